@@ -12,7 +12,7 @@ _LIB_PATH = os.environ.get("DITANGO_B200_LIB") or os.path.join(
     os.path.dirname(os.path.abspath(__file__)), "lib", "libditango_b200.so")
 _lib = None
 
-DTB_F32, DTB_BF16 = 0, 1
+DTB_F32, DTB_BF16, DTB_I8, DTB_E4M3 = 0, 1, 2, 3
 LSE_BHS, LSE_BSH = 0, 1
 MERGE_MAX_STATES = 16
 LAUNCH_OVERLAP_PREVIOUS = 1
@@ -21,7 +21,7 @@ EXPORTS = (
     "dtb_version", "dtb_last_error", "dtb_device_supported", "dtb_read_status",
     "dtb_peek_status_async", "dtb_post_status",
     "dtb_ipc_export_mem", "dtb_ipc_open_mem", "dtb_ipc_close_mem", "dtb_peer_copy_async",
-    "dtb_flash_fwd", "dtb_flash_fwd_ex", "dtb_merge_states", "dtb_copy_chunks",
+    "dtb_flash_fwd", "dtb_flash_fwd_ex", "dtb_merge_states", "dtb_merge_rows", "dtb_copy_chunks",
     "dtb_norm_rope", "dtb_ln_modulate", "dtb_gate_add", "dtb_drift_scratch_bytes", "dtb_drift_accumulate",
     "dtb_drift_noalloc_max_elements", "dtb_drift_accumulate_noalloc",
 )
@@ -74,6 +74,10 @@ def load():
     lib.dtb_merge_states.argtypes = [
         c_int, POINTER(c_void_p), POINTER(c_int), POINTER(c_void_p), POINTER(c_int),
         c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_void_p]
+    lib.dtb_merge_rows.restype = c_int
+    lib.dtb_merge_rows.argtypes = [
+        c_int, POINTER(c_void_p), POINTER(c_int), POINTER(c_void_p), POINTER(c_void_p), POINTER(c_int),
+        c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_void_p]
     lib.dtb_copy_chunks.restype = c_int
     lib.dtb_copy_chunks.argtypes = [
         c_int, POINTER(c_void_p), POINTER(c_void_p), c_int64, c_int64, c_int64, c_int64,

@@ -5,6 +5,7 @@
 #include "flash_fwd_sm100.cuh"
 #include "drift_stats.cuh"
 #include "errors.cuh"
+#include "merge_rows.cuh"
 #include "merge_states.cuh"
 #include "norm_mod.cuh"
 #include "norm_rope.cuh"
@@ -437,6 +438,69 @@ DTB_API int dtb_merge_states(int nstates, const void* const* outs, const int* ou
   if (p.rows == 0) return DTB_OK;
   cudaError_t e = dtb::launch_merge(p, head_dim, d->sm_count, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return fail(DTB_ERR_CUDA, "dtb_merge_states launch failed: %s", cudaGetErrorString(e));
+  return DTB_OK;
+}
+
+DTB_API int dtb_merge_rows(int nstates, const void* const* outs, const int* out_dtypes, const uint8_t* const* exponents,
+                     const float* const* lses, const int* lse_layouts,
+                     float* out, float* lse_out, int lse_out_layout, void* out_bf16,
+                     void* out_codes, int out_codes_dtype, uint8_t* out_exponents,
+                     int batch, int seq, int num_heads, int head_dim, void* stream) {
+  static_assert(DTB_F32 == dtb::kRowsF32 && DTB_BF16 == dtb::kRowsBf16 && DTB_I8 == dtb::kRowsI8 && DTB_E4M3 == dtb::kRowsE4m3, "types");
+  static_assert(DTB_MERGE_MAX_STATES == dtb::kMergeRowsMaxStates, "states");
+  if (nstates < 1 || nstates > DTB_MERGE_MAX_STATES) return fail(DTB_ERR_ARG, "dtb_merge_rows: nstates %d not in [1, %d]", nstates, DTB_MERGE_MAX_STATES);
+  if (head_dim != 64 && head_dim != 128) return fail(DTB_ERR_ARG, "dtb_merge_rows: head_dim %d not in {64, 128}", head_dim);
+  if (!outs || !out_dtypes || !exponents || !lses || !lse_layouts) return fail(DTB_ERR_ARG, "dtb_merge_rows: null argument");
+  if (!out && !out_bf16 && !out_codes) return fail(DTB_ERR_ARG, "dtb_merge_rows: no result buffer was given");
+  if (out_codes && out_codes_dtype != DTB_I8 && out_codes_dtype != DTB_E4M3) return fail(DTB_ERR_ARG, "dtb_merge_rows: bad type %d of the 8-bit result", out_codes_dtype);
+  if (out_codes && !out_exponents) return fail(DTB_ERR_ARG, "dtb_merge_rows: an 8-bit result needs a buffer of exponents");
+  if (lse_out && lse_out_layout != DTB_LSE_BHS && lse_out_layout != DTB_LSE_BSH) return fail(DTB_ERR_ARG, "dtb_merge_rows: bad lse_out_layout %d", lse_out_layout);
+  if (batch < 0 || seq < 0 || num_heads < 1) return fail(DTB_ERR_ARG, "dtb_merge_rows: bad shape");
+  const int64_t rows = static_cast<int64_t>(batch) * seq;
+  if (rows >= (1ll << 31) || rows * num_heads >= (1ll << 31)) return fail(DTB_ERR_ARG, "dtb_merge_rows: more than 2^31 rows");
+  if (!aligned16(out) || !aligned16(out_bf16) || !aligned16(out_codes)) return fail(DTB_ERR_ARG, "dtb_merge_rows: result not 16-byte aligned");
+  dtb::MergeRowsParams p;
+  memset(&p, 0, sizeof(p));
+  int at = 0;
+  for (int pass = 0; pass < 2; ++pass) {           // the states in 8 bits, then the others
+    for (int i = 0; i < nstates; ++i) {
+      const int t = out_dtypes[i];
+      if (t != DTB_F32 && t != DTB_BF16 && t != DTB_I8 && t != DTB_E4M3) return fail(DTB_ERR_ARG, "dtb_merge_rows: bad dtype for state %d", i);
+      const bool narrow = t == DTB_I8 || t == DTB_E4M3;
+      if (narrow != (pass == 0)) continue;
+      if (!outs[i] || (narrow && !exponents[i])) return fail(DTB_ERR_ARG, "dtb_merge_rows: state %d has a null pointer", i);
+      if (!lses[i] && (nstates > 1 || lse_out)) return fail(DTB_ERR_ARG, "dtb_merge_rows: state %d has no lse (only a single state without lse_out may)", i);
+      if (!aligned16(outs[i])) return fail(DTB_ERR_ARG, "dtb_merge_rows: state %d is not 16-byte aligned", i);
+      if (lse_layouts[i] != DTB_LSE_BHS && lse_layouts[i] != DTB_LSE_BSH) return fail(DTB_ERR_ARG, "dtb_merge_rows: bad lse layout for state %d", i);
+      if ((outs[i] == out_bf16 && t != DTB_BF16) || (outs[i] == out_codes) || (outs[i] == out && t != DTB_F32))
+        return fail(DTB_ERR_ARG, "dtb_merge_rows: a result may take the place of a state of its own type only, an 8-bit one of none");
+      if (lse_out && lses[i] == lse_out && lse_layouts[i] != lse_out_layout) return fail(DTB_ERR_ARG, "dtb_merge_rows: in-place lse needs matching layouts");
+      p.values[at] = outs[i];
+      p.exponents[at] = exponents[i];
+      p.lse[at] = lses[i];
+      p.dtype[at] = t;
+      p.lse_layout[at] = lse_layouts[i];
+      ++at;
+    }
+    if (pass == 0) p.narrow = at;
+  }
+  DeviceInfo* d = nullptr;
+  int rc = device_info(&d);
+  if (rc != DTB_OK) return rc;
+  p.nstates = nstates;
+  p.out = out;
+  p.out_bf16 = static_cast<uint16_t*>(out_bf16);
+  p.out_codes = static_cast<uint8_t*>(out_codes);
+  p.out_exponents = out_exponents;
+  p.out_codes_dtype = out_codes_dtype;
+  p.lse_out = lse_out;
+  p.lse_out_layout = lse_out_layout;
+  p.rows = rows * num_heads;
+  p.H = num_heads;
+  p.S = seq;
+  if (p.rows == 0) return DTB_OK;
+  cudaError_t e = dtb::launch_merge_rows(p, head_dim, d->sm_count, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return fail(DTB_ERR_CUDA, "dtb_merge_rows launch failed: %s", cudaGetErrorString(e));
   return DTB_OK;
 }
 

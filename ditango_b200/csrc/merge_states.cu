@@ -13,6 +13,8 @@
 // at 2 x 6851 x 48 x 128 726 us; as it stands 81 us and 306 us; L2 flushed before each launch).
 #include "merge_states.cuh"
 
+#include "row_access.cuh"
+
 #include <math.h>
 
 namespace dtb {
@@ -24,14 +26,6 @@ struct Raw8 {
   uint4 a, b;
 };
 
-__device__ __forceinline__ uint4 ld_stream(const void* p) {
-  uint4 v;
-  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
-}
-__device__ __forceinline__ void st_stream(void* p, uint4 v) {
-  asm volatile("st.global.cs.v4.u32 [%0], {%1,%2,%3,%4};" ::"l"(p), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
-}
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -56,17 +50,6 @@ __device__ __forceinline__ void add_weighted(float (&acc)[8], float w, const Raw
       acc[2 * i + 1] = fmaf(w, __uint_as_float(a[i] & 0xffff0000u), acc[2 * i + 1]);
     }
   }
-}
-
-// Offset of row = (b*S + s)*H + h in an lse tensor.  Rows fit 32 bits (checked by the launcher), so
-// the two divisions are 32-bit.
-__device__ __forceinline__ uint32_t lse_offset(int layout, uint32_t row, uint32_t H, uint32_t S) {
-  if (layout == 1) return row;                    // [B,S,H]
-  const uint32_t tok = row / H;
-  const uint32_t h = row - tok * H;
-  const uint32_t b = tok / S;
-  const uint32_t s = tok - b * S;
-  return (b * H + h) * S + s;                     // [B,H,S]
 }
 
 }  // namespace

@@ -5,12 +5,12 @@ extension is missing or an argument is not a CUDA tensor of the expected kind.
 """
 import ctypes
 import math
-from typing import Optional, Sequence, Tuple
+from typing import NamedTuple, Optional, Sequence, Tuple, Union
 
 import torch
 
 from . import _capi
-from ._capi import DTB_BF16, DTB_F32, LSE_BHS, LSE_BSH
+from ._capi import DTB_BF16, DTB_E4M3, DTB_F32, DTB_I8, LSE_BHS, LSE_BSH
 
 
 class LaunchLog:
@@ -46,6 +46,15 @@ def _need_cuda(*ts):
     for t in ts:
         if t is not None and not t.is_cuda:
             raise _capi.ExtensionError("ditango_b200 kernels take CUDA tensors only")
+
+
+def _need_current_device(*ts):
+    """The kernels run on the current device's current stream: tensors of another device are refused, not reached for."""
+    _need_cuda(*ts)
+    dev = torch.cuda.current_device()
+    for t in ts:
+        if t is not None and t.device.index != dev:
+            raise _capi.ExtensionError(f"tensor on {t.device}, but the current device is cuda:{dev}")
 
 
 def _tok_stride(x: torch.Tensor) -> int:
@@ -179,13 +188,136 @@ def flash_partial(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
     return out, lse
 
 
-def merge_states(states: Sequence[Tuple[torch.Tensor, torch.Tensor, int]], *,
+class QuantizedRows(NamedTuple):
+    """Values of a state in 8 bits: codes [..,H,D] (int8 or float8_e4m3fn) and one exponent byte b per row [..,H]; a value is
+    code * 2^(b - 127).  b = 255 marks a row with an infinity or a NaN, which reads back as NaN."""
+    values: torch.Tensor
+    exponents: torch.Tensor
+
+    @property
+    def shape(self):
+        return self.values.shape
+
+    @property
+    def dtype(self):
+        return self.values.dtype
+
+    @property
+    def device(self):
+        return self.values.device
+
+    @property
+    def nbytes(self) -> int:
+        return self.values.nbytes + self.exponents.nbytes
+
+
+_CODES = {torch.int8: DTB_I8, torch.float8_e4m3fn: DTB_E4M3}
+_VALUES = {torch.float32: DTB_F32, torch.bfloat16: DTB_BF16}
+
+
+def _new_rows(shape, dtype: torch.dtype, device) -> QuantizedRows:
+    if dtype not in _CODES:
+        raise _capi.ExtensionError(f"rows are kept in int8 or float8_e4m3fn, not {dtype}")
+    return QuantizedRows(torch.empty(shape, dtype=dtype, device=device), torch.empty(shape[:-1], dtype=torch.uint8, device=device))
+
+
+def _merge_rows(states, shape, out, lse_out, lse_out_layout, out_bf16, out_rows):
+    """Launch of dtb_merge_rows; states[i] = (values tensor or QuantizedRows, lse or None, layout)."""
+    if len(shape) not in (3, 4):
+        raise _capi.ExtensionError("states are [B,S,H,D] or [T,H,D]")
+    B, S, H, D = (1, *shape) if len(shape) == 3 else shape
+    n = len(states)
+    outs, exps, lses = ((ctypes.c_void_p * n)() for _ in range(3))
+    dts, lays = ((ctypes.c_int * n)() for _ in range(2))
+    for i, (o, l, lay) in enumerate(states):
+        quantized = isinstance(o, QuantizedRows)
+        v, e = o if quantized else (o, None)
+        types = _CODES if quantized else _VALUES
+        _need_current_device(v, e, l)
+        if tuple(v.shape) != tuple(shape) or not v.is_contiguous() or v.dtype not in types:
+            raise _capi.ExtensionError("states must be contiguous, of one shape, and fp32, bf16 or QuantizedRows")
+        if quantized and (tuple(e.shape) != tuple(shape[:-1]) or not e.is_contiguous() or e.dtype != torch.uint8):
+            raise _capi.ExtensionError("exponents must be contiguous uint8, one per row")
+        if l is not None and (l.dtype != torch.float32 or l.numel() != B * S * H or not l.is_contiguous()):
+            raise _capi.ExtensionError("lse must be contiguous fp32 with B*S*H entries")
+        outs[i], dts[i], lays[i] = v.data_ptr(), types[v.dtype], lay
+        exps[i] = e.data_ptr() if quantized else None
+        lses[i] = l.data_ptr() if l is not None else None
+    for t, dtype in ((out, torch.float32), (out_bf16, torch.bfloat16)):
+        _need_current_device(t)
+        if t is not None and (t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous()):
+            raise _capi.ExtensionError(f"a result must be a contiguous {dtype} tensor of the states' shape")
+    if lse_out is not None:
+        _need_current_device(lse_out)
+        if lse_out.dtype != torch.float32 or lse_out.numel() != B * S * H or not lse_out.is_contiguous():
+            raise _capi.ExtensionError("lse_out must be contiguous fp32 with B*S*H entries")
+    if out_rows is not None:
+        _need_current_device(*out_rows)
+        if (out_rows.dtype not in _CODES or tuple(out_rows.shape) != tuple(shape) or out_rows.exponents.dtype != torch.uint8 or
+                tuple(out_rows.exponents.shape) != tuple(shape[:-1]) or not all(t.is_contiguous() for t in out_rows)):
+            raise _capi.ExtensionError("out_rows must be contiguous codes of the states' shape with one uint8 exponent per row")
+    if B * S * H == 0:        # (an empty tensor has no address)
+        return
+    rc = _capi.load().dtb_merge_rows(
+        n, outs, dts, exps, lses, lays, out.data_ptr() if out is not None else None,
+        lse_out.data_ptr() if lse_out is not None else None, lse_out_layout,
+        out_bf16.data_ptr() if out_bf16 is not None else None,
+        out_rows.values.data_ptr() if out_rows is not None else None, _CODES[out_rows.dtype] if out_rows is not None else 0,
+        out_rows.exponents.data_ptr() if out_rows is not None else None, B, S, H, D, _stream_ptr())
+    _capi.check(rc, "dtb_merge_rows")
+    LaunchLog.count += 1
+
+
+def quantize_rows(out: torch.Tensor, dtype: torch.dtype = torch.int8, *, rows: Optional[QuantizedRows] = None) -> QuantizedRows:
+    """The values [..,H,D] of a state (fp32 or bf16, contiguous) in 8 bits, each row by its own power of two; into `rows` where
+    given.  One launch."""
+    if rows is None:
+        _need_current_device(out)
+        rows = _new_rows(out.shape, dtype, out.device)
+    _merge_rows([(out, None, LSE_BSH)], out.shape, None, None, LSE_BSH, None, rows)
+    return rows
+
+
+def dequantize_rows(rows: QuantizedRows, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """The values that `rows` stand for, as fp32 or bf16 (exact in both).  One launch."""
+    if dtype not in _VALUES:
+        raise _capi.ExtensionError("rows are read back as float32 or bfloat16")
+    _need_current_device(*rows)
+    out = torch.empty(rows.shape, dtype=dtype, device=rows.device)
+    f32 = dtype == torch.float32
+    _merge_rows([(rows, None, LSE_BSH)], rows.shape, out if f32 else None, None, LSE_BSH, None if f32 else out, None)
+    return out
+
+
+def merge_states(states: Sequence[Tuple[Union[torch.Tensor, QuantizedRows], torch.Tensor, int]], *,
                  out: Optional[torch.Tensor] = None, lse_out: Optional[torch.Tensor] = None,
                  lse_out_layout: int = LSE_BSH, out_bf16: Optional[torch.Tensor] = None,
-                 want_lse: bool = True, fp32_out: bool = True) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
-    """One-pass merge of partial states.  states[i] = (out_i [B,S,H,D] fp32|bf16 contiguous,
+                 want_lse: bool = True, fp32_out: bool = True,
+                 out_rows: Union[QuantizedRows, torch.dtype, None] = None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """One-pass merge of partial states.  states[i] = (out_i [B,S,H,D] fp32|bf16 contiguous or QuantizedRows,
     lse_i fp32 contiguous, layout_i).  Returns (out fp32 [B,S,H,D], lse_out or None).  With
-    fp32_out=False only the bf16 copy `out_bf16` is written and returned in place of `out`."""
+    fp32_out=False only the bf16 copy `out_bf16` is written and returned in place of `out`.  `out_rows`
+    (QuantizedRows to fill, or the type of new ones: torch.int8, torch.float8_e4m3fn) has the result
+    written in 8 bits too; with fp32_out=False and no `out_bf16` that is what is returned."""
+    if out_rows is not None or any(isinstance(o, QuantizedRows) for o, _, _ in states):
+        shape, device = states[0][0].shape, states[0][0].device
+        if isinstance(out_rows, torch.dtype):
+            out_rows = _new_rows(shape, out_rows, device)
+        if not fp32_out:
+            out = None
+            if out_bf16 is None and out_rows is None:
+                raise _capi.ExtensionError("fp32_out=False needs out_bf16 or out_rows")
+        elif out is None:
+            out = torch.empty(shape, dtype=torch.float32, device=device)
+        if any(l is None for _, l, _ in states):
+            raise _capi.ExtensionError("every state needs its lse")
+        if not want_lse:
+            lse_out = None
+        elif lse_out is None:
+            lead, s, h = tuple(shape[:-3]), shape[-3], shape[-2]
+            lse_out = torch.empty(lead + ((s, h) if lse_out_layout == LSE_BSH else (h, s)), dtype=torch.float32, device=device)
+        _merge_rows(states, shape, out, lse_out, lse_out_layout, out_bf16, out_rows)
+        return (out if out is not None else out_bf16 if out_bf16 is not None else out_rows), lse_out
     lib = _capi.load()
     n = len(states)
     o0 = states[0][0]

@@ -34,6 +34,9 @@ extern "C" {
 /* element types of partial-state outputs */
 #define DTB_F32 0
 #define DTB_BF16 1
+/* values kept in 8 bits with one exponent byte per row (dtb_merge_rows only) */
+#define DTB_I8 2
+#define DTB_E4M3 3
 
 /* layouts of a log-sum-exp tensor that belongs to tokens [B,S] x heads H
  * (packed inputs: B = 1, S = total tokens) */
@@ -173,6 +176,27 @@ DTB_API int dtb_flash_fwd_ex(const void* q, const void* k, const void* v,
 DTB_API int dtb_merge_states(int nstates, const void* const* outs, const int* out_dtypes,
                      const float* const* lses, const int* lse_layouts,
                      float* out, float* lse_out, int lse_out_layout, void* out_bf16,
+                     int batch, int seq, int num_heads, int head_dim, void* stream);
+
+/*
+ * dtb_merge_states for states of which some are held in 8 bits, with a result that may be written in 8 bits; with one
+ * state and no lse it writes a state in 8 bits, or reads it back.  (The reference caches fp32 states, core/cache.py:9-128.)
+ *
+ * A row, one (token, head), of a state in 8 bits is D codes (DTB_I8, or DTB_E4M3) and one exponent byte b; a value is
+ * code * 2^(b - 127), so it is exact in bf16.  Written, b is the smallest byte, at least 8, with max|value| <= M * 2^(b - 127), M
+ * the largest code (127, 448), and a code the nearest to value * 2^(127 - b), ties to even.  A row that holds an infinity or a
+ * NaN has b = 255 and codes 0, and reads back as NaN.
+ *
+ *  outs[i], out_dtypes[i]   [batch, seq, H, D] contiguous, DTB_F32, DTB_BF16, DTB_I8 or DTB_E4M3
+ *  exponents[i]             [batch, seq, H] bytes of a state in 8 bits (not read otherwise)
+ *  lses[i]                  may be NULL for a single state when lse_out is NULL: its weight is then 1
+ *  out, out_bf16, out_codes results in fp32, bf16 and 8 bits (out_codes_dtype, with out_exponents); at least one.  An fp32 or bf16
+ *                           result may be the buffer of a state of its type, lse_out that of a state's lse in its layout.
+ */
+DTB_API int dtb_merge_rows(int nstates, const void* const* outs, const int* out_dtypes, const uint8_t* const* exponents,
+                     const float* const* lses, const int* lse_layouts,
+                     float* out, float* lse_out, int lse_out_layout, void* out_bf16,
+                     void* out_codes, int out_codes_dtype, uint8_t* out_exponents,
                      int batch, int seq, int num_heads, int head_dim, void* stream);
 
 /*
