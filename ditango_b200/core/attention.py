@@ -29,7 +29,7 @@ from .._capi import LSE_BSH
 from ..logger import init_logger
 from ..timer import get_timer
 from ..utils import get_timestep
-from .cache import proCache
+from .cache import QUANTIZED, proCache
 from .config import get_config
 from .redundancy_map import get_redundancy_map
 from .schedule import StepPlan, plan_pair_step, plan_step
@@ -61,6 +61,10 @@ def release_receive_slots(group=None):
         del _SLOTS[key]
 
 
+# values of the config key `cache-dtype`
+_CACHE_DTYPES = {"bf16": torch.bfloat16, "bfloat16": torch.bfloat16, "int8": torch.int8,
+                 "e4m3": torch.float8_e4m3fn, "float8_e4m3fn": torch.float8_e4m3fn}
+
 # Denoising step at which the device status word was last polled by this process (see _run).
 _STATUS_POLL = {"step": None}
 
@@ -74,7 +78,9 @@ class proAttention:
     # torch.bfloat16 the cast is fused into the last kernel of the call and the fp32 copy is never written.
     output_dtype = torch.float32
     # dtype of the values of cached block states (the reference keeps fp32: utils.py:76); bfloat16 halves
-    # the cache's footprint and read traffic.  lse stays fp32.
+    # the cache's footprint and read traffic, int8 and float8_e4m3fn (one power of two per row) quarter it.  lse stays fp32.
+    # A state on its way into 8 bits leaves the attention kernel in bf16, whose rounding (2^-9) is lost in that of the codes, and
+    # is quantised by one launch; the call that made it merges it as it was.
     cache_dtype = torch.float32
     # Overlapping attention launches.  The chunks of a call are attended by one launch each; every launch ends
     # in a partly filled wave and is followed by a launch gap.  A launch made with overlap_previous starts while
@@ -105,8 +111,8 @@ class proAttention:
         # chunk pointer of every rank of the group for this layer; all ranks keep the same copy
         self._pointers = [0] * self.isp_size
         cfg = get_config()
-        if cfg is not None and getattr(cfg, "cache_dtype", None) in ("bf16", "bfloat16"):
-            self.cache_dtype = torch.bfloat16
+        if cfg is not None and getattr(cfg, "cache_dtype", None) in _CACHE_DTYPES:
+            self.cache_dtype = _CACHE_DTYPES[cfg.cache_dtype]
         if cfg is not None and getattr(cfg, "output_dtype", None) in ("bf16", "bfloat16"):
             self.output_dtype = torch.bfloat16
         # Partial states, cached states and their merges keep lse as [B,S,H] ([T,H] packed): one lse per
@@ -248,12 +254,14 @@ class proAttention:
 
         chain, reorder = self._chain_mode()
         self._chain_open = False
+        quantized = self.cache_dtype in QUANTIZED
+        kept = torch.bfloat16 if quantized else self.cache_dtype
 
         def attend(kv, keep=False):
             kw = {}
             if packed:
                 kw = dict(cu_seqlens_q=cu_q, cu_seqlens_k=kv[2], max_seqlen_q=max_q, max_seqlen_k=max_kv)
-            return self._attend(chain, query, kv[0], kv[1], out_dtype=self.cache_dtype if keep else torch.float32, **kw)
+            return self._attend(chain, query, kv[0], kv[1], out_dtype=kept if keep else torch.float32, **kw)
 
         plan = plan_pair_step(N, flags, self._have)
         posted = self._post_hops(plan, plan.n_hops, payload)
@@ -272,6 +280,10 @@ class proAttention:
                   for o, l in (self._chunk_states.get(src, (None, None)),) if l is not None]
         self.stats["cached_blocks_merged"] += len(others) - len(plan.ranks[me].owners)
         out, lse = self._finish(own, others)
+        if quantized:             # behind the launches of the call, so that these may overlap one another
+            for src in plan.ranks[me].owners:
+                o, l = self._chunk_states[src]
+                self._chunk_states[src] = (_engine.quantize_rows(o, self.cache_dtype), l)
         self._last_lse = lse
         self.stats["calls"] += 1
         return out
@@ -352,6 +364,9 @@ class proAttention:
         #    written by the attention kernel in the cache's dtype: no cast pass afterwards.
         fresh = None
         chunk_states = []
+        quantized = self.cache.store_dtype in QUANTIZED or self.cache_dtype in QUANTIZED
+        kept = torch.bfloat16 if quantized else self.cache_dtype
+        to_store = []                          # states to be quantised, behind the launches of the call
         fresh_chunks = sum(1 for o in mine.owners if o != me)
         for hop in range(stride):
             current, handle = posted[hop]
@@ -361,13 +376,16 @@ class proAttention:
                 if own is None:            # (reordered launches attended it before the waits)
                     own = attend(payload, dtype=torch.bfloat16 if direct16 else torch.float32)
             elif keep_chunks:
-                st = attend(current, dtype=self.cache_dtype)
-                if st[0].dtype != self.cache.store_dtype:
-                    self._chain_open = False           # store_block converts: a kernel behind the launch
-                self.cache.store_block(mine.owners[hop], st[0], st[1])
+                st = attend(current, dtype=kept)
+                if quantized:
+                    to_store.append((mine.owners[hop], st))
+                else:
+                    if st[0].dtype != self.cache.store_dtype:
+                        self._chain_open = False           # store_block converts: a kernel behind the launch
+                    self.cache.store_block(mine.owners[hop], st[0], st[1])
                 chunk_states.append((st[0], st[1], LSE_BSH))
             elif keep_block:
-                fresh = attend(current, into=fresh, dtype=self.cache_dtype if fresh_chunks == 1 else torch.float32)
+                fresh = attend(current, into=fresh, dtype=kept if fresh_chunks == 1 else torch.float32)
             else:
                 own = attend(current, into=own)          # nothing is kept: fold into the result
 
@@ -376,7 +394,9 @@ class proAttention:
         # 4. store the fresh block, combine everything in one pass
         if fresh is not None:
             self.cache.store_block(mine.target_block, fresh[0], fresh[1])
-            chunk_states.append((self.cache.out_block_cache[mine.target_block], fresh[1], LSE_BSH))
+            chunk_states.append((fresh[0] if quantized else self.cache.out_block_cache[mine.target_block], fresh[1], LSE_BSH))
+        for owner, st in to_store:
+            self.cache.store_block(owner, st[0], st[1])
         out, lse = self._finish(own, states + chunk_states)
 
         # 5. pointers and cache layout for the next step

@@ -6,7 +6,9 @@ block" as last computed; `update_cache_blocks` re-blocks the list when the next 
 stride (:49-72) and empties the slot that will be recomputed.  Differences: re-blocking merges all
 member slots of a new block in ONE kernel pass (the reference chains pairwise merges, :28-46); the
 block size used by the memory guard is computed from shapes (the reference allocates a zero block to
-measure it, :89-101); slots may optionally hold bf16 `out` to halve the footprint.
+measure it, :89-101); slots may optionally hold bf16 `out` to halve the footprint, or 8-bit rows
+(`QuantizedRows`: codes and one power of two per row) to quarter it, quantised as they are stored and as blocks
+merge; the merge that reads them does so in place of a pass that would unpack them.
 """
 from typing import List, Optional, Tuple
 
@@ -20,6 +22,9 @@ from ..utils import get_timestep
 logger = init_logger(__name__)
 
 State = Tuple[torch.Tensor, torch.Tensor]
+
+# store types whose slots hold QuantizedRows
+QUANTIZED = (torch.int8, torch.float8_e4m3fn)
 
 
 def _device_total_mb() -> float:
@@ -42,7 +47,7 @@ class proCache:
         self.layer_id = layer_id
         self.store_dtype = store_dtype
         self.lse_layout = lse_layout          # layout of every lse handed to store_block ([B,H,S] or [B,S,H])
-        self.out_block_cache: List[Optional[torch.Tensor]] = [None] * isp_size
+        self.out_block_cache: List[Optional[torch.Tensor]] = [None] * isp_size       # (or QuantizedRows)
         self.lse_block_cache: List[Optional[torch.Tensor]] = [None] * isp_size
         self.block_size_mb: Optional[float] = None
         self.memory_constraint = 0.72 * _device_total_mb()
@@ -55,7 +60,7 @@ class proCache:
 
     def store_block(self, block_id: int, out: torch.Tensor, lse: torch.Tensor):
         if out.dtype != self.store_dtype:
-            out = out.to(self.store_dtype)
+            out = _engine.quantize_rows(out, self.store_dtype) if self.store_dtype in QUANTIZED else out.to(self.store_dtype)
         self.out_block_cache[block_id] = out
         self.lse_block_cache[block_id] = lse
 
@@ -79,7 +84,9 @@ class proCache:
             if len(members) == 1:
                 outs[i], lses[i] = members[0][0], members[0][1]
                 continue
-            if self.store_dtype == torch.bfloat16:
+            if self.store_dtype in QUANTIZED:
+                o, l = _engine.merge_states(members, lse_out_layout=self.lse_layout, out_rows=self.store_dtype, fp32_out=False)
+            elif self.store_dtype == torch.bfloat16:
                 # the merged block leaves the kernel as bf16; no fp32 copy is written
                 o = torch.empty(members[0][0].shape, dtype=torch.bfloat16, device=members[0][0].device)
                 _, l = _engine.merge_states(members, lse_out_layout=self.lse_layout, out_bf16=o, fp32_out=False)
@@ -108,10 +115,12 @@ class proCache:
     # ------------------------------------------------------------------ memory guard
     def set_block_size_mb(self, tensor: torch.Tensor) -> float:
         """Size of one cached block for a chunk shaped like `tensor` ([.., H, D]): fp32 values plus
-        one fp32 lse per row, i.e. the bytes of a [.., H, D+1] fp32 tensor."""
+        one fp32 lse per row, i.e. the bytes of a [.., H, D+1] fp32 tensor; 8-bit rows: a byte per value, an
+        exponent byte and the lse per row."""
         if self.block_size_mb is None:
             rows = tensor.numel() // tensor.shape[-1]
-            self.block_size_mb = rows * (tensor.shape[-1] + 1) * 4 / (1024 ** 2)
+            row_bytes = tensor.shape[-1] + 5 if self.store_dtype in QUANTIZED else (tensor.shape[-1] + 1) * 4
+            self.block_size_mb = rows * row_bytes / (1024 ** 2)
         return self.block_size_mb
 
     def pass_memory_check(self, next_isp_stride: int, layer_id: int) -> bool:
@@ -135,7 +144,7 @@ class proCache:
         n = 0
         for o, l in zip(self.out_block_cache, self.lse_block_cache):
             if o is not None:
-                n += o.numel() * o.element_size() + l.numel() * l.element_size()
+                n += o.nbytes + l.nbytes
         return n
 
     def report_cache_status(self, layer_id: int):

@@ -46,3 +46,18 @@ def test_rows_on_the_cpu_and_of_other_types_are_refused():
             call()
     with pytest.raises(ExtensionError):
         ops._new_rows((1, 2, 3, 64), torch.uint8, "cpu")
+
+
+@pytest.mark.parametrize("key,dtype", [("int8", torch.int8), ("e4m3", torch.float8_e4m3fn), ("bf16", torch.bfloat16), ("fp32", torch.float32)])
+def test_the_cache_type_is_a_config_key(key, dtype, tmp_path):
+    from ditango_b200.core.attention import proAttention
+    from ditango_b200.core import config
+    from ditango_b200.core.group_coordinate import SingleRankGroup
+    (tmp_path / "c.yaml").write_text(f"cache-dtype: {key}\n")
+    before = config.DITANGO_CONFIG
+    try:
+        config.init_config(str(tmp_path / "c.yaml"), make_output_dir=False)
+        layer = proAttention(0, SingleRankGroup(torch.device("cpu")))
+        assert layer.cache_dtype == layer.cache.store_dtype == dtype
+    finally:
+        config.DITANGO_CONFIG = before
