@@ -3,6 +3,7 @@
 #include "../../include/ditango_b200.h"
 
 #include "flash_fwd_sm100.cuh"
+#include "flash_window.cuh"
 #include "drift_stats.cuh"
 #include "errors.cuh"
 #include "merge_rows.cuh"
@@ -397,6 +398,84 @@ DTB_API int dtb_flash_fwd_ex(const void* q, const void* k, const void* v,
   return flash_fwd_impl(q, k, v, q_tok_stride, k_tok_stride, v_tok_stride, out, out_dtype, out_tok_stride, lse, lse_layout,
                         accumulate, cu_seqlens_q, cu_seqlens_k, nseg, seqlen_q, seqlen_k, total_q, total_k, num_heads,
                         head_dim, softmax_scale, launch_flags, stream);
+}
+
+DTB_API int dtb_flash_window(const void* q, const void* k, const void* v,
+                     int64_t q_tok_stride, int64_t q_batch_stride, int64_t k_tok_stride, int64_t k_batch_stride,
+                     int64_t v_tok_stride, int64_t v_batch_stride,
+                     void* out, int out_dtype, float* lse, int lse_layout, int accumulate,
+                     const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, const int32_t* seqlens_k,
+                     int nseg, int seqlen_q, int seqlen_k, int64_t total_q, int64_t total_k,
+                     int num_heads, int num_kv_heads, int head_dim, float softmax_scale,
+                     int left, int right, int sinks, int q_start, int k_start, void* stream) {
+  constexpr int kFar = 1 << 30;
+  static_assert(DTB_QUERIES_LAST == dtb::kQueriesLast, "q_start");
+  if (!q || !k || !v || !out || !lse) return fail(DTB_ERR_ARG, "dtb_flash_window: null tensor pointer");
+  if (head_dim != 64 && head_dim != 128) return fail(DTB_ERR_ARG, "dtb_flash_window: head_dim %d not in {64, 128}", head_dim);
+  if (num_heads < 1 || num_heads > 65535 || num_kv_heads < 1 || num_heads % num_kv_heads)
+    return fail(DTB_ERR_ARG, "dtb_flash_window: %d query heads over %d key heads", num_heads, num_kv_heads);
+  if (nseg < 1 || nseg > 65535) return fail(DTB_ERR_ARG, "dtb_flash_window: nseg %d out of range", nseg);
+  if (seqlen_q < 0 || seqlen_k < 0 || total_q < 0 || total_k < 0) return fail(DTB_ERR_ARG, "dtb_flash_window: negative length");
+  if (seqlen_q >= kFar || seqlen_k >= kFar || total_q >= (1ll << 31) || total_k >= (1ll << 31)) return fail(DTB_ERR_ARG, "dtb_flash_window: too many tokens");
+  if ((cu_seqlens_q == nullptr) != (cu_seqlens_k == nullptr)) return fail(DTB_ERR_ARG, "dtb_flash_window: cu_seqlens_q and cu_seqlens_k must both be given or both be null");
+  if (cu_seqlens_q != nullptr && seqlens_k != nullptr) return fail(DTB_ERR_ARG, "dtb_flash_window: seqlens_k is for dense batches");
+  if (cu_seqlens_q == nullptr && (static_cast<int64_t>(nseg) * seqlen_q != total_q || static_cast<int64_t>(nseg) * seqlen_k != total_k))
+    return fail(DTB_ERR_ARG, "dtb_flash_window: total tokens are not nseg*seqlen");
+  if (left < -1 || right < -1 || sinks < 0 || left > kFar || right > kFar || sinks > kFar) return fail(DTB_ERR_ARG, "dtb_flash_window: window (%d, %d) or sinks %d out of range", left, right, sinks);
+  if ((q_start != DTB_QUERIES_LAST && (q_start < -kFar || q_start > kFar)) || k_start < -kFar || k_start > kFar)
+    return fail(DTB_ERR_ARG, "dtb_flash_window: position out of range");
+  const int64_t q_width = static_cast<int64_t>(num_heads) * head_dim, k_width = static_cast<int64_t>(num_kv_heads) * head_dim;
+  if (q_tok_stride < q_width || k_tok_stride < k_width || v_tok_stride < k_width) return fail(DTB_ERR_ARG, "dtb_flash_window: token stride smaller than the heads");
+  if (cu_seqlens_q == nullptr && nseg > 1 && (q_batch_stride < q_width || k_batch_stride < k_width || v_batch_stride < k_width))
+    return fail(DTB_ERR_ARG, "dtb_flash_window: batch stride smaller than the heads");
+  if ((q_tok_stride | q_batch_stride | k_tok_stride | k_batch_stride | v_tok_stride | v_batch_stride) & 7) return fail(DTB_ERR_ARG, "dtb_flash_window: strides must be multiples of 8 elements");
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out)) return fail(DTB_ERR_ARG, "dtb_flash_window: tensor pointers must be 16-byte aligned");
+  if (out_dtype != DTB_F32 && out_dtype != DTB_BF16) return fail(DTB_ERR_ARG, "dtb_flash_window: bad out_dtype %d", out_dtype);
+  if (lse_layout != DTB_LSE_BHS && lse_layout != DTB_LSE_BSH) return fail(DTB_ERR_ARG, "dtb_flash_window: bad lse_layout %d", lse_layout);
+  if (accumulate && out_dtype != DTB_F32) return fail(DTB_ERR_ARG, "dtb_flash_window: accumulate needs an fp32 state");
+  if (!(softmax_scale > 0.f)) return fail(DTB_ERR_ARG, "dtb_flash_window: softmax_scale must be positive");
+  DeviceInfo* d = nullptr;
+  int rc = device_info(&d);
+  if (rc != DTB_OK) return rc;
+  if (seqlen_q == 0 || total_q == 0) return DTB_OK;
+
+  dtb::WindowParams p;
+  memset(&p, 0, sizeof(p));
+  p.f.out = out;
+  p.f.lse = lse;
+  p.f.cu_q = cu_seqlens_q;
+  p.f.cu_k = cu_seqlens_k;
+  p.f.status = d->status_ptr;
+  p.f.out_tok_stride = q_width;
+  p.f.total_q = total_q;
+  p.f.nseg = nseg;
+  p.f.seqlen_q = seqlen_q;
+  p.f.seqlen_k = seqlen_k;
+  p.f.num_heads = num_heads;
+  p.f.scale_log2 = softmax_scale * 1.4426950408889634f;
+  p.f.out_dtype = out_dtype;
+  p.f.lse_layout = lse_layout;
+  p.f.accumulate = accumulate ? 1 : 0;
+  p.q = static_cast<const uint16_t*>(q);
+  p.k = static_cast<const uint16_t*>(k);
+  p.v = static_cast<const uint16_t*>(v);
+  p.q_tok = q_tok_stride;
+  p.q_batch = q_batch_stride;
+  p.k_tok = k_tok_stride;
+  p.k_batch = k_batch_stride;
+  p.v_tok = v_tok_stride;
+  p.v_batch = v_batch_stride;
+  p.seqlens_k = seqlens_k;
+  p.kv_heads = num_kv_heads;
+  p.left = left < 0 ? kFar : left;
+  p.right = right < 0 ? kFar : right;
+  p.sinks = sinks;
+  p.q_start = q_start;
+  p.k_start = k_start;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const cudaError_t e = head_dim == 64 ? dtb::launch_window_rows<64>(p, d->sm_count, s) : dtb::launch_window_rows<128>(p, d->sm_count, s);
+  if (e != cudaSuccess) return fail(DTB_ERR_CUDA, "dtb_flash_window launch failed: %s", cudaGetErrorString(e));
+  return DTB_OK;
 }
 
 DTB_API int dtb_merge_states(int nstates, const void* const* outs, const int* out_dtypes,

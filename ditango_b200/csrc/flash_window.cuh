@@ -1,0 +1,77 @@
+// Parameters and launchers of the windowed attention kernels (flash_window_rows.cu), and which keys a row sees.
+#pragma once
+#include "flash_fwd_sm100.cuh"
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace dtb {
+
+constexpr int kQueriesLast = INT32_MIN;      // q_start: the queries are the last positions of their sequence
+
+struct WindowParams {
+  FlashParams f;                 // (scale, results, lengths; out is contiguous)
+  const uint16_t* q;             // token t of sequence b, head h: q + b * q_batch + t * q_tok + h * D
+  const uint16_t* k;
+  const uint16_t* v;
+  int64_t q_tok, q_batch, k_tok, k_batch, v_tok, v_batch;      // elements; packed: no batch strides
+  const int32_t* seqlens_k;      // keys of each sequence of a dense batch, or null: all seqlen_k
+  int kv_heads;                  // divides f.num_heads
+  int left, right, sinks;        // each within [0, 2^30]
+  int q_start, k_start;          // positions of the first query (or kQueriesLast) and the first key
+};
+
+// The sequence of a CTA: where its queries and keys begin among the tokens, how many there are, and the first query's position
+// counted from the first key.
+struct WindowSeq {
+  int q_begin, q_len, k_begin, k_len;
+  int64_t q_shift;
+};
+
+__device__ __forceinline__ WindowSeq window_seq(const WindowParams& p, int seg) {
+  WindowSeq s;
+  if (p.f.cu_q != nullptr) {
+    s.q_begin = p.f.cu_q[seg];
+    s.q_len = p.f.cu_q[seg + 1] - s.q_begin;
+    s.k_begin = p.f.cu_k[seg];
+    s.k_len = p.f.cu_k[seg + 1] - s.k_begin;
+  } else {
+    s.q_begin = s.k_begin = 0;
+    s.q_len = p.f.seqlen_q;
+    s.k_len = p.f.seqlen_k;
+    if (p.seqlens_k != nullptr) s.k_len = min(p.seqlens_k[seg], s.k_len);
+  }
+  s.q_len = max(min(s.q_len, p.f.seqlen_q), 0);
+  s.k_len = max(min(s.k_len, p.f.seqlen_k), 0);
+  s.q_shift = p.q_start == kQueriesLast ? static_cast<int64_t>(s.k_len) - s.q_len : static_cast<int64_t>(p.q_start) - p.k_start;
+  return s;
+}
+
+// Keys that query i sees: [0, first) and [lo, hi), first <= lo <= hi.  A key at position j is seen from position x when
+// j <= x + right and (j >= x - left or j < sinks).
+struct WindowSpan {
+  int first, lo, hi;
+};
+
+__device__ __forceinline__ int clamp_key(int64_t j, int k_len) { return static_cast<int>(j < 0 ? 0 : j > k_len ? k_len : j); }
+
+__device__ __forceinline__ WindowSpan window_span(const WindowParams& p, const WindowSeq& s, int i) {
+  const int64_t x = s.q_shift + i;
+  const int sinks = clamp_key(static_cast<int64_t>(p.sinks) - p.k_start, s.k_len);
+  WindowSpan w;
+  w.hi = clamp_key(x + p.right + 1, s.k_len);
+  w.first = min(sinks, w.hi);
+  w.lo = min(max(clamp_key(x - p.left, s.k_len), sinks), w.hi);
+  w.lo = max(w.lo, w.first);
+  return w;
+}
+
+// Element offset of a sequence's token in a q / k / v tensor (dense: token inside its sequence; packed: of the whole tensor).
+__device__ __forceinline__ int64_t window_offset(const WindowParams& p, int seg, int64_t tok, int64_t tok_stride, int64_t batch_stride) {
+  return (p.f.cu_q != nullptr ? 0 : seg * batch_stride) + tok * tok_stride;
+}
+
+template <int D>
+cudaError_t launch_window_rows(const WindowParams& p, int sm_count, cudaStream_t stream);
+
+}  // namespace dtb

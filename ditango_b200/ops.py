@@ -188,6 +188,92 @@ def flash_partial(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
     return out, lse
 
 
+def _strides(x: torch.Tensor, packed: bool) -> Tuple[int, int]:
+    """(token, batch) strides in elements of a [B,S,H,D] or packed [T,H,D] tensor whose (H, D) block is dense; that of an axis of
+    length 1, which nothing steps along, is given as a dense tensor's."""
+    H, D = x.shape[-2], x.shape[-1]
+    if (x.stride(-1) != 1 and D != 1) or (x.stride(-2) != D and H != 1):
+        raise _capi.ExtensionError("head and channel dims must be contiguous")
+    tok = x.stride(-3) if x.shape[-3] > 1 else H * D
+    return tok, (0 if packed else x.stride(0) if x.shape[0] > 1 else tok * x.shape[1])
+
+
+def flash_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, left: int = -1, right: int = -1, sinks: int = 0,
+                 q_start: Optional[int] = None, k_start: int = 0, seqlens_k: Optional[torch.Tensor] = None,
+                 out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None, accumulate: bool = False,
+                 out_dtype: torch.dtype = torch.float32, lse_layout: int = LSE_BHS, softmax_scale: Optional[float] = None,
+                 cu_seqlens_q: Optional[torch.Tensor] = None, cu_seqlens_k: Optional[torch.Tensor] = None,
+                 max_seqlen_q: Optional[int] = None, max_seqlen_k: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Attention state of q against one KV chunk with a sliding window and `sinks` first tokens that stay visible.
+
+    The query at position x sees the key at position j when j <= x + right and (j >= x - left or j < sinks); -1 means no limit.
+    Key j of a sequence is at position k_start + j.  Query i is at q_start + i; q_start=None puts the queries at the end of
+    their sequence's keys (position i when there are as many queries as keys, the newest positions when the keys are a cache).
+
+    Dense: q [B,Sq,H,D], k,v [B,Sk,Hk,D] bf16, any batch and token strides that are multiples of 8; Hk divides H.  `seqlens_k`
+    (int32 [B] on the device) gives the number of keys of each sequence, the rest of Sk may hold anything.  Packed
+    (cu_seqlens given): q [Tq,H,D], k,v [Tk,Hk,D].  Returns (out, lse) as flash_partial does, mergeable with its states; with
+    accumulate=True the state is merged into the given fp32 (out, lse) in place.  A row that sees no key has out 0 and lse -inf.
+    """
+    _need_current_device(q, k, v, out, lse, cu_seqlens_q, cu_seqlens_k, seqlens_k)
+    if q.dtype != torch.bfloat16 or k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16:
+        raise _capi.ExtensionError("q, k, v must be bfloat16")
+    packed = cu_seqlens_q is not None
+    if packed != (cu_seqlens_k is not None):
+        raise _capi.ExtensionError("cu_seqlens_q and cu_seqlens_k go together")
+    dims = 3 if packed else 4
+    if q.dim() != dims or k.dim() != dims or v.shape != k.shape or k.shape[-1] != q.shape[-1]:
+        raise _capi.ExtensionError("q is [B,S,H,D] and k, v are [B,S,Hk,D], packed [T,H,D] and [T,Hk,D]")
+    H, D, Hk = q.shape[-2], q.shape[-1], k.shape[-2]
+    if packed:
+        Tq, Tk = q.shape[0], k.shape[0]
+        nseg = cu_seqlens_q.numel() - 1
+        sq = min(Tq, int(max_seqlen_q)) if max_seqlen_q is not None else Tq
+        sk = min(Tk, int(max_seqlen_k)) if max_seqlen_k is not None else Tk
+        if any(c.dtype != torch.int32 or not c.is_contiguous() for c in (cu_seqlens_q, cu_seqlens_k)) or cu_seqlens_k.numel() != nseg + 1:
+            raise _capi.ExtensionError("cu_seqlens must be contiguous int32, as many of q as of k")
+        lse_shape = (H, Tq) if lse_layout == LSE_BHS else (Tq, H)
+    else:
+        nseg, sq, sk = q.shape[0], q.shape[1], k.shape[1]
+        if k.shape[0] != nseg:
+            raise _capi.ExtensionError("q and k must have one batch size")
+        Tq, Tk = nseg * sq, nseg * sk
+        lse_shape = (nseg, H, sq) if lse_layout == LSE_BHS else (nseg, sq, H)
+    if seqlens_k is not None and (packed or seqlens_k.dtype != torch.int32 or seqlens_k.numel() != nseg or not seqlens_k.is_contiguous()):
+        raise _capi.ExtensionError("seqlens_k is contiguous int32 with one length per sequence of a dense batch")
+    if accumulate and (out is None or lse is None or out.dtype != torch.float32):
+        raise _capi.ExtensionError("accumulate needs an existing fp32 (out, lse) state")
+    if out is None:
+        out = torch.empty(q.shape, dtype=out_dtype, device=q.device)
+    if lse is None:
+        lse = torch.empty(lse_shape, dtype=torch.float32, device=q.device)
+    if out.shape != q.shape or not out.is_contiguous() or out.dtype not in _VALUES:
+        raise _capi.ExtensionError("out must be contiguous float32 or bfloat16 of q's shape")
+    if tuple(lse.shape) != lse_shape or not lse.is_contiguous() or lse.dtype != torch.float32:
+        raise _capi.ExtensionError(f"lse must be a contiguous fp32 tensor of shape {lse_shape}")
+    if q.numel() == 0:
+        return out, lse
+    keys, values = (x.data_ptr() or q.data_ptr() for x in (k, v))        # (an empty tensor has no address, and nothing is read)
+    ev = None
+    if LaunchLog.events is not None:
+        ev = (torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True))
+        ev[0].record()
+    rc = _capi.load().dtb_flash_window(
+        q.data_ptr(), keys, values, *_strides(q, packed), *_strides(k, packed), *_strides(v, packed),
+        out.data_ptr(), _VALUES[out.dtype], lse.data_ptr(), lse_layout, int(accumulate),
+        cu_seqlens_q.data_ptr() if packed else None, cu_seqlens_k.data_ptr() if packed else None,
+        seqlens_k.data_ptr() if seqlens_k is not None else None, nseg, sq, sk, Tq, Tk, H, Hk, D,
+        1.0 / math.sqrt(D) if softmax_scale is None else float(softmax_scale), left, right, sinks,
+        _capi.QUERIES_LAST if q_start is None else q_start, k_start, _stream_ptr())
+    _capi.check(rc, "dtb_flash_window")
+    LaunchLog.count += 1
+    if ev is not None:
+        ev[1].record()
+        span = sk if left < 0 or right < 0 else min(sk, left + right + 1 + sinks)      # upper bound of a row's keys
+        LaunchLog.events.append((ev[0], ev[1], 4.0 * nseg * H * sq * span * D))
+    return out, lse
+
+
 class QuantizedRows(NamedTuple):
     """Values of a state in 8 bits: codes [..,H,D] (int8 or float8_e4m3fn) and one exponent byte b per row [..,H]; a value is
     code * 2^(b - 127).  b = 255 marks a row with an infinity or a NaN, which reads back as NaN."""

@@ -158,6 +158,33 @@ DTB_API int dtb_flash_fwd_ex(const void* q, const void* k, const void* v,
                      int num_heads, int head_dim, float softmax_scale, int launch_flags, void* stream);
 
 /*
+ * dtb_flash_fwd with a sliding window and first tokens that stay visible.  (The reference has full attention only.)  The query at
+ * position x sees the key at position j when
+ *     j <= x + right   and   (j >= x - left  or  j < sinks)
+ * Key j of a sequence is at position k_start + j; query i at q_start + i, or with q_start = DTB_QUERIES_LAST at the end of the keys,
+ * the last query at the last key's position.  A row that sees nothing gets out = 0, lse = -inf (with accumulate its state stays).
+ *
+ *  q, k, v        bf16, token t of sequence b at t * tok_stride + b * batch_stride, head h behind it at h * head_dim (batch strides are
+ *                 not read for packed batches).  Strides are multiples of 8 elements, pointers 16-byte aligned.
+ *  out            [total_q, num_heads, head_dim] contiguous; lse, lse_layout, accumulate as for dtb_flash_fwd
+ *  num_kv_heads   divides num_heads: query head h meets key head h / (num_heads / num_kv_heads)
+ *  cu_seqlens_q/k packed batch, as for dtb_flash_fwd: rows outside all segments are left alone
+ *  seqlens_k      NULL, or device int32[nseg]: the keys of each sequence of a dense batch (at most seqlen_k; what the memory holds
+ *                 behind them does not matter)
+ *  left, right    keys visible before and behind the query's own position, -1 for all; sinks first positions
+ * Keys and values that no query of a block of rows sees may hold anything; those that some see must be finite.
+ */
+#define DTB_QUERIES_LAST (-2147483647 - 1)
+DTB_API int dtb_flash_window(const void* q, const void* k, const void* v,
+                     int64_t q_tok_stride, int64_t q_batch_stride, int64_t k_tok_stride, int64_t k_batch_stride,
+                     int64_t v_tok_stride, int64_t v_batch_stride,
+                     void* out, int out_dtype, float* lse, int lse_layout, int accumulate,
+                     const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, const int32_t* seqlens_k,
+                     int nseg, int seqlen_q, int seqlen_k, int64_t total_q, int64_t total_k,
+                     int num_heads, int num_kv_heads, int head_dim, float softmax_scale,
+                     int left, int right, int sinks, int q_start, int k_start, void* stream);
+
+/*
  * N-way merge of partial softmax states in one pass over HBM:
  *     lse_out = log sum_i exp(lse_i),   out = sum_i exp(lse_i - lse_out) * out_i
  * Replaces the chains of update_out_and_lse (utils.py:24-84) at core/attention.py:110-116, :144,

@@ -61,3 +61,30 @@ def test_the_cache_type_is_a_config_key(key, dtype, tmp_path):
         assert layer.cache_dtype == layer.cache.store_dtype == dtype
     finally:
         config.DITANGO_CONFIG = before
+
+
+def _window(lib, *, q=16, k=16, v=16, qt=192, qb=1920, kt=192, kb=1920, vt=192, vb=1920, out=16, odt=0, lse=16, lay=0, acc=0, cq=None, ck=None,
+            sl=None, n=2, sq=10, sk=10, tq=20, tk=20, H=3, Hk=3, D=64, scale=0.1, left=3, right=3, sinks=0, qs=0, ks=0):
+    return lib.dtb_flash_window(q, k, v, qt, qb, kt, kb, vt, vb, out, odt, lse, lay, acc, cq, ck, sl, n, sq, sk, tq, tk, H, Hk, D, scale,
+                                left, right, sinks, qs, ks, None)
+
+
+@pytest.mark.parametrize("args,word", [
+    (dict(q=None), "null"), (dict(lse=None), "null"), (dict(D=80), "head_dim"), (dict(H=3, Hk=2), "query heads"), (dict(Hk=0), "query heads"),
+    (dict(n=0), "nseg"), (dict(sq=-1), "negative"), (dict(n=1, sq=2 ** 30, tq=2 ** 30), "too many"), (dict(cq=16), "cu_seqlens"),
+    (dict(cq=16, ck=16, sl=16), "seqlens_k"), (dict(tq=21), "total"), (dict(tk=19), "total"), (dict(left=-2), "window"), (dict(right=2 ** 30 + 1), "window"),
+    (dict(sinks=-1), "sinks"), (dict(qs=2 ** 30 + 1), "position"), (dict(ks=-2 ** 30 - 1), "position"), (dict(qt=128), "token stride"),
+    (dict(kb=128), "batch stride"), (dict(vt=196), "multiples of 8"), (dict(q=24), "aligned"), (dict(odt=2), "out_dtype"), (dict(lay=2), "lse_layout"),
+    (dict(acc=1, odt=1), "accumulate"), (dict(scale=0.0), "scale"), (dict(scale=float("nan")), "scale")])
+def test_flash_window_refuses(args, word):
+    from ditango_b200 import _capi
+    lib = _capi.load()
+    assert _window(lib, **args) == -1 and word in lib.dtb_last_error().decode()
+
+
+def test_flash_window_takes_gpu_tensors_only():
+    from ditango_b200 import ops
+    from ditango_b200._capi import ExtensionError
+    q = torch.zeros(1, 8, 1, 64, dtype=torch.bfloat16)
+    with pytest.raises(ExtensionError):
+        ops.flash_window(q, q, q, left=3)
