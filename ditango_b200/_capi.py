@@ -5,7 +5,7 @@ device is not compute capability 10.x, calls raise; nothing falls back to PyTorc
 """
 import ctypes
 import os
-from ctypes import c_char_p, c_float, c_int, c_int64, c_void_p, POINTER
+from ctypes import c_char_p, c_double, c_float, c_int, c_int64, c_void_p, POINTER
 
 # DITANGO_B200_LIB points at a library built elsewhere (same ABI); default: the in-tree build.
 _LIB_PATH = os.environ.get("DITANGO_B200_LIB") or os.path.join(
@@ -23,7 +23,7 @@ EXPORTS = (
     "dtb_peek_status_async", "dtb_post_status",
     "dtb_ipc_export_mem", "dtb_ipc_open_mem", "dtb_ipc_close_mem", "dtb_peer_copy_async",
     "dtb_flash_fwd", "dtb_flash_fwd_ex", "dtb_flash_window", "dtb_merge_states", "dtb_merge_rows", "dtb_copy_chunks",
-    "dtb_norm_rope", "dtb_ln_modulate", "dtb_gate_add", "dtb_drift_scratch_bytes", "dtb_drift_accumulate",
+    "dtb_norm_rope", "dtb_norm_rope_grid", "dtb_norm_rope_grid_scratch_bytes", "dtb_norm_rope_grid_backward", "dtb_ln_modulate", "dtb_gate_add", "dtb_drift_scratch_bytes", "dtb_drift_accumulate",
     "dtb_drift_noalloc_max_elements", "dtb_drift_accumulate_noalloc",
 )
 
@@ -92,6 +92,16 @@ def load():
     lib.dtb_norm_rope.argtypes = [
         c_void_p, c_void_p, c_void_p, c_void_p, c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_float,
         c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p]
+    place = [POINTER(c_int), POINTER(c_int), POINTER(c_double), c_int64] + [c_int] * 8
+    side = [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_float]
+    lib.dtb_norm_rope_grid.restype = c_int
+    lib.dtb_norm_rope_grid.argtypes = side + side + [c_int, c_int] + place + [c_void_p]
+    lib.dtb_norm_rope_grid_scratch_bytes.restype = c_int64
+    lib.dtb_norm_rope_grid_scratch_bytes.argtypes = [c_int]
+    side = [c_void_p, c_int64, c_int64, c_void_p, c_float]
+    lib.dtb_norm_rope_grid_backward.restype = c_int
+    lib.dtb_norm_rope_grid_backward.argtypes = ([c_void_p, c_int64, c_int64] * 2 + side + side + [c_void_p] * 6 + [c_int, c_int] + place +
+                                                [c_void_p, c_int64, c_void_p])
     lib.dtb_ln_modulate.restype = c_int
     lib.dtb_ln_modulate.argtypes = [c_void_p, c_void_p, c_void_p, c_void_p, c_float, c_void_p, c_void_p,
                                     c_int, c_int, c_int, c_int, c_void_p]

@@ -62,15 +62,19 @@ def sequence_to_heads(x: torch.Tensor, group) -> torch.Tensor:
 
 @get_timer("ulyssesAttn")
 def ulysses_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, group=None,
-                      softmax_scale: Optional[float] = None) -> torch.Tensor:
+                      softmax_scale: Optional[float] = None, left: int = -1, right: int = -1, sinks: int = 0) -> torch.Tensor:
     """query, key, value: this rank's [B,S_loc,H,D] bf16 -> attention output [B,S_loc,H,D] bf16 over
-    the whole sequence of the group."""
+    the whole sequence of the group; with `left` or `right` given, over the window of that many positions
+    either way and the first `sinks` positions (ops.flash_window)."""
     group = group if group is not None else get_isp_group()
     D = query.shape[-1]
     with get_timer("A2A_1"):
         q, k, v = heads_to_sequence((query, key, value), group)
-    out, _ = _engine.flash_partial(q, k, v, out_dtype=torch.bfloat16,
-                                   softmax_scale=softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(D))
+    scale = softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(D)
+    if left < 0 and right < 0:
+        out, _ = _engine.flash_partial(q, k, v, out_dtype=torch.bfloat16, softmax_scale=scale)
+    else:
+        out, _ = _engine.flash_window(q, k, v, left=left, right=right, sinks=sinks, out_dtype=torch.bfloat16, softmax_scale=scale)
     with get_timer("A2A_2"):
         return sequence_to_heads(out, group)
 

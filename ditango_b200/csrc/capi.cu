@@ -10,12 +10,14 @@
 #include "merge_states.cuh"
 #include "norm_mod.cuh"
 #include "norm_rope.cuh"
+#include "norm_rope_grid.cuh"
 
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -646,6 +648,147 @@ DTB_API int dtb_norm_rope(const void* q, void* q_out, const void* q_weight, cons
   if (p.tokens == 0) return DTB_OK;
   cudaError_t e = dtb::launch_norm_rope(p, head_dim, d->sm_count, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return fail(DTB_ERR_CUDA, "dtb_norm_rope launch failed: %s", cudaGetErrorString(e));
+  return DTB_OK;
+}
+
+// What the forward and the backward pass are given alike.
+static int grid_rope_params(const char* what, dtb::NormRopeGridParams* p, const void* const x[2], const int64_t strides[4], void* const dst[2],
+                            const void* const weight[2], const void* const bias[2], const float eps[2], int dtype,
+                            const int* grid, const int* axes, const double* place, int64_t first, int shards,
+                            int batch, int seq, int text_len, int video_len, int q_heads, int k_heads, int head_dim) {
+  if (!grid || !axes || !place) return fail(DTB_ERR_ARG, "%s: null argument", what);
+  if (head_dim != 64 && head_dim != 128) return fail(DTB_ERR_ARG, "%s: head_dim %d not in {64, 128}", what, head_dim);
+  if (dtype != DTB_F32 && dtype != DTB_BF16) return fail(DTB_ERR_ARG, "%s: bad dtype %d", what, dtype);
+  if (batch < 0 || seq < 0 || q_heads < 1 || k_heads < 1) return fail(DTB_ERR_ARG, "%s: bad shape", what);
+  if (text_len < 0 || video_len < 0 || video_len > seq || text_len > seq - video_len) return fail(DTB_ERR_ARG, "%s: %d text and %d video tokens of %d", what, text_len, video_len, seq);
+  int64_t places = 1;
+  for (int i = 0; i < 3; ++i) {
+    if (grid[i] < 0) return fail(DTB_ERR_ARG, "%s: negative grid", what);
+    places *= grid[i];
+    if (places >= (1ll << 31)) return fail(DTB_ERR_ARG, "%s: grid of 2^31 places or more", what);
+  }
+  int channels = 0;
+  for (int i = 0; i < 3; ++i) {
+    if (axes[i] < 0 || axes[i] > head_dim || axes[i] % 2) return fail(DTB_ERR_ARG, "%s: an axis has %d channels", what, axes[i]);
+    channels += axes[i];
+  }
+  if (channels != head_dim) return fail(DTB_ERR_ARG, "%s: the axes have %d channels, a head %d", what, channels, head_dim);
+  if (first < 0 || shards < 1) return fail(DTB_ERR_ARG, "%s: first token %lld of %d shards", what, static_cast<long long>(first), shards);
+  const int64_t shard_len = places / shards + (places % shards ? 1 : 0);
+  if (shard_len * shards >= (1ll << 31)) return fail(DTB_ERR_ARG, "%s: %d shards of %lld tokens", what, shards, static_cast<long long>(shard_len));
+  if (!(place[0] > 0.) || !std::isfinite(place[0])) return fail(DTB_ERR_ARG, "%s: base must be positive", what);
+  for (int i = 1; i < 7; ++i)
+    if (!std::isfinite(place[i])) return fail(DTB_ERR_ARG, "%s: origin and step must be finite", what);
+  const int width = dtype == DTB_F32 ? 4 : 8;                     // values in 16 bytes
+  const int heads[2] = {q_heads, k_heads};
+  for (int i = 0; i < 2; ++i) {
+    if (!x[i] || !dst[i] || !weight[i]) return fail(DTB_ERR_ARG, "%s: null tensor pointer", what);
+    if (!aligned16(x[i]) || !aligned16(dst[i]) || !aligned16(weight[i]) || !aligned16(bias[i])) return fail(DTB_ERR_ARG, "%s: pointers must be 16-byte aligned", what);
+    if (strides[2 * i] % width || strides[2 * i + 1] % width) return fail(DTB_ERR_ARG, "%s: strides must be multiples of 16 bytes", what);
+    p->src[i] = x[i];
+    p->tok_stride[i] = strides[2 * i];
+    p->batch_stride[i] = strides[2 * i + 1];
+    p->dst[i] = dst[i];
+    p->weight[i] = weight[i];
+    p->bias[i] = bias[i];
+    p->eps[i] = eps[i];
+    p->heads[i] = heads[i];
+  }
+  p->tokens = static_cast<int64_t>(batch) * seq;
+  p->seq = seq;
+  p->text_len = text_len;
+  p->video_len = video_len;
+  p->first = first;
+  p->shards = shards;
+  p->shard_len = static_cast<int>(shard_len);
+  p->shard_places = static_cast<int>(places / shards);
+  p->shard_rest = static_cast<int>(places % shards);
+  p->size_y = grid[1];
+  p->size_x = grid[2];
+  int pair = 0;
+  for (int a = 0; a < 3; ++a) {
+    p->origin[a] = place[1 + a];
+    p->step[a] = place[4 + a];
+    for (int i = 0; i < axes[a]; i += 2, ++pair) {
+      p->turns[pair] = std::pow(place[0], -static_cast<double>(i) / axes[a]) * 0.15915494309189533577;       // / 2 pi
+      p->axis[pair] = static_cast<uint8_t>(a);
+    }
+  }
+  return DTB_OK;
+}
+
+DTB_API int dtb_norm_rope_grid(const void* q, int64_t q_tok_stride, int64_t q_batch_stride, void* q_out, const void* q_weight, const void* q_bias, float q_eps,
+                               const void* k, int64_t k_tok_stride, int64_t k_batch_stride, void* k_out, const void* k_weight, const void* k_bias, float k_eps,
+                               int dtype, int rms, const int* grid, const int* axes, const double* place, int64_t first, int shards,
+                               int batch, int seq, int text_len, int video_len, int q_heads, int k_heads, int head_dim, void* stream) {
+  dtb::NormRopeGridParams p;
+  memset(&p, 0, sizeof(p));
+  const void* x[2] = {q, k};
+  const int64_t strides[4] = {q_tok_stride, q_batch_stride, k_tok_stride, k_batch_stride};
+  void* dst[2] = {q_out, k_out};
+  const void* w[2] = {q_weight, k_weight};
+  const void* b[2] = {q_bias, k_bias};
+  const float eps[2] = {q_eps, k_eps};
+  int rc = grid_rope_params("dtb_norm_rope_grid", &p, x, strides, dst, w, b, eps, dtype, grid, axes, place, first, shards, batch, seq, text_len,
+                            video_len, q_heads, k_heads, head_dim);
+  if (rc != DTB_OK) return rc;
+  DeviceInfo* d = nullptr;
+  if ((rc = device_info(&d)) != DTB_OK) return rc;
+  if (p.tokens == 0) return DTB_OK;
+  cudaError_t e = dtb::launch_norm_rope_grid(p, head_dim, dtype == DTB_BF16, rms != 0, d->sm_count, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return fail(DTB_ERR_CUDA, "dtb_norm_rope_grid launch failed: %s", cudaGetErrorString(e));
+  return DTB_OK;
+}
+
+DTB_API int64_t dtb_norm_rope_grid_scratch_bytes(int head_dim) {
+  DeviceInfo* d = nullptr;
+  if (head_dim != 64 && head_dim != 128) return fail(DTB_ERR_ARG, "dtb_norm_rope_grid_scratch_bytes: head_dim %d not in {64, 128}", head_dim);
+  int rc = device_info(&d);
+  return rc != DTB_OK ? rc : dtb::norm_rope_grid_scratch_bytes(head_dim, d->sm_count);
+}
+
+DTB_API int dtb_norm_rope_grid_backward(const void* dq_out, int64_t dq_tok_stride, int64_t dq_batch_stride,
+                                        const void* dk_out, int64_t dk_tok_stride, int64_t dk_batch_stride,
+                                        const void* q, int64_t q_tok_stride, int64_t q_batch_stride, const void* q_weight, float q_eps,
+                                        const void* k, int64_t k_tok_stride, int64_t k_batch_stride, const void* k_weight, float k_eps,
+                                        void* dq, void* dk, void* dq_weight, void* dq_bias, void* dk_weight, void* dk_bias,
+                                        int dtype, int rms, const int* grid, const int* axes, const double* place, int64_t first, int shards,
+                                        int batch, int seq, int text_len, int video_len, int q_heads, int k_heads, int head_dim,
+                                        void* scratch, int64_t scratch_bytes, void* stream) {
+  dtb::NormRopeGridParams p;
+  memset(&p, 0, sizeof(p));
+  const void* x[2] = {q, k};
+  const int64_t strides[4] = {q_tok_stride, q_batch_stride, k_tok_stride, k_batch_stride};
+  void* dst[2] = {dq, dk};
+  const void* w[2] = {q_weight, k_weight};
+  const void* b[2] = {nullptr, nullptr};
+  const float eps[2] = {q_eps, k_eps};
+  const char* what = "dtb_norm_rope_grid_backward";
+  int rc = grid_rope_params(what, &p, x, strides, dst, w, b, eps, dtype, grid, axes, place, first, shards, batch, seq, text_len, video_len,
+                            q_heads, k_heads, head_dim);
+  if (rc != DTB_OK) return rc;
+  const int width = dtype == DTB_F32 ? 4 : 8;
+  if (!dq_out || !dk_out || !scratch) return fail(DTB_ERR_ARG, "%s: null tensor pointer", what);
+  if (!aligned16(dq_out) || !aligned16(dk_out) || !aligned16(scratch)) return fail(DTB_ERR_ARG, "%s: pointers must be 16-byte aligned", what);
+  if (dq_tok_stride % width || dq_batch_stride % width || dk_tok_stride % width || dk_batch_stride % width) return fail(DTB_ERR_ARG, "%s: strides must be multiples of 16 bytes", what);
+  DeviceInfo* d = nullptr;
+  if ((rc = device_info(&d)) != DTB_OK) return rc;
+  const int64_t need = dtb::norm_rope_grid_scratch_bytes(head_dim, d->sm_count);
+  if (scratch_bytes < need)
+    return fail(DTB_ERR_ARG, "%s: scratch of %lld bytes is smaller than the %lld needed", what, static_cast<long long>(scratch_bytes), static_cast<long long>(need));
+  p.grad[0] = dq_out;
+  p.grad[1] = dk_out;
+  p.grad_tok_stride[0] = dq_tok_stride;
+  p.grad_tok_stride[1] = dk_tok_stride;
+  p.grad_batch_stride[0] = dq_batch_stride;
+  p.grad_batch_stride[1] = dk_batch_stride;
+  p.weight_grad[0] = dq_weight;
+  p.weight_grad[1] = dk_weight;
+  p.bias_grad[0] = dq_bias;
+  p.bias_grad[1] = dk_bias;
+  p.partial = static_cast<float*>(scratch);
+  cudaError_t e = dtb::launch_norm_rope_grid_backward(p, head_dim, dtype == DTB_BF16, rms != 0, d->sm_count, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return fail(DTB_ERR_CUDA, "%s launch failed: %s", what, cudaGetErrorString(e));
   return DTB_OK;
 }
 

@@ -12,12 +12,13 @@ denoising loop; projections and feed-forward are library GEMMs, the attention is
 """
 import math
 from dataclasses import dataclass
-from typing import Tuple
+from typing import Optional, Tuple
 
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
 from torch.autograd import forward_ad
+from torch.autograd.function import once_differentiable
 
 from ..baseline.ulysses import heads_to_sequence, sequence_to_heads
 from ..core.attention import proAttention
@@ -38,6 +39,13 @@ class DiTConfig:
     height: int = 60
     width: int = 90
     text_len: int = 226
+    # "tables": rotary tables over the video tokens; "grid": the norm + rotary kernel forms the angles from a token's place in the
+    # latent grid (and has a backward pass of its own), and no table is stored, sharded or read
+    rotary: str = "tables"
+    # local attention: a video token sees the video tokens of this many frames' worth of positions either way and the text, the text
+    # sees everything; None: full attention.  For mode "ulysses", whose ranks (or whose one rank) hold whole sequences; positions are
+    # those of the gathered sequence, the padding of uneven shards counted.
+    window_frames: Optional[int] = None
 
     @property
     def dim(self) -> int:
@@ -46,6 +54,31 @@ class DiTConfig:
     @property
     def video_tokens(self) -> int:
         return self.frames * (self.height // self.patch_size) * (self.width // self.patch_size)
+
+    @property
+    def grid_rope(self) -> "_engine.GridRope":
+        """The positions that rotary_tables has in tables."""
+        d_t = self.head_dim // 4
+        d_h = (self.head_dim - d_t) // 2
+        return _engine.GridRope((self.frames, self.height // self.patch_size, self.width // self.patch_size), (d_t, d_h, d_h))
+
+
+def grid_tables(rope: "_engine.GridRope", tokens: int, device) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The cos and sin tables [tokens, D] (fp32) of the positions that `rope` gives a sequence's video tokens; 0 at padding."""
+    angles = [((o + st * torch.arange(n, dtype=torch.float64, device=device))[:, None] *
+               rope.base ** (-torch.arange(0, d, 2, dtype=torch.float64, device=device) / max(d, 1))).repeat_interleave(2, dim=1)
+              for n, d, o, st in zip(rope.grid, rope.axes, rope.origin, rope.step)]
+    t, h, w = rope.grid
+    size, rest = divmod(t * h * w, rope.shards)
+    length = size + (1 if rest else 0)
+    n = rope.first + torch.arange(tokens, device=device)
+    shard, at = n // max(length, 1), n % max(length, 1)
+    real = (shard < rope.shards) & (at < size + (shard < rest).long())
+    place = (shard * size + shard.clamp(max=rest) + at)[real]
+    ang = torch.cat([a[i] for a, i in zip(angles, (place // max(h * w, 1), place // max(w, 1) % max(h, 1), place % max(w, 1)))], dim=-1)
+    cos, sin = (torch.zeros(tokens, ang.shape[-1], device=device) for _ in range(2))
+    cos[real], sin[real] = ang.cos().float(), ang.sin().float()
+    return cos, sin
 
 
 def rotary_tables(cfg: DiTConfig, device, dtype=torch.float32) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -160,6 +193,48 @@ def norm_and_rotate(q, k, norm_q, norm_k, cos, sin, text_len: int) -> Tuple[torc
     return tuple(_rotate_video(x, cos, sin, text_len).contiguous() for x in (norm_q(q), norm_k(k)))
 
 
+class _NormRotateGrid(torch.autograd.Function):
+    """The grid form of norm and rotation with its own backward kernels (first derivatives only).  Its backward can be captured
+    into a CUDA graph, under autograd's own condition: no graph of the same leaves made outside of the capture is still alive."""
+
+    @staticmethod
+    def forward(ctx, q, k, q_weight, q_bias, k_weight, k_bias, q_eps, k_eps, rope, text_len, video_len, rms):
+        ctx.save_for_backward(q, k, q_weight, q_bias, k_weight, k_bias)
+        ctx.rest = q_eps, k_eps, rope, text_len, video_len, rms
+        return _engine.norm_rope_grid(q, k, (q_weight, q_bias, q_eps), (k_weight, k_bias, k_eps), rope, text_len=text_len,
+                                      video_len=video_len, rms=rms)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dq, dk):
+        q, k, q_weight, q_bias, k_weight, k_bias = ctx.saved_tensors
+        q_eps, k_eps, rope, text_len, video_len, rms = ctx.rest
+        grads = _engine.norm_rope_grid_backward(dq.contiguous(), dk.contiguous(), q, k, (q_weight, q_bias, q_eps), (k_weight, k_bias, k_eps),
+                                                rope, text_len=text_len, video_len=video_len, rms=rms)
+        return (*(g if need else None for g, need in zip(grads, ctx.needs_input_grad)), *(None,) * 6)
+
+
+def norm_and_rotate_grid(q, k, norm_q, norm_k, rope, text_len: int, video_len: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """norm_and_rotate with the angles from each video token's place in `rope`'s grid (a GridRope).  On a GPU in bf16 this is one
+    kernel, and its gradients are two; elsewhere the tables are formed and the separate operations run."""
+    D = q.shape[-1]
+    if (q.is_cuda and q.device.index == torch.cuda.current_device() and D in (64, 128) and q.shape == k.shape and
+            _plain_bf16(q.device, q, k) and _plain_norm(norm_q, D, q.device) and
+            _plain_norm(norm_k, D, q.device) and not torch.is_autocast_enabled("cuda")):
+        args = (q, k, norm_q.weight, norm_q.bias, norm_k.weight, norm_k.bias)
+        rest = (norm_q.eps, norm_k.eps, rope, text_len, video_len, False)
+        if torch.is_grad_enabled() and any(x.requires_grad for x in args):
+            return _NormRotateGrid.apply(*args, *rest)
+        return _engine.norm_rope_grid(q, k, (args[2], args[3], rest[0]), (args[4], args[5], rest[1]), rope, text_len=text_len, video_len=video_len)
+    video_len = q.shape[1] - text_len if video_len is None else video_len
+    cos, sin = grid_tables(rope, video_len, q.device)
+    outs = []
+    for x in (norm_q(q), norm_k(k)):
+        front, video, behind = x.split([text_len, video_len, x.shape[1] - text_len - video_len], dim=1)
+        outs.append(torch.cat([front, apply_rotary(video, cos, sin), behind], dim=1).contiguous())
+    return tuple(outs)
+
+
 def _plain_modulation(h: torch.Tensor, mod: torch.Tensor) -> bool:
     """Whether the kernels can take `mod`: one bf16 row per sequence of h.  (A row that broadcasts over the batch, another
     dtype or layout -- what a hook on, or a replacement of, the projection may return -- stays with the separate operations.)"""
@@ -236,22 +311,37 @@ class DiTBlock(nn.Module):
             eq, ek, ev = heads_to_sequence(proj(enc), self.group)
             text_all = eq.shape[1]
             q, k, v = (torch.cat([a, b], dim=1) for a, b in ((eq, q), (ek, k), (ev, v)))
-            cos, sin = rope                                          # unsharded (padded) tables
-            q, k = norm_and_rotate(q, k, self.norm_q, self.norm_k, cos, sin, text_all)
-            out, _ = _engine.flash_partial(q, k, v.contiguous(), out_dtype=torch.bfloat16,
-                                           softmax_scale=1.0 / math.sqrt(D))
+            q, k = self._norm_and_rotate(q, k, rope, text_all)           # rope: unsharded (padded) tables, or the whole grid
+            out = self._attend_whole(q, k, v.contiguous(), text_all)
             o_enc = sequence_to_heads(out[:, :text_all].contiguous(), self.group).flatten(2).to(h.dtype)
             o_vid = sequence_to_heads(out[:, text_all:].contiguous(), self.group).flatten(2).to(h.dtype)
             return self.to_out(o_vid), self.to_out(o_enc)
         out = self._attend_joint(torch.cat([enc, h], dim=1), text_len, rope)
         return out[:, text_len:], out[:, :text_len]
 
+    def _norm_and_rotate(self, q, k, rope, text_len):
+        if isinstance(rope, _engine.GridRope):
+            return norm_and_rotate_grid(q, k, self.norm_q, self.norm_k, rope, text_len)
+        cos, sin = rope
+        return norm_and_rotate(q, k, self.norm_q, self.norm_k, cos, sin, text_len)
+
+    def _attend_whole(self, q, k, v, text_len):
+        """Attention of whole sequences [B, text + video, H, D], bf16."""
+        scale = 1.0 / math.sqrt(q.shape[-1])
+        if self.cfg.window_frames is None:
+            return _engine.flash_partial(q, k, v, out_dtype=torch.bfloat16, softmax_scale=scale)[0]
+        reach = self.cfg.window_frames * (self.cfg.video_tokens // self.cfg.frames)
+        # the text sees everything, the video its window and the text
+        text = _engine.flash_window(q[:, :text_len], k, v, out_dtype=torch.bfloat16, softmax_scale=scale, q_start=0)[0]
+        video = _engine.flash_window(q[:, text_len:], k, v, left=reach, right=reach, sinks=text_len, q_start=text_len,
+                                     out_dtype=torch.bfloat16, softmax_scale=scale)[0]
+        return torch.cat([text, video], dim=1)
+
     def _attend_joint(self, x, text_len, rope):
         """Attention of the joint sequence x [B, text + video, dim], projected back."""
         B, H, D = x.shape[0], self.cfg.num_heads, self.cfg.head_dim
         q, k, v = (f(x).view(B, -1, H, D) for f in (self.to_q, self.to_k, self.to_v))
-        cos, sin = rope                                              # this rank's slice of the tables
-        q, k = norm_and_rotate(q, k, self.norm_q, self.norm_k, cos, sin, text_len)
+        q, k = self._norm_and_rotate(q, k, rope, text_len)               # rope: this rank's slice of the tables or of the grid
         out = self.attention.attn(q, k, v.contiguous())
         return self.to_out(out.to(x.dtype).flatten(2))
 
@@ -282,6 +372,10 @@ class CogVideoXDiT(nn.Module):
 
     def __init__(self, cfg: DiTConfig, group, mode: str = "ditango"):
         super().__init__()
+        if cfg.rotary not in ("tables", "grid"):
+            raise ValueError(f"rotary is 'tables' or 'grid', not {cfg.rotary!r}")
+        if cfg.window_frames is not None and (mode != "ulysses" or cfg.window_frames < 0):
+            raise ValueError("window_frames is for mode 'ulysses' and not negative")
         self.cfg, self.group, self.mode = cfg, group, mode
         p = cfg.patch_size
         self.patch_embed = nn.Linear(cfg.in_channels * p * p, cfg.dim)
@@ -310,20 +404,25 @@ class CogVideoXDiT(nn.Module):
         h = self.patch_embed(x.to(dtype))
         enc = self.text_proj(text.to(dtype))
         N, r = self.group.world_size, self.group.rank_in_group
-        if self._rope is None:
+        grid = cfg.rotary == "grid"
+        if self._rope is None and not grid:
             self._rope = rotary_tables(cfg, latents.device)
-        cos, sin = self._rope
+        cos, sin = (None, None) if grid else self._rope
         if N > 1:
             h = split_tensor_uneven(h, N, dim=1, tensor_name="hidden")[r]
             enc = split_tensor_uneven(enc, N, dim=1, tensor_name="encoder_hidden")[r]
-            if self.mode == "ulysses":
+            if grid:
+                pass
+            elif self.mode == "ulysses":
                 # full tables in the gathered order: every rank's shard keeps its zero padding
                 cos = torch.cat(split_tensor_uneven(cos, N, dim=0), dim=0)
                 sin = torch.cat(split_tensor_uneven(sin, N, dim=0), dim=0)
             else:
                 cos, sin = split_tensor_uneven(cos, N, dim=0)[r], split_tensor_uneven(sin, N, dim=0)[r]
+        # (a ulysses rank sees all pieces of the grid, padding in between, a ring rank its own)
+        rope = cfg.grid_rope._replace(shards=N, first=0 if self.mode == "ulysses" else r * h.shape[1]) if grid else (cos, sin)
         for blk in self.blocks:
-            h, enc = blk(h, enc, temb, (cos, sin))
+            h, enc = blk(h, enc, temb, rope)
         if N > 1:
             h = remove_padding_after_gather(self.group.all_gather(h.contiguous(), dim=1), "hidden")
             enc = remove_padding_after_gather(self.group.all_gather(enc.contiguous(), dim=1), "encoder_hidden")

@@ -4,6 +4,7 @@ These are the only places arithmetic happens on the attention path; they raise w
 extension is missing or an argument is not a CUDA tensor of the expected kind.
 """
 import ctypes
+import functools
 import math
 from typing import NamedTuple, Optional, Sequence, Tuple, Union
 
@@ -488,6 +489,91 @@ def norm_rope(q: torch.Tensor, k: torch.Tensor, q_norm: Tuple[torch.Tensor, torc
     _capi.check(rc, "dtb_norm_rope")
     LaunchLog.count += 1
     return qo, ko
+
+
+class GridRope(NamedTuple):
+    """Rotary positions of tokens that are places of a (time, height, width) grid, in row-major order.  An axis with d of a head's
+    channels turns its pair i by (origin + step * index) * base^(-2 i / d).  The places lie in `shards` pieces as split_tensor_uneven
+    makes them, padding included, and `first` is the number of a sequence's first video token among those: 0 for all pieces one
+    after another, r * ceil(places / shards) for rank r's.  Tokens behind the last piece are padding too."""
+    grid: Tuple[int, int, int]
+    axes: Tuple[int, int, int]
+    base: float = 10000.0
+    origin: Tuple[float, float, float] = (0.0, 0.0, 0.0)
+    step: Tuple[float, float, float] = (1.0, 1.0, 1.0)
+    first: int = 0
+    shards: int = 1
+
+
+@functools.lru_cache(maxsize=64)
+def _rope_arrays(grid, axes, base, origin, step):
+    return (ctypes.c_int * 3)(*grid), (ctypes.c_int * 3)(*axes), (ctypes.c_double * 7)(base, *origin, *step)
+
+
+Norm = Tuple[torch.Tensor, Optional[torch.Tensor], float]
+
+
+def _grid_rope_args(q, k, norms, rope, text_len, video_len):
+    """Checks what both passes are given; returns (element type, arguments from `grid` on)."""
+    if q.dim() != 4 or k.dim() != 4 or q.shape[:2] != k.shape[:2] or q.shape[-1] != k.shape[-1]:
+        raise _capi.ExtensionError("q and k are [B,S,H,D] and [B,S,Hk,D]")
+    B, S, H, D = q.shape
+    if q.dtype not in _VALUES or k.dtype != q.dtype:
+        raise _capi.ExtensionError("q and k must be bfloat16 or float32 alike")
+    for w, b, _ in norms:
+        for x in (w,) if b is None else (w, b):
+            if x.dtype != q.dtype or x.numel() != D or not x.is_contiguous():
+                raise _capi.ExtensionError("weights and biases hold D contiguous elements of q's type")
+    arrays = _rope_arrays(tuple(rope.grid), tuple(rope.axes), float(rope.base), tuple(rope.origin), tuple(rope.step))
+    video_len = S - text_len if video_len is None else video_len
+    return _VALUES[q.dtype], (*arrays, rope.first, rope.shards, B, S, text_len, video_len, H, k.shape[2], D)
+
+
+def norm_rope_grid(q: torch.Tensor, k: torch.Tensor, q_norm: Norm, k_norm: Norm, rope: GridRope, *, text_len: int = 0,
+                   video_len: Optional[int] = None, rms: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Layer norm (RMS norm with `rms`) over D of q [B,S,H,D] and k [B,S,Hk,D], bf16 or fp32, norms as (weight, bias or None, eps);
+    then rotary positions of the `video_len` tokens (None: all) behind the first `text_len`, from their place in rope's grid.
+    Any token and batch strides that are multiples of 16 bytes; new contiguous tensors, one launch.  Padding behind the grid's
+    last place comes out as 0, as with zero-padded tables."""
+    _need_current_device(q, k, *q_norm[:2], *k_norm[:2])
+    dtype, rest = _grid_rope_args(q, k, (q_norm, k_norm), rope, text_len, video_len)
+    qo, ko = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k))
+    if q.numel() == 0 or k.numel() == 0:
+        return qo, ko
+    rc = _capi.load().dtb_norm_rope_grid(
+        q.data_ptr(), *_strides(q, False), qo.data_ptr(), q_norm[0].data_ptr(), None if q_norm[1] is None else q_norm[1].data_ptr(), q_norm[2],
+        k.data_ptr(), *_strides(k, False), ko.data_ptr(), k_norm[0].data_ptr(), None if k_norm[1] is None else k_norm[1].data_ptr(), k_norm[2],
+        dtype, int(rms), *rest, _stream_ptr())
+    _capi.check(rc, "dtb_norm_rope_grid")
+    LaunchLog.count += 1
+    return qo, ko
+
+
+def norm_rope_grid_backward(dq: torch.Tensor, dk: torch.Tensor, q: torch.Tensor, k: torch.Tensor, q_norm: Norm, k_norm: Norm, rope: GridRope, *,
+                            text_len: int = 0, video_len: Optional[int] = None, rms: bool = False) -> Tuple[Optional[torch.Tensor], ...]:
+    """Gradients of norm_rope_grid's inputs from those of its results, dq and dk: (q's, k's, q_norm's weight and bias, k_norm's
+    weight and bias), None for a bias that is None.  Two launches; the sums for the weights are taken in a fixed order."""
+    _need_current_device(dq, dk, q, k, *q_norm[:2], *k_norm[:2])
+    dtype, rest = _grid_rope_args(q, k, (q_norm, k_norm), rope, text_len, video_len)
+    if dq.shape != q.shape or dk.shape != k.shape or dq.dtype != q.dtype or dk.dtype != q.dtype:
+        raise _capi.ExtensionError("dq and dk have the shapes and the type of q and k")
+    gq, gk = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k))
+    sums = [None if x is None else torch.empty_like(x) for x in (*q_norm[:2], *k_norm[:2])]
+    if q.numel() == 0 or k.numel() == 0:
+        return (gq, gk, *(None if x is None else x.zero_() for x in sums))
+    lib = _capi.load()
+    need = lib.dtb_norm_rope_grid_scratch_bytes(q.shape[-1])
+    if need < 0:
+        _capi.check(need, "dtb_norm_rope_grid_scratch_bytes")
+    scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
+    rc = lib.dtb_norm_rope_grid_backward(
+        dq.data_ptr(), *_strides(dq, False), dk.data_ptr(), *_strides(dk, False),
+        q.data_ptr(), *_strides(q, False), q_norm[0].data_ptr(), q_norm[2], k.data_ptr(), *_strides(k, False), k_norm[0].data_ptr(), k_norm[2],
+        gq.data_ptr(), gk.data_ptr(), *(None if x is None else x.data_ptr() for x in sums), dtype, int(rms), *rest,
+        scratch.data_ptr(), need, _stream_ptr())
+    _capi.check(rc, "dtb_norm_rope_grid_backward")
+    LaunchLog.count += 2
+    return (gq, gk, *sums)
 
 
 MOD_MAX_DIM = 3072

@@ -255,6 +255,41 @@ DTB_API int dtb_norm_rope(const void* q, void* q_out, const void* q_weight, cons
                           int batch, int seq, int text_len, int num_heads, int head_dim, void* stream);
 
 /*
+ * Norm of each head of the query and key projections (layer norm, or RMS norm with rms != 0), then rotary positions on three axes:
+ * dtb_norm_rope without tables, for tokens that are places of a grid (time, height, width), with its gradients.  Of a sequence's
+ * tokens the first text_len and those behind the video_len after them are normalised only; the n-th video token is number
+ * first + n of the grid's places (row-major) with their padding, and its channel pair i' of axis a, which has axes[a] channels
+ * (interleaved pairs, axes in order), turns by
+ *     (origin_a + step_a * index_a) * base^(-2 i' / axes[a])
+ * The places lie in `shards` pieces of ceil(places / shards) tokens; where they do not divide evenly the first pieces are full and the
+ * others end with padding (what split_tensor_uneven, utils.py:86-136, makes).  Padding, and a token behind the last piece, gets a
+ * result of 0, as from zero-padded tables, and passes no gradient.  The reference forms such tables per model (executor/cogvideox/attention_processor.py:50-72 applies them).
+ *
+ *  q, k            dtype DTB_BF16 or DTB_F32 (weights, biases, results and gradients alike): token s of sequence b, head h at
+ *                  b * batch_stride + s * tok_stride + h * head_dim, strides multiples of 16 bytes
+ *  q_out, k_out    [batch, seq, heads, head_dim] contiguous; they may be q, k where those are contiguous
+ *  q_weight, ...   [head_dim]; a bias may be NULL
+ *  grid, axes      host int[3]: places and channels (even, head_dim in all) of the axes
+ *  place           host double[7]: base, origin[3], step[3]
+ * Backward: dq_out, dk_out are the gradients of the results, with strides of their own; dq, dk contiguous.  dq_weight ... dk_bias
+ * [head_dim] (each may be NULL) are sums over all rows in a fixed order.  scratch: dtb_norm_rope_grid_scratch_bytes(head_dim) bytes
+ * (negative: an error code), 16-byte aligned, of one call at a time.
+ */
+DTB_API int dtb_norm_rope_grid(const void* q, int64_t q_tok_stride, int64_t q_batch_stride, void* q_out, const void* q_weight, const void* q_bias, float q_eps,
+                               const void* k, int64_t k_tok_stride, int64_t k_batch_stride, void* k_out, const void* k_weight, const void* k_bias, float k_eps,
+                               int dtype, int rms, const int* grid, const int* axes, const double* place, int64_t first, int shards,
+                               int batch, int seq, int text_len, int video_len, int q_heads, int k_heads, int head_dim, void* stream);
+DTB_API int64_t dtb_norm_rope_grid_scratch_bytes(int head_dim);
+DTB_API int dtb_norm_rope_grid_backward(const void* dq_out, int64_t dq_tok_stride, int64_t dq_batch_stride,
+                                        const void* dk_out, int64_t dk_tok_stride, int64_t dk_batch_stride,
+                                        const void* q, int64_t q_tok_stride, int64_t q_batch_stride, const void* q_weight, float q_eps,
+                                        const void* k, int64_t k_tok_stride, int64_t k_batch_stride, const void* k_weight, float k_eps,
+                                        void* dq, void* dk, void* dq_weight, void* dq_bias, void* dk_weight, void* dk_bias,
+                                        int dtype, int rms, const int* grid, const int* axes, const double* place, int64_t first, int shards,
+                                        int batch, int seq, int text_len, int video_len, int q_heads, int k_heads, int head_dim,
+                                        void* scratch, int64_t scratch_bytes, void* stream);
+
+/*
  * The two elementwise steps around a transformer block's sub-layers (LayerNormZero modulation and gated residual,
  * executor/cogvideox/cogvideox_transformer_3d.py:139-190), over both streams in one launch each; fp32 arithmetic,
  * one rounding to bf16.  All tensors bf16, contiguous.

@@ -88,3 +88,47 @@ def test_flash_window_takes_gpu_tensors_only():
     q = torch.zeros(1, 8, 1, 64, dtype=torch.bfloat16)
     with pytest.raises(ExtensionError):
         ops.flash_window(q, q, q, left=3)
+
+
+def _grid_rope(lib, *, q=16, qt=192, qb=1920, qo=16, qw=16, qbias=None, k=16, dtype=1, grid=(2, 3, 4), axes=(16, 24, 24), place=(1e4, 0, 0, 0, 1, 1, 1),
+               first=0, shards=1, B=1, S=10, text=2, video=8, H=3, Hk=3, D=64, back=False, scratch=16, scratch_bytes=1 << 30):
+    arrays = (ctypes.c_int * 3)(*grid), (ctypes.c_int * 3)(*axes), (ctypes.c_double * 7)(*place)
+    rest = (dtype, 0, *arrays, first, shards, B, S, text, video, H, Hk, D)
+    if back:
+        return lib.dtb_norm_rope_grid_backward(16, 192, 1920, 16, qt, qb, q, qt, qb, qw, 1e-6, k, 192, 1920, 16, 1e-6, qo, 16, 16, None, 16, None,
+                                               *rest, scratch, scratch_bytes, None)
+    return lib.dtb_norm_rope_grid(q, qt, qb, qo, qw, qbias, 1e-6, k, 192, 1920, 16, 16, None, 1e-6, *rest, None)
+
+
+@pytest.mark.parametrize("back", [False, True])
+@pytest.mark.parametrize("args,word", [
+    (dict(q=None), "null"), (dict(k=None), "null"), (dict(qw=None), "null"), (dict(D=32), "head_dim"), (dict(dtype=2), "dtype"), (dict(H=0), "shape"),
+    (dict(text=3), "text and"), (dict(video=-1), "text and"), (dict(text=-1), "text and"), (dict(grid=(2, -1, 4)), "negative grid"),
+    (dict(grid=(2 ** 16, 2 ** 10, 2 ** 10)), "2^31"), (dict(axes=(16, 25, 23)), "channels"), (dict(axes=(16, 24, 26)), "channels"),
+    (dict(axes=(-2, 34, 32)), "channels"), (dict(first=-1), "first"), (dict(shards=0), "shards"), (dict(place=(0, 0, 0, 0, 1, 1, 1)), "base"),
+    (dict(place=(1e4, float("nan"), 0, 0, 1, 1, 1)), "finite"), (dict(qt=196), "multiples"), (dict(qo=24), "aligned")])
+def test_norm_rope_grid_refuses(args, word, back):
+    from ditango_b200 import _capi
+    lib = _capi.load()
+    assert _grid_rope(lib, back=back, **args) == -1 and word in lib.dtb_last_error().decode()
+
+
+def test_norm_rope_grid_takes_gpu_tensors_only():
+    from ditango_b200 import _capi, ops
+    x, w = torch.zeros(1, 8, 1, 64), torch.ones(64)
+    with pytest.raises(_capi.ExtensionError):
+        ops.norm_rope_grid(x, x, (w, None, 1e-6), (w, None, 1e-6), ops.GridRope((1, 2, 4), (16, 24, 24)))
+    with pytest.raises(_capi.ExtensionError):
+        ops.norm_rope_grid_backward(x, x, x, x, (w, None, 1e-6), (w, None, 1e-6), ops.GridRope((1, 2, 4), (16, 24, 24)))
+
+
+def test_grid_positions_on_the_cpu_take_the_tables():
+    """The general path, on tensors that no kernel takes, gives what norm_and_rotate gives on the model's tables."""
+    from ditango_b200.executor.cogvideox_dit import DiTConfig, norm_and_rotate, norm_and_rotate_grid, rotary_tables
+    cfg = DiTConfig(frames=2, height=6, width=8)
+    torch.manual_seed(0)
+    q, k = (torch.randn(1, 3 + cfg.video_tokens, 2, 64) for _ in range(2))
+    norms = [torch.nn.LayerNorm(64) for _ in range(2)]
+    a = norm_and_rotate(q, k, *norms, *rotary_tables(cfg, "cpu"), 3)
+    b = norm_and_rotate_grid(q, k, *norms, cfg.grid_rope, 3)
+    assert all((x - y).abs().max() < 1e-5 for x, y in zip(a, b))
