@@ -125,6 +125,25 @@ int make_tile_map(CUtensorMap* tm, const void* base, int64_t rows, int64_t width
   return DTB_OK;
 }
 
+// 3-D bf16 view of tokens x batch rows of `width` channels for boxes of 64 channels x 128 tokens, the outer axis of the smaller
+// stride first; *batch_first says which one that is.
+int make_token_map(CUtensorMap* tm, const void* base, int64_t width, int64_t tokens, int64_t tok_stride, int64_t batch, int64_t batch_stride,
+                   int* batch_first, const char* what) {
+  const bool swap = batch > 1 && batch_stride < tok_stride;
+  const int64_t inner = swap ? batch : tokens, outer = swap ? tokens : batch;
+  const int64_t inner_stride = swap ? batch_stride : tok_stride, outer_stride = swap ? tok_stride : batch > 1 ? batch_stride : tok_stride;
+  cuuint64_t gdim[3] = {static_cast<cuuint64_t>(width), static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(outer)};
+  cuuint64_t gstride[2] = {static_cast<cuuint64_t>(inner_stride) * 2, static_cast<cuuint64_t>(outer_stride) * 2};
+  cuuint32_t box[3] = {64, swap ? 1u : 128u, swap ? 128u : 1u};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = g_encode(tm, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), gdim, gstride, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  *batch_first = swap ? 1 : 0;
+  if (r != CUDA_SUCCESS) return fail(DTB_ERR_CUDA, "cuTensorMapEncodeTiled(%s) failed with CUresult %d", what, static_cast<int>(r));
+  return DTB_OK;
+}
+
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // Encoded tensor maps, kept per (base pointer, rows, width, pitch, box rows).  The attention path calls
@@ -402,6 +421,9 @@ DTB_API int dtb_flash_fwd_ex(const void* q, const void* k, const void* v,
                         head_dim, softmax_scale, launch_flags, stream);
 }
 
+// Which launches take the kernel of 128-row tiles.
+static bool takes_window_tiles(int seqlen_q, int group) { return static_cast<int64_t>(seqlen_q) * group > 64 && seqlen_q > 16; }
+
 DTB_API int dtb_flash_window(const void* q, const void* k, const void* v,
                      int64_t q_tok_stride, int64_t q_batch_stride, int64_t k_tok_stride, int64_t k_batch_stride,
                      int64_t v_tok_stride, int64_t v_batch_stride,
@@ -475,7 +497,21 @@ DTB_API int dtb_flash_window(const void* q, const void* k, const void* v,
   p.q_start = q_start;
   p.k_start = k_start;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = head_dim == 64 ? dtb::launch_window_rows<64>(p, d->sm_count, s) : dtb::launch_window_rows<128>(p, d->sm_count, s);
+  cudaError_t e;
+  if (takes_window_tiles(seqlen_q, num_heads / num_kv_heads)) {
+    if ((rc = load_encoder()) != DTB_OK) return rc;
+    const bool packed = cu_seqlens_q != nullptr;
+    const int64_t q_tokens = packed ? total_q : seqlen_q, k_tokens = packed ? total_k : seqlen_k, batch = packed ? 1 : nseg;
+    CUtensorMap tq, tk, tv;
+    // (a tensor map needs a row; without keys none is loaded)
+    if ((rc = make_token_map(&tq, q, q_width, q_tokens, q_tok_stride, batch, q_batch_stride, &p.q_batch_first, "q")) != DTB_OK ||
+        (rc = make_token_map(&tk, k, k_width, std::max<int64_t>(k_tokens, 1), k_tok_stride, batch, k_batch_stride, &p.k_batch_first, "k")) != DTB_OK ||
+        (rc = make_token_map(&tv, v, k_width, std::max<int64_t>(k_tokens, 1), v_tok_stride, batch, v_batch_stride, &p.v_batch_first, "v")) != DTB_OK)
+      return rc;
+    e = head_dim == 64 ? dtb::launch_window_tiles<64>(tq, tk, tv, p, s) : dtb::launch_window_tiles<128>(tq, tk, tv, p, s);
+  } else {
+    e = head_dim == 64 ? dtb::launch_window_rows<64>(p, d->sm_count, s) : dtb::launch_window_rows<128>(p, d->sm_count, s);
+  }
   if (e != cudaSuccess) return fail(DTB_ERR_CUDA, "dtb_flash_window launch failed: %s", cudaGetErrorString(e));
   return DTB_OK;
 }

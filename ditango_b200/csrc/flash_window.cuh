@@ -1,7 +1,9 @@
-// Parameters and launchers of the windowed attention kernels (flash_window_rows.cu), and which keys a row sees.
+// Parameters and launchers of the windowed attention kernels (flash_window_rows.cu for few query rows, flash_window_sm100.cu for
+// many), and which keys a row sees.
 #pragma once
 #include "flash_fwd_sm100.cuh"
 
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -19,6 +21,8 @@ struct WindowParams {
   int kv_heads;                  // divides f.num_heads
   int left, right, sinks;        // each within [0, 2^30]
   int q_start, k_start;          // positions of the first query (or kQueriesLast) and the first key
+  // the order of a tensor map's outer axes, the one with the smaller stride first: 1 batch then token, 0 token then batch
+  int q_batch_first, k_batch_first, v_batch_first;
 };
 
 // The sequence of a CTA: where its queries and keys begin among the tokens, how many there are, and the first query's position
@@ -71,6 +75,9 @@ __device__ __forceinline__ int64_t window_offset(const WindowParams& p, int seg,
   return (p.f.cu_q != nullptr ? 0 : seg * batch_stride) + tok * tok_stride;
 }
 
+// Tensor maps of q, k and v: [heads * D, tokens, batch] (or batch and tokens changed over), boxes of 64 channels x 128 tokens.
+template <int D>
+cudaError_t launch_window_tiles(const CUtensorMap& tm_q, const CUtensorMap& tm_k, const CUtensorMap& tm_v, const WindowParams& p, cudaStream_t stream);
 template <int D>
 cudaError_t launch_window_rows(const WindowParams& p, int sm_count, cudaStream_t stream);
 

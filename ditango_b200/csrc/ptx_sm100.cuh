@@ -57,6 +57,15 @@ __device__ __forceinline__ void tma_load_2d(void* smem_dst, const CUtensorMap* m
       : "memory");
 }
 
+// 3-D tile load: 64 channels from x, tokens from `token` of sequence `batch`, the map's outer axes being (token, batch) or (batch, token).
+__device__ __forceinline__ void tma_load_token(void* smem_dst, const CUtensorMap* m, uint64_t* bar, int x, int token, int batch, int batch_first) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+      ::"r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(x), "r"(batch_first ? batch : token),
+      "r"(batch_first ? token : batch)
+      : "memory");
+}
+
 // ----------------------------------------------------------------------------- TMEM
 __device__ __forceinline__ void tmem_alloc(uint32_t* smem_result, uint32_t ncols) {
   asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(smem_result)),
