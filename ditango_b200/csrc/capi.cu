@@ -421,8 +421,24 @@ DTB_API int dtb_flash_fwd_ex(const void* q, const void* k, const void* v,
                         head_dim, softmax_scale, launch_flags, stream);
 }
 
-// Which launches take the kernel of 128-row tiles.
-static bool takes_window_tiles(int seqlen_q, int group) { return static_cast<int64_t>(seqlen_q) * group > 64 && seqlen_q > 16; }
+// Which launches take the kernel of 128-row tiles: those that it is expected to finish sooner.  It needs a whole walk over the keys of
+// a block of 256 rows for each round of blocks over the SMs, however few there are; the other kernel's time goes with its tiles of
+// 16 rows x 16 keys, spread over all SMs.  Rates as measured, us of (tiles of 16, tiles of 128), one forced after the other:
+//   queries                              16            64            128           256           512
+//   24 heads of 128, window 4096    15.1 / 65.5   36.3 / 66.2   65.2 / 66.4    106 / 67.7    189 / 68.3
+//   24 heads of 128, window 512      9.2 / 17.4   11.8 / 17.8   16.5 / 18.0   26.7 / 19.4   46.2 / 19.6
+//   2 x 48 of 64, window 2700       17.1 / 40.0   40.9 / 41.2   73.8 / 42.9    130 / 44.3    241 / 86.4
+//   4 x 32 over 8 of 64, 1000       10.3 / 20.3   24.9 / 21.6   40.6 / 21.9   76.0 / 22.9    146 / 44.0
+//   4 heads of 64, window 700        5.8 / 16.2    6.5 / 16.2    6.8 / 17.9    7.4 / 18.6    9.1 / 18.8
+static bool takes_window_tiles(const dtb::WindowParams& p, int head_dim, int sm_count) {
+  const int64_t group = p.f.num_heads / p.kv_heads, span = std::min<int64_t>(p.f.seqlen_k, static_cast<int64_t>(p.left) + p.right + p.sinks);
+  const double small_tiles = static_cast<double>((p.f.seqlen_q * group + 15) / 16 * p.kv_heads * p.f.nseg) * ((span + 31) / 16);
+  const double rows_us = 5. + small_tiles / (sm_count * (head_dim == 64 ? 12.8 : 7.2));
+  const int64_t blocks = (p.f.seqlen_q + 255) / 256 * static_cast<int64_t>(p.f.num_heads) * p.f.nseg;
+  const int64_t steps = (std::min<int64_t>(p.f.seqlen_k, span + std::min(p.f.seqlen_q, 128)) + 127) / 128;
+  const double tiles_us = static_cast<double>((blocks + sm_count - 1) / sm_count) * (8. + steps * (head_dim == 64 ? 1.3 : 1.75));
+  return tiles_us < rows_us;
+}
 
 DTB_API int dtb_flash_window(const void* q, const void* k, const void* v,
                      int64_t q_tok_stride, int64_t q_batch_stride, int64_t k_tok_stride, int64_t k_batch_stride,
@@ -498,7 +514,7 @@ DTB_API int dtb_flash_window(const void* q, const void* k, const void* v,
   p.k_start = k_start;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e;
-  if (takes_window_tiles(seqlen_q, num_heads / num_kv_heads)) {
+  if (takes_window_tiles(p, head_dim, d->sm_count)) {
     if ((rc = load_encoder()) != DTB_OK) return rc;
     const bool packed = cu_seqlens_q != nullptr;
     const int64_t q_tokens = packed ? total_q : seqlen_q, k_tokens = packed ? total_k : seqlen_k, batch = packed ? 1 : nseg;
@@ -586,7 +602,7 @@ DTB_API int dtb_merge_rows(int nstates, const void* const* outs, const int* out_
       const bool narrow = t == DTB_I8 || t == DTB_E4M3;
       if (narrow != (pass == 0)) continue;
       if (!outs[i] || (narrow && !exponents[i])) return fail(DTB_ERR_ARG, "dtb_merge_rows: state %d has a null pointer", i);
-      if (!lses[i] && (nstates > 1 || lse_out)) return fail(DTB_ERR_ARG, "dtb_merge_rows: state %d has no lse (only a single state without lse_out may)", i);
+      if (!lses[i]) return fail(DTB_ERR_ARG, "dtb_merge_rows: state %d has no lse", i);
       if (!aligned16(outs[i])) return fail(DTB_ERR_ARG, "dtb_merge_rows: state %d is not 16-byte aligned", i);
       if (lse_layouts[i] != DTB_LSE_BHS && lse_layouts[i] != DTB_LSE_BSH) return fail(DTB_ERR_ARG, "dtb_merge_rows: bad lse layout for state %d", i);
       if ((outs[i] == out_bf16 && t != DTB_BF16) || (outs[i] == out_codes) || (outs[i] == out && t != DTB_F32))
@@ -618,6 +634,35 @@ DTB_API int dtb_merge_rows(int nstates, const void* const* outs, const int* out_
   if (p.rows == 0) return DTB_OK;
   cudaError_t e = dtb::launch_merge_rows(p, head_dim, d->sm_count, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return fail(DTB_ERR_CUDA, "dtb_merge_rows launch failed: %s", cudaGetErrorString(e));
+  return DTB_OK;
+}
+
+// `wide` values (fp32 or bf16) and their rows in 8 bits
+static int check_rows(const char* what, const void* wide, int dtype, const void* codes, int codes_dtype, const uint8_t* exponents, int64_t rows, int head_dim) {
+  if (head_dim != 64 && head_dim != 128) return fail(DTB_ERR_ARG, "%s: head_dim %d not in {64, 128}", what, head_dim);
+  if (dtype != DTB_F32 && dtype != DTB_BF16) return fail(DTB_ERR_ARG, "%s: bad dtype %d", what, dtype);
+  if (codes_dtype != DTB_I8 && codes_dtype != DTB_E4M3) return fail(DTB_ERR_ARG, "%s: bad type %d of the codes", what, codes_dtype);
+  if (rows < 0 || rows >= (1ll << 31)) return fail(DTB_ERR_ARG, "%s: %lld rows", what, static_cast<long long>(rows));
+  if (!wide || !codes || !exponents) return fail(DTB_ERR_ARG, "%s: null tensor pointer", what);
+  if (!aligned16(wide) || !aligned16(codes)) return fail(DTB_ERR_ARG, "%s: pointers must be 16-byte aligned", what);
+  return DTB_OK;
+}
+
+DTB_API int dtb_quantize_rows(const void* values, int dtype, void* codes, int codes_dtype, uint8_t* exponents, int64_t rows, int head_dim, void* stream) {
+  int rc = check_rows("dtb_quantize_rows", values, dtype, codes, codes_dtype, exponents, rows, head_dim);
+  DeviceInfo* d = nullptr;
+  if (rc != DTB_OK || (rc = device_info(&d)) != DTB_OK || rows == 0) return rc;
+  cudaError_t e = dtb::launch_quantize_rows(values, dtype == DTB_BF16, static_cast<uint8_t*>(codes), exponents, codes_dtype, rows, head_dim, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return fail(DTB_ERR_CUDA, "dtb_quantize_rows launch failed: %s", cudaGetErrorString(e));
+  return DTB_OK;
+}
+
+DTB_API int dtb_dequantize_rows(const void* codes, int codes_dtype, const uint8_t* exponents, void* out, int out_dtype, int64_t rows, int head_dim, void* stream) {
+  int rc = check_rows("dtb_dequantize_rows", out, out_dtype, codes, codes_dtype, exponents, rows, head_dim);
+  DeviceInfo* d = nullptr;
+  if (rc != DTB_OK || (rc = device_info(&d)) != DTB_OK || rows == 0) return rc;
+  cudaError_t e = dtb::launch_dequantize_rows(static_cast<const uint8_t*>(codes), exponents, codes_dtype, out, out_dtype == DTB_BF16, rows, head_dim, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return fail(DTB_ERR_CUDA, "dtb_dequantize_rows launch failed: %s", cudaGetErrorString(e));
   return DTB_OK;
 }
 

@@ -28,6 +28,7 @@ constexpr int kThreads = kWarps * 32;
 constexpr int kRows = 16;
 constexpr int kKeys = 16;           // keys of a tile
 constexpr int kStages = 3;
+constexpr int kMostCtas = 8;        // of a cluster
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
@@ -88,14 +89,14 @@ __global__ void __launch_bounds__(kThreads) flash_window_rows_kernel(const Windo
   const int seg = blockIdx.z, kv_head = blockIdx.y;
   const int group = p.f.num_heads / p.kv_heads;
   const WindowSeq s = window_seq(p, seg);
-  const int64_t rows = static_cast<int64_t>(s.q_len) * group;
-  const int64_t row0 = static_cast<int64_t>(blockIdx.x / C) * kRows;
+  const int rows = s.q_len * group, row0 = static_cast<int>(blockIdx.x) / C * kRows;       // (the launcher sees to it that they fit)
   if (row0 >= rows) return;                           // all CTAs of the cluster or none
-  const int n_rows = static_cast<int>(min(static_cast<int64_t>(kRows), rows - row0));
+  const int status = *reinterpret_cast<volatile int*>(p.f.status);
+  const int n_rows = min(kRows, rows - row0);
 
   // what the block sees: the first row reaches furthest to the left, the last one to the right
-  const WindowSpan w0 = window_span(p, s, static_cast<int>(row0 / group));
-  const WindowSpan w1 = window_span(p, s, static_cast<int>((row0 + n_rows - 1) / group));
+  const WindowSpan w0 = window_span(p, s, row0 / group);
+  const WindowSpan w1 = window_span(p, s, (row0 + n_rows - 1) / group);
   const int first = w1.first, lo = max(w0.lo, first);
   const int total = first + max(w1.hi - lo, 0);
   const int n_tiles = (total + kKeys - 1) / kKeys;
@@ -109,7 +110,7 @@ __global__ void __launch_bounds__(kThreads) flash_window_rows_kernel(const Windo
     end[h] = from[h] = to[h] = 0;
     const uint16_t* src = nullptr;
     if (r < n_rows) {
-      const int i = static_cast<int>((row0 + r) / group), g = static_cast<int>((row0 + r) % group);
+      const int i = (row0 + r) / group, g = (row0 + r) % group;
       const WindowSpan w = window_span(p, s, i);
       end[h] = w.first;
       from[h] = w.lo - lo + first;
@@ -157,7 +158,11 @@ __global__ void __launch_bounds__(kThreads) flash_window_rows_kernel(const Windo
   int stage = 0;
   for (int tile = tile0; tile < n_tiles; tile += step) {
     cp_async_wait<kStages - 2>();
-    __syncwarp();
+    __syncwarp();                                     // ... and all lanes have read the tile before it, whose slot the next load takes
+    const int ahead = tile + (kStages - 1) * step;
+    const int slot = stage == 0 ? kStages - 1 : stage - 1;
+    if (ahead < n_tiles) load(ahead, slot);
+    cp_async_commit();
     const uint32_t ks = smem_u32(ring + stage * 2 * M::kTileBytes), vs = ks + M::kTileBytes;
     float sc[2][4] = {};
 #pragma unroll
@@ -210,12 +215,6 @@ __global__ void __launch_bounds__(kThreads) flash_window_rows_kernel(const Windo
       mma16816(o[2 * d], a, b[0], b[1]);
       mma16816(o[2 * d + 1], a, b[2], b[3]);
     }
-    __syncwarp();                                     // all lanes have read what the next load may overwrite
-    const int ahead = tile + (kStages - 1) * step;
-    int slot = stage + kStages - 1;
-    if (slot >= kStages) slot -= kStages;
-    if (ahead < n_tiles) load(ahead, slot);
-    cp_async_commit();
     if (++stage == kStages) stage = 0;
   }
   cp_async_wait<0>();
@@ -258,25 +257,37 @@ __global__ void __launch_bounds__(kThreads) flash_window_rows_kernel(const Windo
   // ... and the CTAs: four columns of a row per thread, the rows' columns dealt out over the cluster
   cluster.sync();
   // after a failure elsewhere nothing is stored (a CTA that left instead would take its shared memory with it)
-  const bool stores = *reinterpret_cast<volatile int*>(p.f.status) == 0;
+  const bool stores = status == 0;
   for (int u = rank * kThreads + threadIdx.x; u < n_rows * (D / 4); u += C * kThreads) {
     const int r = u / (D / 4), col = (u % (D / 4)) * 4;
+    // (all reads of the other CTAs' memory are under way before one is used)
+    float2 ml[kMostCtas];
+    float4 v[kMostCtas];
+#pragma unroll
+    for (int b = 0; b < kMostCtas; ++b) {
+      ml[b] = make_float2(-INFINITY, 0.f);
+      v[b] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (b < C) {
+        ml[b] = cluster.map_shared_rank(s_ml_cta, b)[r];
+        v[b] = *reinterpret_cast<const float4*>(cluster.map_shared_rank(s_o_cta, b) + r * D + col);
+      }
+    }
     float mx = -INFINITY;
-    for (int b = 0; b < C; ++b) mx = fmaxf(mx, cluster.map_shared_rank(s_ml_cta, b)[r].x);
+#pragma unroll
+    for (int b = 0; b < kMostCtas; ++b) mx = fmaxf(mx, ml[b].x);
     const float ref = reference(mx);
     float sum = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int b = 0; b < C; ++b) {
-      const float2 ml = cluster.map_shared_rank(s_ml_cta, b)[r];
-      const float f = ex2((ml.x - ref) * c);
-      const float4 v = *reinterpret_cast<const float4*>(cluster.map_shared_rank(s_o_cta, b) + r * D + col);
-      sum = fmaf(ml.y, f, sum);
-      acc.x = fmaf(v.x, f, acc.x);
-      acc.y = fmaf(v.y, f, acc.y);
-      acc.z = fmaf(v.z, f, acc.z);
-      acc.w = fmaf(v.w, f, acc.w);
+#pragma unroll
+    for (int b = 0; b < kMostCtas; ++b) {
+      const float f = ex2((ml[b].x - ref) * c);
+      sum = fmaf(ml[b].y, f, sum);
+      acc.x = fmaf(v[b].x, f, acc.x);
+      acc.y = fmaf(v[b].y, f, acc.y);
+      acc.z = fmaf(v[b].z, f, acc.z);
+      acc.w = fmaf(v[b].w, f, acc.w);
     }
-    const int i = static_cast<int>((row0 + r) / group), head = kv_head * group + static_cast<int>((row0 + r) % group);
+    const int i = (row0 + r) / group, head = kv_head * group + (row0 + r) % group;
     const int64_t tok = p.f.cu_q != nullptr ? static_cast<int64_t>(s.q_begin) + i : static_cast<int64_t>(seg) * p.f.seqlen_q + i;
     const int64_t li = lse_index(p.f, seg, head, i, tok), oi = tok * p.f.out_tok_stride + static_cast<int64_t>(head) * D + col;
     const bool empty = !(sum > 0.f);                  // no key seen: nothing to write over a state
@@ -328,12 +339,13 @@ cudaError_t launch_window_rows(const WindowParams& p, int sm_count, cudaStream_t
   const int group = p.f.num_heads / p.kv_heads;
   const int64_t row_blocks = (static_cast<int64_t>(p.f.seqlen_q) * group + kRows - 1) / kRows;
   const int64_t blocks = row_blocks * p.kv_heads * p.f.nseg;
-  // as many CTAs to a row block as keep two per SM busy, each with two tiles for every warp
+  // as many CTAs to a row block as give every SM one, each with two tiles for every warp (56 blocks of 188 tiles at D = 64: 13.0 us
+  // with 4, 14.0 with 8; 24 blocks of 272 tiles at D = 128, 8 CTAs either way: 14.5)
   const int64_t span = static_cast<int64_t>(p.left) + p.right + p.sinks + kRows;
   const int64_t tiles = ((span < p.f.seqlen_k ? span : p.f.seqlen_k) + kKeys - 1) / kKeys;
   int C = 1;
-  while (C < 8 && blocks * C < 2 * sm_count && tiles > 2 * kWarps * C) C *= 2;
-  if (row_blocks * C > 0x7fffffff) return cudaErrorInvalidValue;
+  while (C < kMostCtas && blocks * C < sm_count && tiles > 2 * kWarps * C) C *= 2;
+  if ((row_blocks * C + 1) * kRows > 0x7fffffff) return cudaErrorInvalidValue;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(row_blocks * C), p.kv_heads, p.f.nseg);
   cfg.blockDim = dim3(kThreads);

@@ -7,9 +7,8 @@
 // code's rounding is the only one, the value it stands for is a bf16 number (at most 7 bits behind the leading one), and the
 // factor is one byte and goes into the weight.  It costs int8 up to one bit of its 7, and e4m3 (a floating type) nothing.
 // A row with an infinity or a NaN gets b = 255: its codes are 0, and 0 * 2^128 reads back as NaN.
-// With one state and no lse the weight is 1: that writes a state in 8 bits, or reads it back.
 //
-// Bound by HBM.  D / 16 lanes own a row, 16 values each: 16 bytes of a state in 8 bits.  The 8-bit states come first in the
+// Bound by HBM.  In the merge D / 16 lanes own a row, 16 values each: 16 bytes of a state in 8 bits.  The 8-bit states come first in the
 // parameters and are fetched kNarrow at a time, all of those loads and the first wide state's in flight before the weights (which
 // wait for the lse) are formed.  All sums are fp32.
 #include "merge_rows.cuh"
@@ -71,23 +70,27 @@ __device__ __forceinline__ void add_wide(float (&acc)[16], float w, const Wide& 
     }
   }
 }
+// The four codes of a word as floats.
+__device__ __forceinline__ void decode4(uint32_t a, int dtype, float (&f)[4]) {
+  if (dtype == kRowsI8) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) f[k] = static_cast<float>(static_cast<int8_t>(a >> (8 * k)));
+  } else {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(a >> (16 * k)), __NV_E4M3);
+      const float2 x = __half22float2(h);
+      f[2 * k] = x.x;
+      f[2 * k + 1] = x.y;
+    }
+  }
+}
 __device__ __forceinline__ void add_codes(float (&acc)[16], float w, uint4 v, int dtype) {
   const uint32_t a[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     float f[4];
-    if (dtype == kRowsI8) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) f[k] = static_cast<float>(static_cast<int8_t>(a[i] >> (8 * k)));
-    } else {
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(a[i] >> (16 * k)), __NV_E4M3);
-        const float2 x = __half22float2(h);
-        f[2 * k] = x.x;
-        f[2 * k + 1] = x.y;
-      }
-    }
+    decode4(a[i], dtype, f);
 #pragma unroll
     for (int k = 0; k < 4; ++k) acc[4 * i + k] = fmaf(w, f[k], acc[4 * i + k]);
   }
@@ -101,23 +104,20 @@ __device__ __forceinline__ uint32_t exponent_byte(uint32_t top, int dtype) {
                                  : static_cast<int>((top + (0x7fffffu - 0x600000u)) >> 23) - 8;
   return static_cast<uint32_t>(b < kMinExponent ? kMinExponent : b);
 }
-__device__ __forceinline__ uint4 encode(const float (&acc)[16], uint32_t b, int dtype) {
-  if (b == 255u) return make_uint4(0u, 0u, 0u, 0u);
-  const float f = __uint_as_float((254u - b) << 23);
-  uint32_t r[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float x0 = acc[4 * i] * f, x1 = acc[4 * i + 1] * f, x2 = acc[4 * i + 2] * f, x3 = acc[4 * i + 3] * f;
-    if (dtype == kRowsI8) {
-      r[i] = (static_cast<uint32_t>(__float2int_rn(x0)) & 0xffu) | (static_cast<uint32_t>(__float2int_rn(x1)) & 0xffu) << 8 |
-             (static_cast<uint32_t>(__float2int_rn(x2)) & 0xffu) << 16 | static_cast<uint32_t>(__float2int_rn(x3)) << 24;
-    } else {
-      r[i] = static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(x0, x1), __NV_SATFINITE, __NV_E4M3)) |
-             static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(x2, x3), __NV_SATFINITE, __NV_E4M3)) << 16;
-    }
-  }
-  return make_uint4(r[0], r[1], r[2], r[3]);
+// Four values as codes of a row with exponent byte b; f = 2^(127 - b).
+__device__ __forceinline__ uint32_t encode4(float x0, float x1, float x2, float x3, uint32_t b, float f, int dtype) {
+  if (b == 255u) return 0u;
+  x0 *= f;
+  x1 *= f;
+  x2 *= f;
+  x3 *= f;
+  if (dtype == kRowsI8)
+    return (static_cast<uint32_t>(__float2int_rn(x0)) & 0xffu) | (static_cast<uint32_t>(__float2int_rn(x1)) & 0xffu) << 8 |
+           (static_cast<uint32_t>(__float2int_rn(x2)) & 0xffu) << 16 | static_cast<uint32_t>(__float2int_rn(x3)) << 24;
+  return static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(x0, x1), __NV_SATFINITE, __NV_E4M3)) |
+         static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(x2, x3), __NV_SATFINITE, __NV_E4M3)) << 16;
 }
+__device__ __forceinline__ float inverse_of(uint32_t b) { return __uint_as_float((254u - b) << 23); }
 
 }  // namespace
 
@@ -161,17 +161,15 @@ __global__ void __launch_bounds__(kThreads) merge_rows_kernel(const MergeRowsPar
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int i = 0; i < 4; ++i) wide[u].q[i] = make_uint4(0u, 0u, 0u, 0u);
-    if (p.lse[0] != nullptr) {
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+    for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int t = 0; t < kPerLane; ++t) {
-          const int st = lane + t * G;
-          w[u][t] = -INFINITY;
-          if (row_of(u) < p.rows && st < n)
-            w[u][t] = p.lse[st][lse_offset(p.lse_layout[st], static_cast<uint32_t>(row_of(u)), p.H, p.S)];
-        }
-    }
+      for (int t = 0; t < kPerLane; ++t) {
+        const int st = lane + t * G;
+        w[u][t] = -INFINITY;
+        if (row_of(u) < p.rows && st < n)
+          w[u][t] = p.lse[st][lse_offset(p.lse_layout[st], static_cast<uint32_t>(row_of(u)), p.H, p.S)];
+      }
     uint32_t eb[U][kPerLane];
 #pragma unroll
     for (int u = 0; u < U; ++u)
@@ -186,28 +184,22 @@ __global__ void __launch_bounds__(kThreads) merge_rows_kernel(const MergeRowsPar
 
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (p.lse[0] == nullptr) {
-        lse_out[u] = 0.f;
+      float mx = w[u][0];
 #pragma unroll
-        for (int t = 0; t < kPerLane; ++t) w[u][t] = 1.f;
-      } else {
-        float mx = w[u][0];
+      for (int t = 1; t < kPerLane; ++t) mx = fmaxf(mx, w[u][t]);
 #pragma unroll
-        for (int t = 1; t < kPerLane; ++t) mx = fmaxf(mx, w[u][t]);
+      for (int o = G / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(full, mx, o, G));
+      float sum = 0.f;
 #pragma unroll
-        for (int o = G / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(full, mx, o, G));
-        float sum = 0.f;
-#pragma unroll
-        for (int t = 0; t < kPerLane; ++t) {
-          w[u][t] = w[u][t] == -INFINITY ? 0.f : exp2f((w[u][t] - mx) * 1.4426950408889634f);
-          sum += w[u][t];
-        }
-#pragma unroll
-        for (int o = G / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(full, sum, o, G);
-        lse_out[u] = sum > 0.f ? mx + logf(sum) : -INFINITY;
-#pragma unroll
-        for (int t = 0; t < kPerLane; ++t) w[u][t] = sum > 0.f ? __fdiv_rn(w[u][t], sum) : 0.f;
+      for (int t = 0; t < kPerLane; ++t) {
+        w[u][t] = w[u][t] == -INFINITY ? 0.f : exp2f((w[u][t] - mx) * 1.4426950408889634f);
+        sum += w[u][t];
       }
+#pragma unroll
+      for (int o = G / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(full, sum, o, G);
+      lse_out[u] = sum > 0.f ? mx + logf(sum) : -INFINITY;
+#pragma unroll
+      for (int t = 0; t < kPerLane; ++t) w[u][t] = sum > 0.f ? __fdiv_rn(w[u][t], sum) : 0.f;
       // the factor of a state in 8 bits goes into its weight; a weight of 0 stays one
 #pragma unroll
       for (int t = 0; t < kPerLane; ++t)
@@ -260,7 +252,12 @@ __global__ void __launch_bounds__(kThreads) merge_rows_kernel(const MergeRowsPar
         for (int o = G / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(full, top, o, G));
         const uint32_t b = exponent_byte(top, p.out_codes_dtype);
         if (row < p.rows) {
-          st_stream(p.out_codes + off, encode(acc[u], b, p.out_codes_dtype));
+          const float f = inverse_of(b);
+          uint32_t r[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            r[i] = encode4(acc[u][4 * i], acc[u][4 * i + 1], acc[u][4 * i + 2], acc[u][4 * i + 3], b, f, p.out_codes_dtype);
+          st_stream(p.out_codes + off, make_uint4(r[0], r[1], r[2], r[3]));
           if (lane == 0) p.out_exponents[row] = static_cast<uint8_t>(b);
         }
       }
@@ -282,6 +279,144 @@ __global__ void __launch_bounds__(kThreads) merge_rows_kernel(const MergeRowsPar
       }
     }
   }
+}
+
+// A single state written in 8 bits: D / 8 lanes to a row, 8 values each, kRowsPerThread rows whose loads are in flight together.  (The
+// two halves of an fp32 row are loaded one after the other, four values a lane, so that each access is to whole lines.)
+constexpr int kCodeThreads = 256;
+constexpr int kRowsPerThread = 4;
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kCodeThreads) quantize_rows_kernel(const T* values, uint8_t* codes, uint8_t* exponents, int codes_dtype, int64_t rows) {
+  constexpr int G = D / 8, U = kRowsPerThread;
+  constexpr bool f32 = sizeof(T) == 4;
+  const int lane = threadIdx.x % G;
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * (kCodeThreads / G * U) + threadIdx.x / G;
+  uint4 raw[U][f32 ? 2 : 1];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t row = row0 + u * (kCodeThreads / G);
+    raw[u][0] = make_uint4(0u, 0u, 0u, 0u);
+    if (f32) raw[u][f32 ? 1 : 0] = make_uint4(0u, 0u, 0u, 0u);
+    if (row < rows) {
+      raw[u][0] = ld_stream(values + row * D + lane * (f32 ? 4 : 8));
+      if (f32) raw[u][f32 ? 1 : 0] = ld_stream(values + row * D + D / 2 + lane * 4);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t row = row0 + u * (kCodeThreads / G);
+    float x[8];
+    const uint32_t a[4] = {raw[u][0].x, raw[u][0].y, raw[u][0].z, raw[u][0].w};
+    if (f32) {
+      const uint4 v = raw[u][f32 ? 1 : 0];
+      const uint32_t b[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[i] = __uint_as_float(a[i]);
+        x[4 + i] = __uint_as_float(b[i]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[2 * i] = __uint_as_float(a[i] << 16);
+        x[2 * i + 1] = __uint_as_float(a[i] & 0xffff0000u);
+      }
+    }
+    uint32_t top = 0u;                // magnitudes compare as their bits do, NaNs above all
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+#pragma unroll
+    for (int o = G / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o, G));
+    const uint32_t b = exponent_byte(top, codes_dtype);
+    const float f = inverse_of(b);
+    const uint32_t r0 = encode4(x[0], x[1], x[2], x[3], b, f, codes_dtype), r1 = encode4(x[4], x[5], x[6], x[7], b, f, codes_dtype);
+    if (row < rows) {
+      if (f32) {
+        *reinterpret_cast<uint32_t*>(codes + row * D + lane * 4) = r0;
+        *reinterpret_cast<uint32_t*>(codes + row * D + D / 2 + lane * 4) = r1;
+      } else {
+        *reinterpret_cast<uint2*>(codes + row * D + lane * 8) = make_uint2(r0, r1);
+      }
+      if (lane == 0) exponents[row] = static_cast<uint8_t>(b);
+    }
+  }
+}
+
+// ... and read back.
+template <typename T, int D>
+__global__ void __launch_bounds__(kCodeThreads) dequantize_rows_kernel(const uint8_t* codes, const uint8_t* exponents, T* out, int codes_dtype, int64_t rows) {
+  constexpr int G = D / 8, U = kRowsPerThread;
+  const int lane = threadIdx.x % G;
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * (kCodeThreads / G * U) + threadIdx.x / G;
+  uint2 raw[U];
+  uint32_t b[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t row = row0 + u * (kCodeThreads / G);
+    raw[u] = make_uint2(0u, 0u);
+    b[u] = 0u;
+    if (row < rows) {
+      raw[u] = __ldcs(reinterpret_cast<const uint2*>(codes + row * D + lane * 8));
+      b[u] = exponents[row];
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t row = row0 + u * (kCodeThreads / G);
+    if (row >= rows) break;
+    const float f = power_of(b[u]);
+    float x[4], y[4];
+    decode4(raw[u].x, codes_dtype, x);
+    decode4(raw[u].y, codes_dtype, y);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[i] *= f;
+      y[i] *= f;
+    }
+    T* dst = out + row * D + lane * 8;
+    if (sizeof(T) == 4) {
+      reinterpret_cast<float4*>(dst)[0] = make_float4(x[0], x[1], x[2], x[3]);
+      reinterpret_cast<float4*>(dst)[1] = make_float4(y[0], y[1], y[2], y[3]);
+    } else {
+      *reinterpret_cast<uint4*>(dst) = make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]));
+    }
+  }
+}
+
+static unsigned code_blocks(int64_t rows, int head_dim) {
+  const int64_t per_block = kCodeThreads / (head_dim / 8) * kRowsPerThread;
+  return static_cast<unsigned>((rows + per_block - 1) / per_block);
+}
+
+cudaError_t launch_quantize_rows(const void* values, bool bf16, uint8_t* codes, uint8_t* exponents, int codes_dtype, int64_t rows, int head_dim,
+                                 cudaStream_t stream) {
+  const unsigned blocks = code_blocks(rows, head_dim);
+  const uint16_t* h = static_cast<const uint16_t*>(values);
+  const float* f = static_cast<const float*>(values);
+  if (head_dim == 64) {
+    if (bf16) quantize_rows_kernel<uint16_t, 64><<<blocks, kCodeThreads, 0, stream>>>(h, codes, exponents, codes_dtype, rows);
+    else quantize_rows_kernel<float, 64><<<blocks, kCodeThreads, 0, stream>>>(f, codes, exponents, codes_dtype, rows);
+  } else {
+    if (bf16) quantize_rows_kernel<uint16_t, 128><<<blocks, kCodeThreads, 0, stream>>>(h, codes, exponents, codes_dtype, rows);
+    else quantize_rows_kernel<float, 128><<<blocks, kCodeThreads, 0, stream>>>(f, codes, exponents, codes_dtype, rows);
+  }
+  return cudaGetLastError();
+}
+
+cudaError_t launch_dequantize_rows(const uint8_t* codes, const uint8_t* exponents, int codes_dtype, void* out, bool bf16, int64_t rows, int head_dim,
+                                   cudaStream_t stream) {
+  const unsigned blocks = code_blocks(rows, head_dim);
+  uint16_t* h = static_cast<uint16_t*>(out);
+  float* f = static_cast<float*>(out);
+  if (head_dim == 64) {
+    if (bf16) dequantize_rows_kernel<uint16_t, 64><<<blocks, kCodeThreads, 0, stream>>>(codes, exponents, h, codes_dtype, rows);
+    else dequantize_rows_kernel<float, 64><<<blocks, kCodeThreads, 0, stream>>>(codes, exponents, f, codes_dtype, rows);
+  } else {
+    if (bf16) dequantize_rows_kernel<uint16_t, 128><<<blocks, kCodeThreads, 0, stream>>>(codes, exponents, h, codes_dtype, rows);
+    else dequantize_rows_kernel<float, 128><<<blocks, kCodeThreads, 0, stream>>>(codes, exponents, f, codes_dtype, rows);
+  }
+  return cudaGetLastError();
 }
 
 template <int G, int U, int kNarrow>

@@ -13,7 +13,7 @@ constexpr int kRowsF32 = 0, kRowsBf16 = 1, kRowsI8 = 2, kRowsE4m3 = 3;
 struct MergeRowsParams {
   const void* values[kMergeRowsMaxStates];       // [rows, D]; the states in 8 bits come first
   const uint8_t* exponents[kMergeRowsMaxStates]; // [rows], of the states in 8 bits
-  const float* lse[kMergeRowsMaxStates];         // null (a single state): its weight is 1
+  const float* lse[kMergeRowsMaxStates];
   int dtype[kMergeRowsMaxStates];
   int lse_layout[kMergeRowsMaxStates];           // 0 [B,H,S], 1 [B,S,H]
   int narrow;                                    // states in 8 bits
@@ -30,6 +30,11 @@ struct MergeRowsParams {
   int S;
 };
 
+// A single state's values in 8 bits, and back: `rows` (below 2^31) rows of head_dim.
+cudaError_t launch_quantize_rows(const void* values, bool bf16, uint8_t* codes, uint8_t* exponents, int codes_dtype, int64_t rows, int head_dim,
+                                 cudaStream_t stream);
+cudaError_t launch_dequantize_rows(const uint8_t* codes, const uint8_t* exponents, int codes_dtype, void* out, bool bf16, int64_t rows, int head_dim,
+                                   cudaStream_t stream);
 cudaError_t launch_merge_rows(const MergeRowsParams& p, int head_dim, int sm_count, cudaStream_t stream);
 
 }  // namespace dtb

@@ -49,13 +49,38 @@ def _need_cuda(*ts):
             raise _capi.ExtensionError("ditango_b200 kernels take CUDA tensors only")
 
 
-def _need_current_device(*ts):
-    """The kernels run on the current device's current stream: tensors of another device are refused, not reached for."""
-    _need_cuda(*ts)
-    dev = torch.cuda.current_device()
-    for t in ts:
-        if t is not None and t.device.index != dev:
-            raise _capi.ExtensionError(f"tensor on {t.device}, but the current device is cuda:{dev}")
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def _launch_stream(*tensors) -> int:
+    """The current device's current stream, for a launch on `tensors` (None among them is skipped).  Those of another device are
+    refused, not reached for."""
+    dev = None
+    for t in tensors:
+        if t is None:
+            continue
+        d = t.get_device()
+        if d != dev:
+            if d < 0:
+                raise _capi.ExtensionError("ditango_b200 kernels take CUDA tensors only")
+            if dev is not None or d != _current_device():
+                raise _capi.ExtensionError(f"tensor on cuda:{d}, but the current device is cuda:{_current_device()}")
+            dev = d
+    return _stream_ptr() if _raw_stream is None else _raw_stream(dev)
+
+
+def _empty(shape, dtype: torch.dtype, device) -> torch.Tensor:
+    """torch.empty for a few axes, without the time that it takes to find its layout (1.6 us against 3.2)."""
+    strides, n = [], 1
+    for extent in reversed(shape):
+        strides.append(n)
+        n *= extent
+    return torch.empty_strided(shape, strides[::-1], dtype=dtype, device=device)
+
+
+def _empty_like(x: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """A contiguous tensor of x's shape."""
+    return torch.empty_like(x, dtype=dtype) if x.is_contiguous() else _empty(x.shape, dtype, x.device)
 
 
 def _tok_stride(x: torch.Tensor) -> int:
@@ -189,14 +214,17 @@ def flash_partial(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
     return out, lse
 
 
-def _strides(x: torch.Tensor, packed: bool) -> Tuple[int, int]:
-    """(token, batch) strides in elements of a [B,S,H,D] or packed [T,H,D] tensor whose (H, D) block is dense; that of an axis of
+def _strides(x: torch.Tensor, shape) -> Tuple[int, int]:
+    """(token, batch) strides in elements of a tensor [B,S,H,D], or packed [T,H,D], whose (H, D) block is dense; that of an axis of
     length 1, which nothing steps along, is given as a dense tensor's."""
-    H, D = x.shape[-2], x.shape[-1]
-    if (x.stride(-1) != 1 and D != 1) or (x.stride(-2) != D and H != 1):
+    H, D = shape[-2], shape[-1]
+    *outer, head, channel = x.stride()
+    if channel != 1 or (head != D and H != 1):
         raise _capi.ExtensionError("head and channel dims must be contiguous")
-    tok = x.stride(-3) if x.shape[-3] > 1 else H * D
-    return tok, (0 if packed else x.stride(0) if x.shape[0] > 1 else tok * x.shape[1])
+    tok = outer[-1] if shape[-3] > 1 else H * D
+    if len(shape) == 3:
+        return tok, 0
+    return tok, (outer[0] if shape[0] > 1 else tok * shape[1])
 
 
 def flash_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, left: int = -1, right: int = -1, sinks: int = 0,
@@ -216,18 +244,18 @@ def flash_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, left: int
     (cu_seqlens given): q [Tq,H,D], k,v [Tk,Hk,D].  Returns (out, lse) as flash_partial does, mergeable with its states; with
     accumulate=True the state is merged into the given fp32 (out, lse) in place.  A row that sees no key has out 0 and lse -inf.
     """
-    _need_current_device(q, k, v, out, lse, cu_seqlens_q, cu_seqlens_k, seqlens_k)
-    if q.dtype != torch.bfloat16 or k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16:
+    stream = _launch_stream(q, k, v, out, lse, cu_seqlens_q, cu_seqlens_k, seqlens_k)
+    if not q.dtype == k.dtype == v.dtype == torch.bfloat16:
         raise _capi.ExtensionError("q, k, v must be bfloat16")
     packed = cu_seqlens_q is not None
     if packed != (cu_seqlens_k is not None):
         raise _capi.ExtensionError("cu_seqlens_q and cu_seqlens_k go together")
-    dims = 3 if packed else 4
-    if q.dim() != dims or k.dim() != dims or v.shape != k.shape or k.shape[-1] != q.shape[-1]:
+    shape, kshape = q.shape, k.shape
+    if len(shape) != (3 if packed else 4) or len(kshape) != len(shape) or v.shape != kshape or kshape[-1] != shape[-1]:
         raise _capi.ExtensionError("q is [B,S,H,D] and k, v are [B,S,Hk,D], packed [T,H,D] and [T,Hk,D]")
-    H, D, Hk = q.shape[-2], q.shape[-1], k.shape[-2]
     if packed:
-        Tq, Tk = q.shape[0], k.shape[0]
+        Tq, H, D = shape
+        Tk, Hk, _ = kshape
         nseg = cu_seqlens_q.numel() - 1
         sq = min(Tq, int(max_seqlen_q)) if max_seqlen_q is not None else Tq
         sk = min(Tk, int(max_seqlen_k)) if max_seqlen_k is not None else Tk
@@ -235,8 +263,9 @@ def flash_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, left: int
             raise _capi.ExtensionError("cu_seqlens must be contiguous int32, as many of q as of k")
         lse_shape = (H, Tq) if lse_layout == LSE_BHS else (Tq, H)
     else:
-        nseg, sq, sk = q.shape[0], q.shape[1], k.shape[1]
-        if k.shape[0] != nseg:
+        nseg, sq, H, D = shape
+        batch, sk, Hk, _ = kshape
+        if batch != nseg:
             raise _capi.ExtensionError("q and k must have one batch size")
         Tq, Tk = nseg * sq, nseg * sk
         lse_shape = (nseg, H, sq) if lse_layout == LSE_BHS else (nseg, sq, H)
@@ -245,28 +274,32 @@ def flash_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, left: int
     if accumulate and (out is None or lse is None or out.dtype != torch.float32):
         raise _capi.ExtensionError("accumulate needs an existing fp32 (out, lse) state")
     if out is None:
-        out = torch.empty(q.shape, dtype=out_dtype, device=q.device)
-    if lse is None:
-        lse = torch.empty(lse_shape, dtype=torch.float32, device=q.device)
-    if out.shape != q.shape or not out.is_contiguous() or out.dtype not in _VALUES:
+        if out_dtype not in _VALUES:
+            raise _capi.ExtensionError("out must be float32 or bfloat16")
+        out = _empty_like(q, out_dtype)
+    elif out.shape != shape or not out.is_contiguous() or out.dtype not in _VALUES:
         raise _capi.ExtensionError("out must be contiguous float32 or bfloat16 of q's shape")
-    if tuple(lse.shape) != lse_shape or not lse.is_contiguous() or lse.dtype != torch.float32:
+    if lse is None:
+        lse = _empty(lse_shape, torch.float32, q.device)
+    elif tuple(lse.shape) != lse_shape or not lse.is_contiguous() or lse.dtype != torch.float32:
         raise _capi.ExtensionError(f"lse must be a contiguous fp32 tensor of shape {lse_shape}")
     if q.numel() == 0:
         return out, lse
-    keys, values = (x.data_ptr() or q.data_ptr() for x in (k, v))        # (an empty tensor has no address, and nothing is read)
+    # (an empty tensor has no address, and nothing is read)
+    keys, values = k.data_ptr() or q.data_ptr(), v.data_ptr() or q.data_ptr()
     ev = None
     if LaunchLog.events is not None:
         ev = (torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True))
         ev[0].record()
     rc = _capi.load().dtb_flash_window(
-        q.data_ptr(), keys, values, *_strides(q, packed), *_strides(k, packed), *_strides(v, packed),
-        out.data_ptr(), _VALUES[out.dtype], lse.data_ptr(), lse_layout, int(accumulate),
+        q.data_ptr(), keys, values, *_strides(q, shape), *_strides(k, kshape), *_strides(v, kshape),
+        out.data_ptr(), _VALUES[out.dtype], lse.data_ptr(), lse_layout, accumulate,
         cu_seqlens_q.data_ptr() if packed else None, cu_seqlens_k.data_ptr() if packed else None,
-        seqlens_k.data_ptr() if seqlens_k is not None else None, nseg, sq, sk, Tq, Tk, H, Hk, D,
-        1.0 / math.sqrt(D) if softmax_scale is None else float(softmax_scale), left, right, sinks,
-        _capi.QUERIES_LAST if q_start is None else q_start, k_start, _stream_ptr())
-    _capi.check(rc, "dtb_flash_window")
+        None if seqlens_k is None else seqlens_k.data_ptr(), nseg, sq, sk, Tq, Tk, H, Hk, D,
+        D ** -0.5 if softmax_scale is None else softmax_scale, left, right, sinks,
+        _capi.QUERIES_LAST if q_start is None else q_start, k_start, stream)
+    if rc:
+        _capi.check(rc, "dtb_flash_window")
     LaunchLog.count += 1
     if ev is not None:
         ev[1].record()
@@ -302,66 +335,43 @@ _CODES = {torch.int8: DTB_I8, torch.float8_e4m3fn: DTB_E4M3}
 _VALUES = {torch.float32: DTB_F32, torch.bfloat16: DTB_BF16}
 
 
-def _new_rows(shape, dtype: torch.dtype, device) -> QuantizedRows:
+def _new_rows(device, shape, dtype: torch.dtype) -> QuantizedRows:
     if dtype not in _CODES:
         raise _capi.ExtensionError(f"rows are kept in int8 or float8_e4m3fn, not {dtype}")
-    return QuantizedRows(torch.empty(shape, dtype=dtype, device=device), torch.empty(shape[:-1], dtype=torch.uint8, device=device))
+    return QuantizedRows(_empty(shape, dtype, device), _empty(shape[:-1], torch.uint8, device))
 
 
-def _merge_rows(states, shape, out, lse_out, lse_out_layout, out_bf16, out_rows):
-    """Launch of dtb_merge_rows; states[i] = (values tensor or QuantizedRows, lse or None, layout)."""
-    if len(shape) not in (3, 4):
-        raise _capi.ExtensionError("states are [B,S,H,D] or [T,H,D]")
-    B, S, H, D = (1, *shape) if len(shape) == 3 else shape
-    n = len(states)
-    outs, exps, lses = ((ctypes.c_void_p * n)() for _ in range(3))
-    dts, lays = ((ctypes.c_int * n)() for _ in range(2))
-    for i, (o, l, lay) in enumerate(states):
-        quantized = isinstance(o, QuantizedRows)
-        v, e = o if quantized else (o, None)
-        types = _CODES if quantized else _VALUES
-        _need_current_device(v, e, l)
-        if tuple(v.shape) != tuple(shape) or not v.is_contiguous() or v.dtype not in types:
-            raise _capi.ExtensionError("states must be contiguous, of one shape, and fp32, bf16 or QuantizedRows")
-        if quantized and (tuple(e.shape) != tuple(shape[:-1]) or not e.is_contiguous() or e.dtype != torch.uint8):
-            raise _capi.ExtensionError("exponents must be contiguous uint8, one per row")
-        if l is not None and (l.dtype != torch.float32 or l.numel() != B * S * H or not l.is_contiguous()):
-            raise _capi.ExtensionError("lse must be contiguous fp32 with B*S*H entries")
-        outs[i], dts[i], lays[i] = v.data_ptr(), types[v.dtype], lay
-        exps[i] = e.data_ptr() if quantized else None
-        lses[i] = l.data_ptr() if l is not None else None
-    for t, dtype in ((out, torch.float32), (out_bf16, torch.bfloat16)):
-        _need_current_device(t)
-        if t is not None and (t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous()):
-            raise _capi.ExtensionError(f"a result must be a contiguous {dtype} tensor of the states' shape")
-    if lse_out is not None:
-        _need_current_device(lse_out)
-        if lse_out.dtype != torch.float32 or lse_out.numel() != B * S * H or not lse_out.is_contiguous():
-            raise _capi.ExtensionError("lse_out must be contiguous fp32 with B*S*H entries")
-    if out_rows is not None:
-        _need_current_device(*out_rows)
-        if (out_rows.dtype not in _CODES or tuple(out_rows.shape) != tuple(shape) or out_rows.exponents.dtype != torch.uint8 or
-                tuple(out_rows.exponents.shape) != tuple(shape[:-1]) or not all(t.is_contiguous() for t in out_rows)):
-            raise _capi.ExtensionError("out_rows must be contiguous codes of the states' shape with one uint8 exponent per row")
-    if B * S * H == 0:        # (an empty tensor has no address)
-        return
-    rc = _capi.load().dtb_merge_rows(
-        n, outs, dts, exps, lses, lays, out.data_ptr() if out is not None else None,
-        lse_out.data_ptr() if lse_out is not None else None, lse_out_layout,
-        out_bf16.data_ptr() if out_bf16 is not None else None,
-        out_rows.values.data_ptr() if out_rows is not None else None, _CODES[out_rows.dtype] if out_rows is not None else 0,
-        out_rows.exponents.data_ptr() if out_rows is not None else None, B, S, H, D, _stream_ptr())
-    _capi.check(rc, "dtb_merge_rows")
-    LaunchLog.count += 1
+def _check_rows(rows: QuantizedRows, shape):
+    values, exponents = rows
+    if (values.dtype not in _CODES or exponents.dtype != torch.uint8 or values.shape != shape or exponents.shape != shape[:-1] or
+            not values.is_contiguous() or not exponents.is_contiguous()):
+        raise _capi.ExtensionError("rows are contiguous int8 or float8_e4m3fn codes with one contiguous uint8 exponent per row")
+
+
+def _check_result(out, dtype, shape):
+    if out.dtype != dtype or out.shape != shape or not out.is_contiguous():
+        raise _capi.ExtensionError(f"a result must be a contiguous {dtype} tensor of the states' shape")
 
 
 def quantize_rows(out: torch.Tensor, dtype: torch.dtype = torch.int8, *, rows: Optional[QuantizedRows] = None) -> QuantizedRows:
     """The values [..,H,D] of a state (fp32 or bf16, contiguous) in 8 bits, each row by its own power of two; into `rows` where
     given.  One launch."""
+    shape = out.shape
+    if out.dtype not in _VALUES or not out.is_contiguous():
+        raise _capi.ExtensionError("a state's values are contiguous float32 or bfloat16")
     if rows is None:
-        _need_current_device(out)
-        rows = _new_rows(out.shape, dtype, out.device)
-    _merge_rows([(out, None, LSE_BSH)], out.shape, None, None, LSE_BSH, None, rows)
+        stream = _launch_stream(out)
+        rows = _new_rows(out.device, shape, dtype)
+    else:
+        stream = _launch_stream(out, *rows)
+        _check_rows(rows, shape)
+    n = out.numel()
+    if n:                      # (an empty tensor has no address)
+        rc = _capi.load().dtb_quantize_rows(out.data_ptr(), _VALUES[out.dtype], rows.values.data_ptr(), _CODES[rows.values.dtype],
+                                            rows.exponents.data_ptr(), n // shape[-1], shape[-1], stream)
+        if rc:
+            _capi.check(rc, "dtb_quantize_rows")
+        LaunchLog.count += 1
     return rows
 
 
@@ -369,11 +379,72 @@ def dequantize_rows(rows: QuantizedRows, dtype: torch.dtype = torch.float32) -> 
     """The values that `rows` stand for, as fp32 or bf16 (exact in both).  One launch."""
     if dtype not in _VALUES:
         raise _capi.ExtensionError("rows are read back as float32 or bfloat16")
-    _need_current_device(*rows)
-    out = torch.empty(rows.shape, dtype=dtype, device=rows.device)
-    f32 = dtype == torch.float32
-    _merge_rows([(rows, None, LSE_BSH)], rows.shape, out if f32 else None, None, LSE_BSH, None if f32 else out, None)
+    values, exponents = rows
+    shape = values.shape
+    stream = _launch_stream(values, exponents)
+    _check_rows(rows, shape)
+    out = torch.empty_like(values, dtype=dtype)
+    n = values.numel()
+    if n:
+        rc = _capi.load().dtb_dequantize_rows(values.data_ptr(), _CODES[values.dtype], exponents.data_ptr(), out.data_ptr(), _VALUES[dtype],
+                                              n // shape[-1], shape[-1], stream)
+        if rc:
+            _capi.check(rc, "dtb_dequantize_rows")
+        LaunchLog.count += 1
     return out
+
+
+def _merge_rows(states, shape, out, lse_out, lse_out_layout, out_bf16, out_rows):
+    """Launch of dtb_merge_rows; states[i] = (values tensor or QuantizedRows, lse, layout)."""
+    if len(shape) not in (3, 4):
+        raise _capi.ExtensionError("states are [B,S,H,D] or [T,H,D]")
+    B, S, H, D = (1, *shape) if len(shape) == 3 else shape
+    rows = B * S * H
+    n = len(states)
+    tensors, outs, dts, exps, lses, lays = [], [], [], [], [], []
+    for o, l, lay in states:
+        if isinstance(o, QuantizedRows):
+            _check_rows(o, shape)
+            v, e = o
+            tensors.append(e)
+            dts.append(_CODES[v.dtype])
+            exps.append(e.data_ptr())
+        else:
+            v = o
+            if v.dtype not in _VALUES or v.shape != shape or not v.is_contiguous():
+                raise _capi.ExtensionError("states must be contiguous, of one shape, and fp32, bf16 or QuantizedRows")
+            dts.append(_VALUES[v.dtype])
+            exps.append(None)
+        if l.dtype != torch.float32 or l.numel() != rows or not l.is_contiguous():
+            raise _capi.ExtensionError("lse must be contiguous fp32 with B*S*H entries")
+        tensors.append(v)
+        tensors.append(l)
+        outs.append(v.data_ptr())
+        lses.append(l.data_ptr())
+        lays.append(lay)
+    if out is not None:
+        _check_result(out, torch.float32, shape)
+    if out_bf16 is not None:
+        _check_result(out_bf16, torch.bfloat16, shape)
+    if lse_out is not None and (lse_out.dtype != torch.float32 or lse_out.numel() != rows or not lse_out.is_contiguous()):
+        raise _capi.ExtensionError("lse_out must be contiguous fp32 with B*S*H entries")
+    codes = None
+    if out_rows is not None:
+        _check_rows(out_rows, shape)
+        codes = out_rows.values
+        tensors.extend(out_rows)
+    stream = _launch_stream(*tensors, out, out_bf16, lse_out)
+    if rows * D == 0:
+        return
+    pointers, ints = ctypes.c_void_p * n, ctypes.c_int * n
+    rc = _capi.load().dtb_merge_rows(
+        n, pointers(*outs), ints(*dts), pointers(*exps), pointers(*lses), ints(*lays), None if out is None else out.data_ptr(),
+        None if lse_out is None else lse_out.data_ptr(), lse_out_layout, None if out_bf16 is None else out_bf16.data_ptr(),
+        None if codes is None else codes.data_ptr(), 0 if codes is None else _CODES[codes.dtype],
+        None if codes is None else out_rows.exponents.data_ptr(), B, S, H, D, stream)
+    if rc:
+        _capi.check(rc, "dtb_merge_rows")
+    LaunchLog.count += 1
 
 
 def merge_states(states: Sequence[Tuple[Union[torch.Tensor, QuantizedRows], torch.Tensor, int]], *,
@@ -387,22 +458,20 @@ def merge_states(states: Sequence[Tuple[Union[torch.Tensor, QuantizedRows], torc
     (QuantizedRows to fill, or the type of new ones: torch.int8, torch.float8_e4m3fn) has the result
     written in 8 bits too; with fp32_out=False and no `out_bf16` that is what is returned."""
     if out_rows is not None or any(isinstance(o, QuantizedRows) for o, _, _ in states):
-        shape, device = states[0][0].shape, states[0][0].device
+        shape, device = states[0][0].shape, states[0][1].device
         if isinstance(out_rows, torch.dtype):
-            out_rows = _new_rows(shape, out_rows, device)
+            out_rows = _new_rows(device, shape, out_rows)
         if not fp32_out:
             out = None
             if out_bf16 is None and out_rows is None:
                 raise _capi.ExtensionError("fp32_out=False needs out_bf16 or out_rows")
         elif out is None:
-            out = torch.empty(shape, dtype=torch.float32, device=device)
-        if any(l is None for _, l, _ in states):
-            raise _capi.ExtensionError("every state needs its lse")
+            out = _empty(shape, torch.float32, device)
         if not want_lse:
             lse_out = None
         elif lse_out is None:
             lead, s, h = tuple(shape[:-3]), shape[-3], shape[-2]
-            lse_out = torch.empty(lead + ((s, h) if lse_out_layout == LSE_BSH else (h, s)), dtype=torch.float32, device=device)
+            lse_out = _empty(lead + ((s, h) if lse_out_layout == LSE_BSH else (h, s)), torch.float32, device)
         _merge_rows(states, shape, out, lse_out, lse_out_layout, out_bf16, out_rows)
         return (out if out is not None else out_bf16 if out_bf16 is not None else out_rows), lse_out
     lib = _capi.load()
@@ -507,6 +576,7 @@ class GridRope(NamedTuple):
 
 @functools.lru_cache(maxsize=64)
 def _rope_arrays(grid, axes, base, origin, step):
+    """What the C interface reads of a GridRope (host arrays, read at the launch)."""
     return (ctypes.c_int * 3)(*grid), (ctypes.c_int * 3)(*axes), (ctypes.c_double * 7)(base, *origin, *step)
 
 
@@ -514,19 +584,20 @@ Norm = Tuple[torch.Tensor, Optional[torch.Tensor], float]
 
 
 def _grid_rope_args(q, k, norms, rope, text_len, video_len):
-    """Checks what both passes are given; returns (element type, arguments from `grid` on)."""
-    if q.dim() != 4 or k.dim() != 4 or q.shape[:2] != k.shape[:2] or q.shape[-1] != k.shape[-1]:
+    """Checks what both passes are given; returns (shapes, element type, arguments from `grid` on)."""
+    shape, kshape, dtype = q.shape, k.shape, q.dtype
+    if len(shape) != 4 or len(kshape) != 4 or shape[:2] != kshape[:2] or shape[3] != kshape[3]:
         raise _capi.ExtensionError("q and k are [B,S,H,D] and [B,S,Hk,D]")
-    B, S, H, D = q.shape
-    if q.dtype not in _VALUES or k.dtype != q.dtype:
+    B, S, H, D = shape
+    if dtype not in _VALUES or k.dtype != dtype:
         raise _capi.ExtensionError("q and k must be bfloat16 or float32 alike")
     for w, b, _ in norms:
         for x in (w,) if b is None else (w, b):
-            if x.dtype != q.dtype or x.numel() != D or not x.is_contiguous():
+            if x.dtype != dtype or x.numel() != D or not x.is_contiguous():
                 raise _capi.ExtensionError("weights and biases hold D contiguous elements of q's type")
-    arrays = _rope_arrays(tuple(rope.grid), tuple(rope.axes), float(rope.base), tuple(rope.origin), tuple(rope.step))
-    video_len = S - text_len if video_len is None else video_len
-    return _VALUES[q.dtype], (*arrays, rope.first, rope.shards, B, S, text_len, video_len, H, k.shape[2], D)
+    grid, axes, base, origin, step, first, shards = rope
+    arrays = _rope_arrays(tuple(grid), tuple(axes), base, tuple(origin), tuple(step))
+    return shape, kshape, _VALUES[dtype], (*arrays, first, shards, B, S, text_len, S - text_len if video_len is None else video_len, H, kshape[2], D)
 
 
 def norm_rope_grid(q: torch.Tensor, k: torch.Tensor, q_norm: Norm, k_norm: Norm, rope: GridRope, *, text_len: int = 0,
@@ -535,43 +606,54 @@ def norm_rope_grid(q: torch.Tensor, k: torch.Tensor, q_norm: Norm, k_norm: Norm,
     then rotary positions of the `video_len` tokens (None: all) behind the first `text_len`, from their place in rope's grid.
     Any token and batch strides that are multiples of 16 bytes; new contiguous tensors, one launch.  Padding behind the grid's
     last place comes out as 0, as with zero-padded tables."""
-    _need_current_device(q, k, *q_norm[:2], *k_norm[:2])
-    dtype, rest = _grid_rope_args(q, k, (q_norm, k_norm), rope, text_len, video_len)
-    qo, ko = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k))
+    (qw, qb, q_eps), (kw, kb, k_eps) = q_norm, k_norm
+    stream = _launch_stream(q, k, qw, qb, kw, kb)
+    shape, kshape, dtype, rest = _grid_rope_args(q, k, (q_norm, k_norm), rope, text_len, video_len)
+    qo, ko = _empty_like(q, q.dtype), _empty_like(k, k.dtype)
     if q.numel() == 0 or k.numel() == 0:
         return qo, ko
     rc = _capi.load().dtb_norm_rope_grid(
-        q.data_ptr(), *_strides(q, False), qo.data_ptr(), q_norm[0].data_ptr(), None if q_norm[1] is None else q_norm[1].data_ptr(), q_norm[2],
-        k.data_ptr(), *_strides(k, False), ko.data_ptr(), k_norm[0].data_ptr(), None if k_norm[1] is None else k_norm[1].data_ptr(), k_norm[2],
-        dtype, int(rms), *rest, _stream_ptr())
-    _capi.check(rc, "dtb_norm_rope_grid")
+        q.data_ptr(), *_strides(q, shape), qo.data_ptr(), qw.data_ptr(), None if qb is None else qb.data_ptr(), q_eps,
+        k.data_ptr(), *_strides(k, kshape), ko.data_ptr(), kw.data_ptr(), None if kb is None else kb.data_ptr(), k_eps,
+        dtype, rms, *rest, stream)
+    if rc:
+        _capi.check(rc, "dtb_norm_rope_grid")
     LaunchLog.count += 1
     return qo, ko
+
+
+_ROPE_SCRATCH = {}        # (device, D) -> bytes that the backward pass needs
 
 
 def norm_rope_grid_backward(dq: torch.Tensor, dk: torch.Tensor, q: torch.Tensor, k: torch.Tensor, q_norm: Norm, k_norm: Norm, rope: GridRope, *,
                             text_len: int = 0, video_len: Optional[int] = None, rms: bool = False) -> Tuple[Optional[torch.Tensor], ...]:
     """Gradients of norm_rope_grid's inputs from those of its results, dq and dk: (q's, k's, q_norm's weight and bias, k_norm's
     weight and bias), None for a bias that is None.  Two launches; the sums for the weights are taken in a fixed order."""
-    _need_current_device(dq, dk, q, k, *q_norm[:2], *k_norm[:2])
-    dtype, rest = _grid_rope_args(q, k, (q_norm, k_norm), rope, text_len, video_len)
-    if dq.shape != q.shape or dk.shape != k.shape or dq.dtype != q.dtype or dk.dtype != q.dtype:
+    (qw, qb, q_eps), (kw, kb, k_eps) = q_norm, k_norm
+    stream = _launch_stream(dq, dk, q, k, qw, qb, kw, kb)
+    shape, kshape, dtype, rest = _grid_rope_args(q, k, (q_norm, k_norm), rope, text_len, video_len)
+    if dq.shape != shape or dk.shape != kshape or dq.dtype != q.dtype or dk.dtype != q.dtype:
         raise _capi.ExtensionError("dq and dk have the shapes and the type of q and k")
-    gq, gk = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k))
-    sums = [None if x is None else torch.empty_like(x) for x in (*q_norm[:2], *k_norm[:2])]
+    gq, gk = _empty_like(q, q.dtype), _empty_like(k, k.dtype)
+    sums = [None if x is None else torch.empty_like(x) for x in (qw, qb, kw, kb)]
     if q.numel() == 0 or k.numel() == 0:
         return (gq, gk, *(None if x is None else x.zero_() for x in sums))
     lib = _capi.load()
-    need = lib.dtb_norm_rope_grid_scratch_bytes(q.shape[-1])
-    if need < 0:
-        _capi.check(need, "dtb_norm_rope_grid_scratch_bytes")
-    scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
+    key = (q.get_device(), shape[3])
+    need = _ROPE_SCRATCH.get(key)
+    if need is None:
+        need = lib.dtb_norm_rope_grid_scratch_bytes(shape[3])
+        if need < 0:
+            _capi.check(need, "dtb_norm_rope_grid_scratch_bytes")
+        _ROPE_SCRATCH[key] = need
+    scratch = _empty((need,), torch.uint8, q.device)
     rc = lib.dtb_norm_rope_grid_backward(
-        dq.data_ptr(), *_strides(dq, False), dk.data_ptr(), *_strides(dk, False),
-        q.data_ptr(), *_strides(q, False), q_norm[0].data_ptr(), q_norm[2], k.data_ptr(), *_strides(k, False), k_norm[0].data_ptr(), k_norm[2],
-        gq.data_ptr(), gk.data_ptr(), *(None if x is None else x.data_ptr() for x in sums), dtype, int(rms), *rest,
-        scratch.data_ptr(), need, _stream_ptr())
-    _capi.check(rc, "dtb_norm_rope_grid_backward")
+        dq.data_ptr(), *_strides(dq, shape), dk.data_ptr(), *_strides(dk, kshape),
+        q.data_ptr(), *_strides(q, shape), qw.data_ptr(), q_eps, k.data_ptr(), *_strides(k, kshape), kw.data_ptr(), k_eps,
+        gq.data_ptr(), gk.data_ptr(), *[None if x is None else x.data_ptr() for x in sums], dtype, rms, *rest,
+        scratch.data_ptr(), need, stream)
+    if rc:
+        _capi.check(rc, "dtb_norm_rope_grid_backward")
     LaunchLog.count += 2
     return (gq, gk, *sums)
 

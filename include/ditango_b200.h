@@ -206,8 +206,8 @@ DTB_API int dtb_merge_states(int nstates, const void* const* outs, const int* ou
                      int batch, int seq, int num_heads, int head_dim, void* stream);
 
 /*
- * dtb_merge_states for states of which some are held in 8 bits, with a result that may be written in 8 bits; with one
- * state and no lse it writes a state in 8 bits, or reads it back.  (The reference caches fp32 states, core/cache.py:9-128.)
+ * dtb_merge_states for states of which some are held in 8 bits, with a result that may be written in 8 bits.  (The reference caches
+ * fp32 states, core/cache.py:9-128.)
  *
  * A row, one (token, head), of a state in 8 bits is D codes (DTB_I8, or DTB_E4M3) and one exponent byte b; a value is
  * code * 2^(b - 127), so it is exact in bf16.  Written, b is the smallest byte, at least 8, with max|value| <= M * 2^(b - 127), M
@@ -216,7 +216,6 @@ DTB_API int dtb_merge_states(int nstates, const void* const* outs, const int* ou
  *
  *  outs[i], out_dtypes[i]   [batch, seq, H, D] contiguous, DTB_F32, DTB_BF16, DTB_I8 or DTB_E4M3
  *  exponents[i]             [batch, seq, H] bytes of a state in 8 bits (not read otherwise)
- *  lses[i]                  may be NULL for a single state when lse_out is NULL: its weight is then 1
  *  out, out_bf16, out_codes results in fp32, bf16 and 8 bits (out_codes_dtype, with out_exponents); at least one.  An fp32 or bf16
  *                           result may be the buffer of a state of its type, lse_out that of a state's lse in its layout.
  */
@@ -225,6 +224,10 @@ DTB_API int dtb_merge_rows(int nstates, const void* const* outs, const int* out_
                      float* out, float* lse_out, int lse_out_layout, void* out_bf16,
                      void* out_codes, int out_codes_dtype, uint8_t* out_exponents,
                      int batch, int seq, int num_heads, int head_dim, void* stream);
+
+/* A single state's values, `rows` (below 2^31) rows of head_dim, written in 8 bits, and read back as fp32 or bf16. */
+DTB_API int dtb_quantize_rows(const void* values, int dtype, void* codes, int codes_dtype, uint8_t* exponents, int64_t rows, int head_dim, void* stream);
+DTB_API int dtb_dequantize_rows(const void* codes, int codes_dtype, const uint8_t* exponents, void* out, int out_dtype, int64_t rows, int head_dim, void* stream);
 
 /*
  * Strided copy of contiguous chunks: for every (i0,i1,i2) in [n0,n1,n2) copies chunk_bytes from

@@ -45,7 +45,19 @@ def test_rows_on_the_cpu_and_of_other_types_are_refused():
         with pytest.raises(ExtensionError):
             call()
     with pytest.raises(ExtensionError):
-        ops._new_rows((1, 2, 3, 64), torch.uint8, "cpu")
+        ops._new_rows(x.device, x.shape, torch.uint8)
+
+
+def test_single_states_refuse():
+    from ditango_b200 import _capi
+    lib = _capi.load()
+    for rc in (lib.dtb_quantize_rows(16, 2, 16, 2, 16, 5, 64, None), lib.dtb_quantize_rows(16, 0, None, 2, 16, 5, 64, None),
+               lib.dtb_quantize_rows(16, 0, 32, 1, 16, 5, 64, None), lib.dtb_quantize_rows(16, 0, 32, 2, None, 5, 64, None),
+               lib.dtb_quantize_rows(16, 0, 32, 2, 16, -1, 64, None), lib.dtb_quantize_rows(16, 0, 32, 2, 16, 2 ** 31, 64, None),
+               lib.dtb_dequantize_rows(16, 0, 16, 32, 0, 5, 64, None), lib.dtb_dequantize_rows(16, 2, 16, 32, 2, 5, 64, None),
+               lib.dtb_dequantize_rows(16, 2, None, 32, 0, 5, 64, None), lib.dtb_dequantize_rows(16, 2, 16, None, 0, 5, 64, None),
+               lib.dtb_dequantize_rows(16, 2, 16, 32, 0, 5, 80, None)):
+        assert rc == -1
 
 
 @pytest.mark.parametrize("key,dtype", [("int8", torch.int8), ("e4m3", torch.float8_e4m3fn), ("bf16", torch.bfloat16), ("fp32", torch.float32)])
