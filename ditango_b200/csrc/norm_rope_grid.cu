@@ -6,23 +6,33 @@
 //              dw = sum over rows of dy x^,  db = sum of dy
 //   R turns channels (2 i, 2 i + 1) by the angle  (origin + step * index on pair i's axis) * base^(-2 i' / d)
 // The angles come from the token's place in the grid and not from tables: in turns, product and reduction to [-1/2, 1/2] in 64 bits
-// (far positions keep their precision), cosine and sine of what is left in 32.
+// (far positions keep their precision), cosine and sine of what is left in 32.  A CTA forms those of a few tokens at a time, one per
+// thread, in shared memory.
 //
 // Bound by HBM: each value read once and written once.  D / 8 lanes own a head's row, 8 values each, so that pairs lie inside a lane
 // and the means are shuffles inside the row's lanes.  A CTA's rows of lanes are dealt to the heads of one token, and to several tokens
-// where there are fewer heads; a lane's four angles are formed once for all heads it takes.  All arithmetic is fp32, rounded once.
+// where there are fewer heads.  All arithmetic is fp32, rounded once.
+// Measured: forward, 2 x 17776 x 48 x 64 bf16, layer norm, 147 us (874 MB, 5.95 TB/s); backward, 32681 x 24 x 128 bf16, RMS norm, 213 us
+// (1205 MB, 5.65 TB/s).  The way there, us of the two:
+//   every lane the four angles of its own pairs, a token's loads issued together      216 / 381
+//   angles by the CTA, queries loaded while keys are worked on                        170 / 259
+//   channel pairs in packed arithmetic, fixed distances between heads (a quarter fewer instructions)    171 / 243
+//   loads by asynchronous copies into a ring, so that more warps fit                  147 / 213
 // The sums for the weights stay in a lane's registers over all its rows, are added up in the CTA and then over CTAs, in a fixed order.
 #include "norm_rope_grid.cuh"
 
-#include "ptx_sm100.cuh"
+#include "flash_common.cuh"
 
 namespace dtb {
 
 namespace {
 
-constexpr int kThreads = 128;
-constexpr int kBackwardPerSm = 4;       // CTAs of the backward pass per SM and tensor (what the scratch is sized for)
+using namespace flash;              // packed fp32 pairs
 
+constexpr int kThreads = 128;
+constexpr int kBackwardPerSm = 3;       // CTAs of the backward pass per SM and tensor (what the scratch is sized for)
+
+// Eight values as they lie in memory.
 template <typename T>
 struct Raw8;
 template <>
@@ -33,23 +43,38 @@ template <>
 struct Raw8<float> {
   uint4 a, b;
 };
-__device__ __forceinline__ void load8(Raw8<uint16_t>& r, const uint16_t* p) { r.a = __ldcs(reinterpret_cast<const uint4*>(p)); }
+__device__ __forceinline__ void load8(Raw8<uint16_t>& r, const uint16_t* p) { r.a = *reinterpret_cast<const uint4*>(p); }
 __device__ __forceinline__ void load8(Raw8<float>& r, const float* p) {
-  r.a = __ldcs(reinterpret_cast<const uint4*>(p));
-  r.b = __ldcs(reinterpret_cast<const uint4*>(p) + 1);
+  r.a = *reinterpret_cast<const uint4*>(p);
+  r.b = *(reinterpret_cast<const uint4*>(p) + 1);
 }
-__device__ __forceinline__ void unpack8(const Raw8<uint16_t>& r, float (&x)[8]) {
+// The same by an asynchronous copy into shared memory (kThreads pieces of 16 bytes apart); zeros where not `valid`.
+__device__ __forceinline__ void copy16(uint4* to, const void* from, bool valid) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(to)), "l"(from), "r"(valid ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy8(uint4* to, const uint16_t* from, bool valid) { copy16(to, from, valid); }
+__device__ __forceinline__ void copy8(uint4* to, const float* from, bool valid) {
+  copy16(to, from, valid);
+  copy16(to + kThreads, from + 4, valid);
+}
+__device__ __forceinline__ void read8(Raw8<uint16_t>& r, const uint4* from) { r.a = from[0]; }
+__device__ __forceinline__ void read8(Raw8<float>& r, const uint4* from) {
+  r.a = from[0];
+  r.b = from[kThreads];
+}
+
+// Eight values are held as the four channel pairs that turn together, (re, im) in one 64-bit register pair: half the instructions
+// for whatever treats both alike.
+__device__ __forceinline__ void unpack8(const Raw8<uint16_t>& r, uint64_t (&x)[4]) {
   const uint32_t w[4] = {r.a.x, r.a.y, r.a.z, r.a.w};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    x[2 * i] = __uint_as_float(w[i] << 16);
-    x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-  }
+  for (int i = 0; i < 4; ++i) x[i] = pack2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
 }
-__device__ __forceinline__ void unpack8(const Raw8<float>& r, float (&x)[8]) {
-  const uint32_t w[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
-#pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(w[i]);
+__device__ __forceinline__ void unpack8(const Raw8<float>& r, uint64_t (&x)[4]) {
+  x[0] = pack2(__uint_as_float(r.a.x), __uint_as_float(r.a.y));
+  x[1] = pack2(__uint_as_float(r.a.z), __uint_as_float(r.a.w));
+  x[2] = pack2(__uint_as_float(r.b.x), __uint_as_float(r.b.y));
+  x[3] = pack2(__uint_as_float(r.b.z), __uint_as_float(r.b.w));
 }
 __device__ __forceinline__ void store8(uint16_t* p, const float (&x)[8]) {
   *reinterpret_cast<uint4*>(p) =
@@ -68,239 +93,318 @@ __device__ __forceinline__ float row_sum(float v) {
   for (int o = kLanes / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o, kLanes);
   return v;
 }
+__device__ __forceinline__ float sum_of(uint64_t v) {
+  float a, b;
+  unpack2(v, a, b);
+  return a + b;
+}
 
 // x becomes x^ = (x - mean) rstd; returns rstd.
 template <int D, bool kRms>
-__device__ __forceinline__ float standardise(float (&x)[8], float eps) {
+__device__ __forceinline__ float standardise(uint64_t (&x)[4], float eps) {
   constexpr int kLanes = D / 8;
   if (!kRms) {
-    const float mean = row_sum<kLanes>(((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]))) * (1.f / D);
+    const float mean = row_sum<kLanes>(sum_of(add2(add2(x[0], x[1]), add2(x[2], x[3])))) * (1.f / D);
+    const uint64_t shift = pack2(-mean, -mean);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] -= mean;
+    for (int i = 0; i < 4; ++i) x[i] = add2(x[i], shift);
   }
-  float sq = 0.f;
+  const uint64_t sq = fma2(x[0], x[0], fma2(x[1], x[1], fma2(x[2], x[2], mul2(x[3], x[3]))));
+  const float rstd = rsqrtf(row_sum<kLanes>(sum_of(sq)) * (1.f / D) + eps);
+  const uint64_t scale = pack2(rstd, rstd);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) sq = fmaf(x[i], x[i], sq);
-  const float rstd = rsqrtf(row_sum<kLanes>(sq) * (1.f / D) + eps);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] *= rstd;
+  for (int i = 0; i < 4; ++i) x[i] = mul2(x[i], scale);
   return rstd;
 }
 
-// What happens to a token behind the norm.
-enum Place { kText, kTurned, kPadding };
+// Angle of pair `pair` of token `tok` as (cos, sin): (1, 0) for text, (0, 0), which no angle has, for padding.
+__device__ __forceinline__ float2 rotation(const NormRopeGridParams& p, int64_t tok, int pair) {
+  const int s = static_cast<int>(tok % p.seq) - p.text_len;
+  if (s < 0 || s >= p.video_len) return make_float2(1.f, 0.f);
+  const int64_t n = p.first + s;
+  if (n >= static_cast<int64_t>(p.shards) * p.shard_len) return make_float2(0.f, 0.f);
+  const uint32_t shard = static_cast<uint32_t>(n) / static_cast<uint32_t>(p.shard_len), in = static_cast<uint32_t>(n) - shard * p.shard_len;
+  const uint32_t rest = static_cast<uint32_t>(p.shard_rest);
+  if (in >= p.shard_places + (shard < rest ? 1u : 0u)) return make_float2(0.f, 0.f);
+  const uint32_t at = shard * p.shard_places + min(shard, rest) + in, row = at / static_cast<uint32_t>(p.size_x);
+  const uint32_t t = row / static_cast<uint32_t>(p.size_y);
+  const int a = p.axis[pair];
+  const uint32_t index = a == 0 ? t : a == 1 ? row - t * p.size_y : at - row * p.size_x;
+  const double turn = (p.origin[a] + p.step[a] * index) * p.turns[pair];
+  float2 r;
+  sincospif(2.f * static_cast<float>(turn - rint(turn)), &r.y, &r.x);
+  return r;
+}
 
-// Frequencies and axes of a lane's four pairs, and the angles of a token.
-struct Pairs {
-  double turns[4];
-  int axis[4];
-  __device__ __forceinline__ void load(const NormRopeGridParams& p, int col) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      turns[i] = p.turns[col / 2 + i];
-      axis[i] = p.axis[col / 2 + i];
-    }
-  }
-  __device__ __forceinline__ Place place(const NormRopeGridParams& p, int64_t tok, float (&cs)[4], float (&sn)[4]) const {
-    const int s = static_cast<int>(tok % p.seq) - p.text_len;
-    if (s < 0 || s >= p.video_len) return kText;
-    const int64_t n = p.first + s;
-    if (n >= static_cast<int64_t>(p.shards) * p.shard_len) return kPadding;
-    const uint32_t shard = static_cast<uint32_t>(n) / static_cast<uint32_t>(p.shard_len), in = static_cast<uint32_t>(n) - shard * p.shard_len;
-    const uint32_t rest = static_cast<uint32_t>(p.shard_rest);
-    if (in >= p.shard_places + (shard < rest ? 1u : 0u)) return kPadding;
-    const uint32_t at = shard * p.shard_places + min(shard, rest) + in, row = at / static_cast<uint32_t>(p.size_x);
-    const uint32_t t = row / static_cast<uint32_t>(p.size_y);
-    const double pos[3] = {p.origin[0] + p.step[0] * t, p.origin[1] + p.step[1] * (row - t * p.size_y),
-                           p.origin[2] + p.step[2] * (at - row * p.size_x)};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const double turn = (axis[i] == 0 ? pos[0] : axis[i] == 1 ? pos[1] : pos[2]) * turns[i];
-      sincospif(2.f * static_cast<float>(turn - rint(turn)), &sn[i], &cs[i]);
-    }
-    return kTurned;
-  }
-};
-
-// How a CTA's rows of lanes are dealt: `width` of them (a power of two) to a token's heads.
+// How a CTA goes through the tokens: batches of `batch` tokens, in steps of `tokens` tokens times `width` heads (a power of two).
 template <int D>
 struct Deal {
   static constexpr int kLanes = D / 8;
   static constexpr int kRowsOfLanes = kThreads / kLanes;
-  int width, tokens, head0, sub;
-  __device__ __forceinline__ explicit Deal(int heads) {
+  static constexpr int kPairs = D / 2;
+  static constexpr int kBatch = kRowsOfLanes;                 // most tokens of a batch: one to each row of lanes
+  int width, tokens, batch;
+  __host__ __device__ __forceinline__ explicit Deal(int heads) {
     width = 1;
     while (width < kRowsOfLanes && width < heads) width *= 2;
     tokens = kRowsOfLanes / width;
-    const int row = threadIdx.x / kLanes;
-    head0 = row % width;
-    sub = row / width;
+    // at least as many tokens as there are threads for their angles
+    batch = tokens > kThreads / kPairs ? tokens : kThreads / kPairs;
+  }
+  // The angles of the batch from token `first` on.  One batch's are written while slower warps may still read those of the one
+  // before it, hence two buffers and one barrier.
+  __device__ __forceinline__ void angles(const NormRopeGridParams& p, float2 (*to)[kPairs], int64_t first, int n) const {
+    for (int i = threadIdx.x; i < n * kPairs; i += kThreads)
+      if (first + i / kPairs < p.tokens) to[i / kPairs][i % kPairs] = rotation(p, first + i / kPairs, i % kPairs);
+    __syncthreads();
   }
 };
 
+// The four rotations of a lane's pairs.
+__device__ __forceinline__ void load_turns(const float2* from, float (&cs)[4], float (&sn)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; i += 2) {
+    const float4 v = *reinterpret_cast<const float4*>(from + i);
+    cs[i] = v.x;
+    sn[i] = v.y;
+    cs[i + 1] = v.z;
+    sn[i + 1] = v.w;
+  }
+}
+__device__ __forceinline__ bool is_padding(const float (&cs)[4], const float (&sn)[4]) { return cs[0] == 0.f && sn[0] == 0.f; }
+
 }  // namespace
 
-template <typename T, int D, bool kRms>
-__global__ void __launch_bounds__(kThreads) norm_rope_grid_kernel(const __grid_constant__ NormRopeGridParams p) {
-  constexpr int kLanes = D / 8;
-  constexpr int U = 3;                    // heads of each tensor whose loads are in flight together
-  const int col = (threadIdx.x % kLanes) * 8;
-  const Deal<D> deal(max(p.heads[0], p.heads[1]));
-  Pairs pairs;
-  pairs.load(p, col);
-  float w[2][8], b[2][8];
+// The steps of a CTA in their order: batch, tokens of the batch, heads of a token, queries then keys (kTensors = 2).
+template <int kTensors>
+struct Cursor {
+  int64_t base;           // first token of the batch
+  int t, h0, x;
+  __device__ __forceinline__ void next(int step_tokens, int step_heads, int batch, int heads, int64_t stride) {
+    if (kTensors == 2 && (x ^= 1) != 0) return;
+    if ((h0 += step_heads) < heads) return;
+    h0 = 0;
+    if ((t += step_tokens) < batch) return;
+    t = 0;
+    base += stride;
+  }
+};
+
+// How a kernel with U heads to a thread and step goes through the tokens.  kFull: there are at least as many heads as rows of lanes, so
+// that a step is of one token (the same for all threads) and the heads of a thread lie a constant apart.
+template <int D, int U, bool kFull>
+struct Pace {
+  using Deal = dtb::Deal<D>;
+  static constexpr int kBatch = kFull ? kThreads / Deal::kPairs : Deal::kBatch;       // most tokens of a batch
+  int width, tokens, batch, head0, sub;
+  __device__ __forceinline__ explicit Pace(const Deal& deal) {
+    constexpr int kLanes = D / 8;
+    width = kFull ? Deal::kRowsOfLanes : deal.width;
+    tokens = kFull ? 1 : deal.tokens;
+    batch = kFull ? kBatch : deal.batch;
+    head0 = kFull ? threadIdx.x / kLanes : threadIdx.x / kLanes % width;
+    sub = kFull ? 0 : threadIdx.x / kLanes / width;
+  }
+};
+
+// What a thread works on it copies itself, kAhead steps before, into its own places of a ring in shared memory: no barrier, and no
+// registers for what is under way.
+template <typename T, int D, bool kRms, bool kFull>
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 6 : 5) norm_rope_grid_kernel(const __grid_constant__ NormRopeGridParams p) {
+  // heads of a step, 16-byte pieces of a lane's part of a row, steps whose loads are under way
+  constexpr int U = 3, kPieces = sizeof(T) / 2, kAhead = sizeof(T) == 2 ? 4 : 2;
+  using Pace = Pace<D, U, kFull>;
+  __shared__ __align__(16) float2 s_turn[2][Pace::kBatch][D / 2];
+  __shared__ uint4 s_ring[kAhead][U * kPieces][kThreads];
+  const int col = (threadIdx.x % (D / 8)) * 8;
+  const int most = max(p.heads[0], p.heads[1]);
+  const Deal<D> deal(most);
+  const Pace pace(deal);
+  uint64_t w[2][4], b[2][4];
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
     Raw8<T> r;
     load8(r, static_cast<const T*>(p.weight[x]) + col);
     unpack8(r, w[x]);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) b[x][i] = 0.f;
-    if (p.bias[x] != nullptr) {
-      load8(r, static_cast<const T*>(p.bias[x]) + col);
-      unpack8(r, b[x]);
-    }
+    r = Raw8<T>{};
+    if (p.bias[x] != nullptr) load8(r, static_cast<const T*>(p.bias[x]) + col);
+    unpack8(r, b[x]);
   }
-  const int most = max(p.heads[0], p.heads[1]);
-  // (the bound is the same for all lanes of a warp: the shuffles use the full mask)
-  for (int64_t tok0 = static_cast<int64_t>(blockIdx.x) * deal.tokens; tok0 < p.tokens; tok0 += static_cast<int64_t>(gridDim.x) * deal.tokens) {
-    const int64_t tok = tok0 + deal.sub;
-    const bool live = tok < p.tokens;
-    const int64_t seq_no = tok / p.seq, s = tok - seq_no * p.seq;
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * pace.batch;
+  Cursor<2> at{static_cast<int64_t>(blockIdx.x) * pace.batch, 0, 0, 0}, ahead = at;
+  int slot = 0;
+  auto copy = [&]() {
+    const int x = ahead.x;
+    const int64_t tok = ahead.base + ahead.t + pace.sub;
+    if (ahead.base < p.tokens) {
+      const int64_t seq_no = tok / p.seq;
+      const T* src = static_cast<const T*>(x ? p.src[1] : p.src[0]) + seq_no * (x ? p.batch_stride[1] : p.batch_stride[0]) +
+                     (tok - seq_no * p.seq) * (x ? p.tok_stride[1] : p.tok_stride[0]) + col + (ahead.h0 + pace.head0) * D;
+      const int heads = tok < p.tokens ? (x ? p.heads[1] : p.heads[0]) - ahead.h0 - pace.head0 : 0;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (u * pace.width < heads) copy8(&s_ring[slot][u * kPieces][threadIdx.x], src + u * pace.width * D, true);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    ahead.next(pace.tokens, U * pace.width, pace.batch, most, stride);
+    if (++slot == kAhead) slot = 0;
+  };
+  // (rows that were not loaded are worked on all the same and not stored: a row's lanes keep to themselves)
+  auto work = [&](int x, int64_t tok, int h0, const float2* turns) {
     float cs[4], sn[4];
-    Place place = kText;
-    bool placed = false;
-    for (int h0 = 0; h0 < most; h0 += U * deal.width) {
-      Raw8<T> raw[2][U];
+    load_turns(turns, cs, sn);
+    const bool padding = is_padding(cs, sn);
+    T* dst = static_cast<T*>(x ? p.dst[1] : p.dst[0]) + tok * ((x ? p.heads[1] : p.heads[0]) * D) + col + (h0 + pace.head0) * D;
+    const int heads = tok < p.tokens ? (x ? p.heads[1] : p.heads[0]) - h0 - pace.head0 : 0;
 #pragma unroll
-      for (int x = 0; x < 2; ++x)
+    for (int u = 0; u < U; ++u) {
+      Raw8<T> raw;
+      read8(raw, &s_ring[slot][u * kPieces][threadIdx.x]);
+      if (padding) raw = Raw8<T>{};             // (it may hold anything, and 0 times that need not be 0)
+      uint64_t v[4];
+      unpack8(raw, v);
+      standardise<D, kRms>(v, x ? p.eps[1] : p.eps[0]);
+      float z[8];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int h = h0 + u * deal.width + deal.head0;
-          raw[x][u] = Raw8<T>{};
-          if (live && h < p.heads[x])
-            load8(raw[x][u], static_cast<const T*>(p.src[x]) + seq_no * p.batch_stride[x] + s * p.tok_stride[x] + static_cast<int64_t>(h) * D + col);
-        }
-      if (!placed) {                       // under the loads
-        if (live) place = pairs.place(p, tok, cs, sn);
-        placed = true;
+      for (int i = 0; i < 4; ++i) {
+        float re, im;
+        unpack2(fma2(v[i], w[x][i], b[x][i]), re, im);
+        z[2 * i] = re * cs[i] - im * sn[i];
+        z[2 * i + 1] = im * cs[i] + re * sn[i];
       }
+      if (u * pace.width < heads) store8(dst + u * pace.width * D, z);
+    }
+  };
+  for (int i = 0; i < kAhead; ++i) copy();
+  int buffer = 0;
+  // (all bounds are the same for all threads of the CTA: barriers and shuffles)
+  for (; at.base < p.tokens; at.base += stride) {
+    const float2(*turns)[D / 2] = s_turn[buffer];
+    deal.angles(p, s_turn[buffer], at.base, pace.batch);
+    buffer ^= 1;
+    for (int t = 0; t < pace.batch; t += pace.tokens) {
+      const int64_t tok = at.base + t + pace.sub;
+      for (int h0 = 0; h0 < most; h0 += U * pace.width) {
 #pragma unroll
-      for (int x = 0; x < 2; ++x)
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int h = h0 + u * deal.width + deal.head0;
-          float v[8];
-          unpack8(raw[x][u], v);
-          standardise<D, kRms>(v, p.eps[x]);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = fmaf(v[i], w[x][i], b[x][i]);
-          if (place == kTurned) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float re = v[2 * i], im = v[2 * i + 1];
-              v[2 * i] = re * cs[i] - im * sn[i];
-              v[2 * i + 1] = im * cs[i] + re * sn[i];
-            }
-          } else if (place == kPadding) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = 0.f;
-          }
-          if (live && h < p.heads[x]) store8(static_cast<T*>(p.dst[x]) + (tok * p.heads[x] + h) * D + col, v);
+        for (int x = 0; x < 2; ++x) {
+          asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
+          work(x, tok, h0, &turns[t + pace.sub][col / 2]);
+          copy();
         }
+      }
     }
   }
 }
 
-// grid: (CTAs, tensor)
-template <typename T, int D, bool kRms>
-__global__ void __launch_bounds__(kThreads) norm_rope_grid_backward_kernel(const __grid_constant__ NormRopeGridParams p) {
+// grid: (CTAs, tensor).  kBias: sums for a bias are wanted.
+template <typename T, int D, bool kRms, bool kFull, bool kBias>
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 6 : 4) norm_rope_grid_backward_kernel(const __grid_constant__ NormRopeGridParams p) {
   constexpr int kLanes = D / 8;
-  constexpr int U = 2;
-  __shared__ float s_sum[kThreads / kLanes][2 * D];
+  constexpr int U = sizeof(T) == 2 ? 3 : 2, kPieces = sizeof(T) / 2, kAhead = 2;
+  using Pace = Pace<D, U, kFull>;
+  constexpr int kRing = kAhead * 2 * U * kPieces * kThreads, kSums = kThreads / kLanes * 2 * D / 4;      // pieces of 16 bytes
+  __shared__ __align__(16) float2 s_turn[2][Pace::kBatch][D / 2];
+  __shared__ uint4 s_ring[kRing > kSums ? kRing : kSums];           // [step][x, gradient][head][thread]; in the end the sums
   const int x = blockIdx.y;
   const int heads = p.heads[x];
   const int col = (threadIdx.x % kLanes) * 8;
   const Deal<D> deal(heads);
-  Pairs pairs;
-  pairs.load(p, col);
-  float w[8], dw[8], db[8];
+  const Pace pace(deal);
+  uint64_t w[4], dw[4], db[4];
   {
     Raw8<T> r;
     load8(r, static_cast<const T*>(p.weight[x]) + col);
     unpack8(r, w);
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) dw[i] = db[i] = 0.f;
+  for (int i = 0; i < 4; ++i) dw[i] = db[i] = pack2(0.f, 0.f);
   const float eps = p.eps[x];
-  const T* src = static_cast<const T*>(p.src[x]) + col;
-  const T* grad = static_cast<const T*>(p.grad[x]) + col;
-  T* dst = static_cast<T*>(p.dst[x]) + col;
-  for (int64_t tok0 = static_cast<int64_t>(blockIdx.x) * deal.tokens; tok0 < p.tokens; tok0 += static_cast<int64_t>(gridDim.x) * deal.tokens) {
-    const int64_t tok = tok0 + deal.sub;
-    const bool live = tok < p.tokens;
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * pace.batch;
+  Cursor<1> at{static_cast<int64_t>(blockIdx.x) * pace.batch, 0, 0, 0}, ahead = at;
+  int slot = 0;
+  auto place = [&](int which, int u) { return s_ring + ((slot * 2 + which) * U + u) * kPieces * kThreads + threadIdx.x; };
+  // (a row that is not there is 0 and adds nothing)
+  auto copy = [&]() {
+    const int64_t tok = min(ahead.base + ahead.t + pace.sub, p.tokens - 1);
     const int64_t seq_no = tok / p.seq, s = tok - seq_no * p.seq;
+    const int left = ahead.base + ahead.t + pace.sub < p.tokens ? heads - ahead.h0 - pace.head0 : 0;
+    const int first = col + (ahead.h0 + pace.head0) * D;
+    const T* src = static_cast<const T*>(p.src[x]) + seq_no * p.batch_stride[x] + s * p.tok_stride[x];
+    const T* grad = static_cast<const T*>(p.grad[x]) + seq_no * p.grad_batch_stride[x] + s * p.grad_tok_stride[x];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool there = u * pace.width < left;
+      const int h = there ? first + u * pace.width * D : col;
+      copy8(place(0, u), src + h, there);
+      copy8(place(1, u), grad + h, there);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    ahead.next(pace.tokens, U * pace.width, pace.batch, heads, stride);
+    if (++slot == kAhead) slot = 0;
+  };
+  auto work = [&](int64_t tok, int h0, const float2* turns) {
     float cs[4], sn[4];
-    Place place = kText;
-    bool placed = false;
-    for (int h0 = 0; h0 < heads; h0 += U * deal.width) {
-      Raw8<T> rx[U], rg[U];
+    load_turns(turns, cs, sn);
+    const bool padding = is_padding(cs, sn);
+    T* dst = static_cast<T*>(p.dst[x]) + tok * (heads * D) + col + (h0 + pace.head0) * D;
+    const int left = tok < p.tokens ? heads - h0 - pace.head0 : 0;
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int h = h0 + u * deal.width + deal.head0;
-        rx[u] = rg[u] = Raw8<T>{};
-        if (live && h < heads) {
-          load8(rx[u], src + seq_no * p.batch_stride[x] + s * p.tok_stride[x] + static_cast<int64_t>(h) * D);
-          load8(rg[u], grad + seq_no * p.grad_batch_stride[x] + s * p.grad_tok_stride[x] + static_cast<int64_t>(h) * D);
-        }
+    for (int u = 0; u < U; ++u) {
+      Raw8<T> rx, rg;
+      read8(rx, place(0, u));
+      read8(rg, place(1, u));
+      if (padding) rx = rg = Raw8<T>{};               // (padding, and its gradient, may hold anything)
+      uint64_t v[4], g[4];
+      unpack8(rx, v);
+      unpack8(rg, g);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float re, im;
+        unpack2(g[i], re, im);
+        g[i] = pack2(re * cs[i] + im * sn[i], im * cs[i] - re * sn[i]);
       }
-      if (!placed) {
-        if (live) place = pairs.place(p, tok, cs, sn);
-        placed = true;
+      const float rstd = standardise<D, kRms>(v, eps);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        dw[i] = fma2(g[i], v[i], dw[i]);
+        if (kBias) db[i] = add2(db[i], g[i]);
+        g[i] = mul2(g[i], w[i]);
       }
+      const uint64_t gx = fma2(g[0], v[0], fma2(g[1], v[1], fma2(g[2], v[2], mul2(g[3], v[3]))));
+      // dx = rstd g - rstd mean(g) - v rstd mean(g v)
+      const float of_v = row_sum<kLanes>(sum_of(gx)) * (1.f / D) * -rstd;
+      const float shift = kRms ? 0.f : row_sum<kLanes>(sum_of(add2(add2(g[0], g[1]), add2(g[2], g[3])))) * (1.f / D) * -rstd;
+      const uint64_t scale = pack2(rstd, rstd), factor = pack2(of_v, of_v), shifts = pack2(shift, shift);
+      float z[8];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int h = h0 + u * deal.width + deal.head0;
-        float v[8], g[8];
-        unpack8(rx[u], v);
-        unpack8(rg[u], g);
-        if (place == kTurned) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float re = g[2 * i], im = g[2 * i + 1];
-            g[2 * i] = re * cs[i] + im * sn[i];
-            g[2 * i + 1] = im * cs[i] - re * sn[i];
-          }
-        } else if (place == kPadding) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) g[i] = 0.f;
-        }
-        const float rstd = standardise<D, kRms>(v, eps);
-        float sum_g = 0.f, sum_gx = 0.f;
-        const bool counts = live && h < heads && place != kPadding;      // (a row that is cut off may hold anything)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if (counts) {
-            dw[i] = fmaf(g[i], v[i], dw[i]);
-            db[i] += g[i];
-          }
-          g[i] *= w[i];
-          sum_g += g[i];
-          sum_gx = fmaf(g[i], v[i], sum_gx);
-        }
-        const float mean_gx = row_sum<kLanes>(sum_gx) * (1.f / D);
-        const float mean_g = kRms ? 0.f : row_sum<kLanes>(sum_g) * (1.f / D);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) g[i] = place == kPadding ? 0.f : rstd * ((g[i] - mean_g) - v[i] * mean_gx);
-        if (live && h < heads) store8(dst + (tok * heads + h) * D, g);
+      for (int i = 0; i < 4; ++i) unpack2(fma2(v[i], factor, kRms ? mul2(g[i], scale) : fma2(g[i], scale, shifts)), z[2 * i], z[2 * i + 1]);
+      if (u * pace.width < left) store8(dst + u * pace.width * D, z);
+    }
+  };
+  if (p.tokens > 0) {
+    for (int i = 0; i < kAhead; ++i) copy();
+  }
+  int buffer = 0;
+  for (; at.base < p.tokens; at.base += stride) {
+    const float2(*turns)[D / 2] = s_turn[buffer];
+    deal.angles(p, s_turn[buffer], at.base, pace.batch);
+    buffer ^= 1;
+    for (int t = 0; t < pace.batch; t += pace.tokens) {
+      for (int h0 = 0; h0 < heads; h0 += U * pace.width) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
+        work(at.base + t + pace.sub, h0, &turns[t + pace.sub][col / 2]);
+        copy();
       }
     }
   }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncthreads();                                     // the ring's memory takes the sums
+  float(*s_sum)[2 * D] = reinterpret_cast<float(*)[2 * D]>(s_ring);
   const int row = threadIdx.x / kLanes;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    s_sum[row][col + i] = dw[i];
-    s_sum[row][D + col + i] = db[i];
+  for (int i = 0; i < 4; ++i) {
+    unpack2(dw[i], s_sum[row][col + 2 * i], s_sum[row][col + 2 * i + 1]);
+    unpack2(db[i], s_sum[row][D + col + 2 * i], s_sum[row][D + col + 2 * i + 1]);
   }
   __syncthreads();
   float* to = p.partial + (static_cast<int64_t>(x) * gridDim.x + blockIdx.x) * (2 * D);
@@ -334,33 +438,36 @@ __global__ void __launch_bounds__(1024) norm_rope_grid_sums_kernel(const __grid_
   }
 }
 
-template <int D>
-static int tokens_per_cta(int heads) {
-  constexpr int rows = kThreads / (D / 8);
-  int width = 1;
-  while (width < rows && width < heads) width *= 2;
-  return rows / width;
-}
-
 template <typename T, int D, bool kRms>
 static cudaError_t launch_forward(const NormRopeGridParams& p, int sm_count, cudaStream_t stream) {
-  const int per_cta = tokens_per_cta<D>(p.heads[0] > p.heads[1] ? p.heads[0] : p.heads[1]);
-  const int64_t need = (p.tokens + per_cta - 1) / per_cta, cap = static_cast<int64_t>(sm_count) * 16;
-  norm_rope_grid_kernel<T, D, kRms><<<static_cast<unsigned>(need < cap ? need : cap), kThreads, 0, stream>>>(p);
+  const int most = p.heads[0] > p.heads[1] ? p.heads[0] : p.heads[1];
+  const int batch = Deal<D>(most).batch;
+  const int64_t need = (p.tokens + batch - 1) / batch, cap = static_cast<int64_t>(sm_count) * (sizeof(T) == 2 ? 6 : 5);
+  const unsigned ctas = static_cast<unsigned>(need < cap ? need : cap);
+  if (most >= Deal<D>::kRowsOfLanes) norm_rope_grid_kernel<T, D, kRms, true><<<ctas, kThreads, 0, stream>>>(p);
+  else norm_rope_grid_kernel<T, D, kRms, false><<<ctas, kThreads, 0, stream>>>(p);
+  return cudaGetLastError();
+}
+
+template <typename T, int D, bool kRms, bool kBias>
+static cudaError_t launch_backward_as(const NormRopeGridParams& p, int sm_count, cudaStream_t stream) {
+  const int least = p.heads[0] < p.heads[1] ? p.heads[0] : p.heads[1], most = p.heads[0] + p.heads[1] - least;
+  const int batch = Deal<D>(most).batch;
+  const int64_t need = (p.tokens + batch - 1) / batch, cap = static_cast<int64_t>(sm_count) * kBackwardPerSm;
+  // (without tokens one CTA still writes its sums, which are 0)
+  const int ctas = static_cast<int>(need < 1 ? 1 : need < cap ? need : cap);
+  if (least >= Deal<D>::kRowsOfLanes) norm_rope_grid_backward_kernel<T, D, kRms, true, kBias><<<dim3(ctas, 2), kThreads, 0, stream>>>(p);
+  else norm_rope_grid_backward_kernel<T, D, kRms, false, kBias><<<dim3(ctas, 2), kThreads, 0, stream>>>(p);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  norm_rope_grid_sums_kernel<T, D><<<dim3(2 * D / 32, 2), 1024, 0, stream>>>(p, ctas);
   return cudaGetLastError();
 }
 
 template <typename T, int D, bool kRms>
 static cudaError_t launch_backward(const NormRopeGridParams& p, int sm_count, cudaStream_t stream) {
-  const int per_cta = tokens_per_cta<D>(p.heads[0] < p.heads[1] ? p.heads[0] : p.heads[1]);
-  const int64_t need = (p.tokens + per_cta - 1) / per_cta, cap = static_cast<int64_t>(sm_count) * kBackwardPerSm;
-  // (without tokens one CTA still writes its sums, which are 0)
-  const int ctas = static_cast<int>(need < 1 ? 1 : need < cap ? need : cap);
-  norm_rope_grid_backward_kernel<T, D, kRms><<<dim3(ctas, 2), kThreads, 0, stream>>>(p);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
-  norm_rope_grid_sums_kernel<T, D><<<dim3(2 * D / 32, 2), 1024, 0, stream>>>(p, ctas);
-  return cudaGetLastError();
+  return p.bias_grad[0] != nullptr || p.bias_grad[1] != nullptr ? launch_backward_as<T, D, kRms, true>(p, sm_count, stream)
+                                                                : launch_backward_as<T, D, kRms, false>(p, sm_count, stream);
 }
 
 cudaError_t launch_norm_rope_grid(const NormRopeGridParams& p, int head_dim, bool bf16, bool rms, int sm_count, cudaStream_t stream) {

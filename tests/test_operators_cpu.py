@@ -102,14 +102,14 @@ def test_flash_window_takes_gpu_tensors_only():
         ops.flash_window(q, q, q, left=3)
 
 
-def _grid_rope(lib, *, q=16, qt=192, qb=1920, qo=16, qw=16, qbias=None, k=16, dtype=1, grid=(2, 3, 4), axes=(16, 24, 24), place=(1e4, 0, 0, 0, 1, 1, 1),
+def _grid_rope(lib, *, q=16, qt=192, qb=1920, qo=16, qw=16, qbias=None, q_eps=1e-6, k=16, dtype=1, grid=(2, 3, 4), axes=(16, 24, 24), place=(1e4, 0, 0, 0, 1, 1, 1),
                first=0, shards=1, B=1, S=10, text=2, video=8, H=3, Hk=3, D=64, back=False, scratch=16, scratch_bytes=1 << 30):
     arrays = (ctypes.c_int * 3)(*grid), (ctypes.c_int * 3)(*axes), (ctypes.c_double * 7)(*place)
     rest = (dtype, 0, *arrays, first, shards, B, S, text, video, H, Hk, D)
     if back:
-        return lib.dtb_norm_rope_grid_backward(16, 192, 1920, 16, qt, qb, q, qt, qb, qw, 1e-6, k, 192, 1920, 16, 1e-6, qo, 16, 16, None, 16, None,
+        return lib.dtb_norm_rope_grid_backward(16, 192, 1920, 16, qt, qb, q, qt, qb, qw, q_eps, k, 192, 1920, 16, 1e-6, qo, 16, 16, None, 16, None,
                                                *rest, scratch, scratch_bytes, None)
-    return lib.dtb_norm_rope_grid(q, qt, qb, qo, qw, qbias, 1e-6, k, 192, 1920, 16, 16, None, 1e-6, *rest, None)
+    return lib.dtb_norm_rope_grid(q, qt, qb, qo, qw, qbias, q_eps, k, 192, 1920, 16, 16, None, 1e-6, *rest, None)
 
 
 @pytest.mark.parametrize("back", [False, True])
@@ -118,7 +118,7 @@ def _grid_rope(lib, *, q=16, qt=192, qb=1920, qo=16, qw=16, qbias=None, k=16, dt
     (dict(text=3), "text and"), (dict(video=-1), "text and"), (dict(text=-1), "text and"), (dict(grid=(2, -1, 4)), "negative grid"),
     (dict(grid=(2 ** 16, 2 ** 10, 2 ** 10)), "2^31"), (dict(axes=(16, 25, 23)), "channels"), (dict(axes=(16, 24, 26)), "channels"),
     (dict(axes=(-2, 34, 32)), "channels"), (dict(first=-1), "first"), (dict(shards=0), "shards"), (dict(place=(0, 0, 0, 0, 1, 1, 1)), "base"),
-    (dict(place=(1e4, float("nan"), 0, 0, 1, 1, 1)), "finite"), (dict(qt=196), "multiples"), (dict(qo=24), "aligned")])
+    (dict(place=(1e4, float("nan"), 0, 0, 1, 1, 1)), "finite"), (dict(q_eps=0.0), "eps"), (dict(q_eps=float("nan")), "eps"), (dict(qt=196), "multiples"), (dict(qo=24), "aligned")])
 def test_norm_rope_grid_refuses(args, word, back):
     from ditango_b200 import _capi
     lib = _capi.load()
