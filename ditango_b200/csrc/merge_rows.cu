@@ -146,6 +146,7 @@ __global__ void __launch_bounds__(kThreads) merge_rows_kernel(const __grid_const
   const int64_t tile = static_cast<int64_t>(blockIdx.x) * kTile;
   const int lane = threadIdx.x % G;
   uint4 code[kNarrow];
+  Wide wide;
   auto load_codes = [&](int c0, int64_t row) {
 #pragma unroll
     for (int k = 0; k < kNarrow; ++k)
@@ -213,11 +214,11 @@ __global__ void __launch_bounds__(kThreads) merge_rows_kernel(const __grid_const
       if (c0 + kNarrow < n8) load_codes(c0 + kNarrow, row);
     }
     load_codes(0, row + kRows);
+    if (n8 < n && live) load_wide(wide, p.values[n8], p.dtype[n8], off);
     for (int st = n8; st < n; ++st) {
-      Wide wide = {};
-      if (live) load_wide(wide, p.values[st], p.dtype[st], off);
       const float w = s_w[st][r];
       if (live && w != 0.f) add_wide(sum, w, wide, p.dtype[st]);
+      if (st + 1 < n && live) load_wide(wide, p.values[st + 1], p.dtype[st + 1], off);
     }
 
     float acc[16];

@@ -394,32 +394,36 @@ def dequantize_rows(rows: QuantizedRows, dtype: torch.dtype = torch.float32) -> 
     return out
 
 
+_ARRAYS = {n: (ctypes.c_void_p * n, ctypes.c_int * n) for n in range(1, _capi.MERGE_MAX_STATES + 1)}
+
+
 def _merge_rows(states, shape, out, lse_out, lse_out_layout, out_bf16, out_rows):
     """Launch of dtb_merge_rows; states[i] = (values tensor or QuantizedRows, lse, layout)."""
-    if len(shape) not in (3, 4):
-        raise _capi.ExtensionError("states are [B,S,H,D] or [T,H,D]")
-    B, S, H, D = (1, *shape) if len(shape) == 3 else shape
-    rows = B * S * H
     n = len(states)
-    tensors, outs, dts, exps, lses, lays = [], [], [], [], [], []
+    if len(shape) not in (3, 4) or n not in _ARRAYS:
+        raise _capi.ExtensionError(f"1 to {_capi.MERGE_MAX_STATES} states of [B,S,H,D] or [T,H,D]")
+    B, S, H, D = (1, *shape) if len(shape) == 3 else shape
+    rows, row_shape = B * S * H, shape[:-1]
+    tensors, outs, dts, exps, lses, lays = [out, out_bf16, lse_out], [], [], [], [], []
     for o, l, lay in states:
-        if isinstance(o, QuantizedRows):
-            _check_rows(o, shape)
+        if type(o) is QuantizedRows:
             v, e = o
+            if e.dtype != torch.uint8 or e.shape != row_shape or not e.is_contiguous():
+                raise _capi.ExtensionError("exponents are contiguous uint8, one per row")
             tensors.append(e)
-            dts.append(_CODES[v.dtype])
             exps.append(e.data_ptr())
+            dtype = _CODES.get(v.dtype)
         else:
             v = o
-            if v.dtype not in _VALUES or v.shape != shape or not v.is_contiguous():
-                raise _capi.ExtensionError("states must be contiguous, of one shape, and fp32, bf16 or QuantizedRows")
-            dts.append(_VALUES[v.dtype])
             exps.append(None)
+            dtype = _VALUES.get(v.dtype)
+        if dtype is None or v.shape != shape or not v.is_contiguous():
+            raise _capi.ExtensionError("states must be contiguous, of one shape, and fp32, bf16 or QuantizedRows")
         if l.dtype != torch.float32 or l.numel() != rows or not l.is_contiguous():
             raise _capi.ExtensionError("lse must be contiguous fp32 with B*S*H entries")
-        tensors.append(v)
-        tensors.append(l)
+        tensors += (v, l)
         outs.append(v.data_ptr())
+        dts.append(dtype)
         lses.append(l.data_ptr())
         lays.append(lay)
     if out is not None:
@@ -428,20 +432,20 @@ def _merge_rows(states, shape, out, lse_out, lse_out_layout, out_bf16, out_rows)
         _check_result(out_bf16, torch.bfloat16, shape)
     if lse_out is not None and (lse_out.dtype != torch.float32 or lse_out.numel() != rows or not lse_out.is_contiguous()):
         raise _capi.ExtensionError("lse_out must be contiguous fp32 with B*S*H entries")
-    codes = None
+    codes, code, exponents = None, 0, None
     if out_rows is not None:
         _check_rows(out_rows, shape)
-        codes = out_rows.values
-        tensors.extend(out_rows)
-    stream = _launch_stream(*tensors, out, out_bf16, lse_out)
+        codes, exponents = out_rows
+        tensors += out_rows
+        code = _CODES[codes.dtype]
+    stream = _launch_stream(*tensors)
     if rows * D == 0:
         return
-    pointers, ints = ctypes.c_void_p * n, ctypes.c_int * n
+    pointers, ints = _ARRAYS[n]
     rc = _capi.load().dtb_merge_rows(
         n, pointers(*outs), ints(*dts), pointers(*exps), pointers(*lses), ints(*lays), None if out is None else out.data_ptr(),
         None if lse_out is None else lse_out.data_ptr(), lse_out_layout, None if out_bf16 is None else out_bf16.data_ptr(),
-        None if codes is None else codes.data_ptr(), 0 if codes is None else _CODES[codes.dtype],
-        None if codes is None else out_rows.exponents.data_ptr(), B, S, H, D, stream)
+        None if codes is None else codes.data_ptr(), code, None if exponents is None else exponents.data_ptr(), B, S, H, D, stream)
     if rc:
         _capi.check(rc, "dtb_merge_rows")
     LaunchLog.count += 1
@@ -457,7 +461,7 @@ def merge_states(states: Sequence[Tuple[Union[torch.Tensor, QuantizedRows], torc
     fp32_out=False only the bf16 copy `out_bf16` is written and returned in place of `out`.  `out_rows`
     (QuantizedRows to fill, or the type of new ones: torch.int8, torch.float8_e4m3fn) has the result
     written in 8 bits too; with fp32_out=False and no `out_bf16` that is what is returned."""
-    if out_rows is not None or any(isinstance(o, QuantizedRows) for o, _, _ in states):
+    if out_rows is not None or any(type(o) is QuantizedRows for o, _, _ in states):
         shape, device = states[0][0].shape, states[0][1].device
         if isinstance(out_rows, torch.dtype):
             out_rows = _new_rows(device, shape, out_rows)
