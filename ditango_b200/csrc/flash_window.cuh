@@ -25,12 +25,17 @@ struct WindowParams {
   int q_batch_first, k_batch_first, v_batch_first;
 };
 
-// The sequence of a CTA: where its queries and keys begin among the tokens, how many there are, and the first query's position
-// counted from the first key.
+// A sequence: where its queries and keys begin among the tokens, how many there are, and which keys its first query sees: [0, sinks) as
+// far as it sees them, and from `from` up to `to`, which move on by one with every query.
 struct WindowSeq {
   int q_begin, q_len, k_begin, k_len;
-  int64_t q_shift;
+  int from, to, sinks;
 };
+
+__device__ __forceinline__ int clamp_position(int64_t x) {
+  constexpr int64_t kFar = 1 << 30;                 // beyond all keys, and a query's number can still be added
+  return static_cast<int>(x < -kFar ? -kFar : x > kFar ? kFar : x);
+}
 
 __device__ __forceinline__ WindowSeq window_seq(const WindowParams& p, int seg) {
   WindowSeq s;
@@ -47,7 +52,11 @@ __device__ __forceinline__ WindowSeq window_seq(const WindowParams& p, int seg) 
   }
   s.q_len = max(min(s.q_len, p.f.seqlen_q), 0);
   s.k_len = max(min(s.k_len, p.f.seqlen_k), 0);
-  s.q_shift = p.q_start == kQueriesLast ? static_cast<int64_t>(s.k_len) - s.q_len : static_cast<int64_t>(p.q_start) - p.k_start;
+  // the first query's position, counted from the first key
+  const int64_t x = p.q_start == kQueriesLast ? static_cast<int64_t>(s.k_len) - s.q_len : static_cast<int64_t>(p.q_start) - p.k_start;
+  s.from = clamp_position(x - p.left);
+  s.to = clamp_position(x + p.right + 1);
+  s.sinks = max(min(clamp_position(static_cast<int64_t>(p.sinks) - p.k_start), s.k_len), 0);
   return s;
 }
 
@@ -57,18 +66,14 @@ struct WindowSpan {
   int first, lo, hi;
 };
 
-__device__ __forceinline__ int clamp_key(int64_t j, int k_len) { return static_cast<int>(j < 0 ? 0 : j > k_len ? k_len : j); }
-
-__device__ __forceinline__ WindowSpan window_span(const WindowParams& p, const WindowSeq& s, int i) {
-  const int64_t x = s.q_shift + i;
-  const int sinks = clamp_key(static_cast<int64_t>(p.sinks) - p.k_start, s.k_len);
+__device__ __forceinline__ WindowSpan window_span(int from, int to, int sinks, int k_len, int i) {
   WindowSpan w;
-  w.hi = clamp_key(x + p.right + 1, s.k_len);
+  w.hi = min(max(to + i, 0), k_len);
   w.first = min(sinks, w.hi);
-  w.lo = min(max(clamp_key(x - p.left, s.k_len), sinks), w.hi);
-  w.lo = max(w.lo, w.first);
+  w.lo = max(min(max(from + i, sinks), w.hi), w.first);
   return w;
 }
+__device__ __forceinline__ WindowSpan window_span(const WindowSeq& s, int i) { return window_span(s.from, s.to, s.sinks, s.k_len, i); }
 
 // Element offset of a sequence's token in a q / k / v tensor (dense: token inside its sequence; packed: of the whole tensor).
 __device__ __forceinline__ int64_t window_offset(const WindowParams& p, int seg, int64_t tok, int64_t tok_stride, int64_t batch_stride) {

@@ -95,8 +95,8 @@ __global__ void __launch_bounds__(kThreads) flash_window_rows_kernel(const Windo
   const int n_rows = min(kRows, rows - row0);
 
   // what the block sees: the first row reaches furthest to the left, the last one to the right
-  const WindowSpan w0 = window_span(p, s, row0 / group);
-  const WindowSpan w1 = window_span(p, s, (row0 + n_rows - 1) / group);
+  const WindowSpan w0 = window_span(s, row0 / group);
+  const WindowSpan w1 = window_span(s, (row0 + n_rows - 1) / group);
   const int first = w1.first, lo = max(w0.lo, first);
   const int total = first + max(w1.hi - lo, 0);
   const int n_tiles = (total + kKeys - 1) / kKeys;
@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(kThreads) flash_window_rows_kernel(const Windo
     const uint16_t* src = nullptr;
     if (r < n_rows) {
       const int i = (row0 + r) / group, g = (row0 + r) % group;
-      const WindowSpan w = window_span(p, s, i);
+      const WindowSpan w = window_span(s, i);
       end[h] = w.first;
       from[h] = w.lo - lo + first;
       to[h] = w.hi - lo + first;

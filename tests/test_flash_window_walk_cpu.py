@@ -17,51 +17,69 @@ STUBS = r"""
 #include <cstdint>
 #include <cstdio>
 #include <cstdlib>
+#include <vector>
 #define __device__
 #define __forceinline__ inline
-#define __restrict__
 using std::max; using std::min;
 struct CUtensorMap { int x; };
 constexpr int kQueriesLast = INT32_MIN;
-struct FlashParams { int* status; const int32_t *cu_q, *cu_k; int seqlen_q, seqlen_k; };
-struct WindowParams { FlashParams f; const int32_t* seqlens_k; int left, right, sinks, q_start, k_start, q_batch_first, k_batch_first, v_batch_first; };
+struct FlashParams { int* status; const int32_t *cu_q, *cu_k; int seqlen_q, seqlen_k, num_heads, nseg; };
+struct WindowParams { FlashParams f; const int32_t* seqlens_k; int kv_heads, left, right, sinks, q_start, k_start, q_batch_first, k_batch_first, v_batch_first; };
 %(seq)s
 %(span)s
 %(constants)s
 %(cfg)s
 %(walk)s
+%(item)s
 constexpr int D = %(head_dim)d;
 using C = Cfg<D>;
 constexpr int NB = C::kSBufs;
-constexpr int kRing = C::kStages;
-uint64_t q_full[2], kv_full[kRing], kv_empty[kRing], s_full[NB], p_lo[NB], p_hi[NB], pv_done[2], o_final[2], v_tail[2];
-uint8_t s_q[kQT * C::kTileBytes], s_kv[kRing * C::kKvTileBytes];
+struct Arrays {
+  uint64_t q_full[2 * C::kQBufs], q_empty[C::kQBufs], kv_full[C::kStages], kv_empty[C::kStages], s_full[NB], p_lo[NB], p_hi[NB], pv_done[2];
+  uint64_t o_final[2], o_free[2], work_full[kWork], work_empty[kWork], v_tail[kTails], claim[1];
+  uint8_t s_q[C::kQBufs * kQT * C::kTileBytes], s_kv[C::kStages * C::kTileBytes], s_claim[16];
+  Item s_work[kWork];
+} sh_;
+template <int>
+struct Shared {
+  uint64_t *q_full = sh_.q_full, *q_empty = sh_.q_empty, *kv_full = sh_.kv_full, *kv_empty = sh_.kv_empty, *s_full = sh_.s_full, *p_lo = sh_.p_lo;
+  uint64_t *p_hi = sh_.p_hi, *pv_done = sh_.pv_done, *o_final = sh_.o_final, *o_free = sh_.o_free, *work_full = sh_.work_full;
+  uint64_t *work_empty = sh_.work_empty, *v_tail = sh_.v_tail, *claim = sh_.claim;
+  uint8_t *s_q = sh_.s_q, *s_kv = sh_.s_kv, *s_claim = sh_.s_claim;
+  Item* s_work = sh_.s_work;
+  explicit Shared(uint8_t*) {}
+};
+uint32_t opaque_zero() { return 0; }
 CUtensorMap tm_q, tm_k, tm_v;
 struct uint4 { uint32_t x, y, z, w; };
 uint4 make_uint4(uint32_t, uint32_t, uint32_t, uint32_t) { return uint4{1, 1, 1, 1}; }
 constexpr uint32_t idesc_bf16_f32(int, int, bool, bool) { return 0; }
-uint32_t smem_u32(const void* x) { return x == s_q ? 0u : uint32_t(kQT * C::kTileBytes); }
+uint32_t smem_u32(const void* x) { return x == sh_.s_q ? 0u : uint32_t(C::kQBufs * kQT * C::kTileBytes); }
 uint64_t smem_desc_sw128(uint32_t addr, uint32_t, uint32_t) { return addr >> 4; }
+std::vector<Item> items;
 void event(const char* what, const uint64_t* bar, int extra) {
-#define BAR(b) if (bar >= b && bar < b + sizeof(b) / 8) std::printf("%%s %%s %%d %%d\n", what, #b, int(bar - b), extra)
-  BAR(q_full); BAR(kv_full); BAR(kv_empty); BAR(s_full); BAR(p_lo); BAR(p_hi); BAR(pv_done); BAR(o_final); BAR(v_tail);
+#define BAR(b) if (bar >= sh_.b && bar < sh_.b + sizeof(sh_.b) / 8) std::printf("%%s %%s %%d %%d\n", what, #b, int(bar - sh_.b), extra)
+  BAR(q_full); BAR(q_empty); BAR(o_free); BAR(kv_full); BAR(kv_empty); BAR(s_full); BAR(p_lo); BAR(p_hi); BAR(pv_done); BAR(o_final); BAR(v_tail);
+  BAR(work_full); BAR(work_empty); BAR(claim);
 }
 bool wait_or_abort(uint64_t* bar, uint32_t parity, int*, int) { event("wait", bar, int(parity)); return true; }
 void mbar_expect_tx(uint64_t* bar, uint32_t) { event("expect", bar, 0); }
 void mbar_arrive(uint64_t* bar) {
-  int cleared = 0, first = -1;        // rows of 128 bytes that were cleared
-  for (int i = 0; i < int(sizeof(s_kv) / 128); ++i) {
-    if (s_kv[i * 128] != 0) { ++cleared; if (first < 0) first = i; }
+  if (bar >= sh_.work_full && bar < sh_.work_full + kWork) items.push_back(sh_.s_work[bar - sh_.work_full]);
+  if (bar >= sh_.v_tail && bar < sh_.v_tail + kTails) {
+    int cleared = 0, first = -1;        // rows of 128 bytes that were cleared
+    for (int i = 0; i < int(sizeof(sh_.s_kv) / 128); ++i)
+      if (sh_.s_kv[i * 128] != 0) { ++cleared; if (first < 0) first = i; }
+    for (auto& x : sh_.s_kv) x = 0;
+    std::printf("cleared %%d %%d\n", cleared, first);
   }
-  for (auto& x : s_kv) x = 0;
-  std::printf("cleared %%d %%d\n", cleared, first);
   event("arrive", bar, 0);
 }
 void fence_proxy_async_smem() {}
 void prefetch_tmap(const CUtensorMap*) {}
 void tma_load_token(void* dst, const CUtensorMap* m, uint64_t*, int x, int token, int batch, int) {
   std::printf("load %%s %%d %%d\n", m == &tm_q ? "q" : m == &tm_k ? "k" : "v",
-              m == &tm_q ? int((uint8_t*)dst - s_q) / kSlabBytes : int((uint8_t*)dst - s_kv) / kSlabBytes, token);
+              m == &tm_q ? int((uint8_t*)dst - sh_.s_q) / kSlabBytes : int((uint8_t*)dst - sh_.s_kv) / kSlabBytes, token);
 }
 void mma_commit(uint64_t* bar) { event("commit", bar, 0); }
 void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t, uint32_t) { std::printf("S %%u %%llu %%llu\n", d, (unsigned long long)a, (unsigned long long)b); }
@@ -70,23 +88,47 @@ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t, uint32_t acc) {
 }
 void tc_fence_after() {}
 bool elect_one() { return true; }
+// blocks of the launch in their order, every `stride`th of them to this CTA
+int next_block, stride, n_blocks, row_blocks;
+struct { int x, y, z; } blockIdx;
+void claim_request(void*, uint64_t* bar) { event("arrive", bar, 0); }
+bool claim_answer(const void*, int& x, int& y, int& z) {
+  next_block += stride;
+  if (next_block >= n_blocks) return false;
+  x = next_block %% row_blocks; y = next_block / row_blocks; z = 0;
+  return true;
+}
 int main(int, char** argv) {
   WindowParams p = {};
   p.f.seqlen_q = std::atoi(argv[1]); p.f.seqlen_k = std::atoi(argv[2]); p.left = std::atoi(argv[3]); p.right = std::atoi(argv[4]);
   p.sinks = std::atoi(argv[5]); p.q_start = std::atoi(argv[6]); p.k_start = std::atoi(argv[7]);
-  const int q0 = std::atoi(argv[8]), head = 0, kv_head = 0, batch = 0;
-  const WindowSeq s = window_seq(p, 0);
-  const Walk walk(p, s, q0, min(q0 + kQT * kBM, s.q_len) - 1);
-  std::printf("walk %%d %%d %%d %%d\n", walk.steps, walk.tiles, walk.skew, walk.N);
-  for (int i = q0; i < min(q0 + kQT * kBM, s.q_len); ++i) { WindowSpan w = window_span(p, s, i); std::printf("row %%d %%d %%d %%d\n", i, w.first, w.lo, w.hi); }
-  for (int u = 0; u < kQT * walk.steps; ++u) { const int t = walk.tile_of(u); std::printf("unit %%d %%d %%d %%d\n", u, t, walk.begin(t), walk.valid(t)); }
-  if (walk.steps <= 0) return 0;
-  const int n_units = kQT * walk.steps;
+  p.f.num_heads = std::atoi(argv[8]); p.kv_heads = p.f.num_heads; p.f.nseg = 1; next_block = std::atoi(argv[9]); stride = std::atoi(argv[10]);
+  row_blocks = (p.f.seqlen_q + 255) / 256;
+  n_blocks = row_blocks * p.f.num_heads;
+  blockIdx.x = next_block %% row_blocks; blockIdx.y = next_block / row_blocks; blockIdx.z = 0;
+  uint8_t* smem = nullptr;
   const uint32_t tmem_base = 0;
   std::printf("loader 0\n");
 %(loader)s
   std::printf("issuer 0\n");
+  uint32_t fetched = 0;
+  auto fetch = [&](const Shared<D>& sh) {
+    event("wait", &sh.work_full[fetched %% kWork], (fetched / kWork) & 1);
+    const uint32_t slot = fetched++ %% kWork;
+    sh.s_work[slot] = items[fetched - 1];
+    return sh.s_work[slot].walk.steps >= 0 ? int(slot) : -1;
+  };
 %(issuer)s
+  std::printf("blocks 0\n");
+  for (const Item& w : items) {
+    if (w.walk.steps < 0) break;
+    std::printf("block %%d %%d %%d %%d\n", w.q0, w.walk.steps, w.walk.N, w.walk.n);
+    for (int i = w.q0; i < min(w.q0 + 256, w.q_len); ++i) {
+      const WindowSpan s = window_span(w.from, w.to, w.sinks, w.k_len, i);
+      std::printf("row %%d %%d %%d %%d\n", i, s.first, s.lo, s.hi);
+    }
+    for (int u = 0; u < 2 * w.walk.steps; ++u) { const int t = w.walk.tile_of(u); std::printf("unit %%d %%d %%d %%d\n", u, t, w.walk.begin(t), w.walk.valid(t)); }
+  }
 }
 """
 
@@ -104,8 +146,8 @@ def replay(tmp_path_factory):
     span = window[window.index("struct WindowSpan"):window.index("// Element offset")]
     parts = dict(constants=constants, seq=seq, span=span, cfg="template <int D>\nstruct Cfg " + _block(kernel, kernel.index("struct Cfg")) + ";",
                  walk="struct Walk " + _block(kernel, kernel.index("struct Walk")) + ";",
-                 loader=_block(kernel, kernel.index("if (elect_one())", kernel.index("- TMA producer"))),
-                 issuer=_block(kernel, kernel.index("if (elect_one())", kernel.index("- MMA issuer"))))
+                 item="struct Item " + _block(kernel, kernel.index("struct Item")) + ";",
+                 loader=_role(kernel, "- blocks and TMA loads"), issuer=_role(kernel, "- MMA issuer"))
     built = {}
     for head_dim in (64, 128):
         d = tmp_path_factory.mktemp("walk")
@@ -123,12 +165,17 @@ def replay(tmp_path_factory):
     return run
 
 
-def _play(head_dim, loader, issuer, n_units):
-    """Runs the two event lists against each other; returns the products as (kind, unit half, slab of the ring, token loaded there)."""
-    slabs, stages, nb = head_dim // 64, {64: 10, 128: 5}[head_dim], {64: 3, 128: 2}[head_dim]
+def _role(kernel, title):
+    """A role's own view of shared memory and the code of its elected thread, as a scope."""
+    return "{ const Shared<D> sh(smem);\n" + _block(kernel, kernel.index("if (elect_one())", kernel.index(title))) + "\n}"
+
+
+def _play(head_dim, loader, issuer):
+    """Runs the two event lists against each other; returns the products as (event, slab of the ring, what was loaded there)."""
+    slabs, stages, q_bytes = head_dim // 64, {64: 8, 128: 4}[head_dim], {64: 4, 128: 2}[head_dim] * 128 * head_dim * 2
     phase = {}                              # (barrier, index) -> completed phases
     ring = {}                               # slab of the ring -> (tensor, token)
-    done, products, cleared = lambda b: phase.get(b, 0), [], {}
+    done, products = lambda b: phase.get(b, 0), []
 
     def passes(ev):
         # (a wait on a parity passes while the phase under way has the other one)
@@ -136,7 +183,7 @@ def _play(head_dim, loader, issuer, n_units):
 
     def complete(b):
         phase[b] = done(b) + 1
-    at = [0, 0]
+    at, loads = [0, 0], 0
     while at[0] < len(loader) or at[1] < len(issuer):
         moved = False
         while at[0] < len(loader):
@@ -149,10 +196,9 @@ def _play(head_dim, loader, issuer, n_units):
                 if ev[1] != "q":
                     assert int(ev[2]) // slabs == int(last[1])
                     ring[int(ev[2])] = (ev[1], int(ev[3]))
-                if sum(e[0] == "load" for e in loader[:at[0] + 1]) % slabs == 0:
+                loads += 1
+                if loads % slabs == 0:
                     complete(last)
-            elif ev[0] == "cleared":
-                cleared[last[1]] = (int(ev[1]), int(ev[2]))
             elif ev[0] == "arrive":
                 complete((ev[1], ev[2]))
             at[0] += 1
@@ -163,12 +209,16 @@ def _play(head_dim, loader, issuer, n_units):
             if ev[0] == "wait" and ev[1] in ("p_lo", "p_hi"):
                 assert done(("s_full", ev[2])) > done((ev[1], ev[2]))
                 complete((ev[1], ev[2]))
+            # ... and O is read once it is final
+            if ev[0] == "wait" and ev[1] == "o_free":
+                assert done(("o_final", ev[2])) > done(("o_free", ev[2]))
+                complete((ev[1], ev[2]))
             if ev[0] == "wait" and not passes(ev):
                 break
-            if ev[0] == "commit":
+            if ev[0] in ("commit", "arrive"):
                 complete((ev[1], ev[2]))
             elif ev[0] in ("S", "PV"):
-                off = int(ev[3]) * 16 - 2 * 128 * head_dim * 2            # from the ring's start
+                off = int(ev[3]) * 16 - q_bytes            # from the ring's start
                 slab = off // (128 * 128)
                 assert 0 <= slab < stages * slabs
                 products.append((ev, slab, ring[slab]))
@@ -178,74 +228,94 @@ def _play(head_dim, loader, issuer, n_units):
     return products, phase
 
 
+def _blocks(ev):
+    """[(q0, steps, N, n, rows, units)]"""
+    out = []
+    for e in ev[ev.index(["blocks", "0"]) + 1:]:
+        n = [int(x) for x in e[1:]]
+        if e[0] == "block":
+            out.append((*n, [], []))
+        else:
+            out[-1][4 if e[0] == "row" else 5].append(tuple(n))
+    return out
+
+
 CASES = [  # Sq, Sk, left, right, sinks, q_start, k_start
     (300, 300, 100, 100, 0, 0, 0), (700, 700, 200, 200, 130, 0, 0), (1000, 4000, 1500, 0, 226, 3000, 0), (513, 2000, 300, 77, 13, 700, 0),
     (256, 256, 0, 0, 0, 0, 0), (600, 600, 0, 0, 300, 0, 0), (400, 450, 100, 500, 405, 0, 400), (400, 450, 50, 0, 950, 1000, 900),
     (1024, 1024, 2 ** 30, 2 ** 30, 0, 0, 0), (800, 3000, 128, 127, 128, 1100, 0), (300, 100, 20, 10, 4, -50, 0), (2000, 2000, 255, 256, 64, 0, 0),
-    (260, 5000, 700, 700, 1, 2500, 0), (500, 60, 10, 10, 0, 0, 0)]
+    (260, 5000, 700, 700, 1, 2500, 0), (500, 60, 10, 10, 0, 0, 0), (1500, 1500, 20, 20, 5, 0, 0), (1500, 1500, 100, 0, 0, 0, 0)]
 
 
 @pytest.mark.parametrize("head_dim", [64, 128])
 @pytest.mark.parametrize("case", CASES)
-def test_every_unit_meets_its_tile_and_every_row_its_keys(replay, case, head_dim):
+@pytest.mark.parametrize("heads,grid", [(1, 1), (3, 2), (2, 148)])
+def test_every_unit_meets_its_tile_and_every_row_its_keys(replay, case, head_dim, heads, grid):
     Sq, Sk, left, right, sinks, q_start, k_start = case
-    for q0 in range(0, Sq, 256):
-        ev = replay(head_dim, *case, q0)
-        cut = [i for i, e in enumerate(ev) if e[0] in ("loader", "issuer")]
-        head = ev[:cut[0]] if cut else ev
-        steps, tiles, skew, N = (int(x) for x in head[0][1:])
-        units = [tuple(int(x) for x in e[1:]) for e in head if e[0] == "unit"]
-        rows = [tuple(int(x) for x in e[1:]) for e in head if e[0] == "row"]
-        assert len(units) == 2 * steps
-        for i, first, lo, hi in rows:
-            x = q_start + i
-            seen = [j for j in range(Sk) if j + k_start <= x + right and (j + k_start >= x - left or j + k_start < sinks)]
-            assert seen == list(range(first)) + list(range(lo, hi))
-            # the columns that the kernel lets the row see, unit by unit of its Q tile
-            met = []
-            for u, tile, base, valid in units[(i - q0) // 128::2]:
-                c0, c1 = (lo - base, hi - base) if tile < N else (0, first - base)
-                assert min(c1, 128) <= valid             # nothing behind the tile's last key
-                met += range(base + max(c0, 0), base + min(max(c1, 0), 128))
-            assert sorted(met) == seen
-        if not steps:
-            assert not cut and all(first == 0 and lo >= hi for _, first, lo, hi in rows)
-            continue
-        loader, issuer = ev[cut[0] + 1:cut[1]], ev[cut[1] + 1:]
-        products, phase = _play(head_dim, loader, issuer, 2 * steps)
-        # S: one after another, from the unit's tile of K; PV: the same of V, over the steps of 16 keys that hold one
-        slabs = head_dim // 64
+    n_blocks = -(-Sq // 256) * heads
+    covered, slabs, q_bufs = 0, head_dim // 64, {64: 2, 128: 1}[head_dim]
+    for cta in range(min(grid, n_blocks)):
+        ev = replay(head_dim, *case, heads, cta, grid)
+        blocks = _blocks(ev)
+        covered += len(blocks)
+        for q0, steps, N, n, rows, units in blocks:
+            assert len(units) == 2 * steps
+            for i, first, lo, hi in rows:
+                x = q_start + i
+                seen = [j for j in range(Sk) if j + k_start <= x + right and (j + k_start >= x - left or j + k_start < sinks)]
+                assert seen == list(range(first)) + list(range(lo, hi))
+                # the columns that the kernel lets the row see, unit by unit of its Q tile
+                met = []
+                for u, tile, base, valid in units[(i - q0) // 128::2]:
+                    c0, c1 = (lo - base, hi - base) if tile < N else (0, first - base)
+                    assert min(c1, 128) <= valid             # nothing behind the tile's last key
+                    met += range(base + max(c0, 0), base + min(max(c1, 0), 128))
+                assert sorted(met) == seen
+            if not steps:
+                assert all(first == 0 and lo >= hi for _, first, lo, hi in rows)
+        at = ev.index(["issuer", "0"])
+        loader, issuer = ev[1:at], ev[at + 1:ev.index(["blocks", "0"])]
+        real = [b for b in blocks if b[1] > 0]
+        units = [(*u, i % q_bufs) for i, b in enumerate(real) for u in b[5]]
+        products, phase = _play(head_dim, loader, issuer)
+        # S: one after another, from the unit's tile of K and its block's queries; PV: the same of V, over the steps of 16 keys that hold one
         s = [p for p in products if p[0][0] == "S"]
         assert len(s) == len(units) * head_dim // 16
         for n, (e, slab, held) in enumerate(s):
-            u, tile, base, valid = units[n // (head_dim // 16)]
-            assert held == ("k", base) and int(e[2]) * 16 // (128 * head_dim * 2) == u % 2
+            u, tile, base, valid, q_buf = units[n // (head_dim // 16)]
+            assert held == ("k", base) and int(e[2]) * 16 // (128 * head_dim * 2) == 2 * q_buf + u % 2
         pv = [p for p in products if p[0][0] == "PV"]
         k = 0
-        for u, tile, base, valid in units:
+        for u, tile, base, valid, _ in units:
             for step in range(-(-valid // 16)):
                 e, slab, held = pv[k]
-                inside = (int(e[3]) * 16 - 2 * 128 * head_dim * 2) % (128 * 128 * slabs)
+                inside = int(e[3]) * 16 % (128 * 128 * slabs)
                 assert held == ("v", base) and inside == step * 2048 and int(e[4]) == int(u > 1 or step > 0)
                 k += 1
         assert k == len(pv)
         # tiles that are not full are cleared behind their last key, up to a multiple of 16
         clears = [(int(e[1]), int(e[2])) for e in loader if e[0] == "cleared"]
-        ragged = list(dict.fromkeys((tile, valid) for _, tile, _, valid in units if valid % 16))
-        assert len(clears) == len(ragged) <= 2
+        ragged = [r for b in blocks for r in dict.fromkeys((tile, valid) for _, tile, _, valid in b[5] if valid % 16)]
+        assert len(clears) == len(ragged) <= 2 * len(blocks)
         for (count, first), (_, valid) in zip(clears, ragged):
             assert count == (16 - valid % 16) * slabs and first % 128 == valid
+        if not real:
+            continue
         # the last commits are those that the epilogue waits for, each with its last products in front of it
         finals = [i for i, e in enumerate(issuer) if e[:2] == ["commit", "o_final"]]
         last_mma = max(i for i, e in enumerate(issuer) if e[0] in ("S", "PV"))
-        assert [issuer[i][2] for i in finals] == ["0", "1"] and finals[-1] == len(issuer) - 1
+        assert [issuer[i][2] for i in finals] == ["0", "1"] * len(real) and finals[-1] == len(issuer) - 1
         assert all(i < last_mma for i, e in enumerate(issuer) if e[0] == "commit" and e[1] != "o_final")
-        if head_dim == 64:
-            assert all(phase.get(("pv_done", str(h)), 0) == steps - 1 for h in (0, 1))
+        # one completion of pv_done for every unit, but the CTA's last two
+        assert all(phase.get(("pv_done", str(h)), 0) == sum(b[1] for b in real) - 1 for h in (0, 1))
+        # the queries' memory is given back behind the last S that reads it
+        given = [sum(x[0] == "S" for x in issuer[:i]) for i, e in enumerate(issuer) if e[:2] == ["commit", "q_empty"]]
+        assert given == [sum(2 * b[1] for b in real[:i + 1]) * head_dim // 16 for i in range(len(real))]
+    assert covered == n_blocks
 
 
 def test_windows_that_no_end_cuts_take_a_tile_less(replay):
-    """2701 keys for each row: 22 tiles hold those of 128 rows, 23 those of 256."""
-    ev = replay(64, 17776, 17776, 1350, 1350, 226, 0, 0, 256 * 30)
-    steps, tiles, skew, N = (int(x) for x in ev[0][1:])
-    assert (skew, N, steps) == (1, 24, 23 + 2)
+    """2701 keys for each row: 23 tiles hold those of 128 rows, 24 those of 256; two more hold the 226 first ones."""
+    ev = replay(64, 17776, 17776, 1350, 1350, 226, 0, 0, 1, 30, 70)
+    q0, steps, N, n, _, _ = _blocks(ev)[0]
+    assert (q0, N, n, steps) == (256 * 30, 24, 23, 23 + 2)
