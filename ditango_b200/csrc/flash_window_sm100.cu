@@ -48,7 +48,6 @@ constexpr int kOutWarp = 8;         // first of four
 constexpr int kTmaWarp = 12;
 constexpr int kMmaWarp = 13;
 constexpr int kSplit = 64;          // keys of a tile whose probabilities are handed over first
-constexpr int kPolyPairs = 1;       // pairs of every 8 pairs of scores, exponentiated on the FMA units
 constexpr int kWork = 4;            // blocks under way in a CTA
 constexpr int kWorkReaders = 8 + 4 + 1;
 constexpr int kClaimAhead = 8;      // steps before a block's last at which the next block is asked for
@@ -124,6 +123,23 @@ __device__ __forceinline__ uint32_t run_of_bits(int a, int b) {
   asm("shl.b32 %0, 1, %1;" : "=r"(x) : "r"(min(max(a, 0), 32)));
   asm("shl.b32 %0, 1, %1;" : "=r"(y) : "r"(min(max(b, 0), 32)));
   return (y - 1u) & ~(x - 1u);
+}
+
+// 64 bf16 columns of a warp's 32 rows, a row per lane, to rows `pitch` elements apart: through shared memory (4 KB of the warp's), so that
+// 8 lanes write the 128 contiguous bytes of a row.  The 16-byte pieces are XOR-swizzled by row against bank conflicts.
+__device__ __forceinline__ void store_rows64_bf16(uint8_t* stage, uint16_t* dst, int64_t pitch, int rows, const uint32_t* row) {
+  const int lane = threadIdx.x & 31, r0 = lane >> 3, piece = lane & 7;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    *reinterpret_cast<uint4*>(stage + lane * 128 + ((i ^ (lane & 7)) << 4)) = make_uint4(row[4 * i], row[4 * i + 1], row[4 * i + 2], row[4 * i + 3]);
+  __syncwarp();
+#pragma unroll
+  for (int it = 0; it < 8; ++it) {
+    const int r = it * 4 + r0;
+    const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 128 + ((piece ^ (r & 7)) << 4));
+    if (r < rows) *reinterpret_cast<uint4*>(dst + r * pitch + piece * 8) = v;
+  }
+  __syncwarp();        // the stage is written again for the next columns
 }
 
 // Where things are in shared memory.  Every role makes its own from an address that the compiler cannot see through (see
@@ -624,16 +640,39 @@ flash_window_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
           if (!ok) break;
           tc_fence_after();
           if (lane < rows) p.f.lse[li] = lse_out;
+          auto o_read = [&]() {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.o_free[tile]);
+          };
+          if (p.f.out_dtype != 0) {
+            // bf16: 64 columns at a time, rounded as they are read, so that the next block's products do not wait long for O.  (A block of
+            // 25 steps, D = 64 and 128: 35.5 and 54.5 us; 36.6 and 54.8 with 32 fp32 columns staged at a time, 36.5 and 56.0 with
+            // every lane storing its row from registers.)
+            uint16_t* dst = static_cast<uint16_t*>(p.f.out) + tok0 * p.f.out_tok_stride + col;
+#pragma unroll 1
+            for (int x = 0; x < D / 64; ++x) {
+              uint32_t orow[32];
+#pragma unroll
+              for (int q = 0; q < 2; ++q) {
+                uint32_t v[32];
+                tmem_ld32(o_taddr + x * 64 + q * 32, v);
+                tmem_wait_ld<32>(v);
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                  orow[q * 16 + i] = pack_bf16x2(__uint_as_float(v[2 * i]) * w_new, __uint_as_float(v[2 * i + 1]) * w_new);
+              }
+              if (x == D / 64 - 1) o_read();
+              if (rows > 0) store_rows64_bf16(stage, dst + x * 64, p.f.out_tok_stride, rows, orow);
+            }
+            continue;
+          }
 #pragma unroll
           for (int q = 0; q < D / 32; ++q) {
             uint32_t orow[32];
             tmem_ld32(o_taddr + q * 32, orow);
             tmem_wait_ld<32>(orow);
-            if (q == D / 32 - 1) {
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&sh.o_free[tile]);
-            }
+            if (q == D / 32 - 1) o_read();
             OldRows old;
             if (accumulate) load_old_rows32(p.f, tok0, rows, col + q * 32, old);
             if (rows > 0) store_rows32(p.f, stage, tok0, rows, col + q * 32, orow, old, w_new, w_old);
@@ -748,7 +787,8 @@ flash_window_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
               m = m_new;
             }
           }
-          // p = 2^(s*c - m*c), at most 2^8; 0 for what is hidden, also while m is -inf
+          // p = 2^(s*c - m*c), at most 2^8; 0 for what is hidden, also while m is -inf.  (All on the ex2 unit: with one pair of eight on
+          // the FMA units, which the kernels without masks gain from, a block of 25 steps took 36.6 us in place of 35.9.)
           const float ref = m == -INFINITY ? 0.f : -m * c;
           const uint64_t c2 = pack2(c, c), nmc2 = pack2(ref, ref);
           uint64_t sum0 = pack2(0.f, 0.f), sum1 = sum0;
@@ -756,7 +796,7 @@ flash_window_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
 #pragma unroll
             for (int i = i0; i < i1; i += 2) {
               const uint64_t x = fma2(pack2(__uint_as_float(sr[i]), __uint_as_float(sr[i + 1])), c2, nmc2);
-              const uint64_t pp = ((i >> 1) & 7) >= 8 - kPolyPairs ? exp2_poly2(x) : exp2_mufu2(x);
+              const uint64_t pp = exp2_mufu2(x);
               if (i & 2) sum1 = add2(sum1, pp); else sum0 = add2(sum0, pp);
               float p0, p1;
               unpack2(pp, p0, p1);
