@@ -421,23 +421,60 @@ DTB_API int dtb_flash_fwd_ex(const void* q, const void* k, const void* v,
                         head_dim, softmax_scale, launch_flags, stream);
 }
 
-// Which launches take the kernel of 128-row tiles: those that it is expected to finish sooner.  It needs a whole walk over the keys of
-// a block of 256 rows for each round of blocks over the SMs, however few there are; the other kernel's time goes with its tiles of
-// 16 rows x 16 keys, spread over all SMs.  Rates as measured, us of (tiles of 16, tiles of 128), one forced after the other:
-//   queries                              16            64            128           256           512
-//   24 heads of 128, window 4096    15.1 / 65.5   36.3 / 66.2   65.2 / 66.4    106 / 67.7    189 / 68.3
-//   24 heads of 128, window 512      9.2 / 17.4   11.8 / 17.8   16.5 / 18.0   26.7 / 19.4   46.2 / 19.6
-//   2 x 48 of 64, window 2700       17.1 / 40.0   40.9 / 41.2   73.8 / 42.9    130 / 44.3    241 / 86.4
-//   4 x 32 over 8 of 64, 1000       10.3 / 20.3   24.9 / 21.6   40.6 / 21.9   76.0 / 22.9    146 / 44.0
-//   4 heads of 64, window 700        5.8 / 16.2    6.5 / 16.2    6.8 / 17.9    7.4 / 18.6    9.1 / 18.8
-static bool takes_window_tiles(const dtb::WindowParams& p, int head_dim, int sm_count) {
-  const int64_t group = p.f.num_heads / p.kv_heads, span = std::min<int64_t>(p.f.seqlen_k, static_cast<int64_t>(p.left) + p.right + p.sinks);
-  const double small_tiles = static_cast<double>((p.f.seqlen_q * group + 15) / 16 * p.kv_heads * p.f.nseg) * ((span + 31) / 16);
-  const double rows_us = 5. + small_tiles / (sm_count * (head_dim == 64 ? 12.8 : 7.2));
-  const int64_t blocks = (p.f.seqlen_q + 255) / 256 * static_cast<int64_t>(p.f.num_heads) * p.f.nseg;
-  const int64_t steps = (std::min<int64_t>(p.f.seqlen_k, span + std::min(p.f.seqlen_q, 128)) + 127) / 128;
-  const double tiles_us = static_cast<double>((blocks + sm_count - 1) / sm_count) * (8. + steps * (head_dim == 64 ? 1.3 : 1.75));
-  return tiles_us < rows_us;
+// Which kernel a launch takes, and the parts that the tiles of 128 split their keys into: what is expected to finish first.  Tiles of 128
+// need a walk over the keys of a block of 256 rows for each round of blocks over the SMs, however few there are; parts shorten it where
+// blocks leave SMs idle, for a merge behind them and states in fp32 (all parts run at once: more than a part per idle SM gained
+// nothing, e.g. 24 heads of 64 with 1024 rows 57.1 us whole, 56.6 in three).  Tiles of 16 rows x 16 keys are spread over all SMs.
+// Packed batches are not split: rows behind the last sequence have no state that a merge could leave alone.
+// us in tiles of 16 / of 128 whole / in the best number of parts, each forced:
+//   queries                            32                 64                 256                512                 1024
+//   24 heads of 128, window 4096  22.0/66.1/26.3(6)  35.9/66.1/26.3(6)   106/67.7/31(6)      189/68.3/54(2)        -/68.9/-
+//   24 heads of 128, window 512    9.9/18.8/17.0(4)  12.2/19.1/17.5(4)  27.1/20.5/22.7(4)  46.3/21.4/27.1(2)  84.3/22.1/42.1(2)
+//   24 heads of 64, window 4096   14.3/54.4/22.4(6)  22.7/54.3/22.8(6)  56.4/55.4/25.5(6)   105/56.6/34.4(3)   185/57.1/56.6(3)
+//   2 x 48 of 64, window 2700     29.4/41.0/39.9(3)  40.9/41.2/41.3(3)   130/45.0/50.7(3)   241/80.4/86.0(3)   473/118/157(2)
+//   32 over 8 of 128, window 4096 22.2/68.6/30.6(4)  36.4/68.9/31.0(4)   127/70.6/36.5(4)   226/71.1/54.2(2)   436/72.4/95.6(2)
+//   4 x 32 over 8 of 64, 1000     15.0/23.1/31.6(2)  25.0/23.2/32.6(2)  75.5/24.5/41.9(2)   146/41.5/70.3(2)   285/73.2/119(2)
+//   8 over 1 of 128, window 8192  21.7/ 124/30.2(8)  22.3/ 124/30.3(8)  63.2/ 126/33.9(8)   120/ 126/36.1(8)   236/132/50.6(4)
+//   4 heads of 64, window 700      5.7/16.9/13.9(8)   6.4/16.7/14.5(8)   7.4/19.7/18.3(4)   9.0/19.9/18.4(4)  12.6/19.9/18.9(4)
+//   4 heads of 128, window 2000    8.6/37.3/18.3(6)  11.3/39.4/18.9(8)  15.2/41.2/24.1(6)  22.3/41.3/24.0(6)  37.3/41.7/25.6(6)
+struct WindowPlan {
+  int splits;               // 0: tiles of 16 rows; else tiles of 128 over the keys in that many parts
+  int64_t scratch_bytes;    // for more than one part
+};
+static WindowPlan plan_window(int64_t nseg, int64_t seqlen_q, int64_t seqlen_k, int64_t num_heads, int64_t kv_heads, int head_dim,
+                              int64_t left, int64_t right, int64_t sinks, int sm_count, bool may_split) {
+  const int64_t group = num_heads / kv_heads, span = std::min(seqlen_k, left + right + sinks);
+  const double small_tiles = static_cast<double>((seqlen_q * group + 15) / 16 * kv_heads * nseg) * ((span + 31) / 16);
+  double best = 5. + small_tiles / (sm_count * (head_dim == 64 ? 12.8 : 7.2));
+  WindowPlan plan = {0, 0};
+  const int64_t blocks = (seqlen_q + 255) / 256 * num_heads * nseg, rows = nseg * seqlen_q * num_heads;
+  const int64_t steps = (std::min(seqlen_k, span + std::min<int64_t>(seqlen_q, 128)) + 127) / 128;
+  const double start = head_dim == 64 ? 6. : 4., block = head_dim == 64 ? 5. : 4., step = head_dim == 64 ? 1.32 : 1.8;
+  for (int64_t s = 1; s < dtb::kMergeMaxStates; ++s) {
+    double us = start + static_cast<double>((blocks * s + sm_count - 1) / sm_count) * (block + (steps + s - 1) / s * step);
+    if (s > 1) {
+      if (!may_split || seqlen_q <= 16 || s > steps || blocks * s > sm_count || nseg * s > 65535 || s * nseg * seqlen_q >= (1ll << 31)) break;
+      us += 5. + 4. * std::min<int64_t>(seqlen_q, 256) / 256. + static_cast<double>(s * rows * head_dim) * 4. / 5e6;
+    }
+    if (us < best) {
+      best = us;
+      plan.splits = static_cast<int>(s);
+      plan.scratch_bytes = s > 1 ? s * rows * (head_dim + 1) * 4 : 0;
+    }
+  }
+  return plan;
+}
+
+DTB_API int64_t dtb_flash_window_scratch_bytes(int nseg, int seqlen_q, int seqlen_k, int num_heads, int num_kv_heads, int head_dim,
+                                               int left, int right, int sinks) {
+  if (nseg < 1 || seqlen_q < 0 || seqlen_k < 0 || num_heads < 1 || num_kv_heads < 1 || num_heads % num_kv_heads || (head_dim != 64 && head_dim != 128))
+    return fail(DTB_ERR_ARG, "dtb_flash_window_scratch_bytes: bad shape");
+  if (left < -1 || right < -1 || sinks < 0) return fail(DTB_ERR_ARG, "dtb_flash_window_scratch_bytes: window (%d, %d) or sinks %d out of range", left, right, sinks);
+  DeviceInfo* d = nullptr;
+  int rc = device_info(&d);
+  if (rc != DTB_OK) return rc;
+  return plan_window(nseg, seqlen_q, seqlen_k, num_heads, num_kv_heads, head_dim, left < 0 ? seqlen_k : left, right < 0 ? seqlen_k : right, sinks,
+                     d->sm_count, true).scratch_bytes;
 }
 
 DTB_API int dtb_flash_window(const void* q, const void* k, const void* v,
@@ -447,7 +484,8 @@ DTB_API int dtb_flash_window(const void* q, const void* k, const void* v,
                      const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, const int32_t* seqlens_k,
                      int nseg, int seqlen_q, int seqlen_k, int64_t total_q, int64_t total_k,
                      int num_heads, int num_kv_heads, int head_dim, float softmax_scale,
-                     int left, int right, int sinks, int q_start, int k_start, void* stream) {
+                     int left, int right, int sinks, int q_start, int k_start,
+                     void* scratch, int64_t scratch_bytes, void* stream) {
   constexpr int kFar = 1 << 30;
   static_assert(DTB_QUERIES_LAST == dtb::kQueriesLast, "q_start");
   if (!q || !k || !v || !out || !lse) return fail(DTB_ERR_ARG, "dtb_flash_window: null tensor pointer");
@@ -470,6 +508,7 @@ DTB_API int dtb_flash_window(const void* q, const void* k, const void* v,
     return fail(DTB_ERR_ARG, "dtb_flash_window: batch stride smaller than the heads");
   if ((q_tok_stride | q_batch_stride | k_tok_stride | k_batch_stride | v_tok_stride | v_batch_stride) & 7) return fail(DTB_ERR_ARG, "dtb_flash_window: strides must be multiples of 8 elements");
   if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out)) return fail(DTB_ERR_ARG, "dtb_flash_window: tensor pointers must be 16-byte aligned");
+  if (!aligned16(scratch)) return fail(DTB_ERR_ARG, "dtb_flash_window: scratch must be 16-byte aligned");
   if (out_dtype != DTB_F32 && out_dtype != DTB_BF16) return fail(DTB_ERR_ARG, "dtb_flash_window: bad out_dtype %d", out_dtype);
   if (lse_layout != DTB_LSE_BHS && lse_layout != DTB_LSE_BSH) return fail(DTB_ERR_ARG, "dtb_flash_window: bad lse_layout %d", lse_layout);
   if (accumulate && out_dtype != DTB_F32) return fail(DTB_ERR_ARG, "dtb_flash_window: accumulate needs an fp32 state");
@@ -514,7 +553,41 @@ DTB_API int dtb_flash_window(const void* q, const void* k, const void* v,
   p.k_start = k_start;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e;
-  if (takes_window_tiles(p, head_dim, d->sm_count)) {
+  const WindowPlan plan = plan_window(nseg, seqlen_q, seqlen_k, num_heads, num_kv_heads, head_dim, left < 0 ? seqlen_k : left,
+                                      right < 0 ? seqlen_k : right, sinks, d->sm_count, scratch != nullptr && cu_seqlens_q == nullptr);
+  if (scratch_bytes < plan.scratch_bytes)
+    return fail(DTB_ERR_ARG, "dtb_flash_window: scratch of %lld bytes is smaller than the %lld needed", static_cast<long long>(scratch_bytes),
+                static_cast<long long>(plan.scratch_bytes));
+  if (plan.splits > 0) {
+    dtb::MergeParams m;
+    if (plan.splits > 1) {
+      // the parts' states in scratch, merged with the state that is there into the result
+      const int64_t rows = total_q * num_heads;
+      float* parts = static_cast<float*>(scratch);
+      memset(&m, 0, sizeof(m));
+      auto add = [&](const void* o, const float* l, int layout) {
+        m.outs[m.nstates] = o;
+        m.lse[m.nstates] = l;
+        m.out_dtype[m.nstates] = DTB_F32;
+        m.lse_layout[m.nstates++] = layout;
+      };
+      if (accumulate) add(out, lse, lse_layout);
+      for (int i = 0; i < plan.splits; ++i) add(parts + i * rows * head_dim, parts + plan.splits * rows * head_dim + i * rows, DTB_LSE_BSH);
+      m.out = out_dtype == DTB_F32 ? static_cast<float*>(out) : nullptr;
+      m.out_bf16 = out_dtype == DTB_BF16 ? static_cast<uint16_t*>(out) : nullptr;
+      m.lse_out = lse;
+      m.lse_out_layout = lse_layout;
+      m.rows = rows;
+      m.H = num_heads;
+      m.S = seqlen_q;
+      m.status = d->status_ptr;
+      p.f.out = parts;
+      p.f.lse = parts + plan.splits * rows * head_dim;
+      p.f.out_dtype = DTB_F32;
+      p.f.lse_layout = DTB_LSE_BSH;
+      p.f.accumulate = 0;
+    }
+    p.splits = plan.splits;
     if ((rc = load_encoder()) != DTB_OK) return rc;
     const bool packed = cu_seqlens_q != nullptr;
     const int64_t q_tokens = packed ? total_q : seqlen_q, k_tokens = packed ? total_k : seqlen_k, batch = packed ? 1 : nseg;
@@ -525,6 +598,7 @@ DTB_API int dtb_flash_window(const void* q, const void* k, const void* v,
         (rc = make_token_map(&tv, v, k_width, std::max<int64_t>(k_tokens, 1), v_tok_stride, batch, v_batch_stride, &p.v_batch_first, "v")) != DTB_OK)
       return rc;
     e = head_dim == 64 ? dtb::launch_window_tiles<64>(tq, tk, tv, p, s) : dtb::launch_window_tiles<128>(tq, tk, tv, p, s);
+    if (e == cudaSuccess && plan.splits > 1) e = dtb::launch_merge(m, head_dim, d->sm_count, s);
   } else {
     e = head_dim == 64 ? dtb::launch_window_rows<64>(p, d->sm_count, s) : dtb::launch_window_rows<128>(p, d->sm_count, s);
   }

@@ -23,6 +23,9 @@ struct WindowParams {
   int q_start, k_start;          // positions of the first query (or kQueriesLast) and the first key
   // the order of a tensor map's outer axes, the one with the smaller stride first: 1 batch then token, 0 token then batch
   int q_batch_first, k_batch_first, v_batch_first;
+  // Parts that the keys of a block of 256 rows are split into, each attended like a block of its own.  With more than one, f.out and
+  // f.lse (fp32, [B,S,H]) hold the parts' states one after another, f.total_q tokens each, for a merge.
+  int splits;
 };
 
 // A sequence: where its queries and keys begin among the tokens, how many there are, and which keys its first query sees: [0, sinks) as
@@ -66,14 +69,15 @@ struct WindowSpan {
   int first, lo, hi;
 };
 
-__device__ __forceinline__ WindowSpan window_span(int from, int to, int sinks, int k_len, int i) {
+// `k_end`: no key from there on; `k_floor`: the window holds no key before it (sinks, or more where a block's keys are split).
+__device__ __forceinline__ WindowSpan window_span(int from, int to, int sinks, int k_end, int k_floor, int i) {
   WindowSpan w;
-  w.hi = min(max(to + i, 0), k_len);
+  w.hi = min(max(to + i, 0), k_end);
   w.first = min(sinks, w.hi);
-  w.lo = max(min(max(from + i, sinks), w.hi), w.first);
+  w.lo = max(min(max(from + i, k_floor), w.hi), w.first);
   return w;
 }
-__device__ __forceinline__ WindowSpan window_span(const WindowSeq& s, int i) { return window_span(s.from, s.to, s.sinks, s.k_len, i); }
+__device__ __forceinline__ WindowSpan window_span(const WindowSeq& s, int i) { return window_span(s.from, s.to, s.sinks, s.k_len, s.sinks, i); }
 
 // Element offset of a sequence's token in a q / k / v tensor (dense: token inside its sequence; packed: of the whole tensor).
 __device__ __forceinline__ int64_t window_offset(const WindowParams& p, int seg, int64_t tok, int64_t tok_stride, int64_t batch_stride) {

@@ -6,7 +6,7 @@
 // Warp roles (512 threads, four warpgroups):
 //   warps 0-7    softmax, a warpgroup per Q tile; a finished row leaves its reference and sum in shared memory
 //   warps 8-11   results: O out of tensor memory, normalisation, merge with the state in global memory, stores
-//   warp  12     blocks, their plans, TMA loads
+//   warp  12     blocks, their plans, TMA loads; the results of blocks that see no key
 //   warp  13     MMA issuer
 //   warps 14-15  no role
 //
@@ -23,10 +23,13 @@
 // PV runs the steps of 16 keys that hold one, and the rows behind the last key, which may hold anything, are cleared in shared memory
 // by the thread that loads them, which waits for that one load.
 //
-// Blocks are short (a window of 2700 keys: 25 steps, 32 us), so what happens once per block counts.  The next block's plan is made, its
+// Blocks are short (a window of 2700 keys: 25 steps, 36 us at D = 64), so what happens once per block counts.  The next block's plan is made, its
 // queries and first keys loaded and its first scores computed while the softmax warps finish the block before it, and results leave by
 // warps of their own.  The grid has a CTA per block, as if all were to run; CTAs claim further blocks by cluster launch control.  Every
 // phase of a barrier is over for all that look at it before the next one can complete; see flash_fwd_persistent_sm100.cu.
+//
+// With few blocks their keys are split into parts of as many tiles each, which are attended like blocks of their own and merged by the
+// state merge's kernel behind this one (24 heads of 128, 64 queries, window 4096: 66 -> 26 us in six parts).
 #include "flash_common.cuh"
 #include "flash_window.cuh"
 
@@ -66,7 +69,7 @@ struct Cfg {
   // barriers: q_full[QB][2], q_empty[QB], kv_full[S], kv_empty[S], s_full[NB], p_lo[NB], p_hi[NB], pv_done[2], o_final[2],
   // o_free[2], ml_full[2], ml_empty[2], work_full[W], work_empty[W], v_tail[T], claim
   static constexpr int kBars = 3 * kQBufs + 2 * kStages + 3 * kSBufs + 10 + 2 * kWork + kTails + 1;
-  static constexpr int kSmemBytes = 1024 + (kQBufs * kQT + kStages) * kTileBytes + kStageOut + kQT * kBM * 8 + kWork * 64 + 16 +
+  static constexpr int kSmemBytes = 1024 + (kQBufs * kQT + kStages) * kTileBytes + kStageOut + kQT * kBM * 8 + kWork * 64 + D * 4 + 16 +
                                     kBars * 8 + 16;
   static constexpr uint32_t kTmemCols = 512;
   static constexpr uint32_t kColS = 0;                    // + buffer * 128
@@ -81,18 +84,19 @@ struct Walk {
   int lo, win;        // the window's first key and length
   int first;          // first tokens
   int N, n;           // tiles of the window, window steps of a Q tile: N, or N - 1 where Q tile 1 is a tile ahead
-  int steps;          // steps in all; 0: nothing to see, -1: no more blocks
+  int steps;          // steps in all; 0: nothing to see (such a block only the loader meets), -1: no more blocks
 
   // for the rows i0 to i1
-  __device__ __forceinline__ void plan(const WindowSeq& s, int i0, int i1) {
-    const WindowSpan a = window_span(s, i0), z = window_span(s, i1);
+  __device__ __forceinline__ void plan(int from, int to, int sinks, int k_end, int k_floor, int i0, int i1) {
+    auto span = [&](int i) { return window_span(from, to, sinks, k_end, k_floor, i); };
+    const WindowSpan a = span(i0), z = span(i1);
     first = z.first;
-    lo = max(a.lo, first);
+    lo = max(a.lo, min(k_floor, z.hi));
     win = max(z.hi - lo, 0);
     N = (win + kBN - 1) / kBN;
     n = N;
     if (i1 - i0 >= kBM && N >= 2) {
-      const WindowSpan last_of_0 = window_span(s, i0 + kBM - 1), first_of_1 = window_span(s, i0 + kBM);
+      const WindowSpan last_of_0 = span(i0 + kBM - 1), first_of_1 = span(i0 + kBM);
       if (first_of_1.lo >= lo + kBN && last_of_0.hi <= lo + kBN * (N - 1)) n = N - 1;
     }
     steps = n + (first + kBN - 1) / kBN;
@@ -112,8 +116,8 @@ struct Item {
   Walk walk;
   int q0, head, seg;
   int q_begin, q_len;            // where its sequence begins in the results, and its length
-  int from, to, sinks, k_len;    // of its sequence, see WindowSeq
-  int unused;
+  int from, to, sinks;           // of its sequence, see WindowSeq
+  int k_end, k_floor;            // see window_span
 };
 static_assert(sizeof(Item) == 64, "shared-memory layout");
 
@@ -142,6 +146,21 @@ __device__ __forceinline__ void store_rows64_bf16(uint8_t* stage, uint16_t* dst,
   __syncwarp();        // the stage is written again for the next columns
 }
 
+// The results of a block that sees no key, by one thread: empty states (out = 0, lse = -inf).  A state that it were folded into stays
+// as it is.
+template <int D>
+__device__ __forceinline__ void write_none(const FlashParams& p, const Item& w, const uint8_t* zeros) {
+  if (p.accumulate) return;
+  const int size = p.out_dtype == 0 ? 4 : 2;
+#pragma unroll 1
+  for (int i = w.q0; i < min(w.q0 + kQT * kBM, w.q_len); ++i) {
+    const int64_t tok = static_cast<int64_t>(w.q_begin) + i;
+    p.lse[lse_index(p, w.seg, w.head, i, tok)] = -INFINITY;
+    bulk_store(static_cast<uint8_t*>(p.out) + (tok * p.out_tok_stride + w.head * D) * size, zeros, D * size);
+  }
+  bulk_store_commit();
+}
+
 // Where things are in shared memory.  Every role makes its own from an address that the compiler cannot see through (see
 // flash_fwd_persistent_sm100.cu).
 template <int D>
@@ -152,6 +171,7 @@ struct Shared {
   uint8_t* s_out;
   float2* s_ml;           // [tile][row]: reference and sum of a finished row
   Item* s_work;
+  uint8_t* s_zero;        // a row of zeros
   uint8_t* s_claim;
   uint64_t* q_full;       // [block buffer][tile]
   uint64_t* q_empty;      // [block buffer]: the block's last S has read both tiles
@@ -177,7 +197,8 @@ struct Shared {
     s_out = s_kv + C::kStages * C::kTileBytes;
     s_ml = reinterpret_cast<float2*>(s_out + C::kStageOut);
     s_work = reinterpret_cast<Item*>(s_ml + kQT * kBM);
-    s_claim = reinterpret_cast<uint8_t*>(s_work + kWork);
+    s_zero = reinterpret_cast<uint8_t*>(s_work + kWork);
+    s_claim = s_zero + D * 4;
     q_full = reinterpret_cast<uint64_t*>(s_claim + 16);
     q_empty = q_full + 2 * C::kQBufs;
     kv_full = q_empty + C::kQBufs;
@@ -227,7 +248,7 @@ __device__ __forceinline__ bool claim_answer(const void* response16, int& x, int
 
 }  // namespace
 
-// grid: (row blocks, heads, sequences)
+// grid: (row blocks, heads, sequences x parts)
 template <int D>
 __global__ void __launch_bounds__(kThreads, 1)
 flash_window_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
@@ -272,6 +293,10 @@ flash_window_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     for (int i = 0; i < kTails; ++i) mbar_init(&sh.v_tail[i], 1);
     mbar_init(sh.claim, 1);
     fence_mbar_init();
+  }
+  if (warp == kMmaWarp + 1 && lane < D / 4) {
+    reinterpret_cast<uint4*>(sh.s_zero)[lane] = make_uint4(0u, 0u, 0u, 0u);
+    fence_proxy_async_smem();
   }
   if (warp == kMmaWarp) {
     tmem_alloc(sh.tmem_slot, C::kTmemCols);
@@ -335,27 +360,44 @@ flash_window_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         };
         for (;;) {
           Item w;
+          const int seg = bz / p.splits, part = bz % p.splits;
           w.head = by;
-          w.seg = bz;
+          w.seg = seg;
           w.q0 = bx * (kQT * kBM);
-          w.unused = 0;
-          const WindowSeq s = window_seq(p, bz);
-          w.q_begin = p.f.cu_q != nullptr ? s.q_begin : bz * p.f.seqlen_q;
+          const WindowSeq s = window_seq(p, seg);
+          w.q_begin = p.f.cu_q != nullptr ? s.q_begin : seg * p.f.seqlen_q + part * static_cast<int>(p.f.total_q);
           w.q_len = s.q_len;
           w.from = s.from;
           w.to = s.to;
           w.sinks = s.sinks;
-          w.k_len = s.k_len;
+          w.k_end = s.k_len;
+          w.k_floor = s.sinks;
           asked = false;
           if (w.q0 < w.q_len) {
-            w.walk.plan(s, w.q0, min(w.q0 + kQT * kBM, w.q_len) - 1);
-            if (!publish(w)) break;
+            const int i1 = min(w.q0 + kQT * kBM, w.q_len) - 1;
+            w.walk.plan(w.from, w.to, w.sinks, w.k_end, w.k_floor, w.q0, i1);
+            if (p.splits > 1) {
+              // as many tiles to each part, the first tokens to the last one
+              const int begin = w.walk.lo, end = begin + w.walk.win;
+              const int keys = (w.walk.N + (w.walk.first + kBN - 1) / kBN + p.splits - 1) / p.splits * kBN;
+              w.k_floor = min(begin + part * keys, end);
+              if (part + 1 < p.splits) {
+                w.k_end = min(w.k_floor + keys, end);
+                w.sinks = 0;
+              }
+              w.walk.plan(w.from, w.to, w.sinks, w.k_end, w.k_floor, w.q0, i1);
+            }
             const Walk walk = w.walk;
             const int n_units = 2 * walk.steps;
-            if (n_units > 0) {
+            if (n_units == 0) {
+              // The other roles do not meet it.  (The issuer asks for the block behind the one under way before it ends that one: with
+              // a run of such blocks in between, more than there are slots, each role would wait for another.)
+              write_none<D>(p.f, w, sh.s_zero);
+            } else {
+              if (!publish(w)) break;
               const int qb = items % C::kQBufs, q_round = items / C::kQBufs;
               const int kv_head = by / (p.f.num_heads / p.kv_heads);
-              const int batch = p.f.cu_q != nullptr ? 0 : bz;
+              const int batch = p.f.cu_q != nullptr ? 0 : seg;
               int k_tile = -1, v_tile = -1;
               auto load_kv = [&](const CUtensorMap* tm, int tile, int batch_first) {
                 const int stage = it % C::kStages;
@@ -420,6 +462,7 @@ flash_window_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
             break;
           }
         }
+        bulk_store_wait();               // the zeros have been read
       }
       __syncwarp();
     } else {
@@ -468,14 +511,12 @@ flash_window_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         Walk ahead;                // of the block whose S are issued; PV's may still be a block behind
         int ahead_units = 0;
         auto next_item = [&]() {
-          for (;;) {
-            const int slot = fetch(sh);
-            if (slot < 0) return false;
-            ahead = sh.s_work[slot].walk;
-            mbar_arrive(&sh.work_empty[slot]);
-            ahead_units = 2 * ahead.steps;
-            if (ahead_units > 0) return true;
-          }
+          const int slot = fetch(sh);
+          if (slot < 0) return false;
+          ahead = sh.s_work[slot].walk;
+          mbar_arrive(&sh.work_empty[slot]);
+          ahead_units = 2 * ahead.steps;
+          return true;
         };
         int k_stage = 0, v_stage = 0, tails = 0;
         int q_tile = 0;            // of the block ahead: its first tile in s_q, ...
@@ -608,15 +649,9 @@ flash_window_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       const bool accumulate = p.f.accumulate != 0;
       uint32_t item_use = 0;
       for (int slot; (slot = fetch_warp(sh)) >= 0;) {
-        const int steps = sh.s_work[slot].walk.steps, q0 = sh.s_work[slot].q0, head = sh.s_work[slot].head, seg = sh.s_work[slot].seg;
+        const int q0 = sh.s_work[slot].q0, head = sh.s_work[slot].head, seg = sh.s_work[slot].seg;
         const int q_begin = sh.s_work[slot].q_begin, q_len = sh.s_work[slot].q_len;
         give_back(sh, slot);
-        if (steps == 0) {
-          if (!accumulate)
-            for (int r = static_cast<int>(threadIdx.x) - kOutWarp * 32; r < kQT * kBM; r += 128)
-              write_empty_row<D>(p.f, seg, head, q_begin, q_len, q0 + r);
-          continue;
-        }
         bool ok = true;
 #pragma unroll 1
         for (int tile = 0; ok && tile < kQT; ++tile) {
@@ -695,7 +730,7 @@ flash_window_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       int buf = tile;            // S / P buffer of the next key tile
       uint32_t use = 0;          // parity of its barriers
       uint32_t pv_use = 1;       // parity of PV of the key tile before
-      uint32_t items = 0;
+      uint32_t ml_use = 2;        // parity of the reads of the rows before; 2: there are none
       bool ok = true;
       for (int slot; ok && (slot = fetch_warp(sh)) >= 0;) {
         // The columns of a step's tile that the row sees, [c0, c1); both move on by a tile a step, and at the first tokens, `window`
@@ -706,14 +741,13 @@ flash_window_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
           left = w.walk.steps;
           window = w.walk.n;
           // (a row behind the last one sees what the last one sees)
-          const WindowSpan span = window_span(w.from, w.to, w.sinks, w.k_len, min(w.q0 + tile * kBM + quarter * 32 + lane, w.q_len - 1));
+          const WindowSpan span = window_span(w.from, w.to, w.sinks, w.k_end, w.k_floor, min(w.q0 + tile * kBM + quarter * 32 + lane, w.q_len - 1));
           const int base = w.walk.lo + ((w.walk.N - window) & tile) * kBN;
           c0 = span.lo - base;
           c1 = span.hi - base;
           first = span.first;
         }
         give_back(sh, slot);
-        if (left == 0) continue;
         float m = -INFINITY;     // running max of raw scores (lazily updated); -inf: the row has seen no key yet
         float l = 0.f;           // running sum of exp2((s - m) * c)
         bool begun = false;
@@ -824,12 +858,12 @@ flash_window_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
           if (buf >= NB) { buf -= NB; use ^= 1; }
         }
         if (!ok) break;
-        if (items > 0) ok = warp_wait_or_abort(&sh.ml_empty[tile], (items - 1) & 1, p.f.status, 43);
+        if (ml_use < 2) ok = warp_wait_or_abort(&sh.ml_empty[tile], ml_use, p.f.status, 43);
         if (!ok) break;          // the rows before these have not been read
         sh.s_ml[tile * kBM + quarter * 32 + lane] = make_float2(m, l);
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.ml_full[tile]);
-        ++items;
+        ml_use = (ml_use & 1) ^ (ml_use < 2);
       }
     }
   }
@@ -864,7 +898,7 @@ cudaError_t launch_window_tiles(const CUtensorMap& tq, const CUtensorMap& tk, co
       configured[dev & 63] = true;
     }
   }
-  const dim3 grid((p.f.seqlen_q + kQT * kBM - 1) / (kQT * kBM), p.f.num_heads, p.f.nseg);
+  const dim3 grid((p.f.seqlen_q + kQT * kBM - 1) / (kQT * kBM), p.f.num_heads, p.f.nseg * p.splits);
   flash_window_kernel<D><<<grid, kThreads, C::kSmemBytes, stream>>>(tq, tk, tv, p);
   return cudaGetLastError();
 }

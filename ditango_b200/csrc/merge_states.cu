@@ -68,6 +68,7 @@ __global__ void __launch_bounds__(128) merge_states_kernel(const MergeParams p) 
   const int group_in_warp = (threadIdx.x % 32) / G;
   const unsigned full = 0xffffffffu;
   const int n = p.nstates;
+  if (p.status != nullptr && *reinterpret_cast<const volatile int*>(p.status) != 0) return;
 
   auto load_chunk = [&](int c0, int64_t base, Raw8 (&v)[CH][U]) {
 #pragma unroll

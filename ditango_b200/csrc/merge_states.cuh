@@ -20,6 +20,7 @@ struct MergeParams {
   int nstates;
   int H;
   int S;
+  const int* status;                    // null, or a status word: with it set nothing is written
 };
 
 struct CopyParams {

@@ -287,20 +287,28 @@ def flash_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, left: int
         return out, lse
     # (an empty tensor has no address, and nothing is read)
     keys, values = k.data_ptr() or q.data_ptr(), v.data_ptr() or q.data_ptr()
+    lib = _capi.load()
+    scratch, scratch_bytes = None, 0
+    if not packed and sq > 16:         # (fewer queries never have their keys split)
+        scratch_bytes = lib.dtb_flash_window_scratch_bytes(nseg, sq, sk, H, Hk, D, left, right, sinks)
+        if scratch_bytes < 0:
+            _capi.check(scratch_bytes, "dtb_flash_window_scratch_bytes")
+        if scratch_bytes:
+            scratch = _empty((scratch_bytes,), torch.uint8, q.device)
     ev = None
     if LaunchLog.events is not None:
         ev = (torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True))
         ev[0].record()
-    rc = _capi.load().dtb_flash_window(
+    rc = lib.dtb_flash_window(
         q.data_ptr(), keys, values, *_strides(q, shape), *_strides(k, kshape), *_strides(v, kshape),
         out.data_ptr(), _VALUES[out.dtype], lse.data_ptr(), lse_layout, accumulate,
         cu_seqlens_q.data_ptr() if packed else None, cu_seqlens_k.data_ptr() if packed else None,
         None if seqlens_k is None else seqlens_k.data_ptr(), nseg, sq, sk, Tq, Tk, H, Hk, D,
         D ** -0.5 if softmax_scale is None else softmax_scale, left, right, sinks,
-        _capi.QUERIES_LAST if q_start is None else q_start, k_start, stream)
+        _capi.QUERIES_LAST if q_start is None else q_start, k_start, None if scratch is None else scratch.data_ptr(), scratch_bytes, stream)
     if rc:
         _capi.check(rc, "dtb_flash_window")
-    LaunchLog.count += 1
+    LaunchLog.count += 1 if scratch is None else 2
     if ev is not None:
         ev[1].record()
         span = sk if left < 0 or right < 0 else min(sk, left + right + 1 + sinks)      # upper bound of a row's keys

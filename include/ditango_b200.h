@@ -172,6 +172,8 @@ DTB_API int dtb_flash_fwd_ex(const void* q, const void* k, const void* v,
  *  seqlens_k      NULL, or device int32[nseg]: the keys of each sequence of a dense batch (at most seqlen_k; what the memory holds
  *                 behind them does not matter)
  *  left, right    keys visible before and behind the query's own position, -1 for all; sinks first positions
+ *  scratch        dtb_flash_window_scratch_bytes(...) bytes, 16-byte aligned, of one call at a time, for the states of parts that the keys
+ *                 are split into; 0 bytes where they are not.  NULL: they are not split.  (Packed batches never are.)
  * Keys and values that no query of a block of rows sees may hold anything; those that some see must be finite.
  */
 #define DTB_QUERIES_LAST (-2147483647 - 1)
@@ -182,7 +184,10 @@ DTB_API int dtb_flash_window(const void* q, const void* k, const void* v,
                      const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, const int32_t* seqlens_k,
                      int nseg, int seqlen_q, int seqlen_k, int64_t total_q, int64_t total_k,
                      int num_heads, int num_kv_heads, int head_dim, float softmax_scale,
-                     int left, int right, int sinks, int q_start, int k_start, void* stream);
+                     int left, int right, int sinks, int q_start, int k_start,
+                     void* scratch, int64_t scratch_bytes, void* stream);
+DTB_API int64_t dtb_flash_window_scratch_bytes(int nseg, int seqlen_q, int seqlen_k, int num_heads, int num_kv_heads, int head_dim,
+                                               int left, int right, int sinks);
 
 /*
  * N-way merge of partial softmax states in one pass over HBM:

@@ -264,3 +264,206 @@ def test_a_posted_status_keeps_results_from_being_written():
         assert (out == 3).all() and (lse == 3).all()
         ops.flash_window(q, k, k, left=100, right=0, out=out, lse=lse)
         assert not (out == 3).any()
+
+
+def _check_on_gpu(out, lse, q, k, v, b, *, left, right, sinks, at, heads, k_start=0):
+    """Some heads of one sequence against 64 bits on the device."""
+    group = q.shape[2] // k.shape[2]
+    seen = _visible(q.shape[1], k.shape[1], left, right, sinks, at, k_start)
+    for h in heads:
+        want = _exact(*(x.double() for x in (q[b, :, h:h + 1], k[b, :, h // group:h // group + 1], v[b, :, h // group:h // group + 1])), seen.cuda())
+        _check(out[b, :, h:h + 1], lse[b, :, h:h + 1], *(x.cpu() for x in want))
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("accumulate", [False, True])
+def test_many_blocks_of_rows_that_see_nothing(D, accumulate):
+    """Sequences without a key, one after another, between those that have some: more of their blocks than a CTA has blocks under way."""
+    from ditango_b200 import ops
+    B, Sq, Sk, H = 9, 600, 700, 40
+    q, k, v = (_rand((B, n, H, D), n + D).cuda() for n in (Sq, Sk, Sk))
+    v[:] = v.flip(1)
+    lens = [Sk, 0, 0, 0, 0, 0, 333, 0, 17]
+    sl = torch.tensor(lens, dtype=torch.int32).cuda()
+    out, lse = ops.flash_window(q, k, v, left=150, right=90, sinks=70, q_start=0, seqlens_k=sl, lse_layout=ops.LSE_BSH)
+    assert ops.read_status() == 0
+    if accumulate:
+        ops.flash_window(q, k, v, left=150, right=90, sinks=70, q_start=0, seqlens_k=sl, lse_layout=ops.LSE_BSH, out=out, lse=lse, accumulate=True)
+        lse -= math.log(2.0)                    # the same state twice
+    for b, n in enumerate(lens):
+        if n:
+            _check_on_gpu(out, lse, q, k[:, :n], v[:, :n], b, left=150, right=90, sinks=70, at=0, heads=(0, H - 1))
+        else:
+            assert (out[b] == 0).all() and (lse[b] == -math.inf).all()
+    assert ops.read_status() == 0
+
+
+# Launches large enough for the tiles of 128 rows, whole or with their keys split into parts (which takes scratch): B, Sq, Sk, H, Hk, window
+LARGE = {"whole": (1, 700, 1500, 32, 8, dict(left=500, right=60, sinks=30)), "parts": (1, 200, 4500, 24, 6, dict(left=4000, right=0, sinks=70)),
+         "two": (3, 300, 4500, 12, 12, dict(left=4100, right=130, sinks=140))}
+large = pytest.mark.parametrize("kind,D", [(kind, D) for kind in LARGE for D in (64, 128)])
+
+
+def _large(kind, D, seed=0):
+    B, Sq, Sk, H, Hk, window = LARGE[kind]
+    g = torch.Generator(device="cuda").manual_seed(seed + D)
+    return *(torch.randn(B, n, h, D, generator=g, device="cuda").to(torch.bfloat16) for n, h in ((Sq, H), (Sk, Hk), (Sk, Hk))), window
+
+
+def _heads(q):
+    return 0, 5, q.shape[2] - 1
+
+
+@large
+def test_only_launches_that_leave_sms_idle_are_split(kind, D):
+    from ditango_b200 import _capi
+    B, Sq, Sk, H, Hk, w = LARGE[kind]
+    lib = _capi.load()
+    size = lib.dtb_flash_window_scratch_bytes(B, Sq, Sk, H, Hk, D, w["left"], w["right"], w["sinks"])
+    state = B * Sq * H * (D + 1) * 4
+    assert size % state == 0 and (size >= 2 * state) == (kind != "whole")
+    assert lib.dtb_flash_window_scratch_bytes(B, 16, Sk, H, Hk, D, w["left"], w["right"], w["sinks"]) == 0
+
+
+@large
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shift", [0, -77, 9000])
+def test_large_launches_match_the_definition(kind, D, dtype, shift):
+    """At the end of their keys, a little before it, and far behind it, where only the first tokens are seen."""
+    from ditango_b200 import ops
+    q, k, v, w = _large(kind, D)
+    at = k.shape[1] - q.shape[1] + shift
+    out, lse = ops.flash_window(q, k, v, **w, q_start=at, out_dtype=dtype, lse_layout=ops.LSE_BSH)
+    out2, lse2 = ops.flash_window(q, k, v, **w, q_start=at, out_dtype=dtype)
+    assert torch.equal(out, out2) and torch.equal(lse, lse2.transpose(1, 2))
+    for b in range(q.shape[0]):
+        _check_on_gpu(out, lse, q, k, v, b, **w, at=at, heads=_heads(q))
+    assert ops.read_status() == 0
+
+
+@large
+def test_large_launches_of_different_lengths(kind, D):
+    from ditango_b200 import ops
+    q, k, v, w = _large(kind, D)
+    lens = [1, 999, 0] if len(q) == 3 else [999]
+    for b, n in enumerate(lens):
+        k[b, n:], v[b, n:] = math.nan, math.inf
+    out, lse = ops.flash_window(q, k, v, **w, seqlens_k=torch.tensor(lens, dtype=torch.int32).cuda(), lse_layout=ops.LSE_BSH)
+    for b, n in enumerate(lens):
+        _check_on_gpu(out, lse, q, k[:, :n], v[:, :n], b, **w, at=n - q.shape[1], heads=_heads(q))
+    assert ops.read_status() == 0
+
+
+@large
+def test_keys_that_no_large_launch_sees_may_hold_anything(kind, D):
+    from ditango_b200 import ops
+    q, k, v, w = _large(kind, D)
+    w = dict(w, left=w["left"] // 2)
+    at = 2 * k.shape[1] // 3 - q.shape[1]
+    seen = _visible(q.shape[1], k.shape[1], *w.values(), at, 0).any(0).cuda()
+    assert not seen.all()
+    k[:, ~seen], v[:, ~seen] = math.inf, math.nan
+    out, lse = ops.flash_window(q, k, v, **w, q_start=at, lse_layout=ops.LSE_BSH)
+    k[:, ~seen], v[:, ~seen] = 0, 0
+    _check_on_gpu(out, lse, q, k, v, 0, **w, at=at, heads=_heads(q))
+
+
+@large
+@pytest.mark.parametrize("layout", [0, 1])
+def test_large_chunks_folded_into_a_state_are_the_whole(kind, D, layout):
+    from ditango_b200 import ops
+    q, k, v, w = _large(kind, D)
+    at, cut = k.shape[1] - q.shape[1], k.shape[1] // 2 + 13
+    out, lse = ops.flash_window(q, k[:, :cut], v[:, :cut], **w, q_start=at, lse_layout=layout)
+    again = ops.flash_window(q, k[:, cut:], v[:, cut:], **w, q_start=at, k_start=cut, out=out, lse=lse, accumulate=True, lse_layout=layout)
+    assert again[0] is out and again[1] is lse
+    _check_on_gpu(out, lse if layout else lse.transpose(1, 2), q, k, v, 0, **w, at=at, heads=_heads(q))
+    before = out.clone(), lse.clone()
+    ops.flash_window(q, k, v, left=w["left"], right=w["right"], q_start=10 ** 6, out=out, lse=lse, accumulate=True, lse_layout=layout)
+    assert torch.equal(out, before[0]) and torch.equal(lse, before[1])
+    assert ops.read_status() == 0
+
+
+@large
+def test_large_launches_on_views_of_one_projection(kind, D):
+    """Queries and keys as slices of a tensor with other things beside them, batch or sequence first."""
+    from ditango_b200 import ops
+    q, k, v, w = _large(kind, D)
+    H, Hk, S = q.shape[2], k.shape[2], k.shape[1]
+    for first in (True, False):
+        x = torch.full((q.shape[0], S, H + 2 * Hk + 1, D) if first else (S, q.shape[0], H + 2 * Hk + 1, D), math.nan, dtype=torch.bfloat16, device="cuda")
+        y = x if first else x.transpose(0, 1)
+        views = y[:, S - q.shape[1]:, :H], y[:, :, H:H + Hk], y[:, :, H + Hk:H + 2 * Hk]
+        for to, of in zip(views, (q, k, v)):
+            to.copy_(of)
+        want, got = ops.flash_window(q, k, v, **w), ops.flash_window(*views, **w)
+        assert torch.equal(want[0], got[0]) and torch.equal(want[1], got[1])
+
+
+@large
+def test_large_launches_captured_twice_beside_others(kind, D):
+    """Graphs replayed at once on two streams have scratch of their own, and a launch between them too."""
+    from ditango_b200 import ops
+    (q, k, v, w), (q2, _, _, _) = _large(kind, D), _large(kind, D, seed=1)
+    queries = q.clone(), q2.clone()
+    want = [ops.flash_window(x, k, v, **w) for x in queries]
+    graphs = []
+    for x in queries:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            graphs.append((graph, ops.flash_window(x, k, v, **w), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for graph, _, stream in graphs:
+            with torch.cuda.stream(stream):
+                graph.replay()
+        between = ops.flash_window(q, k, v, **w)
+    torch.cuda.synchronize()
+    assert torch.equal(between[0], want[0][0])
+    for (_, got, _), x in zip(graphs, want):
+        assert torch.equal(got[0], x[0]) and torch.equal(got[1], x[1])
+
+
+@large
+def test_large_launches_after_a_failure_write_nothing(kind, D):
+    from ditango_b200 import ops
+    q, k, v, w = _large(kind, D)
+    out, lse = torch.full(q.shape, 3.0, device="cuda"), torch.full((q.shape[0], q.shape[2], q.shape[1]), 3.0, device="cuda")
+    try:
+        ops.post_status(77)
+        ops.flash_window(q, k, v, **w, out=out, lse=lse)
+    finally:
+        assert ops.read_status() == 77
+    assert (out == 3).all() and (lse == 3).all()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_large_packed_sequences(D):
+    from ditango_b200 import ops
+    q, k, v, w = _large("whole", D)
+    q, k, v = q[0], k[0], v[0]
+    qs, ks = [0, 300, 300, 301, 561, 690], [0, 300, 340, 640, 640, 1400]
+    k[1400:], v[1400:] = math.nan, math.nan
+    out, lse = torch.full(q.shape, 7.0, device="cuda"), torch.full(q.shape[:2], 7.0, device="cuda")
+    ops.flash_window(q, k, v, **w, out=out, lse=lse, lse_layout=ops.LSE_BSH, cu_seqlens_q=torch.tensor(qs, dtype=torch.int32).cuda(),
+                     cu_seqlens_k=torch.tensor(ks, dtype=torch.int32).cuda())
+    assert (out[690:] == 7).all() and (lse[690:] == 7).all()
+    for a, b, c, d in zip(qs, qs[1:], ks, ks[1:]):
+        if b > a:
+            _check_on_gpu(*(x[None] for x in (out[a:b], lse[a:b], q[a:b], k[c:d], v[c:d])), 0, **w, at=(d - c) - (b - a), heads=_heads(q[None]))
+    assert ops.read_status() == 0
+
+
+def test_scratch_that_is_too_small_is_refused():
+    from ditango_b200 import _capi
+    q, k, v, w = _large("parts", 64)
+    (B, Sq, Sk, H, Hk, _), lib = LARGE["parts"], _capi.load()
+    out, lse, scratch = torch.full(q.shape, 3.0, device="cuda"), torch.full((B, H, Sq), 3.0, device="cuda"), torch.empty(1024, dtype=torch.uint8, device="cuda")
+    args = (q.data_ptr(), k.data_ptr(), v.data_ptr(), H * 64, 0, Hk * 64, 0, Hk * 64, 0, out.data_ptr(), 0, lse.data_ptr(), 0, 0, None, None, None, B, Sq, Sk,
+            Sq, Sk, H, Hk, 64, 0.125, w["left"], w["right"], w["sinks"], _capi.QUERIES_LAST, 0)
+    stream = torch.cuda.current_stream().cuda_stream
+    assert lib.dtb_flash_window(*args, scratch.data_ptr(), 1024, stream) == -1 and "scratch" in lib.dtb_last_error().decode()
+    torch.cuda.synchronize()
+    assert (out == 3).all() and (lse == 3).all()
+    assert lib.dtb_flash_window(*args, None, 0, stream) == 0            # without scratch the keys stay whole
+    _check_on_gpu(out, lse.transpose(1, 2), q, k, v, 0, **w, at=Sk - Sq, heads=_heads(q))

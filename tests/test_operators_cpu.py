@@ -76,9 +76,9 @@ def test_the_cache_type_is_a_config_key(key, dtype, tmp_path):
 
 
 def _window(lib, *, q=16, k=16, v=16, qt=192, qb=1920, kt=192, kb=1920, vt=192, vb=1920, out=16, odt=0, lse=16, lay=0, acc=0, cq=None, ck=None,
-            sl=None, n=2, sq=10, sk=10, tq=20, tk=20, H=3, Hk=3, D=64, scale=0.1, left=3, right=3, sinks=0, qs=0, ks=0):
+            sl=None, n=2, sq=10, sk=10, tq=20, tk=20, H=3, Hk=3, D=64, scale=0.1, left=3, right=3, sinks=0, qs=0, ks=0, scratch=None):
     return lib.dtb_flash_window(q, k, v, qt, qb, kt, kb, vt, vb, out, odt, lse, lay, acc, cq, ck, sl, n, sq, sk, tq, tk, H, Hk, D, scale,
-                                left, right, sinks, qs, ks, None)
+                                left, right, sinks, qs, ks, scratch, 0, None)
 
 
 @pytest.mark.parametrize("args,word", [
@@ -87,11 +87,21 @@ def _window(lib, *, q=16, k=16, v=16, qt=192, qb=1920, kt=192, kb=1920, vt=192, 
     (dict(cq=16, ck=16, sl=16), "seqlens_k"), (dict(tq=21), "total"), (dict(tk=19), "total"), (dict(left=-2), "window"), (dict(right=2 ** 30 + 1), "window"),
     (dict(sinks=-1), "sinks"), (dict(qs=2 ** 30 + 1), "position"), (dict(ks=-2 ** 30 - 1), "position"), (dict(qt=128), "token stride"),
     (dict(kb=128), "batch stride"), (dict(vt=196), "multiples of 8"), (dict(q=24), "aligned"), (dict(odt=2), "out_dtype"), (dict(lay=2), "lse_layout"),
-    (dict(acc=1, odt=1), "accumulate"), (dict(scale=0.0), "scale"), (dict(scale=float("nan")), "scale")])
+    (dict(acc=1, odt=1), "accumulate"), (dict(scale=0.0), "scale"), (dict(scale=float("nan")), "scale"),
+    (dict(scratch=24), "scratch")])
 def test_flash_window_refuses(args, word):
     from ditango_b200 import _capi
     lib = _capi.load()
     assert _window(lib, **args) == -1 and word in lib.dtb_last_error().decode()
+
+
+@pytest.mark.parametrize("args,word", [((0, 9, 9, 2, 2, 64, 1, 1, 0), "shape"), ((1, -1, 9, 2, 2, 64, 1, 1, 0), "shape"), ((1, 9, 9, 3, 2, 64, 1, 1, 0), "shape"),
+                                       ((1, 9, 9, 2, 0, 64, 1, 1, 0), "shape"), ((1, 9, 9, 2, 2, 32, 1, 1, 0), "shape"), ((1, 9, 9, 2, 2, 64, -2, 1, 0), "window"),
+                                       ((1, 9, 9, 2, 2, 64, 1, 1, -1), "sinks")])
+def test_flash_window_scratch_refuses(args, word):
+    from ditango_b200 import _capi
+    lib = _capi.load()
+    assert lib.dtb_flash_window_scratch_bytes(*args) == -1 and word in lib.dtb_last_error().decode()
 
 
 def test_flash_window_takes_gpu_tensors_only():
