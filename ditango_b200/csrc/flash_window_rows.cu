@@ -290,7 +290,7 @@ __global__ void __launch_bounds__(kThreads) flash_window_rows_kernel(const Windo
     const int i = (row0 + r) / group, head = kv_head * group + (row0 + r) % group;
     const int64_t tok = p.f.cu_q != nullptr ? static_cast<int64_t>(s.q_begin) + i : static_cast<int64_t>(seg) * p.f.seqlen_q + i;
     const int64_t li = lse_index(p.f, seg, head, i, tok), oi = tok * p.f.out_tok_stride + static_cast<int64_t>(head) * D + col;
-    const bool empty = !(sum > 0.f);                  // no key seen: nothing to write over a state
+    const bool empty = sum == 0.f;                    // no key seen: nothing to write over a state  (a NaN among the scores is not empty)
     if (stores && !(empty && p.f.accumulate != 0)) {
       const float lse = empty ? -INFINITY : (mx * c + log2f(sum)) * kLn2;
       float w_new = 0.f, w_old = 0.f, lse_out = lse;

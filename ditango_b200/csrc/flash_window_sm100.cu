@@ -668,9 +668,9 @@ flash_window_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
           const float2 ml = sh.s_ml[tile * kBM + quarter * 32 + lane];
           __syncwarp();
           if (lane == 0) mbar_arrive(&sh.ml_empty[tile]);
-          // a row that has seen no key is an empty state, and leaves a state that it is folded into as it is
+          // a row that has seen no key is an empty state, and leaves a state that it is folded into as it is (a NaN among its scores is not that)
           float w_new = 0.f, w_old = lse_old != -INFINITY ? 1.f : 0.f, lse_out = lse_old;
-          if (ml.y > 0.f) merge_weights(accumulate, lse_old, (ml.x * c + log2f(ml.y)) * kLn2, ml.y, w_new, w_old, lse_out);
+          if (ml.y != 0.f) merge_weights(accumulate, lse_old, (ml.x * c + log2f(ml.y)) * kLn2, ml.y, w_new, w_old, lse_out);
           ok = warp_wait_or_abort(&sh.o_final[tile], item_use, p.f.status, 41);
           if (!ok) break;
           tc_fence_after();

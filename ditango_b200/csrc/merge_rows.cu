@@ -175,7 +175,7 @@ __global__ void __launch_bounds__(kThreads) merge_rows_kernel(const __grid_const
         sum += l == -INFINITY ? 0.f : ex2((l - mx) * 1.4426950408889634f);
       }
       // the factor of a state in 8 bits goes into its weight; a weight of 0 stays one
-      const float scale = sum > 0.f ? __fdividef(1.f, sum) : 0.f;
+      const float scale = sum == 0.f ? 0.f : __fdividef(1.f, sum);       // (a NaN among the lse goes on into the result)
       for (int c = 0; c < n; c += 8) {
         uint32_t b[8];
 #pragma unroll
@@ -188,7 +188,7 @@ __global__ void __launch_bounds__(kThreads) merge_rows_kernel(const __grid_const
           }
       }
       if (p.lse_out != nullptr)
-        p.lse_out[lse_offset(p.lse_out_layout, static_cast<uint32_t>(row), p.H, p.S)] = sum > 0.f ? mx + logf(sum) : -INFINITY;
+        p.lse_out[lse_offset(p.lse_out_layout, static_cast<uint32_t>(row), p.H, p.S)] = sum == 0.f ? -INFINITY : mx + logf(sum);
     }
   }
   __syncthreads();

@@ -20,7 +20,9 @@ struct MergeParams {
   int nstates;
   int H;
   int S;
-  const int* status;                    // null, or a status word: with it set nothing is written
+  // Null, or for a launch that completes one of attention a status word: with it set nothing is written, and a row with a NaN among its
+  // lse becomes NaN (otherwise an empty state).
+  const int* status;
 };
 
 struct CopyParams {

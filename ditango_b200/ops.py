@@ -227,6 +227,9 @@ def _strides(x: torch.Tensor, shape) -> Tuple[int, int]:
     return tok, (outer[0] if shape[0] > 1 else tok * shape[1])
 
 
+_FAR = 1 << 30           # (ctypes would cut off what an int does not hold)
+
+
 def flash_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, left: int = -1, right: int = -1, sinks: int = 0,
                  q_start: Optional[int] = None, k_start: int = 0, seqlens_k: Optional[torch.Tensor] = None,
                  out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None, accumulate: bool = False,
@@ -245,6 +248,9 @@ def flash_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, left: int
     accumulate=True the state is merged into the given fp32 (out, lse) in place.  A row that sees no key has out 0 and lse -inf.
     """
     stream = _launch_stream(q, k, v, out, lse, cu_seqlens_q, cu_seqlens_k, seqlens_k)
+    at = 0 if q_start is None else q_start
+    if not (-1 <= left <= _FAR and -1 <= right <= _FAR and 0 <= sinks <= _FAR and -_FAR <= k_start <= _FAR and -_FAR <= at <= _FAR):
+        raise _capi.ExtensionError("left, right, sinks and positions are within 2^30")
     if not q.dtype == k.dtype == v.dtype == torch.bfloat16:
         raise _capi.ExtensionError("q, k, v must be bfloat16")
     packed = cu_seqlens_q is not None
@@ -589,6 +595,8 @@ class GridRope(NamedTuple):
 @functools.lru_cache(maxsize=64)
 def _rope_arrays(grid, axes, base, origin, step):
     """What the C interface reads of a GridRope (host arrays, read at the launch)."""
+    if not all(0 <= n < 1 << 31 for n in (*grid, *axes)):
+        raise _capi.ExtensionError("a grid's extents and an axis's channels are not negative and below 2^31")
     return (ctypes.c_int * 3)(*grid), (ctypes.c_int * 3)(*axes), (ctypes.c_double * 7)(base, *origin, *step)
 
 
@@ -601,6 +609,9 @@ def _grid_rope_args(q, k, norms, rope, text_len, video_len):
     if len(shape) != 4 or len(kshape) != 4 or shape[:2] != kshape[:2] or shape[3] != kshape[3]:
         raise _capi.ExtensionError("q and k are [B,S,H,D] and [B,S,Hk,D]")
     B, S, H, D = shape
+    video_len = S - text_len if video_len is None else video_len
+    if text_len < 0 or video_len < 0 or text_len + video_len > S:
+        raise _capi.ExtensionError("text and video tokens lie within the sequence")
     if dtype not in _VALUES or k.dtype != dtype:
         raise _capi.ExtensionError("q and k must be bfloat16 or float32 alike")
     for w, b, _ in norms:
@@ -608,8 +619,10 @@ def _grid_rope_args(q, k, norms, rope, text_len, video_len):
             if x.dtype != dtype or x.numel() != D or not x.is_contiguous():
                 raise _capi.ExtensionError("weights and biases hold D contiguous elements of q's type")
     grid, axes, base, origin, step, first, shards = rope
+    if not 0 < shards < 1 << 31 or not 0 <= first < 1 << 62:
+        raise _capi.ExtensionError("shards and first are positions among the pieces")
     arrays = _rope_arrays(tuple(grid), tuple(axes), base, tuple(origin), tuple(step))
-    return shape, kshape, _VALUES[dtype], (*arrays, first, shards, B, S, text_len, S - text_len if video_len is None else video_len, H, kshape[2], D)
+    return shape, kshape, _VALUES[dtype], (*arrays, first, shards, B, S, text_len, video_len, H, kshape[2], D)
 
 
 def norm_rope_grid(q: torch.Tensor, k: torch.Tensor, q_norm: Norm, k_norm: Norm, rope: GridRope, *, text_len: int = 0,
@@ -622,7 +635,7 @@ def norm_rope_grid(q: torch.Tensor, k: torch.Tensor, q_norm: Norm, k_norm: Norm,
     stream = _launch_stream(q, k, qw, qb, kw, kb)
     shape, kshape, dtype, rest = _grid_rope_args(q, k, (q_norm, k_norm), rope, text_len, video_len)
     qo, ko = _empty_like(q, q.dtype), _empty_like(k, k.dtype)
-    if q.numel() == 0 or k.numel() == 0:
+    if q.numel() == 0 and k.numel() == 0:
         return qo, ko
     rc = _capi.load().dtb_norm_rope_grid(
         q.data_ptr(), *_strides(q, shape), qo.data_ptr(), qw.data_ptr(), None if qb is None else qb.data_ptr(), q_eps,
@@ -648,7 +661,7 @@ def norm_rope_grid_backward(dq: torch.Tensor, dk: torch.Tensor, q: torch.Tensor,
         raise _capi.ExtensionError("dq and dk have the shapes and the type of q and k")
     gq, gk = _empty_like(q, q.dtype), _empty_like(k, k.dtype)
     sums = [None if x is None else torch.empty_like(x) for x in (qw, qb, kw, kb)]
-    if q.numel() == 0 or k.numel() == 0:
+    if q.numel() == 0 and k.numel() == 0:
         return (gq, gk, *(None if x is None else x.zero_() for x in sums))
     lib = _capi.load()
     key = (q.get_device(), shape[3])

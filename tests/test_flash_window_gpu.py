@@ -467,3 +467,37 @@ def test_scratch_that_is_too_small_is_refused():
     assert (out == 3).all() and (lse == 3).all()
     assert lib.dtb_flash_window(*args, None, 0, stream) == 0            # without scratch the keys stay whole
     _check_on_gpu(out, lse.transpose(1, 2), q, k, v, 0, **w, at=Sk - Sq, heads=_heads(q))
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("kind", ["few", *LARGE])
+def test_a_nan_among_the_scores_shows(kind, D):
+    """In the rows that see it, and as lse too, and when the state is folded into another; other rows are what they were."""
+    from ditango_b200 import ops
+    q, k, v, w = _large("parts" if kind == "few" else kind, D)
+    if kind == "few":
+        q = q[:, :9]
+    Sq, Sk = q.shape[1], k.shape[1]
+    w = dict(w, left=w["left"] // 2 if kind != "whole" else 100, sinks=0)
+    want = ops.flash_window(q, k, v, **w, lse_layout=ops.LSE_BSH)
+    j = Sk - Sq - w["left"] + Sq // 2                   # seen by the rows in front of the middle
+    k[0, j, 0] = math.nan
+    seen = _visible(Sq, Sk, *w.values(), Sk - Sq, 0)[:, j].cuda()
+    assert seen.any() and not seen.all()
+    group = q.shape[2] // k.shape[2]
+    for state in (None, tuple(x.clone() for x in want)):
+        kw = {} if state is None else dict(out=state[0], lse=state[1], accumulate=True)
+        out, lse = ops.flash_window(q, k, v, **w, lse_layout=ops.LSE_BSH, **kw)
+        assert out[0, seen, :group].isnan().all() and lse[0, seen, :group].isnan().all()
+        assert not out[0, ~seen].isnan().any() and not out[:, :, group:].isnan().any() and not lse[0, ~seen].isnan().any()
+        if state is None:
+            assert torch.equal(out[0, ~seen], want[0][0, ~seen]) and torch.equal(lse[:, :, group:], want[1][:, :, group:])
+    assert ops.read_status() == 0
+
+
+@pytest.mark.parametrize("kw", [dict(left=2 ** 32), dict(right=-2 ** 32 - 1), dict(sinks=2 ** 32 + 1), dict(q_start=2 ** 32), dict(k_start=-2 ** 33)])
+def test_numbers_that_an_int_does_not_hold_are_refused(kw):
+    from ditango_b200 import _capi, ops
+    x = torch.zeros(1, 4, 1, 64, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(_capi.ExtensionError):
+        ops.flash_window(x, x, x, **kw)

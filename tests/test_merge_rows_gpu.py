@@ -181,3 +181,11 @@ def test_empty_tensors_launch_nothing():
     from ditango_b200 import ops
     rows = ops.quantize_rows(torch.empty(2, 0, 3, 64, device="cuda"))
     assert rows.shape == (2, 0, 3, 64) and ops.dequantize_rows(rows).shape == (2, 0, 3, 64)
+
+
+def test_a_nan_among_the_lse_shows():
+    from ditango_b200 import ops
+    outs, lses = torch.randn(2, 1, 5, 3, 64, device="cuda"), torch.randn(2, 1, 5, 3, device="cuda")
+    lses[0, 0, 2, 1] = math.nan
+    out, lse = ops.merge_states([(ops.quantize_rows(outs[0]), lses[0], ops.LSE_BSH), (outs[1], lses[1], ops.LSE_BSH)])
+    assert out[0, 2, 1].isnan().all() and int(out.isnan().sum()) == 64 and lse.isnan().nonzero().tolist() == [[0, 2, 1]]

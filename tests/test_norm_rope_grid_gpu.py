@@ -355,3 +355,22 @@ def test_ulysses_attention_with_a_window():
     p = (torch.einsum("bihd,bjhd->bhij", q.double(), k.double()) / 8).masked_fill(~seen, -math.inf).softmax(-1)
     want, spread = (torch.einsum("bhij,bjhd->bihd", p, t) for t in (v.double(), v.double().abs()))
     assert ((out - want).abs() <= (2.0 ** -8 + 2e-4) * spread + 2.0 ** -8 * want.abs()).all()
+
+
+@pytest.mark.parametrize("rope,kw", [(dict(grid=(1, 2, 2 ** 32 + 2)), {}), (dict(shards=2 ** 32 + 1), {}), (dict(first=-1), {}), ({}, dict(text_len=2 ** 32)),
+                                     ({}, dict(text_len=-1)), ({}, dict(video_len=5)), ({}, dict(text_len=2, video_len=3))])
+def test_numbers_that_an_int_does_not_hold_are_refused(rope, kw):
+    from ditango_b200 import _capi, ops
+    x, w = torch.zeros(1, 4, 1, 64, device="cuda"), torch.ones(64, device="cuda")
+    rope = ops.GridRope(**dict(dict(grid=(1, 2, 2), axes=(16, 24, 24)), **rope))
+    with pytest.raises(_capi.ExtensionError):
+        ops.norm_rope_grid(x, x, (w, None, 1e-6), (w, None, 1e-6), rope, **kw)
+    with pytest.raises(_capi.ExtensionError):
+        ops.norm_rope_grid_backward(x, x, x, x, (w, None, 1e-6), (w, None, 1e-6), rope, **kw)
+
+
+def test_no_heads_on_one_side_are_refused():
+    from ditango_b200 import _capi, ops
+    x, w = torch.zeros(1, 4, 1, 64, device="cuda"), torch.ones(64, device="cuda")
+    with pytest.raises(_capi.ExtensionError):
+        ops.norm_rope_grid(x, x[:, :, :0], (w, None, 1e-6), (w, None, 1e-6), ops.GridRope((1, 2, 2), (16, 24, 24)))
