@@ -24,6 +24,7 @@ from ..baseline.ulysses import heads_to_sequence, sequence_to_heads
 from ..core.attention import proAttention
 from ..utils import remove_padding_after_gather, split_tensor_uneven, update_timestep
 from .. import ops as _engine
+from ..ops import GridRope
 
 
 @dataclass
@@ -56,14 +57,14 @@ class DiTConfig:
         return self.frames * (self.height // self.patch_size) * (self.width // self.patch_size)
 
     @property
-    def grid_rope(self) -> "_engine.GridRope":
+    def grid_rope(self) -> GridRope:
         """The positions that rotary_tables has in tables."""
         d_t = self.head_dim // 4
         d_h = (self.head_dim - d_t) // 2
-        return _engine.GridRope((self.frames, self.height // self.patch_size, self.width // self.patch_size), (d_t, d_h, d_h))
+        return GridRope((self.frames, self.height // self.patch_size, self.width // self.patch_size), (d_t, d_h, d_h))
 
 
-def grid_tables(rope: "_engine.GridRope", tokens: int, device) -> Tuple[torch.Tensor, torch.Tensor]:
+def grid_tables(rope: GridRope, tokens: int, device) -> Tuple[torch.Tensor, torch.Tensor]:
     """The cos and sin tables [tokens, D] (fp32) of the positions that `rope` gives a sequence's video tokens; 0 at padding."""
     angles = [((o + st * torch.arange(n, dtype=torch.float64, device=device))[:, None] *
                rope.base ** (-torch.arange(0, d, 2, dtype=torch.float64, device=device) / max(d, 1))).repeat_interleave(2, dim=1)
@@ -320,7 +321,7 @@ class DiTBlock(nn.Module):
         return out[:, text_len:], out[:, :text_len]
 
     def _norm_and_rotate(self, q, k, rope, text_len):
-        if isinstance(rope, _engine.GridRope):
+        if isinstance(rope, GridRope):
             return norm_and_rotate_grid(q, k, self.norm_q, self.norm_k, rope, text_len)
         cos, sin = rope
         return norm_and_rotate(q, k, self.norm_q, self.norm_k, cos, sin, text_len)
