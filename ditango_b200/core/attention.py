@@ -79,7 +79,7 @@ class proAttention:
     output_dtype = torch.float32
     # dtype of the values of cached block states (the reference keeps fp32: utils.py:76); bfloat16 halves
     # the cache's footprint and read traffic, int8 and float8_e4m3fn (one power of two per row) quarter it.  lse stays fp32.
-    # A state on its way into 8 bits leaves the attention kernel in bf16, whose rounding (2^-9) is lost in that of the codes, and
+    # A state on its way into 8 bits leaves the attention kernel in bf16, whose rounding (2^-8) is lost in that of the codes, and
     # is quantised by one launch; the call that made it merges it as it was.
     cache_dtype = torch.float32
     # Overlapping attention launches.  The chunks of a call are attended by one launch each; every launch ends

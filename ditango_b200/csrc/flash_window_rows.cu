@@ -8,8 +8,10 @@
 // fixed order: one launch, no workspace, no atomics.
 //
 // Bound by HBM for few rows (a key and a value are read once per 16 rows); mma.sync, because 16 rows fill an instruction of it and a
-// 128-row tile of tcgen05 would be empty for the most part.  P is rounded to bf16 for the product (2^-9 of each weight, as in the
-// other attention kernels), sums and states are fp32.
+// 128-row tile of tcgen05 would be empty for the most part.  P is rounded to bf16 for the product (by 2^-8 of each weight at
+// most, as in the other attention kernels), sums and states are fp32.
+// Measured, launches in a graph: a token of 24 heads of 128 against 4352 keys 13.8 us (53 MB, 3.9 TB/s), three tokens of seven sequences, 32
+// over 8 heads of 64, against 3013 keys 12.6 us (43 MB, 3.4 TB/s).  With hardly any keys a launch takes 5 us; the rest is at the rate of HBM.
 #include "flash_common.cuh"
 #include "flash_window.cuh"
 

@@ -28,6 +28,8 @@
 // warps of their own.  The grid has a CTA per block, as if all were to run; CTAs claim further blocks by cluster launch control.  Every
 // phase of a barrier is over for all that look at it before the next one can complete; see flash_fwd_persistent_sm100.cu.
 //
+// Measured: 2 x 17776 x 48 x 64, windows of 1350 either way and 226 first tokens, 1655 us (740 TFLOP/s of what the rows see; the ex2 unit 73 %
+// busy), 29764 x 24 x 128, windows of 3600 and 256 first tokens, 2330 us (1097; the power cap, and 8 us a block that no product fills).
 // With few blocks their keys are split into parts of as many tiles each, which are attended like blocks of their own and merged by the
 // state merge's kernel behind this one (24 heads of 128, 64 queries, window 4096: 66 -> 26 us in six parts).
 #include "flash_common.cuh"
@@ -682,7 +684,7 @@ flash_window_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
           };
           if (p.f.out_dtype != 0) {
             // bf16: 64 columns at a time, rounded as they are read, so that the next block's products do not wait long for O.  (A block of
-            // 25 steps, D = 64 and 128: 35.5 and 54.5 us; 36.6 and 54.8 with 32 fp32 columns staged at a time, 36.5 and 56.0 with
+            // 25 steps, D = 64 and 128: 35.5 and 55.0 us; 36.6 and 54.8 with 32 fp32 columns staged at a time, 36.5 and 56.0 with
             // every lane storing its row from registers.)
             uint16_t* dst = static_cast<uint16_t*>(p.f.out) + tok0 * p.f.out_tok_stride + col;
 #pragma unroll 1
@@ -822,7 +824,8 @@ flash_window_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
             }
           }
           // p = 2^(s*c - m*c), at most 2^8; 0 for what is hidden, also while m is -inf.  (All on the ex2 unit: with one pair of eight on
-          // the FMA units, which the kernels without masks gain from, a block of 25 steps took 36.6 us in place of 35.9.)
+          // the FMA units, which the kernels without masks gain from, a block of 25 steps at D = 64 took 37.3 us in place of 35.7; with the
+          // next tile's scores asked for under the second half, where they are there by then, 38.2.)
           const float ref = m == -INFINITY ? 0.f : -m * c;
           const uint64_t c2 = pack2(c, c), nmc2 = pack2(ref, ref);
           uint64_t sum0 = pack2(0.f, 0.f), sum1 = sum0;
