@@ -85,7 +85,7 @@ def load():
         c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_void_p]
     lib.dtb_merge_rows.restype = c_int
     lib.dtb_merge_rows.argtypes = [
-        c_int, POINTER(c_void_p), POINTER(c_int), POINTER(c_void_p), POINTER(c_void_p), POINTER(c_int),
+        c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,        # (arrays by their addresses)
         c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_void_p]
     lib.dtb_quantize_rows.restype = lib.dtb_dequantize_rows.restype = c_int
     lib.dtb_quantize_rows.argtypes = [c_void_p, c_int, c_void_p, c_int, c_void_p, c_int64, c_int, c_void_p]

@@ -408,7 +408,8 @@ def dequantize_rows(rows: QuantizedRows, dtype: torch.dtype = torch.float32) -> 
     return out
 
 
-_ARRAYS = {n: (ctypes.c_void_p * n, ctypes.c_int * n) for n in range(1, _capi.MERGE_MAX_STATES + 1)}
+# for n states: types of one array that holds their values', exponents' and lse's addresses, one of their types and layouts
+_ARRAYS = {n: (ctypes.c_void_p * (3 * n), ctypes.c_int * (2 * n)) for n in range(1, _capi.MERGE_MAX_STATES + 1)}
 
 
 def _merge_rows(states, shape, out, lse_out, lse_out_layout, out_bf16, out_rows):
@@ -418,28 +419,28 @@ def _merge_rows(states, shape, out, lse_out, lse_out_layout, out_bf16, out_rows)
         raise _capi.ExtensionError(f"1 to {_capi.MERGE_MAX_STATES} states of [B,S,H,D] or [T,H,D]")
     B, S, H, D = (1, *shape) if len(shape) == 3 else shape
     rows, row_shape = B * S * H, shape[:-1]
-    tensors, outs, dts, exps, lses, lays = [out, out_bf16, lse_out], [], [], [], [], []
-    for o, l, lay in states:
+    tensors, (pointers, ints) = [out, out_bf16, lse_out], _ARRAYS[n]
+    addresses, kinds = pointers(), ints()
+    for i, (o, l, lay) in enumerate(states):
         if type(o) is QuantizedRows:
             v, e = o
             if e.dtype != torch.uint8 or e.shape != row_shape or not e.is_contiguous():
                 raise _capi.ExtensionError("exponents are contiguous uint8, one per row")
-            tensors.append(e)
-            exps.append(e.data_ptr())
+            tensors += (v, e, l)
+            addresses[n + i] = e.data_ptr()
             dtype = _CODES.get(v.dtype)
         else:
             v = o
-            exps.append(None)
+            tensors += (v, l)
             dtype = _VALUES.get(v.dtype)
         if dtype is None or v.shape != shape or not v.is_contiguous():
             raise _capi.ExtensionError("states must be contiguous, of one shape, and fp32, bf16 or QuantizedRows")
         if l.dtype != torch.float32 or l.numel() != rows or not l.is_contiguous():
             raise _capi.ExtensionError("lse must be contiguous fp32 with B*S*H entries")
-        tensors += (v, l)
-        outs.append(v.data_ptr())
-        dts.append(dtype)
-        lses.append(l.data_ptr())
-        lays.append(lay)
+        addresses[i] = v.data_ptr()
+        addresses[2 * n + i] = l.data_ptr()
+        kinds[i] = dtype
+        kinds[n + i] = lay
     if out is not None:
         _check_result(out, torch.float32, shape)
     if out_bf16 is not None:
@@ -455,9 +456,9 @@ def _merge_rows(states, shape, out, lse_out, lse_out_layout, out_bf16, out_rows)
     stream = _launch_stream(*tensors)
     if rows * D == 0:
         return
-    pointers, ints = _ARRAYS[n]
+    at, kinds_at = ctypes.addressof(addresses), ctypes.addressof(kinds)
     rc = _capi.load().dtb_merge_rows(
-        n, pointers(*outs), ints(*dts), pointers(*exps), pointers(*lses), ints(*lays), None if out is None else out.data_ptr(),
+        n, at, kinds_at, at + 8 * n, at + 16 * n, kinds_at + 4 * n, None if out is None else out.data_ptr(),
         None if lse_out is None else lse_out.data_ptr(), lse_out_layout, None if out_bf16 is None else out_bf16.data_ptr(),
         None if codes is None else codes.data_ptr(), code, None if exponents is None else exponents.data_ptr(), B, S, H, D, stream)
     if rc:
@@ -475,7 +476,7 @@ def merge_states(states: Sequence[Tuple[Union[torch.Tensor, QuantizedRows], torc
     fp32_out=False only the bf16 copy `out_bf16` is written and returned in place of `out`.  `out_rows`
     (QuantizedRows to fill, or the type of new ones: torch.int8, torch.float8_e4m3fn) has the result
     written in 8 bits too; with fp32_out=False and no `out_bf16` that is what is returned."""
-    if out_rows is not None or any(type(o) is QuantizedRows for o, _, _ in states):
+    if out_rows is not None or QuantizedRows in [type(o) for o, _, _ in states]:
         shape, device = states[0][0].shape, states[0][1].device
         if isinstance(out_rows, torch.dtype):
             out_rows = _new_rows(device, shape, out_rows)
