@@ -865,13 +865,9 @@ static int grid_rope_params(const char* what, dtb::NormRopeGridParams* p, const 
   for (int a = 0; a < 3; ++a) {
     p->origin[a] = place[1 + a];
     p->step[a] = place[4 + a];
-    // base^(-2 i / d) / 2 pi by products: off by i 2^-52 of itself at most, the less the faster a pair turns
-    const double ratio = axes[a] > 0 ? std::pow(place[0], -2. / axes[a]) : 0.;
-    double turn = 0.15915494309189533577;
     for (int i = 0; i < axes[a]; i += 2, ++pair) {
-      p->turns[pair] = turn;
+      p->turns[pair] = std::pow(place[0], -static_cast<double>(i) / axes[a]) * 0.15915494309189533577;       // / 2 pi
       p->axis[pair] = static_cast<uint8_t>(a);
-      turn *= ratio;
     }
   }
   return DTB_OK;
