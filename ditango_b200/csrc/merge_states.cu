@@ -13,6 +13,7 @@
 // at 2 x 6851 x 48 x 128 726 us; as it stands 81 us and 306 us; L2 flushed before each launch).
 #include "merge_states.cuh"
 
+#include "flash_common.cuh"
 #include "row_access.cuh"
 
 #include <math.h>
@@ -69,6 +70,7 @@ __global__ void __launch_bounds__(128) merge_states_kernel(const MergeParams p) 
   const unsigned full = 0xffffffffu;
   const int n = p.nstates;
   const bool shows_nan = p.status != nullptr;
+  if (shows_nan) grid_dependency_wait();               // (launched while the kernel before it ends)
   if (shows_nan && *reinterpret_cast<const volatile int*>(p.status) != 0) return;
 
   auto load_chunk = [&](int c0, int64_t base, Raw8 (&v)[CH][U]) {
@@ -190,11 +192,8 @@ static cudaError_t launch_merge_cfg(const MergeParams& p, int G, int sm_count, c
   const int64_t cap = static_cast<int64_t>(sm_count) * per_sm;
   int blocks = static_cast<int>(blocks_needed < cap ? blocks_needed : cap);
   if (blocks < 1) blocks = 1;
-  if (G == 8)
-    merge_states_kernel<8, U, CH><<<blocks, kThreads, 0, stream>>>(p);
-  else
-    merge_states_kernel<16, U, CH><<<blocks, kThreads, 0, stream>>>(p);
-  return cudaGetLastError();
+  return flash::launch_attention_kernel(G == 8 ? merge_states_kernel<8, U, CH> : merge_states_kernel<16, U, CH>, dim3(blocks), kThreads, 0, stream,
+                                        p.status != nullptr, p);
 }
 
 // Rows per thread x states per fetch are chosen so that eight or nine row pieces are outstanding per thread whatever the

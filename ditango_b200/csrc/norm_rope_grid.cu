@@ -399,6 +399,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 6 : 4) norm_rope_gr
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncthreads();                                     // the ring's memory takes the sums
+  grid_launch_dependents();                            // the kernel that adds them up may be set up meanwhile; it waits for this one's end
   float(*s_sum)[2 * D] = reinterpret_cast<float(*)[2 * D]>(s_ring);
   const int row = threadIdx.x / kLanes;
 #pragma unroll
@@ -460,8 +461,7 @@ static cudaError_t launch_backward_as(const NormRopeGridParams& p, int sm_count,
   else norm_rope_grid_backward_kernel<T, D, kRms, false, kBias><<<dim3(ctas, 2), kThreads, 0, stream>>>(p);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  norm_rope_grid_sums_kernel<T, D><<<dim3(2 * D / 32, 2), 1024, 0, stream>>>(p, ctas);
-  return cudaGetLastError();
+  return launch_attention_kernel(norm_rope_grid_sums_kernel<T, D>, dim3(2 * D / 32, 2), 1024, 0, stream, true, p, ctas);
 }
 
 template <typename T, int D, bool kRms>

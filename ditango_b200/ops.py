@@ -246,6 +246,8 @@ def flash_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, left: int
     (int32 [B] on the device) gives the number of keys of each sequence, the rest of Sk may hold anything.  Packed
     (cu_seqlens given): q [Tq,H,D], k,v [Tk,Hk,D].  Returns (out, lse) as flash_partial does, mergeable with its states; with
     accumulate=True the state is merged into the given fp32 (out, lse) in place.  A row that sees no key has out 0 and lse -inf.
+    Keys and values that no query near by (in its 256) sees may hold anything, the others must be finite.  Few queries against many
+    keys of a dense batch take two launches and scratch from the allocator of the current stream.
     """
     stream = _launch_stream(q, k, v, out, lse, cu_seqlens_q, cu_seqlens_k, seqlens_k)
     at = 0 if q_start is None else q_start
