@@ -45,10 +45,6 @@ using namespace flash;
 
 constexpr int kThreads = 512;
 constexpr int kRegsLaunch = 128;    // what __launch_bounds__(512, 1) allots; checked before the first launch
-constexpr int kRegsSoftmax = 176;
-constexpr int kRegsOutput = 104;
-constexpr int kRegsOther = 56;
-static_assert(2 * kRegsSoftmax + kRegsOutput + kRegsOther == 4 * kRegsLaunch, "register split");
 constexpr int kOutWarp = 8;         // first of four
 constexpr int kTmaWarp = 12;
 constexpr int kMmaWarp = 13;
@@ -63,6 +59,11 @@ constexpr int kTails = 8;
 template <int D>
 struct Cfg {
   static constexpr int kSlabs = D / 64;
+  // registers of a thread of each role (a block of 25 steps the one way and the other: D = 64 35.7 and 36.6 us, D = 128 54.9 and 54.1)
+  static constexpr int kRegsSoftmax = D == 64 ? 176 : 160;
+  static constexpr int kRegsOutput = D == 64 ? 104 : 128;
+  static constexpr int kRegsOther = D == 64 ? 56 : 64;
+  static_assert(2 * kRegsSoftmax + kRegsOutput + kRegsOther == 4 * kRegsLaunch, "register split");
   static constexpr int kTileBytes = 128 * D * 2;          // one Q, K or V tile
   static constexpr int kQBufs = D == 64 ? 2 : 1;          // blocks whose queries are in shared memory
   static constexpr int kStages = D == 64 ? 8 : 4;
@@ -329,7 +330,7 @@ flash_window_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
   };
 
   if (warp >= kTmaWarp) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kRegsOther));
     if (aborted || warp > kMmaWarp) {
       // fall through to the tear-down
     } else if (warp == kTmaWarp) {
@@ -641,7 +642,7 @@ flash_window_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     }
   } else if (warp >= kOutWarp) {
     // -------------------------------------------------------------- results
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOutput));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kRegsOutput));
     if (!aborted) {
       const Shared<D> sh(smem + opaque_zero());
       const int quarter = warp & 3;
@@ -721,7 +722,7 @@ flash_window_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     }
   } else {
     // -------------------------------------------------------------- softmax
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kRegsSoftmax));
     if (!aborted) {
       const Shared<D> sh(smem + opaque_zero());
       const int tile = warp >> 2;
