@@ -861,14 +861,11 @@ static int grid_rope_params(const char* what, dtb::NormRopeGridParams* p, const 
   p->shard_rest = static_cast<int>(places % shards);
   p->size_y = grid[1];
   p->size_x = grid[2];
-  int pair = 0;
   for (int a = 0; a < 3; ++a) {
     p->origin[a] = place[1 + a];
     p->step[a] = place[4 + a];
-    for (int i = 0; i < axes[a]; i += 2, ++pair) {
-      p->turns[pair] = std::pow(place[0], -static_cast<double>(i) / axes[a]) * 0.15915494309189533577;       // / 2 pi
-      p->axis[pair] = static_cast<uint8_t>(a);
-    }
+    p->ratio[a] = axes[a] > 0 ? std::pow(place[0], -2. / axes[a]) : 1.;
+    p->pairs_end[a] = (a == 0 ? 0 : p->pairs_end[a - 1]) + axes[a] / 2;
   }
   return DTB_OK;
 }
@@ -938,12 +935,9 @@ DTB_API int dtb_norm_rope_grid_backward(const void* dq_out, int64_t dq_tok_strid
   p.grad_tok_stride[1] = dk_tok_stride;
   p.grad_batch_stride[0] = dq_batch_stride;
   p.grad_batch_stride[1] = dk_batch_stride;
-  p.weight_grad[0] = dq_weight;
-  p.weight_grad[1] = dk_weight;
-  p.bias_grad[0] = dq_bias;
-  p.bias_grad[1] = dk_bias;
+  const dtb::NormRopeGridSums sums = {{dq_weight, dk_weight}, {dq_bias, dk_bias}};
   p.partial = static_cast<float*>(scratch);
-  cudaError_t e = dtb::launch_norm_rope_grid_backward(p, head_dim, dtype == DTB_BF16, rms != 0, d->sm_count, static_cast<cudaStream_t>(stream));
+  cudaError_t e = dtb::launch_norm_rope_grid_backward(p, sums, head_dim, dtype == DTB_BF16, rms != 0, d->sm_count, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return fail(DTB_ERR_CUDA, "%s launch failed: %s", what, cudaGetErrorString(e));
   return DTB_OK;
 }

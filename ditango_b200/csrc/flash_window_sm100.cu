@@ -29,7 +29,7 @@
 // phase of a barrier is over for all that look at it before the next one can complete; see flash_fwd_persistent_sm100.cu.
 //
 // Measured: 2 x 17776 x 48 x 64, windows of 1350 either way and 226 first tokens, 1655 us (740 TFLOP/s of what the rows see; the ex2 unit 73 %
-// busy), 29764 x 24 x 128, windows of 3600 and 256 first tokens, 2330 us (1097; the power cap, and 8 us a block that no product fills).
+// busy), 29764 x 24 x 128, windows of 3600 and 256 first tokens, 2250 us (1136; the power cap, and 8 us a block that no product fills).
 // With few blocks their keys are split into parts of as many tiles each, which are attended like blocks of their own and merged by the
 // state merge's kernel behind this one (24 heads of 128, 64 queries, window 4096: 66 -> 26 us in six parts).
 #include "flash_common.cuh"

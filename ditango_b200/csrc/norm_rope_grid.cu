@@ -12,12 +12,13 @@
 // Bound by HBM: each value read once and written once.  D / 8 lanes own a head's row, 8 values each, so that pairs lie inside a lane
 // and the means are shuffles inside the row's lanes.  A CTA's rows of lanes are dealt to the heads of one token, and to several tokens
 // where there are fewer heads.  All arithmetic is fp32, rounded once.
-// Measured: forward, 2 x 17776 x 48 x 64 bf16, layer norm, 147 us (874 MB, 5.95 TB/s); backward, 32681 x 24 x 128 bf16, RMS norm, 213 us
-// (1205 MB, 5.65 TB/s).  The way there, us of the two:
+// Measured: forward, 2 x 17776 x 48 x 64 bf16, layer norm, 148 us (874 MB, 5.9 TB/s); backward, 32681 x 24 x 128 bf16, RMS norm, 202 us
+// (1205 MB, 5.96 TB/s).  The way there, us of the two:
 //   every lane the four angles of its own pairs, a token's loads issued together      216 / 381
 //   angles by the CTA, queries loaded while keys are worked on                        170 / 259
 //   channel pairs in packed arithmetic, fixed distances between heads (a quarter fewer instructions)    171 / 243
 //   loads by asynchronous copies into a ring, so that more warps fit                  147 / 213
+//   a pair's rate formed by the thread that has its angles (it was read from a table among the parameters)     148 / 202
 // The sums for the weights stay in a lane's registers over all its rows, are added up in the CTA and then over CTAs, in a fixed order.
 #include "norm_rope_grid.cuh"
 
@@ -117,8 +118,23 @@ __device__ __forceinline__ float standardise(uint64_t (&x)[4], float eps) {
   return rstd;
 }
 
+__device__ __forceinline__ int axis_of(const NormRopeGridParams& p, int pair) { return pair < p.pairs_end[0] ? 0 : pair < p.pairs_end[1] ? 1 : 2; }
+// Where pair `pair` stands at index 0 and what it moves by with the index, in turns.  (A power by squaring, off by 2^-52 of itself per
+// pair in front of it on its axis, the less the faster the pair turns.  A table of all pairs among the parameters was read at another
+// place by each thread and made a launch a microsecond longer.)
+__device__ __forceinline__ double2 rate_of(const NormRopeGridParams& p, int pair) {
+  const int a = axis_of(p, pair), i = pair - (a == 0 ? 0 : p.pairs_end[a - 1]);
+  double rate = 0.15915494309189533577, power = p.ratio[a];       // 1 / 2 pi
+#pragma unroll
+  for (int bit = 1; bit < 64; bit *= 2) {
+    if ((i & bit) != 0) rate *= power;
+    power *= power;
+  }
+  return make_double2(p.origin[a] * rate, p.step[a] * rate);
+}
+
 // Angle of pair `pair` of token `tok` as (cos, sin): (1, 0) for text, (0, 0), which no angle has, for padding.
-__device__ __forceinline__ float2 rotation(const NormRopeGridParams& p, int64_t tok, int pair) {
+__device__ __forceinline__ float2 rotation(const NormRopeGridParams& p, double2 rate, int64_t tok, int pair) {
   const int s = static_cast<int>(tok % p.seq) - p.text_len;
   if (s < 0 || s >= p.video_len) return make_float2(1.f, 0.f);
   const int64_t n = p.first + s;
@@ -128,9 +144,9 @@ __device__ __forceinline__ float2 rotation(const NormRopeGridParams& p, int64_t 
   if (in >= p.shard_places + (shard < rest ? 1u : 0u)) return make_float2(0.f, 0.f);
   const uint32_t at = shard * p.shard_places + min(shard, rest) + in, row = at / static_cast<uint32_t>(p.size_x);
   const uint32_t t = row / static_cast<uint32_t>(p.size_y);
-  const int a = p.axis[pair];
+  const int a = axis_of(p, pair);
   const uint32_t index = a == 0 ? t : a == 1 ? row - t * p.size_y : at - row * p.size_x;
-  const double turn = (p.origin[a] + p.step[a] * index) * p.turns[pair];
+  const double turn = fma(rate.y, static_cast<double>(index), rate.x);
   float2 r;
   sincospif(2.f * static_cast<float>(turn - rint(turn)), &r.y, &r.x);
   return r;
@@ -153,9 +169,9 @@ struct Deal {
   }
   // The angles of the batch from token `first` on.  One batch's are written while slower warps may still read those of the one
   // before it, hence two buffers and one barrier.
-  __device__ __forceinline__ void angles(const NormRopeGridParams& p, float2 (*to)[kPairs], int64_t first, int n) const {
+  __device__ __forceinline__ void angles(const NormRopeGridParams& p, double2 rate, float2 (*to)[kPairs], int64_t first, int n) const {
     for (int i = threadIdx.x; i < n * kPairs; i += kThreads)
-      if (first + i / kPairs < p.tokens) to[i / kPairs][i % kPairs] = rotation(p, first + i / kPairs, i % kPairs);
+      if (first + i / kPairs < p.tokens) to[i / kPairs][i % kPairs] = rotation(p, rate, first + i / kPairs, threadIdx.x % kPairs);
     __syncthreads();
   }
 };
@@ -276,11 +292,12 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 6 : 5) norm_rope_gr
     }
   };
   for (int i = 0; i < kAhead; ++i) copy();
+  const double2 rate = rate_of(p, threadIdx.x % (D / 2));        // (a thread forms the angles of one pair only)
   int buffer = 0;
   // (all bounds are the same for all threads of the CTA: barriers and shuffles)
   for (; at.base < p.tokens; at.base += stride) {
     const float2(*turns)[D / 2] = s_turn[buffer];
-    deal.angles(p, s_turn[buffer], at.base, pace.batch);
+    deal.angles(p, rate, s_turn[buffer], at.base, pace.batch);
     buffer ^= 1;
     for (int t = 0; t < pace.batch; t += pace.tokens) {
       const int64_t tok = at.base + t + pace.sub;
@@ -384,10 +401,11 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 6 : 4) norm_rope_gr
   if (p.tokens > 0) {
     for (int i = 0; i < kAhead; ++i) copy();
   }
+  const double2 rate = rate_of(p, threadIdx.x % (D / 2));        // (a thread forms the angles of one pair only)
   int buffer = 0;
   for (; at.base < p.tokens; at.base += stride) {
     const float2(*turns)[D / 2] = s_turn[buffer];
-    deal.angles(p, s_turn[buffer], at.base, pace.batch);
+    deal.angles(p, rate, s_turn[buffer], at.base, pace.batch);
     buffer ^= 1;
     for (int t = 0; t < pace.batch; t += pace.tokens) {
       for (int h0 = 0; h0 < heads; h0 += U * pace.width) {
@@ -419,11 +437,11 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 6 : 4) norm_rope_gr
 
 // Sums of the CTAs' rows.  grid: (2 D / 32, tensor); 32 columns, 32 threads to a column.
 template <typename T, int D>
-__global__ void __launch_bounds__(1024) norm_rope_grid_sums_kernel(const __grid_constant__ NormRopeGridParams p, int rows) {
+__global__ void __launch_bounds__(1024) norm_rope_grid_sums_kernel(const __grid_constant__ NormRopeGridSums to, const float* partial, int rows) {
   __shared__ float s_sum[32][33];
   grid_dependency_wait();
   const int x = blockIdx.y, c = blockIdx.x * 32 + (threadIdx.x & 31), slice = threadIdx.x >> 5;
-  const float* from = p.partial + static_cast<int64_t>(x) * rows * (2 * D) + c;
+  const float* from = partial + static_cast<int64_t>(x) * rows * (2 * D) + c;
   float sum = 0.f;
 #pragma unroll 4
   for (int r = slice; r < rows; r += 32) sum += from[static_cast<int64_t>(r) * (2 * D)];
@@ -434,7 +452,7 @@ __global__ void __launch_bounds__(1024) norm_rope_grid_sums_kernel(const __grid_
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if ((threadIdx.x & 31) == 0) {
     const int at = blockIdx.x * 32 + slice;
-    void* dst = at < D ? p.weight_grad[x] : p.bias_grad[x];
+    void* dst = at < D ? to.weight_grad[x] : to.bias_grad[x];
     if (dst != nullptr) store1(static_cast<T*>(dst) + (at < D ? at : at - D), sum);
   }
 }
@@ -451,7 +469,7 @@ static cudaError_t launch_forward(const NormRopeGridParams& p, int sm_count, cud
 }
 
 template <typename T, int D, bool kRms, bool kBias>
-static cudaError_t launch_backward_as(const NormRopeGridParams& p, int sm_count, cudaStream_t stream) {
+static cudaError_t launch_backward_as(const NormRopeGridParams& p, const NormRopeGridSums& sums, int sm_count, cudaStream_t stream) {
   const int least = p.heads[0] < p.heads[1] ? p.heads[0] : p.heads[1], most = p.heads[0] + p.heads[1] - least;
   const int batch = Deal<D>(most).batch;
   const int64_t need = (p.tokens + batch - 1) / batch, cap = static_cast<int64_t>(sm_count) * kBackwardPerSm;
@@ -461,13 +479,13 @@ static cudaError_t launch_backward_as(const NormRopeGridParams& p, int sm_count,
   else norm_rope_grid_backward_kernel<T, D, kRms, false, kBias><<<dim3(ctas, 2), kThreads, 0, stream>>>(p);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  return launch_attention_kernel(norm_rope_grid_sums_kernel<T, D>, dim3(2 * D / 32, 2), 1024, 0, stream, true, p, ctas);
+  return launch_attention_kernel(norm_rope_grid_sums_kernel<T, D>, dim3(2 * D / 32, 2), 1024, 0, stream, true, sums, static_cast<const float*>(p.partial), ctas);
 }
 
 template <typename T, int D, bool kRms>
-static cudaError_t launch_backward(const NormRopeGridParams& p, int sm_count, cudaStream_t stream) {
-  return p.bias_grad[0] != nullptr || p.bias_grad[1] != nullptr ? launch_backward_as<T, D, kRms, true>(p, sm_count, stream)
-                                                                : launch_backward_as<T, D, kRms, false>(p, sm_count, stream);
+static cudaError_t launch_backward(const NormRopeGridParams& p, const NormRopeGridSums& sums, int sm_count, cudaStream_t stream) {
+  return sums.bias_grad[0] != nullptr || sums.bias_grad[1] != nullptr ? launch_backward_as<T, D, kRms, true>(p, sums, sm_count, stream)
+                                                                      : launch_backward_as<T, D, kRms, false>(p, sums, sm_count, stream);
 }
 
 cudaError_t launch_norm_rope_grid(const NormRopeGridParams& p, int head_dim, bool bf16, bool rms, int sm_count, cudaStream_t stream) {
@@ -481,13 +499,13 @@ cudaError_t launch_norm_rope_grid(const NormRopeGridParams& p, int head_dim, boo
 
 int64_t norm_rope_grid_scratch_bytes(int head_dim, int sm_count) { return 2ll * sm_count * kBackwardPerSm * 2 * head_dim * 4; }
 
-cudaError_t launch_norm_rope_grid_backward(const NormRopeGridParams& p, int head_dim, bool bf16, bool rms, int sm_count, cudaStream_t stream) {
+cudaError_t launch_norm_rope_grid_backward(const NormRopeGridParams& p, const NormRopeGridSums& sums, int head_dim, bool bf16, bool rms, int sm_count, cudaStream_t stream) {
   if (head_dim == 64) {
-    if (bf16) return rms ? launch_backward<uint16_t, 64, true>(p, sm_count, stream) : launch_backward<uint16_t, 64, false>(p, sm_count, stream);
-    return rms ? launch_backward<float, 64, true>(p, sm_count, stream) : launch_backward<float, 64, false>(p, sm_count, stream);
+    if (bf16) return rms ? launch_backward<uint16_t, 64, true>(p, sums, sm_count, stream) : launch_backward<uint16_t, 64, false>(p, sums, sm_count, stream);
+    return rms ? launch_backward<float, 64, true>(p, sums, sm_count, stream) : launch_backward<float, 64, false>(p, sums, sm_count, stream);
   }
-  if (bf16) return rms ? launch_backward<uint16_t, 128, true>(p, sm_count, stream) : launch_backward<uint16_t, 128, false>(p, sm_count, stream);
-  return rms ? launch_backward<float, 128, true>(p, sm_count, stream) : launch_backward<float, 128, false>(p, sm_count, stream);
+  if (bf16) return rms ? launch_backward<uint16_t, 128, true>(p, sums, sm_count, stream) : launch_backward<uint16_t, 128, false>(p, sums, sm_count, stream);
+  return rms ? launch_backward<float, 128, true>(p, sums, sm_count, stream) : launch_backward<float, 128, false>(p, sums, sm_count, stream);
 }
 
 }  // namespace dtb

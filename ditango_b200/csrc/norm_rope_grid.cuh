@@ -15,8 +15,6 @@ struct NormRopeGridParams {
   void* dst[2];                  // results, or gradients of src: [batch, seq, heads, D] contiguous
   const void* weight[2];         // [D]
   const void* bias[2];           // [D] or null
-  void* weight_grad[2];          // backward: [D], or null
-  void* bias_grad[2];
   float* partial;                // backward: scratch, a row of 2 D sums for each CTA
   float eps[2];
   int heads[2];
@@ -30,13 +28,19 @@ struct NormRopeGridParams {
   int shards, shard_len, shard_places, shard_rest;
   int size_y, size_x;
   double origin[3], step[3];
-  double turns[64];              // of pair i: base^(-2 i' / d) / 2 pi, i' its place among the d channels of its axis
-  uint8_t axis[64];
+  // the i'th pair of an axis with d channels turns by base^(-2 i / d) = ratio^i; axis a has the pairs up to pairs_end[a]
+  double ratio[3];
+  int pairs_end[3];
 };
 
 cudaError_t launch_norm_rope_grid(const NormRopeGridParams& p, int head_dim, bool bf16, bool rms, int sm_count, cudaStream_t stream);
 // Bytes behind p.partial that the backward pass needs.
 int64_t norm_rope_grid_scratch_bytes(int head_dim, int sm_count);
-cudaError_t launch_norm_rope_grid_backward(const NormRopeGridParams& p, int head_dim, bool bf16, bool rms, int sm_count, cudaStream_t stream);
+// What the sums become: [D] each, or null.
+struct NormRopeGridSums {
+  void* weight_grad[2];
+  void* bias_grad[2];
+};
+cudaError_t launch_norm_rope_grid_backward(const NormRopeGridParams& p, const NormRopeGridSums& sums, int head_dim, bool bf16, bool rms, int sm_count, cudaStream_t stream);
 
 }  // namespace dtb
