@@ -171,7 +171,8 @@ struct Deal {
   // before it, hence two buffers and one barrier.
   __device__ __forceinline__ void angles(const NormRopeGridParams& p, double2 rate, float2 (*to)[kPairs], int64_t first, int n) const {
     for (int i = threadIdx.x; i < n * kPairs; i += kThreads)
-      if (first + i / kPairs < p.tokens) to[i / kPairs][i % kPairs] = rotation(p, rate, first + i / kPairs, threadIdx.x % kPairs);
+      // (tokens behind the last are padding: what shared memory holds there would be multiplied by 0, and need not be a number)
+      to[i / kPairs][i % kPairs] = first + i / kPairs < p.tokens ? rotation(p, rate, first + i / kPairs, threadIdx.x % kPairs) : make_float2(0.f, 0.f);
     __syncthreads();
   }
 };

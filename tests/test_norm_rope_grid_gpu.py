@@ -374,3 +374,19 @@ def test_no_heads_on_one_side_are_refused():
     x, w = torch.zeros(1, 4, 1, 64, device="cuda"), torch.ones(64, device="cuda")
     with pytest.raises(_capi.ExtensionError):
         ops.norm_rope_grid(x, x[:, :, :0], (w, None, 1e-6), (w, None, 1e-6), ops.GridRope((1, 2, 2), (16, 24, 24)))
+
+
+@pytest.mark.parametrize("H,D", [(1, 64), (3, 64), (24, 64), (1, 128), (8, 128)])
+@pytest.mark.parametrize("tokens", [1, 3, 9, 131])
+def test_what_shared_memory_held_before_does_not_matter(H, D, tokens):
+    """Launches whose last CTA has room for more tokens than there are, behind launches that leave NaN in the shared memory of all SMs."""
+    from ditango_b200 import ops
+    q, k, norms, g = _inputs(1, tokens, H, H, D, torch.float32, True, tokens)
+    dq, dk = (torch.randn(1, tokens, H, D, generator=g).cuda() for _ in range(2))
+    args = (q.cuda(), k.cuda(), *_cuda(norms), _rope((1, 1, tokens), D))
+    want = ops.norm_rope_grid_backward(dq, dk, *args)
+    nan = torch.full((16, 2000, 24, 128), math.nan, dtype=torch.bfloat16, device="cuda")
+    for _ in range(5):
+        ops.flash_window(nan[:, :1], nan, nan, left=1999, right=0)
+        got = ops.norm_rope_grid_backward(dq, dk, *args)
+        assert all(x.isfinite().all() and torch.equal(x, y) for x, y in zip(got, want))
