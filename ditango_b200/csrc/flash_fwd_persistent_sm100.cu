@@ -406,15 +406,21 @@ flash_fwd_persistent_kernel(const __grid_constant__ CUtensorMap tm_q, const __gr
           if (++stage == C::kStages) { stage = 0; round ^= 1; }
           return true;
         };
-        int n = 0, tail = 0, slot = 0;      // of the current item: key tiles, keys of the last one, work slot
+        int n = 0, tail = 0, slot = 0;      // of the current item: key tiles, keys of the last one, work slot (below 0: there is none)
+        // the next item: whether it has keys; one without is given back at once
+        auto look = [&]() {
+          slot = fetch(sh);
+          if (slot < 0) return false;
+          n = sh.s_work[slot].n_tiles;
+          tail = sh.s_work[slot].k_len - (n - 1) * kBN;
+          if (n == 0) mbar_arrive(&sh.work_empty[slot]);
+          return n > 0;
+        };
+        // the next item with keys
         auto next_item = [&]() {
           for (;;) {
-            slot = fetch(sh);
+            if (look()) return true;
             if (slot < 0) return false;
-            n = sh.s_work[slot].n_tiles;
-            tail = sh.s_work[slot].k_len - (n - 1) * kBN;
-            if (n > 0) return true;
-            mbar_arrive(&sh.work_empty[slot]);
           }
         };
         int k_stage = 0, v_stage = 0;
@@ -424,6 +430,10 @@ flash_fwd_persistent_kernel(const __grid_constant__ CUtensorMap tm_q, const __gr
         bool first = true;
         int buf = 0;               // S / P buffer of the next PV; units are numbered through all items
         uint32_t use = 0;          // parity of its barriers
+        auto next_queries = [&]() {
+          q_tile += kQT;
+          if (q_tile == kQT * C::kQBufs) { q_tile = 0; q_use ^= 1; }
+        };
         // S(un) of the current item into buffer `b`: operands, K fetched for the first Q tile ...
         uint64_t s_a = 0, s_b = 0;
         auto ready_s = [&](int un) {
@@ -450,9 +460,22 @@ flash_fwd_persistent_kernel(const __grid_constant__ CUtensorMap tm_q, const __gr
           commit_s(un, b);
           return true;
         };
-        bool ok = next_item();
-        for (int u = 0; ok && u < NB && u < 2 * n; ++u) ok = put_s(u, u);
-        while (ok) {
+        bool ok = true, more = false;       // more: the item's first units are under way, issued as the one before it ended
+        for (;;) {
+          if (!more) {
+            if (slot < 0 || !next_item()) break;
+            if (!first) {          // what the loop below commits when it knows of another item
+              mma_commit(&sh.pv_done[0]);
+              mma_commit(&sh.pv_done[1]);
+              mma_commit(&sh.kv_empty[v_stage]);
+              next_queries();
+            }
+#pragma unroll
+            for (int u = 0, b = buf; ok && u < NB && u < 2 * n; ++u) {
+              ok = put_s(u, b);
+              if (++b == NB) b = 0;
+            }
+          }
           const int n_units = 2 * n;
           for (int u = 0; ok && u < n_units - 2; ++u) {
             const int tile = u & 1;
@@ -483,14 +506,15 @@ flash_fwd_persistent_kernel(const __grid_constant__ CUtensorMap tm_q, const __gr
           }
           // The last key tile, and in the S buffers that its units leave the first units of the next item, so that the softmax
           // warps find their scores while O is still being read: the third buffer is free now, the others behind their PV.
+          // An item without keys is not passed over here: the result warps have it behind this one's O, so that a run of them,
+          // longer than there are slots, would leave the loader waiting for those warps, and them and this thread for each other.
           const int tail_steps = (tail + 15) >> 4;
           const bool one = n == 1;
           ok = ok && next_kv(v_stage, 23) && ((tail & 15) == 0 || wait_or_abort(&sh.v_tail[slot], ((fetched - 1) / kWork) & 1, p.status, 28));
           mbar_arrive(&sh.work_empty[slot]);
-          const bool more = ok && next_item();
+          more = ok && look();
           if (more) {
-            q_tile += kQT;
-            if (q_tile == kQT * C::kQBufs) { q_tile = 0; q_use ^= 1; }
+            next_queries();
             ok = put_s(0, buf == 0 ? NB - 1 : buf - 1);
           }
 #pragma unroll 1
@@ -517,7 +541,7 @@ flash_fwd_persistent_kernel(const __grid_constant__ CUtensorMap tm_q, const __gr
             }
             if (++buf == NB) { buf = 0; use ^= 1; }
           }
-          if (!more) break;
+          if (!ok) break;
           first = false;
           o_use ^= 1;
         }

@@ -245,3 +245,37 @@ def test_two_streams_at_once():
     for w, results in zip(want, got):
         assert all(torch.equal(o, w[0]) and torch.equal(l, w[1]) for o, l in results)
     assert ops.read_status() == 0
+
+
+@pytest.mark.parametrize("lens_k", [[700] + [0] * 15, [300, 0, 129, 0, 0, 640] + [0] * 9 + [17], [0] * 3 + [1] + [0] * 11 + [255]], ids=["first", "mixed", "short"])
+def test_runs_of_sequences_without_keys(lens_k):
+    """More blocks without keys behind one that has some than a CTA has slots for: they are passed, and leave what is folded into as it is."""
+    from ditango_b200 import ops
+    H, Sq, n = 200, 257, len(lens_k)
+    cu_q, cu_k = (torch.tensor([0] + torch.tensor(x).cumsum(0).tolist(), dtype=torch.int32, device="cuda") for x in ([Sq] * n, lens_k))
+    q, k, v = (x[0] for x in _qkv(1, Sq * n, sum(lens_k), H, 64, seed=3))
+    assert 2 * n * H > 5 * 8 * _sms()
+    kw = dict(cu_seqlens_q=cu_q, cu_seqlens_k=cu_k, max_seqlen_q=Sq, max_seqlen_k=max(lens_k), lse_layout=ops.LSE_BSH)
+
+    def check(o, l, empty_out, empty_lse):
+        for s, keys in enumerate(lens_k):
+            rows, at = slice(Sq * s, Sq * (s + 1)), slice(int(cu_k[s]), int(cu_k[s + 1]))
+            if not keys:
+                assert (o[rows] == empty_out).all() and (l[rows] == empty_lse).all()
+                continue
+            for h in (0, H - 1):
+                x = q[rows, h].double() @ k[at, h].double().T / 8
+                assert (o[rows, h].double() - torch.softmax(x, -1) @ v[at, h].double()).abs().max() <= v.double().abs().max() * 2.0 ** -8
+                want = torch.logsumexp(x, -1)
+                assert ((l[rows, h].double() - want).abs() <= 1e-6 * (1 + want.abs())).all()
+
+    out, lse = ops.flash_partial(q, k, v, **kw)
+    assert ops.read_status() == 0
+    check(out, lse, 0.0, -math.inf)
+    again = ops.flash_partial(q, k, v, **kw)
+    assert torch.equal(again[0], out) and torch.equal(again[1], lse)
+    # a state of weight e^-1000 beside what is seen: nothing but the rows without keys keep it
+    o, l = torch.full_like(out, 3.0), torch.full_like(lse, -1000.0)
+    ops.flash_partial(q, k, v, out=o, lse=l, accumulate=True, **kw)
+    check(o, l, 3.0, -1000.0)
+    assert ops.read_status() == 0
