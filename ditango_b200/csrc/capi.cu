@@ -546,8 +546,8 @@ DTB_API int dtb_flash_window(const void* q, const void* k, const void* v,
   p.v_batch = v_batch_stride;
   p.seqlens_k = seqlens_k;
   p.kv_heads = num_kv_heads;
-  p.left = left < 0 ? kFar : left;
-  p.right = right < 0 ? kFar : right;
+  p.left = left;
+  p.right = right;
   p.sinks = sinks;
   p.q_start = q_start;
   p.k_start = k_start;

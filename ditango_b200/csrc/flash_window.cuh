@@ -19,7 +19,7 @@ struct WindowParams {
   int64_t q_tok, q_batch, k_tok, k_batch, v_tok, v_batch;      // elements; packed: no batch strides
   const int32_t* seqlens_k;      // keys of each sequence of a dense batch, or null: all seqlen_k
   int kv_heads;                  // divides f.num_heads
-  int left, right, sinks;        // each within [0, 2^30]
+  int left, right, sinks;        // each within [0, 2^30]; left, right -1: no limit
   int q_start, k_start;          // positions of the first query (or kQueriesLast) and the first key
   // the order of a tensor map's outer axes, the one with the smaller stride first: 1 batch then token, 0 token then batch
   int q_batch_first, k_batch_first, v_batch_first;
@@ -35,8 +35,8 @@ struct WindowSeq {
   int from, to, sinks;
 };
 
+constexpr int kFar = 1 << 30;                       // beyond all keys, and a query's number can still be added
 __device__ __forceinline__ int clamp_position(int64_t x) {
-  constexpr int64_t kFar = 1 << 30;                 // beyond all keys, and a query's number can still be added
   return static_cast<int>(x < -kFar ? -kFar : x > kFar ? kFar : x);
 }
 
@@ -57,8 +57,8 @@ __device__ __forceinline__ WindowSeq window_seq(const WindowParams& p, int seg) 
   s.k_len = max(min(s.k_len, p.f.seqlen_k), 0);
   // the first query's position, counted from the first key
   const int64_t x = p.q_start == kQueriesLast ? static_cast<int64_t>(s.k_len) - s.q_len : static_cast<int64_t>(p.q_start) - p.k_start;
-  s.from = clamp_position(x - p.left);
-  s.to = clamp_position(x + p.right + 1);
+  s.from = p.left < 0 ? -kFar : clamp_position(x - p.left);
+  s.to = p.right < 0 ? kFar : clamp_position(x + p.right + 1);
   s.sinks = max(min(clamp_position(static_cast<int64_t>(p.sinks) - p.k_start), s.k_len), 0);
   return s;
 }

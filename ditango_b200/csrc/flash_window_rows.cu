@@ -343,8 +343,9 @@ cudaError_t launch_window_rows(const WindowParams& p, int sm_count, cudaStream_t
   const int64_t blocks = row_blocks * p.kv_heads * p.f.nseg;
   // as many CTAs to a row block as give every SM one, each with two tiles for every warp (56 blocks of 188 tiles at D = 64: 13.0 us
   // with 4, 14.0 with 8; 24 blocks of 272 tiles at D = 128, 8 CTAs either way: 14.5)
-  const int64_t span = static_cast<int64_t>(p.left) + p.right + p.sinks + kRows;
-  const int64_t tiles = ((span < p.f.seqlen_k ? span : p.f.seqlen_k) + kKeys - 1) / kKeys;
+  int64_t span = static_cast<int64_t>(p.left) + p.right + p.sinks + kRows;
+  if (p.left < 0 || p.right < 0 || span > p.f.seqlen_k) span = p.f.seqlen_k;
+  const int64_t tiles = (span + kKeys - 1) / kKeys;
   int C = 1;
   while (C < kMostCtas && blocks * C < sm_count && tiles > 2 * kWarps * C) C *= 2;
   if ((row_blocks * C + 1) * kRows > 0x7fffffff) return cudaErrorInvalidValue;

@@ -501,3 +501,13 @@ def test_numbers_that_an_int_does_not_hold_are_refused(kw):
     x = torch.zeros(1, 4, 1, 64, dtype=torch.bfloat16, device="cuda")
     with pytest.raises(_capi.ExtensionError):
         ops.flash_window(x, x, x, **kw)
+
+
+@pytest.mark.parametrize("Sq,H", [(1, 2), (40, 2), (300, 24)])
+@pytest.mark.parametrize("left,right,sinks,q_start,k_start", [
+    (-1, 0, 0, 2 ** 30, 0), (-1, 5, 0, 2 ** 30, -2 ** 30), (-1, -1, 0, 2 ** 30, -2 ** 30), (-1, -1, 0, -2 ** 30, 2 ** 30), (40, -1, 0, -2 ** 30, 0),
+    (40, -1, 0, 2 ** 30, -2 ** 30), (2 ** 30, 2 ** 30, 0, 2 ** 30, -2 ** 30)])
+def test_no_limit_is_none_at_any_position(Sq, H, left, right, sinks, q_start, k_start):
+    """At the ends of the positions that are accepted, where a limit of 2^30 does hide keys."""
+    q, k, v = _rand((1, Sq, H, 64), 1), _rand((1, 450, H, 64), 2), _rand((1, 450, H, 64), 3)
+    _run_and_check(q, k, v, left=left, right=right, sinks=sinks, q_start=q_start, k_start=k_start)

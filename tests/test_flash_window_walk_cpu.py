@@ -344,3 +344,25 @@ def test_windows_that_no_end_cuts_take_a_tile_less(replay):
     ev = replay(64, 17776, 17776, 1350, 1350, 226, 0, 0, 1, 30, 70, 1)
     q0, steps, N, n = _blocks(ev)[0][:4]
     assert (q0, N, n, steps) == (256 * 30, 24, 23, 23 + 2)
+
+
+FAR = 2 ** 30
+
+
+@pytest.mark.parametrize("left,right,sinks,q_start,k_start", [
+    (-1, 0, 0, FAR, 0), (-1, 5, 0, FAR, -FAR), (-1, -1, 0, FAR, -FAR), (-1, -1, 0, -FAR, FAR), (40, -1, 0, -FAR, 0), (40, -1, 7, -FAR, FAR),
+    (-1, 0, 0, -FAR, 0), (40, -1, 0, FAR, -FAR), (40, -1, 3, FAR, 0), (FAR, FAR, 0, FAR, -FAR), (FAR, FAR, 0, -FAR, FAR), (FAR, 0, 0, FAR, 0)])
+@pytest.mark.parametrize("splits", [1, 3])
+def test_no_limit_is_none_at_any_position(replay, left, right, sinks, q_start, k_start, splits):
+    """At the ends of the positions that are accepted, where a limit of 2^30 does hide keys."""
+    Sq, Sk = 600, 300
+    seen, blocks = {}, 0
+    for block in range(3 * splits):
+        for q0, steps, N, n, head, part, rows, units in _blocks(replay(64, Sq, Sk, left, right, sinks, q_start, k_start, 1, block, 3 * splits, splits)):
+            blocks += 1
+            for i, first, lo, hi in rows:
+                seen.setdefault(i, []).extend(list(range(first)) + list(range(lo, hi)))
+    assert blocks == 3 * splits and len(seen) == Sq
+    for i, keys in seen.items():
+        x = q_start + i
+        assert sorted(keys) == [j for j in range(Sk) if (right < 0 or j + k_start <= x + right) and (left < 0 or j + k_start >= x - left or j + k_start < sinks)]
