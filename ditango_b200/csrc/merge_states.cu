@@ -69,9 +69,10 @@ __global__ void __launch_bounds__(128) merge_states_kernel(const MergeParams p) 
   const int group_in_warp = (threadIdx.x % 32) / G;
   const unsigned full = 0xffffffffu;
   const int n = p.nstates;
-  const bool shows_nan = p.status != nullptr;
-  if (shows_nan) grid_dependency_wait();               // (launched while the kernel before it ends)
-  if (shows_nan && *reinterpret_cast<const volatile int*>(p.status) != 0) return;
+  if (p.status != nullptr) {
+    grid_dependency_wait();                            // (launched while the kernel before it ends)
+    if (*reinterpret_cast<const volatile int*>(p.status) != 0) return;
+  }
 
   auto load_chunk = [&](int c0, int64_t base, Raw8 (&v)[CH][U]) {
 #pragma unroll
@@ -134,8 +135,8 @@ __global__ void __launch_bounds__(128) merge_states_kernel(const MergeParams p) 
 #pragma unroll
       for (int o = G / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(full, sum, o, G);
 #pragma unroll
-      for (int t = 0; t < kPerLane; ++t) w[u][t] = (sum > 0.f || (shows_nan && sum != 0.f)) ? e[t] / sum : 0.f;
-      lse_out[u] = (sum > 0.f || (shows_nan && sum != 0.f)) ? mx + __logf(sum) : -INFINITY;
+      for (int t = 0; t < kPerLane; ++t) w[u][t] = (sum != 0.f) ? e[t] / sum : 0.f;       // (a NaN among the lse goes on into the result)
+      lse_out[u] = (sum != 0.f) ? mx + __logf(sum) : -INFINITY;
     }
     float acc[U][8];
 #pragma unroll

@@ -20,8 +20,8 @@ struct MergeParams {
   int nstates;
   int H;
   int S;
-  // Null, or for a launch that completes the one of attention before it a status word: the launch may be set up while that one ends, with
-  // the word set nothing is written, and a row with a NaN among its lse becomes NaN (otherwise an empty state).
+  // Null, or for a launch that completes the one of attention before it a status word: the launch may be set up while that one ends, and
+  // with the word set nothing is written.
   const int* status;
 };
 

@@ -203,7 +203,7 @@ DTB_API int64_t dtb_flash_window_scratch_bytes(int nseg, int seqlen_q, int seqle
  *                When it is given, `out` may be NULL and the fp32 result is not written at all.
  *  batch, seq    tokens are [batch, seq]; they matter for DTB_LSE_BHS indexing only.
  *  States whose lse is -inf on a row contribute nothing; a row empty in all states gets
- *  out = 0, lse = -inf.
+ *  out = 0, lse = -inf.  A NaN among a row's lse makes its out and lse NaN.
  */
 DTB_API int dtb_merge_states(int nstates, const void* const* outs, const int* out_dtypes,
                      const float* const* lses, const int* lse_layouts,

@@ -189,3 +189,27 @@ def test_a_nan_among_the_lse_shows():
     lses[0, 0, 2, 1] = math.nan
     out, lse = ops.merge_states([(ops.quantize_rows(outs[0]), lses[0], ops.LSE_BSH), (outs[1], lses[1], ops.LSE_BSH)])
     assert out[0, 2, 1].isnan().all() and int(out.isnan().sum()) == 64 and lse.isnan().nonzero().tolist() == [[0, 2, 1]]
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("kinds", [(F, F), (H16, F), (H16, H16, H16), (F,) * 5, (F, H16) * 8, (F,), (F, I), (E, H16, F)], ids=str)
+def test_a_nan_among_the_lse_shows_whatever_the_states_are_held_in(kinds, D):
+    """In its own row alone, whichever state has it, beside empty states too; a row of empty states stays one."""
+    from ditango_b200 import ops
+    n, shape = len(kinds), (2, 37, 3, D)
+    g = torch.Generator().manual_seed(n)
+    outs, lses = torch.randn(n, *shape, generator=g), torch.randn(n, *shape[:-1], generator=g)
+    lses[:, 0, 4, 1] = -math.inf                 # nothing in any state
+    lses[:, 0, 5, 1], lses[n - 1, 0, 5, 1] = -math.inf, math.nan       # a NaN beside empty states
+    lses[n // 2, 1, 36, 2] = math.nan
+    lses[0, 1, 0, 0] = math.nan
+    bad = [[0, 5, 1], [1, 0, 0], [1, 36, 2]]
+    for layout in (ops.LSE_BSH, ops.LSE_BHS):
+        mine = [(ops.quantize_rows(o.cuda(), k) if k in CODES else o.to(k).cuda(), (l if layout == 1 else l.transpose(1, 2)).contiguous().cuda(), layout)
+                for k, o, l in zip(kinds, outs, lses)]
+        b16 = torch.empty(shape, dtype=torch.bfloat16, device="cuda")
+        out, lse = ops.merge_states(mine, lse_out_layout=layout, out_bf16=b16)
+        lse = lse if layout == 1 else lse.transpose(1, 2)
+        for x in (out, b16):
+            assert x.isnan().all(-1).nonzero().tolist() == bad and int(x.isnan().sum()) == len(bad) * D
+        assert lse.isnan().nonzero().tolist() == bad and (lse == -math.inf).nonzero().tolist() == [[0, 4, 1]] and (out[0, 4, 1] == 0).all()
