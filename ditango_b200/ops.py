@@ -476,11 +476,13 @@ def merge_states(states: Sequence[Tuple[Union[torch.Tensor, QuantizedRows], torc
     """One-pass merge of partial states.  states[i] = (out_i [B,S,H,D] fp32|bf16 contiguous or QuantizedRows,
     lse_i fp32 contiguous, layout_i).  Returns (out fp32 [B,S,H,D], lse_out or None).  With
     fp32_out=False only the bf16 copy `out_bf16` is written and returned in place of `out`.  `out_rows`
-    (QuantizedRows to fill, or the type of new ones: torch.int8, torch.float8_e4m3fn) has the result
-    written in 8 bits too; with fp32_out=False and no `out_bf16` that is what is returned."""
+    (QuantizedRows to fill) has the result written in 8 bits too; with fp32_out=False and no `out_bf16`
+    that is what is returned, and a type (torch.int8, torch.float8_e4m3fn) asks for new ones."""
     if out_rows is not None or QuantizedRows in [type(o) for o, _, _ in states]:
         shape, device = states[0][0].shape, states[0][1].device
         if isinstance(out_rows, torch.dtype):
+            if fp32_out or out_bf16 is not None:
+                raise _capi.ExtensionError("out_rows is a type only where its rows are what is returned: fp32_out=False and no out_bf16")
             out_rows = _new_rows(device, shape, out_rows)
         if not fp32_out:
             out = None

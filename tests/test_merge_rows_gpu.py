@@ -213,3 +213,18 @@ def test_a_nan_among_the_lse_shows_whatever_the_states_are_held_in(kinds, D):
         for x in (out, b16):
             assert x.isnan().all(-1).nonzero().tolist() == bad and int(x.isnan().sum()) == len(bad) * D
         assert lse.isnan().nonzero().tolist() == bad and (lse == -math.inf).nonzero().tolist() == [[0, 4, 1]] and (out[0, 4, 1] == 0).all()
+
+
+@pytest.mark.parametrize("code", CODES)
+def test_results_of_several_types_at_once_are_those_of_separate_calls(code):
+    from ditango_b200 import ops
+    shape = (2, 97, 7, 128)
+    mine, _ = _states(shape, (code, F, code, H16), torch.Generator().manual_seed(3))
+    rows, lse = ops.merge_states(mine, out_rows=code, fp32_out=False)
+    mine_rows, b16 = ops._new_rows("cuda", shape, code), torch.empty(shape, dtype=torch.bfloat16, device="cuda")
+    out, lse2 = ops.merge_states(mine, out_bf16=b16, out_rows=mine_rows)
+    assert torch.equal(mine_rows.values.view(torch.uint8), rows.values.view(torch.uint8)) and torch.equal(mine_rows.exponents, rows.exponents)
+    assert torch.equal(out, ops.merge_states(mine)[0]) and torch.equal(b16, out.to(torch.bfloat16)) and torch.equal(lse, lse2)
+    again = ops._new_rows("cuda", shape, code)
+    got, _ = ops.merge_states(mine, out_bf16=b16, out_rows=again, fp32_out=False)
+    assert got is b16 and torch.equal(again.exponents, rows.exponents)

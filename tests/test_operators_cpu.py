@@ -154,3 +154,18 @@ def test_grid_positions_on_the_cpu_take_the_tables():
     a = norm_and_rotate(q, k, *norms, *rotary_tables(cfg, "cpu"), 3)
     b = norm_and_rotate_grid(q, k, *norms, cfg.grid_rope, 3)
     assert all((x - y).abs().max() < 1e-5 for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(fp32_out=False, out_bf16=True), dict(out_bf16=True), dict(out=True)])
+def test_new_rows_that_the_caller_would_not_get_are_refused(kw):
+    """A merge returns one result: rows beside another one are the caller's."""
+    from ditango_b200 import ops
+    from ditango_b200._capi import ExtensionError
+    x, lse = torch.zeros(1, 2, 3, 64), torch.zeros(1, 2, 3)
+    kw = {k: v if k == "fp32_out" else torch.empty_like(x, dtype=torch.bfloat16 if k == "out_bf16" else torch.float32) for k, v in kw.items()}
+    with pytest.raises(ExtensionError, match="out_rows is a type only"):
+        ops.merge_states([(x, lse, ops.LSE_BSH)], out_rows=torch.int8, **kw)
+    rows = ops._new_rows(x.device, x.shape, torch.int8)
+    for given in (dict(out_rows=torch.int8, fp32_out=False), dict(out_rows=rows, **kw)):     # (taken, and then refused for their device)
+        with pytest.raises(ExtensionError, match="CUDA tensors only"):
+            ops.merge_states([(x, lse, ops.LSE_BSH)], **given)
