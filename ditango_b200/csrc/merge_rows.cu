@@ -184,7 +184,8 @@ __global__ void __launch_bounds__(kThreads) merge_rows_kernel(const __grid_const
         for (int k = 0; k < 8; ++k)
           if (c + k < n) {
             const float l = s_w[c + k][threadIdx.x];
-            s_w[c + k][threadIdx.x] = l == -INFINITY ? 0.f : ex2((l - mx) * 1.4426950408889634f) * scale * power_of(b[k]);
+            const float w = l == -INFINITY ? 0.f : ex2((l - mx) * 1.4426950408889634f) * scale;
+            s_w[c + k][threadIdx.x] = w == 0.f ? 0.f : w * power_of(b[k]);        // (power_of may be infinite)
           }
       }
       if (p.lse_out != nullptr)

@@ -228,3 +228,25 @@ def test_results_of_several_types_at_once_are_those_of_separate_calls(code):
     again = ops._new_rows("cuda", shape, code)
     got, _ = ops.merge_states(mine, out_bf16=b16, out_rows=again, fp32_out=False)
     assert got is b16 and torch.equal(again.exponents, rows.exponents)
+
+
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("gap", [math.inf, 1e4, 200.0])
+def test_a_weight_that_is_0_in_fp32_keeps_what_is_not_finite_out(gap, D, code):
+    """A state that far below the others may hold anything, in 8 bits as in the wide types; a little nearer a NaN shows."""
+    from ditango_b200 import ops
+    shape = (1, 33, 3, D)
+    g = torch.Generator().manual_seed(D)
+    x, bad = torch.randn(shape, generator=g).cuda(), torch.randn(shape, generator=g)
+    bad[0, 5:20, 1, 7], bad[0, 9, 2, 0] = math.nan, math.inf
+    lse = torch.randn(shape[:-1], generator=g).cuda()
+    for kind in (code, F, H16):
+        rows = ops.quantize_rows(bad.cuda(), code) if kind in CODES else bad.to(kind).cuda()
+        mine = [(rows, lse - gap, ops.LSE_BSH), (x, lse, ops.LSE_BSH)]
+        out, out_lse = ops.merge_states(mine)
+        assert torch.equal(out, x) and torch.equal(out_lse, lse)
+        back = ops.merge_states(mine, out_rows=code, fp32_out=False)[0]
+        assert torch.equal(back.exponents, ops.quantize_rows(x, code).exponents) and int(back.exponents.max()) < 255
+        near, _ = ops.merge_states([(rows, lse - 20, ops.LSE_BSH), (x, lse, ops.LSE_BSH)])
+        assert near[0, 5:20, 1].isnan().any() and not near[0, 5:20, 0].isnan().any()
