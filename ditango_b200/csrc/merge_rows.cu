@@ -40,16 +40,19 @@ __device__ __forceinline__ float power_of(uint32_t b) { return __uint_as_float(b
 struct Wide {
   uint4 q[4];
 };
-__device__ __forceinline__ uint4 load16(const void* p) { return __ldg(static_cast<const uint4*>(p)); }
+// Codes and exponents, which no result may take the place of, are read as memory that nobody writes meanwhile; wide values and lse,
+// whose place a result may take, by ordinary loads (plain ones, which the compiler issues in front of the codes' arithmetic: a load
+// that it may not move took a call on one int8 and one fp32 state of 14882 x 24 x 128 from 84 to 94 us).
+__device__ __forceinline__ uint4 load_codes16(const void* p) { return __ldg(static_cast<const uint4*>(p)); }
 __device__ __forceinline__ void load_wide(Wide& w, const void* values, int dtype, int64_t off) {
   if (dtype == kRowsF32) {
     const float* src = static_cast<const float*>(values) + off;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w.q[i] = load16(src + 4 * i);
+    for (int i = 0; i < 4; ++i) w.q[i] = *reinterpret_cast<const uint4*>(src + 4 * i);
   } else {
     const uint16_t* src = static_cast<const uint16_t*>(values) + off;
-    w.q[0] = load16(src);
-    w.q[1] = load16(src + 8);
+    w.q[0] = *reinterpret_cast<const uint4*>(src);
+    w.q[1] = *reinterpret_cast<const uint4*>(src + 8);
   }
 }
 // The values of a lane are eight pairs of fp32.
@@ -150,7 +153,7 @@ __global__ void __launch_bounds__(kThreads) merge_rows_kernel(const __grid_const
   auto load_codes = [&](int c0, int64_t row) {
 #pragma unroll
     for (int k = 0; k < kNarrow; ++k)
-      if (c0 + k < n8 && row < p.rows) code[k] = load16(static_cast<const uint8_t*>(p.values[c0 + k]) + row * D + lane * 16);
+      if (c0 + k < n8 && row < p.rows) code[k] = load_codes16(static_cast<const uint8_t*>(p.values[c0 + k]) + row * D + lane * 16);
   };
   // (under way while the weights are formed)
   load_codes(0, tile + threadIdx.x / G);
@@ -163,7 +166,7 @@ __global__ void __launch_bounds__(kThreads) merge_rows_kernel(const __grid_const
         float l[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k)
-          l[k] = c + k < n ? __ldg(p.lse[c + k] + lse_offset(p.lse_layout[c + k], static_cast<uint32_t>(row), p.H, p.S)) : -INFINITY;
+          l[k] = c + k < n ? p.lse[c + k][lse_offset(p.lse_layout[c + k], static_cast<uint32_t>(row), p.H, p.S)] : -INFINITY;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           if (c + k < n) s_w[c + k][threadIdx.x] = l[k];

@@ -1,5 +1,7 @@
 """What the entry points of the operators refuse, on tensors and pointers that never reach a GPU."""
 import ctypes
+import os
+import re
 
 import pytest
 import torch
@@ -169,3 +171,14 @@ def test_new_rows_that_the_caller_would_not_get_are_refused(kw):
     for given in (dict(out_rows=torch.int8, fp32_out=False), dict(out_rows=rows, **kw)):     # (taken, and then refused for their device)
         with pytest.raises(ExtensionError, match="CUDA tensors only"):
             ops.merge_states([(x, lse, ops.LSE_BSH)], **given)
+
+
+def test_what_a_result_may_take_the_place_of_is_read_by_ordinary_loads():
+    """Loads for memory that stays as it is during a kernel are for codes and exponents alone: dtb_merge_rows may write the result over a
+    state's wide values, and lse_out over its lse."""
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "ditango_b200", "csrc")
+    source = re.sub(r"//[^\n]*", "", open(os.path.join(csrc, "merge_rows.cu")).read())
+    lines = [line for line in source.splitlines() if re.search(r"__ldg|ld\.global\.nc|__restrict__", line)]
+    assert len(lines) == 2 and "load_codes16(const void* p)" in lines[0] and "p.exponents[" in lines[1]
+    uses = [line for line in source.splitlines() if "load_codes16(" in line][1:]
+    assert len(uses) == 1 and "c0 + k < n8" in uses[0]               # the first n8 states are those in 8 bits
