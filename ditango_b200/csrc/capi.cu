@@ -681,6 +681,7 @@ DTB_API int dtb_merge_rows(int nstates, const void* const* outs, const int* out_
       if (lse_layouts[i] != DTB_LSE_BHS && lse_layouts[i] != DTB_LSE_BSH) return fail(DTB_ERR_ARG, "dtb_merge_rows: bad lse layout for state %d", i);
       if ((outs[i] == out_bf16 && t != DTB_BF16) || (outs[i] == out_codes) || (outs[i] == out && t != DTB_F32))
         return fail(DTB_ERR_ARG, "dtb_merge_rows: a result may take the place of a state of its own type only, an 8-bit one of none");
+      if (out_codes && narrow && exponents[i] == out_exponents) return fail(DTB_ERR_ARG, "dtb_merge_rows: the exponents of an 8-bit result are those of state %d", i);
       if (lse_out && lses[i] == lse_out && lse_layouts[i] != lse_out_layout) return fail(DTB_ERR_ARG, "dtb_merge_rows: in-place lse needs matching layouts");
       p.values[at] = outs[i];
       p.exponents[at] = exponents[i];

@@ -222,7 +222,8 @@ DTB_API int dtb_merge_states(int nstates, const void* const* outs, const int* ou
  *  outs[i], out_dtypes[i]   [batch, seq, H, D] contiguous, DTB_F32, DTB_BF16, DTB_I8 or DTB_E4M3
  *  exponents[i]             [batch, seq, H] bytes of a state in 8 bits (not read otherwise)
  *  out, out_bf16, out_codes results in fp32, bf16 and 8 bits (out_codes_dtype, with out_exponents); at least one.  An fp32 or bf16
- *                           result may be the buffer of a state of its type, lse_out that of a state's lse in its layout.
+ *                           result may be the buffer of a state of its type, lse_out that of a state's lse in its layout.  An
+ *                           8-bit result's codes and exponents are buffers of their own.
  */
 DTB_API int dtb_merge_rows(int nstates, const void* const* outs, const int* out_dtypes, const uint8_t* const* exponents,
                      const float* const* lses, const int* lse_layouts,

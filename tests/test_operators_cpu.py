@@ -182,3 +182,10 @@ def test_what_a_result_may_take_the_place_of_is_read_by_ordinary_loads():
     assert len(lines) == 2 and "load_codes16(const void* p)" in lines[0] and "p.exponents[" in lines[1]
     uses = [line for line in source.splitlines() if "load_codes16(" in line][1:]
     assert len(uses) == 1 and "c0 + k < n8" in uses[0]               # the first n8 states are those in 8 bits
+
+
+def test_merge_rows_refuses_a_state_s_exponents_for_the_result():
+    from ditango_b200 import _capi
+    lib = _capi.load()
+    assert _merge_rows(lib, n=2, outs=(16, 32), dts=(0, 3), exps=(None, 48), lses=(16, 16), lays=(1, 1), codes=64, code_e=48) == -1
+    assert "exponents of an 8-bit result" in lib.dtb_last_error().decode()
