@@ -17,6 +17,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -840,7 +841,8 @@ static int grid_rope_params(const char* what, dtb::NormRopeGridParams* p, const 
   for (int i = 0; i < 2; ++i) {
     if (!x[i] || !dst[i] || !weight[i]) return fail(DTB_ERR_ARG, "%s: null tensor pointer", what);
     if (!aligned16(x[i]) || !aligned16(dst[i]) || !aligned16(weight[i]) || !aligned16(bias[i])) return fail(DTB_ERR_ARG, "%s: pointers must be 16-byte aligned", what);
-    if (!(eps[i] > 0.f)) return fail(DTB_ERR_ARG, "%s: eps must be positive", what);
+    // (the kernels count smaller numbers as 0, and 0 has no inverse root)
+    if (!(eps[i] >= FLT_MIN)) return fail(DTB_ERR_ARG, "%s: eps must be positive, and not below the smallest normal float", what);
     if (strides[2 * i] % width || strides[2 * i + 1] % width) return fail(DTB_ERR_ARG, "%s: strides must be multiples of 16 bytes", what);
     p->src[i] = x[i];
     p->tok_stride[i] = strides[2 * i];

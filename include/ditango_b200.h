@@ -277,7 +277,7 @@ DTB_API int dtb_norm_rope(const void* q, void* q_out, const void* q_weight, cons
  *  q, k            dtype DTB_BF16 or DTB_F32 (weights, biases, results and gradients alike): token s of sequence b, head h at
  *                  b * batch_stride + s * tok_stride + h * head_dim, strides multiples of 16 bytes
  *  q_out, k_out    [batch, seq, heads, head_dim] contiguous; they may be q, k where those are contiguous
- *  q_weight, ...   [head_dim]; a bias may be NULL; q_eps, k_eps above 0
+ *  q_weight, ...   [head_dim]; a bias may be NULL; q_eps, k_eps normal numbers above 0
  *  grid, axes      host int[3]: places and channels (even, head_dim in all) of the axes
  *  place           host double[7]: base, origin[3], step[3]
  * Backward: dq_out, dk_out are the gradients of the results, with strides of their own; dq, dk contiguous.  dq_weight ... dk_bias

@@ -189,3 +189,12 @@ def test_merge_rows_refuses_a_state_s_exponents_for_the_result():
     lib = _capi.load()
     assert _merge_rows(lib, n=2, outs=(16, 32), dts=(0, 3), exps=(None, 48), lses=(16, 16), lays=(1, 1), codes=64, code_e=48) == -1
     assert "exponents of an 8-bit result" in lib.dtb_last_error().decode()
+
+
+@pytest.mark.parametrize("back", [False, True])
+@pytest.mark.parametrize("eps", [1e-40, 1.1e-38, -1e-6])
+def test_norm_rope_grid_refuses_an_eps_that_the_kernels_count_as_0(eps, back):
+    from ditango_b200 import _capi
+    lib = _capi.load()
+    assert _grid_rope(lib, back=back, q_eps=eps) == -1 and "eps" in lib.dtb_last_error().decode()
+    assert _grid_rope(lib, back=back, q_eps=1.2e-38, S=0, text=0, video=0) != -1 or "eps" not in lib.dtb_last_error().decode()
