@@ -830,7 +830,7 @@ static int grid_rope_params(const char* what, dtb::NormRopeGridParams* p, const 
     channels += axes[i];
   }
   if (channels != head_dim) return fail(DTB_ERR_ARG, "%s: the axes have %d channels, a head %d", what, channels, head_dim);
-  if (first < 0 || shards < 1) return fail(DTB_ERR_ARG, "%s: first token %lld of %d shards", what, static_cast<long long>(first), shards);
+  if (first < 0 || first > (1ll << 62) || shards < 1) return fail(DTB_ERR_ARG, "%s: first token %lld of %d shards", what, static_cast<long long>(first), shards);
   const int64_t shard_len = places / shards + (places % shards ? 1 : 0);
   if (shard_len * shards >= (1ll << 31)) return fail(DTB_ERR_ARG, "%s: %d shards of %lld tokens", what, shards, static_cast<long long>(shard_len));
   if (!(place[0] > 0.) || !std::isfinite(place[0])) return fail(DTB_ERR_ARG, "%s: base must be positive", what);

@@ -280,6 +280,7 @@ DTB_API int dtb_norm_rope(const void* q, void* q_out, const void* q_weight, cons
  *  q_weight, ...   [head_dim]; a bias may be NULL; q_eps, k_eps normal numbers above 0
  *  grid, axes      host int[3]: places and channels (even, head_dim in all) of the axes
  *  place           host double[7]: base, origin[3], step[3]
+ *  first           0 to 2^62
  * Backward: dq_out, dk_out are the gradients of the results, with strides of their own; dq, dk contiguous.  dq_weight ... dk_bias
  * [head_dim] (each may be NULL) are sums over all rows in a fixed order.  scratch: dtb_norm_rope_grid_scratch_bytes(head_dim) bytes
  * (negative: an error code), 16-byte aligned, of one call at a time.

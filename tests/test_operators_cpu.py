@@ -198,3 +198,11 @@ def test_norm_rope_grid_refuses_an_eps_that_the_kernels_count_as_0(eps, back):
     lib = _capi.load()
     assert _grid_rope(lib, back=back, q_eps=eps) == -1 and "eps" in lib.dtb_last_error().decode()
     assert _grid_rope(lib, back=back, q_eps=1.2e-38, S=0, text=0, video=0) != -1 or "eps" not in lib.dtb_last_error().decode()
+
+
+@pytest.mark.parametrize("back", [False, True])
+@pytest.mark.parametrize("first", [2 ** 63 - 1, 2 ** 62 + 1])
+def test_norm_rope_grid_refuses_a_first_token_that_cannot_be_counted_on_from(first, back):
+    from ditango_b200 import _capi
+    lib = _capi.load()
+    assert _grid_rope(lib, back=back, first=first) == -1 and "first token" in lib.dtb_last_error().decode()
