@@ -626,7 +626,8 @@ def _grid_rope_args(q, k, norms, rope, text_len, video_len):
     grid, axes, base, origin, step, first, shards = rope
     if not 0 < shards < 1 << 31 or not 0 <= first < 1 << 62:
         raise _capi.ExtensionError("shards and first are positions among the pieces")
-    arrays = _rope_arrays(tuple(grid), tuple(axes), base, tuple(origin), tuple(step))
+    # (as plain numbers: what is kept goes by their values, and a tensor among them would be known by its identity)
+    arrays = _rope_arrays(tuple(grid), tuple(axes), float(base), tuple(map(float, origin)), tuple(map(float, step)))
     return shape, kshape, _VALUES[dtype], (*arrays, first, shards, B, S, text_len, video_len, H, kshape[2], D)
 
 

@@ -206,3 +206,15 @@ def test_norm_rope_grid_refuses_a_first_token_that_cannot_be_counted_on_from(fir
     from ditango_b200 import _capi
     lib = _capi.load()
     assert _grid_rope(lib, back=back, first=first) == -1 and "first token" in lib.dtb_last_error().decode()
+
+
+def test_a_grid_s_numbers_are_taken_by_their_values():
+    """A tensor among them that changes in place changes what the next call is given."""
+    from ditango_b200 import ops
+    q, w = torch.zeros(1, 8, 2, 64), torch.ones(64)
+    base, at, step = torch.tensor(1e4), torch.tensor(0.5, dtype=torch.float64), torch.tensor(1.0)
+    rope = ops.GridRope((1, 2, 4), (16, 24, 24), base=base, origin=(0.0, at, 0.0), step=(1.0, 1.0, step))
+    place = lambda: list(ops._grid_rope_args(q, q, ((w, None, 1e-6),) * 2, rope, 0, None)[3][2])
+    assert place() == [1e4, 0.0, 0.5, 0.0, 1.0, 1.0, 1.0]
+    base.fill_(500.0), at.fill_(-3.25), step.fill_(2.0)
+    assert place() == [500.0, 0.0, -3.25, 0.0, 1.0, 1.0, 2.0]
