@@ -34,6 +34,11 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 }
 // 2^(b - 127); 0 for b = 0, infinity for b = 255
 __device__ __forceinline__ float power_of(uint32_t b) { return __uint_as_float(b << 23); }
+// a b where a may be smaller than the smallest normal number (which a plain product counts as 0 under the compiler's fast arithmetic)
+__device__ __forceinline__ float scaled(float a, float b) {
+  asm("mul.rn.f32 %0, %1, %2;" : "=f"(a) : "f"(a), "f"(b));
+  return a;
+}
 
 // The values of a lane are eight pairs of fp32.
 // 16 values of a wide state as loaded: fp32 in all four, bf16 in the first two.
@@ -126,8 +131,8 @@ __device__ __forceinline__ uint32_t encode4(float x0, float x1, float x2, float 
     const uint32_t t2 = __float_as_uint(fmaf(x2, f, kWhole)), t3 = __float_as_uint(fmaf(x3, f, kWhole));
     return __byte_perm(__byte_perm(t0, t1, 0x0040), __byte_perm(t2, t3, 0x0040), 0x5410);
   }
-  return static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(x0 * f, x1 * f), __NV_SATFINITE, __NV_E4M3)) |
-         static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(x2 * f, x3 * f), __NV_SATFINITE, __NV_E4M3)) << 16;
+  return static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(scaled(x0, f), scaled(x1, f)), __NV_SATFINITE, __NV_E4M3)) |
+         static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(scaled(x2, f), scaled(x3, f)), __NV_SATFINITE, __NV_E4M3)) << 16;
 }
 __device__ __forceinline__ float inverse_of(uint32_t b) { return __uint_as_float((254u - b) << 23); }
 

@@ -250,3 +250,27 @@ def test_a_weight_that_is_0_in_fp32_keeps_what_is_not_finite_out(gap, D, code):
         assert torch.equal(back.exponents, ops.quantize_rows(x, code).exponents) and int(back.exponents.max()) < 255
         near, _ = ops.merge_states([(rows, lse - 20, ops.LSE_BSH), (x, lse, ops.LSE_BSH)])
         assert near[0, 5:20, 1].isnan().any() and not near[0, 5:20, 0].isnan().any()
+
+
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("dtype", [F, H16])
+@pytest.mark.parametrize("D", [64, 128])
+def test_values_below_the_smallest_normal_number(D, dtype, code):
+    """Rows whose values are smaller than 2^-126, all of them or some: codes and what they stand for, through a merge too."""
+    from ditango_b200 import ops
+    g = torch.Generator().manual_seed(D)
+    x = (torch.randn(1, 60, 3, D, generator=g).double() * torch.exp2(-100 - torch.arange(60, dtype=torch.float64) / 2)[None, :, None, None]).to(dtype)
+    assert (x.double().abs().amax(-1) < 2.0 ** -126).any()
+    rows = ops.quantize_rows(x.cuda(), code)
+    scale = torch.exp2(127 - rows.exponents.cpu().double())[..., None]
+    assert torch.equal(rows.exponents.cpu().int(), _smallest_exponents(x, code).int())
+    want = (x.double() * scale).round() if code == torch.int8 else (x.double() * scale).float().to(code).float().double()
+    got = rows.values.cpu().double() if code == torch.int8 else rows.values.cpu().float().double()
+    assert torch.equal(got, want) and (got[:, 52:] != 0).any() == (code != torch.int8)
+    for back in (F, H16):
+        assert torch.equal(ops.dequantize_rows(rows, back).cpu().double(), _values(rows))
+    lse = torch.zeros(1, 60, 3, device="cuda")
+    out, _ = ops.merge_states([(rows, lse, ops.LSE_BSH)])
+    assert torch.equal(out.cpu().double(), _values(rows))
+    again, _ = ops.merge_states([(rows, lse, ops.LSE_BSH)], out_rows=code, fp32_out=False)
+    assert torch.equal(_values(again), _values(rows))
