@@ -424,8 +424,9 @@ DTB_API int dtb_flash_fwd_ex(const void* q, const void* k, const void* v,
 
 // Which kernel a launch takes, and the parts that the tiles of 128 split their keys into: what is expected to finish first.  Tiles of 128
 // need a walk over the keys of a block of 256 rows for each round of blocks over the SMs, however few there are; parts shorten it where
-// blocks leave SMs idle, for a merge behind them and states in fp32 (all parts run at once: more than a part per idle SM gained
-// nothing, e.g. 24 heads of 64 with 1024 rows 57.1 us whole, 56.6 in three).  Tiles of 16 rows x 16 keys are spread over all SMs.
+// blocks leave SMs idle, for a merge behind them and states in fp32 (all parts run at once: with 34 tiles of keys more than a part per
+// idle SM gained nothing, e.g. 24 heads of 64 with 1024 rows 57.1 us whole, 56.6 in three; longer walks were not measured so).
+// Tiles of 16 rows x 16 keys are taken to be spread over all SMs, which 8 CTAs to a block of 16 rows cannot do for few key heads.
 // Packed batches are not split: rows behind the last sequence have no state that a merge could leave alone.
 // us in tiles of 16 / of 128 whole / in the best number of parts, each forced:
 //   queries                            32                 64                 256                512                 1024

@@ -41,7 +41,7 @@ class DiTConfig:
     width: int = 90
     text_len: int = 226
     # "tables": rotary tables over the video tokens; "grid": the norm + rotary kernel forms the angles from a token's place in the
-    # latent grid (and has a backward pass of its own), and no table is stored, sharded or read
+    # latent grid, and no table is stored, sharded or read
     rotary: str = "tables"
     # local attention: a video token sees the video tokens of this many frames' worth of positions either way and the text, the text
     # sees everything; None: full attention.  For mode "ulysses", whose ranks (or whose one rank) hold whole sequences; positions are
@@ -217,7 +217,8 @@ class _NormRotateGrid(torch.autograd.Function):
 
 def norm_and_rotate_grid(q, k, norm_q, norm_k, rope, text_len: int, video_len: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """norm_and_rotate with the angles from each video token's place in `rope`'s grid (a GridRope).  On a GPU in bf16 this is one
-    kernel, and its gradients are two; elsewhere the tables are formed and the separate operations run."""
+    kernel, and its gradients are two (for a differentiable attention behind it, which this transformer's is not); elsewhere the tables
+    are formed and the separate operations run."""
     D = q.shape[-1]
     if (q.is_cuda and q.device.index == torch.cuda.current_device() and D in (64, 128) and q.shape == k.shape and
             _plain_bf16(q.device, q, k) and _plain_norm(norm_q, D, q.device) and

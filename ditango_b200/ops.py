@@ -242,10 +242,12 @@ def flash_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, left: int
     Key j of a sequence is at position k_start + j.  Query i is at q_start + i; q_start=None puts the queries at the end of
     their sequence's keys (position i when there are as many queries as keys, the newest positions when the keys are a cache).
 
-    Dense: q [B,Sq,H,D], k,v [B,Sk,Hk,D] bf16, any batch and token strides that are multiples of 8; Hk divides H.  `seqlens_k`
+    Dense: q [B,Sq,H,D], k,v [B,Sk,Hk,D] bf16, any batch and token strides that are multiples of 8 and not below a token's heads
+    (an expanded batch is refused); Hk divides H.  `seqlens_k`
     (int32 [B] on the device) gives the number of keys of each sequence, the rest of Sk may hold anything.  Packed
     (cu_seqlens given): q [Tq,H,D], k,v [Tk,Hk,D].  Returns (out, lse) as flash_partial does, mergeable with its states; with
     accumulate=True the state is merged into the given fp32 (out, lse) in place.  A row that sees no key has out 0 and lse -inf.
+    Scores, sums and states are fp32; a weight is rounded to bf16 (2^-8 of itself at most) for the product with v, as in flash_partial.
     Keys and values that no query near by (in its 256) sees may hold anything, the others must be finite.  Few queries against many
     keys of a dense batch take two launches and scratch from the allocator of the current stream.
     """
