@@ -210,7 +210,9 @@ class _NormRotateGrid(torch.autograd.Function):
     def backward(ctx, dq, dk):
         q, k, q_weight, q_bias, k_weight, k_bias = ctx.saved_tensors
         q_eps, k_eps, rope, text_len, video_len, rms = ctx.rest
-        grads = _engine.norm_rope_grid_backward(dq.contiguous(), dk.contiguous(), q, k, (q_weight, q_bias, q_eps), (k_weight, k_bias, k_eps),
+        # (a part of another gradient may begin anywhere, the kernel takes 16 bytes at a time)
+        dq, dk = (x.clone() if x.data_ptr() % 16 else x for x in (dq.contiguous(), dk.contiguous()))
+        grads = _engine.norm_rope_grid_backward(dq, dk, q, k, (q_weight, q_bias, q_eps), (k_weight, k_bias, k_eps),
                                                 rope, text_len=text_len, video_len=video_len, rms=rms)
         return (*(g if need else None for g, need in zip(grads, ctx.needs_input_grad)), *(None,) * 6)
 

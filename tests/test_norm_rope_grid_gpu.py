@@ -390,3 +390,20 @@ def test_what_shared_memory_held_before_does_not_matter(H, D, tokens):
         ops.flash_window(nan[:, :1], nan, nan, left=1999, right=0)
         got = ops.norm_rope_grid_backward(dq, dk, *args)
         assert all(x.isfinite().all() and torch.equal(x, y) for x, y in zip(got, want))
+
+
+@pytest.mark.parametrize("front", [1, 3, 8])
+def test_a_gradient_that_begins_anywhere_in_memory(front):
+    """Behind `front` other values of one tensor, as the gradient of a concatenation does."""
+    from ditango_b200.executor.cogvideox_dit import norm_and_rotate_grid
+    torch.manual_seed(2)
+    rope = _rope((2, 3, 4), 64)
+    nq, nk = (nn.LayerNorm(64, eps=1e-6).cuda().to(torch.bfloat16) for _ in range(2))
+    x = torch.randn(1, 24, 2, 64, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    leaves = [x, *nq.parameters(), *nk.parameters()]
+    dz = torch.randn(front + 2 * x.numel(), device="cuda").to(torch.bfloat16)
+    outs = norm_and_rotate_grid(x, x, nq, nk, rope, 0)
+    got = torch.autograd.grad(torch.cat([x.new_zeros(front), *(o.flatten() for o in outs)]), leaves, dz)
+    a, b = (d.clone().view_as(x) for d in dz[front:].chunk(2))
+    want = torch.autograd.grad(norm_and_rotate_grid(x, x, nq, nk, rope, 0), leaves, (a, b))
+    assert all(torch.equal(g, w) for g, w in zip(got, want))
