@@ -218,13 +218,14 @@ class _NormRotateGrid(torch.autograd.Function):
 
 
 def norm_and_rotate_grid(q, k, norm_q, norm_k, rope, text_len: int, video_len: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor]:
-    """norm_and_rotate with the angles from each video token's place in `rope`'s grid (a GridRope).  On a GPU in bf16 this is one
-    kernel, and its gradients are two (for a differentiable attention behind it, which this transformer's is not); elsewhere the tables
+    """norm_and_rotate with the angles from each video token's place in `rope`'s grid (a GridRope).  On a GPU in bf16, with an eps
+    that the kernel takes, this is one kernel, and its gradients are two (for a differentiable attention behind it, which this transformer's is not); elsewhere the tables
     are formed and the separate operations run."""
     D = q.shape[-1]
     if (q.is_cuda and q.device.index == torch.cuda.current_device() and D in (64, 128) and q.shape == k.shape and
             _plain_bf16(q.device, q, k) and _plain_norm(norm_q, D, q.device) and
-            _plain_norm(norm_k, D, q.device) and not torch.is_autocast_enabled("cuda")):
+            _plain_norm(norm_k, D, q.device) and min(norm_q.eps, norm_k.eps) >= torch.finfo(torch.float32).tiny and
+            not torch.is_autocast_enabled("cuda")):
         args = (q, k, norm_q.weight, norm_q.bias, norm_k.weight, norm_k.bias)
         rest = (norm_q.eps, norm_k.eps, rope, text_len, video_len, False)
         if torch.is_grad_enabled() and any(x.requires_grad for x in args):

@@ -407,3 +407,22 @@ def test_a_gradient_that_begins_anywhere_in_memory(front):
     a, b = (d.clone().view_as(x) for d in dz[front:].chunk(2))
     want = torch.autograd.grad(norm_and_rotate_grid(x, x, nq, nk, rope, 0), leaves, (a, b))
     assert all(torch.equal(g, w) for g, w in zip(got, want))
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e-40])
+def test_norms_without_an_eps_take_the_separate_operations(eps):
+    """What has an inverse root without one (no row is constant here) stays as it was; the kernel refuses such an eps."""
+    from ditango_b200 import _capi, ops
+    from ditango_b200.executor.cogvideox_dit import norm_and_rotate_grid
+    torch.manual_seed(3)
+    rope = _rope((2, 3, 4), 64)
+    q, k = (torch.randn(1, 24, 2, 64, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    nq, nk = (nn.LayerNorm(64, eps=e).cuda().to(torch.bfloat16) for e in (eps, 1e-6))
+    for norms in ((nq, nk), (nk, nq)):
+        n = ops.LaunchLog.count
+        outs = norm_and_rotate_grid(q, k, *norms, rope, 0)
+        assert ops.LaunchLog.count == n
+        for a, b in zip(outs, norm_and_rotate_grid(q, k, nk, nk, rope, 0)):     # (1e-6 beside a variance of 1; bf16 at every step)
+            assert (a.float() - b.float()).abs().max() <= 2.0 ** -5 * b.float().abs().max()
+        with pytest.raises(_capi.ExtensionError, match="eps"):
+            ops.norm_rope_grid(q, k, *((m.weight, m.bias, m.eps) for m in norms), rope)
