@@ -22,7 +22,8 @@ EXPORTS = (
     "dtb_version", "dtb_last_error", "dtb_device_supported", "dtb_read_status",
     "dtb_peek_status_async", "dtb_post_status",
     "dtb_ipc_export_mem", "dtb_ipc_open_mem", "dtb_ipc_close_mem", "dtb_peer_copy_async",
-    "dtb_flash_fwd", "dtb_flash_fwd_ex", "dtb_flash_window", "dtb_flash_window_scratch_bytes", "dtb_merge_states", "dtb_merge_rows", "dtb_quantize_rows",
+    "dtb_flash_fwd", "dtb_flash_fwd_ex", "dtb_flash_window", "dtb_flash_window_scratch_bytes",
+    "dtb_extend_pages", "dtb_release_pages", "dtb_write_pages", "dtb_flash_paged", "dtb_flash_paged_scratch_bytes", "dtb_merge_states", "dtb_merge_rows", "dtb_quantize_rows",
     "dtb_dequantize_rows", "dtb_copy_chunks",
     "dtb_norm_rope", "dtb_norm_rope_grid", "dtb_norm_rope_grid_scratch_bytes", "dtb_norm_rope_grid_backward", "dtb_ln_modulate", "dtb_gate_add", "dtb_drift_scratch_bytes", "dtb_drift_accumulate",
     "dtb_drift_noalloc_max_elements", "dtb_drift_accumulate_noalloc",
@@ -79,6 +80,16 @@ def load():
         c_int, c_int, c_int, c_int64, c_int64, c_int, c_int, c_int, c_float, c_int, c_int, c_int, c_int, c_int, c_void_p, c_int64, c_void_p]
     lib.dtb_flash_window_scratch_bytes.restype = c_int64
     lib.dtb_flash_window_scratch_bytes.argtypes = [c_int] * 9
+    lib.dtb_extend_pages.restype = lib.dtb_release_pages.restype = lib.dtb_write_pages.restype = lib.dtb_flash_paged.restype = c_int
+    lib.dtb_extend_pages.argtypes = [c_void_p] * 5 + [c_int] * 4 + [c_void_p, c_int64] + [c_void_p] * 5
+    lib.dtb_release_pages.argtypes = [c_void_p] * 7 + [c_int] * 4 + [c_void_p] * 3
+    pool = [c_void_p, c_int64, c_int64, c_int64]
+    lib.dtb_write_pages.argtypes = [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p] + pool * 2 + [c_int] * 4 + [c_void_p]
+    lib.dtb_flash_paged.argtypes = (
+        [c_void_p, c_int64, c_int64] + pool * 2 + [c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int] +
+        [c_int, c_int, c_int, c_int64, c_int, c_int, c_int, c_float, c_int, c_int, c_int, c_void_p, c_int64, c_void_p])
+    lib.dtb_flash_paged_scratch_bytes.restype = c_int64
+    lib.dtb_flash_paged_scratch_bytes.argtypes = [c_int] * 6
     lib.dtb_merge_states.restype = c_int
     lib.dtb_merge_states.argtypes = [
         c_int, POINTER(c_void_p), POINTER(c_int), POINTER(c_void_p), POINTER(c_int),

@@ -3,6 +3,7 @@
 #include "../../include/ditango_b200.h"
 
 #include "flash_fwd_sm100.cuh"
+#include "flash_paged.cuh"
 #include "flash_window.cuh"
 #include "drift_stats.cuh"
 #include "errors.cuh"
@@ -11,6 +12,7 @@
 #include "norm_mod.cuh"
 #include "norm_rope.cuh"
 #include "norm_rope_grid.cuh"
+#include "pages.cuh"
 
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -141,6 +143,25 @@ int make_token_map(CUtensorMap* tm, const void* base, int64_t width, int64_t tok
                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   *batch_first = swap ? 1 : 0;
+  if (r != CUDA_SUCCESS) return fail(DTB_ERR_CUDA, "cuTensorMapEncodeTiled(%s) failed with CUresult %d", what, static_cast<int>(r));
+  return DTB_OK;
+}
+
+// 4-D bf16 view of a pool of pages [channel, token, head, page] for boxes of 64 channels x box_rows tokens, of token and head the one with the
+// smaller stride first; *head_first says which one that is.
+int make_page_map(CUtensorMap* tm, const void* base, int64_t head_dim, int64_t page_size, int64_t tok_stride, int64_t heads, int64_t head_stride,
+                  int64_t pages, int64_t page_stride, int box_rows, int* head_first, const char* what) {
+  const bool swap = head_stride < tok_stride;
+  const int64_t inner = swap ? heads : page_size, outer = swap ? page_size : heads;
+  cuuint64_t gdim[4] = {static_cast<cuuint64_t>(head_dim), static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(outer), static_cast<cuuint64_t>(pages)};
+  cuuint64_t gstride[3] = {static_cast<cuuint64_t>(swap ? head_stride : tok_stride) * 2, static_cast<cuuint64_t>(swap ? tok_stride : head_stride) * 2,
+                           static_cast<cuuint64_t>(page_stride) * 2};
+  cuuint32_t box[4] = {64, swap ? 1u : static_cast<cuuint32_t>(box_rows), swap ? static_cast<cuuint32_t>(box_rows) : 1u, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult r = g_encode(tm, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), gdim, gstride, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  *head_first = swap ? 1 : 0;
   if (r != CUDA_SUCCESS) return fail(DTB_ERR_CUDA, "cuTensorMapEncodeTiled(%s) failed with CUresult %d", what, static_cast<int>(r));
   return DTB_OK;
 }
@@ -605,6 +626,256 @@ DTB_API int dtb_flash_window(const void* q, const void* k, const void* v,
     e = head_dim == 64 ? dtb::launch_window_rows<64>(p, d->sm_count, s) : dtb::launch_window_rows<128>(p, d->sm_count, s);
   }
   if (e != cudaSuccess) return fail(DTB_ERR_CUDA, "dtb_flash_window launch failed: %s", cudaGetErrorString(e));
+  return DTB_OK;
+}
+
+// Pages hold a power of two of tokens, 16 at least; returns the exponent, or -1.
+static int page_shift_of(int page_size) {
+  if (page_size < 16 || page_size > (1 << 20) || (page_size & (page_size - 1))) return -1;
+  int shift = 0;
+  while ((1 << shift) < page_size) ++shift;
+  return shift;
+}
+
+// What the table's rows and the pool may be: [streams, columns] and pages of 1 << shift tokens, all numbers of tokens in 31 bits.
+static int check_table(const char* what, int streams, int columns, int pages, int shift) {
+  if (streams < 1 || columns < 1 || pages < 1) return fail(DTB_ERR_ARG, "%s: a table of %d x %d and %d pages", what, streams, columns, pages);
+  if (shift < 0) return fail(DTB_ERR_ARG, "%s: a page size is a power of two from 16 to 2^20", what);
+  if ((static_cast<int64_t>(columns) << shift) >= (1ll << 30) || (static_cast<int64_t>(pages) << shift) >= (1ll << 31))
+    return fail(DTB_ERR_ARG, "%s: too many tokens in a row of the table or in the pool", what);
+  return DTB_OK;
+}
+
+DTB_API int dtb_extend_pages(int32_t* table, const int32_t* seqlens, const int32_t* new_lens, const int32_t* free_pages, const int32_t* free_count,
+                             int streams, int columns, int pages, int page_size, int32_t* slots, int64_t tokens, int32_t* cu_seqlens,
+                             int32_t* seqlens_out, int32_t* free_count_out, int32_t* missing, void* stream) {
+  const int shift = page_shift_of(page_size);
+  int rc = check_table("dtb_extend_pages", streams, columns, pages, shift);
+  if (rc != DTB_OK) return rc;
+  if (streams > dtb::kMostStreams) return fail(DTB_ERR_ARG, "dtb_extend_pages: more than %d streams", dtb::kMostStreams);
+  if (!table || !seqlens || !new_lens || !free_pages || !free_count || !cu_seqlens || !seqlens_out || !free_count_out || !missing || (!slots && tokens))
+    return fail(DTB_ERR_ARG, "dtb_extend_pages: null pointer");
+  if (tokens < 0 || tokens >= (1ll << 31) - 4) return fail(DTB_ERR_ARG, "dtb_extend_pages: %lld tokens", static_cast<long long>(tokens));
+  if (!aligned16(slots)) return fail(DTB_ERR_ARG, "dtb_extend_pages: slots must be 16-byte aligned");
+  DeviceInfo* d = nullptr;
+  if ((rc = device_info(&d)) != DTB_OK) return rc;
+  const dtb::ExtendParams p = {table, seqlens, new_lens, free_pages, free_count, slots, cu_seqlens, seqlens_out, free_count_out, missing,
+                               streams, columns, pages, shift, static_cast<int>(tokens)};
+  const cudaError_t e = dtb::launch_extend_pages(p, d->sm_count, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return fail(DTB_ERR_CUDA, "dtb_extend_pages launch failed: %s", cudaGetErrorString(e));
+  return DTB_OK;
+}
+
+DTB_API int dtb_release_pages(const int32_t* table, int32_t* table_out, const int32_t* seqlens, const int32_t* begin, const int32_t* end,
+                              int32_t* free_pages, const int32_t* free_count, int streams, int columns, int pages, int page_size,
+                              int32_t* seqlens_out, int32_t* free_count_out, void* stream) {
+  const int shift = page_shift_of(page_size);
+  int rc = check_table("dtb_release_pages", streams, columns, pages, shift);
+  if (rc != DTB_OK) return rc;
+  if (!table || !table_out || !seqlens || !begin || !end || !free_pages || !free_count || !seqlens_out || !free_count_out)
+    return fail(DTB_ERR_ARG, "dtb_release_pages: null pointer");
+  const int64_t items = static_cast<int64_t>(streams) * ((columns + dtb::kReleaseColumns - 1) / dtb::kReleaseColumns);
+  if (items > static_cast<int64_t>(dtb::kReleaseItems) * dtb::kReleaseCtas)
+    return fail(DTB_ERR_ARG, "dtb_release_pages: a table of %d x %d is too large", streams, columns);
+  DeviceInfo* d = nullptr;
+  if ((rc = device_info(&d)) != DTB_OK) return rc;
+  const dtb::ReleaseParams p = {table, table_out, seqlens, begin, end, free_pages, free_count, seqlens_out, free_count_out, streams, columns, pages, shift};
+  const cudaError_t e = dtb::launch_release_pages(p, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return fail(DTB_ERR_CUDA, "dtb_release_pages launch failed: %s", cudaGetErrorString(e));
+  return DTB_OK;
+}
+
+// Strides of a pool [pages, P, heads, head_dim]: multiples of 16 bytes, and none below what lies inside.
+static int check_pool(const char* what, const char* name, const void* base, int pages, int page_size, int heads, int head_dim, int64_t page_stride,
+                      int64_t tok_stride, int64_t head_stride) {
+  if (!base) return fail(DTB_ERR_ARG, "%s: null tensor pointer", what);
+  if (!aligned16(base) || ((page_stride | tok_stride | head_stride) & 7)) return fail(DTB_ERR_ARG, "%s: %s must be 16-byte aligned, strides multiples of 8 elements", what, name);
+  if (tok_stride < head_dim || head_stride < head_dim || page_stride < head_dim || std::max(page_stride, std::max(tok_stride, head_stride)) >= (1ll << 38))
+    return fail(DTB_ERR_ARG, "%s: %s has a stride below a row's %d elements or beyond 2^38", what, name, head_dim);
+  // (of each two axes that are stepped along, one lies within a step of the other)
+  auto apart = [](int64_t na, int64_t sa, int64_t nb, int64_t sb) { return na == 1 || nb == 1 || sa >= nb * sb || sb >= na * sa; };
+  if (!apart(page_size, tok_stride, heads, head_stride) || !apart(pages, page_stride, page_size, tok_stride) || !apart(pages, page_stride, heads, head_stride))
+    return fail(DTB_ERR_ARG, "%s: %s has strides by which elements lie over one another", what, name);
+  return DTB_OK;
+}
+
+DTB_API int dtb_write_pages(const void* k, const void* v, int64_t k_tok_stride, int64_t v_tok_stride, int64_t tokens, const int32_t* slots,
+                            void* k_pages, int64_t k_page_stride, int64_t k_page_tok_stride, int64_t k_head_stride,
+                            void* v_pages, int64_t v_page_stride, int64_t v_page_tok_stride, int64_t v_head_stride,
+                            int pages, int page_size, int num_kv_heads, int head_dim, void* stream) {
+  const int shift = page_shift_of(page_size);
+  int rc = check_table("dtb_write_pages", 1, 1, pages, shift);
+  if (rc != DTB_OK) return rc;
+  if (head_dim != 64 && head_dim != 128) return fail(DTB_ERR_ARG, "dtb_write_pages: head_dim %d not in {64, 128}", head_dim);
+  if (num_kv_heads < 1 || num_kv_heads > 65535) return fail(DTB_ERR_ARG, "dtb_write_pages: %d key heads", num_kv_heads);
+  if (tokens < 0 || tokens >= (1ll << 31)) return fail(DTB_ERR_ARG, "dtb_write_pages: %lld tokens", static_cast<long long>(tokens));
+  if (!k || !v || !slots) return fail(DTB_ERR_ARG, "dtb_write_pages: null tensor pointer");
+  const int64_t width = static_cast<int64_t>(num_kv_heads) * head_dim;
+  if (k_tok_stride < width || v_tok_stride < width || ((k_tok_stride | v_tok_stride) & 7) || !aligned16(k) || !aligned16(v))
+    return fail(DTB_ERR_ARG, "dtb_write_pages: tokens must be 16-byte aligned, their strides multiples of 8 elements and not below the heads");
+  if ((rc = check_pool("dtb_write_pages", "k_pages", k_pages, pages, page_size, num_kv_heads, head_dim, k_page_stride, k_page_tok_stride, k_head_stride)) != DTB_OK ||
+      (rc = check_pool("dtb_write_pages", "v_pages", v_pages, pages, page_size, num_kv_heads, head_dim, v_page_stride, v_page_tok_stride, v_head_stride)) != DTB_OK)
+    return rc;
+  DeviceInfo* d = nullptr;
+  if ((rc = device_info(&d)) != DTB_OK) return rc;
+  if (tokens == 0) return DTB_OK;
+  dtb::WriteParams p = {};
+  p.src[0] = static_cast<const uint16_t*>(k);
+  p.src[1] = static_cast<const uint16_t*>(v);
+  p.src_tok[0] = k_tok_stride;
+  p.src_tok[1] = v_tok_stride;
+  p.dst[0] = static_cast<uint16_t*>(k_pages);
+  p.dst[1] = static_cast<uint16_t*>(v_pages);
+  p.dst_page[0] = k_page_stride;
+  p.dst_page[1] = v_page_stride;
+  p.dst_tok[0] = k_page_tok_stride;
+  p.dst_tok[1] = v_page_tok_stride;
+  p.dst_head[0] = k_head_stride;
+  p.dst_head[1] = v_head_stride;
+  p.slots = slots;
+  p.tokens = static_cast<int>(tokens);
+  p.heads = num_kv_heads;
+  p.head_shift = head_dim == 64 ? 6 : 7;
+  p.page_shift = shift;
+  p.capacity = static_cast<int64_t>(pages) << shift;
+  const cudaError_t e = dtb::launch_write_pages(p, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return fail(DTB_ERR_CUDA, "dtb_write_pages launch failed: %s", cudaGetErrorString(e));
+  return DTB_OK;
+}
+
+// Which kernels a launch over pages takes.
+struct PagedPlan {
+  int few_rows;                  // sequences with at most this many queries go to the kernel of few rows; -1: none do
+  bool tiles;                    // there may be others
+  dtb::PagedRowsPlan rows;
+  int64_t scratch_bytes;
+};
+static PagedPlan plan_paged(int64_t nseg, int64_t seqlen_q, int64_t seqlen_k, int64_t num_heads, int64_t kv_heads, int head_dim, int sm_count) {
+  PagedPlan plan = {};
+  const int64_t group = num_heads / kv_heads;
+  plan.few_rows = static_cast<int>(std::max<int64_t>(128 / group, 1));
+  plan.tiles = seqlen_q > plan.few_rows;
+  plan.rows = dtb::plan_paged_rows(static_cast<int>(std::min<int64_t>(std::min<int64_t>(seqlen_q, plan.few_rows) * group, 64)), head_dim, sm_count);
+  plan.scratch_bytes = plan.rows.scratch_bytes;
+  return plan;
+}
+
+static int check_paged_shape(const char* what, int nseg, int seqlen_q, int seqlen_k, int num_heads, int num_kv_heads, int head_dim) {
+  if (head_dim != 64 && head_dim != 128) return fail(DTB_ERR_ARG, "%s: head_dim %d not in {64, 128}", what, head_dim);
+  if (num_heads < 1 || num_heads > 65535 || num_kv_heads < 1 || num_heads % num_kv_heads) return fail(DTB_ERR_ARG, "%s: %d query heads over %d key heads", what, num_heads, num_kv_heads);
+  if (nseg < 1 || nseg > 65535) return fail(DTB_ERR_ARG, "%s: nseg %d out of range", what, nseg);
+  if (seqlen_q < 0 || seqlen_k < 0 || seqlen_q >= (1 << 30) || seqlen_k >= (1 << 30)) return fail(DTB_ERR_ARG, "%s: length out of range", what);
+  if (static_cast<int64_t>(seqlen_q) * num_heads >= (1ll << 31)) return fail(DTB_ERR_ARG, "%s: too many rows in a sequence", what);
+  return DTB_OK;
+}
+
+DTB_API int64_t dtb_flash_paged_scratch_bytes(int nseg, int seqlen_q, int seqlen_k, int num_heads, int num_kv_heads, int head_dim) {
+  int rc = check_paged_shape("dtb_flash_paged_scratch_bytes", nseg, seqlen_q, seqlen_k, num_heads, num_kv_heads, head_dim);
+  if (rc != DTB_OK) return rc;
+  DeviceInfo* d = nullptr;
+  if ((rc = device_info(&d)) != DTB_OK) return rc;
+  return plan_paged(nseg, seqlen_q, seqlen_k, num_heads, num_kv_heads, head_dim, d->sm_count).scratch_bytes;
+}
+
+DTB_API int dtb_flash_paged(const void* q, int64_t q_tok_stride, int64_t q_batch_stride,
+                            const void* k_pages, int64_t k_page_stride, int64_t k_tok_stride, int64_t k_head_stride,
+                            const void* v_pages, int64_t v_page_stride, int64_t v_tok_stride, int64_t v_head_stride,
+                            int pages, int page_size, const int32_t* table, int columns, const int32_t* seqlens_k, const int32_t* cu_seqlens_q,
+                            void* out, int out_dtype, float* lse, int lse_layout, int accumulate,
+                            int nseg, int seqlen_q, int seqlen_k, int64_t total_q, int num_heads, int num_kv_heads, int head_dim, float softmax_scale,
+                            int left, int right, int sinks, void* scratch, int64_t scratch_bytes, void* stream) {
+  constexpr const char* kWhat = "dtb_flash_paged";
+  int rc = check_paged_shape(kWhat, nseg, seqlen_q, seqlen_k, num_heads, num_kv_heads, head_dim);
+  if (rc != DTB_OK) return rc;
+  const int shift = page_shift_of(page_size);
+  if ((rc = check_table(kWhat, nseg, columns, pages, shift)) != DTB_OK) return rc;
+  if ((static_cast<int64_t>(nseg) * columns << shift) >= (1ll << 31)) return fail(DTB_ERR_ARG, "%s: the table's %d rows have room for 2^31 tokens or more", kWhat, nseg);
+  if (!q || !out || !lse || !table || !seqlens_k) return fail(DTB_ERR_ARG, "%s: null tensor pointer", kWhat);
+  if (total_q < 0 || total_q >= (1ll << 31)) return fail(DTB_ERR_ARG, "%s: too many tokens", kWhat);
+  if (cu_seqlens_q == nullptr && static_cast<int64_t>(nseg) * seqlen_q != total_q) return fail(DTB_ERR_ARG, "%s: total tokens are not nseg*seqlen", kWhat);
+  constexpr int kFar = 1 << 30;
+  if (left < -1 || right < -1 || sinks < 0 || left > kFar || right > kFar || sinks > kFar) return fail(DTB_ERR_ARG, "%s: window (%d, %d) or sinks %d out of range", kWhat, left, right, sinks);
+  const int64_t q_width = static_cast<int64_t>(num_heads) * head_dim;
+  if (q_tok_stride < q_width || (cu_seqlens_q == nullptr && nseg > 1 && q_batch_stride < q_width)) return fail(DTB_ERR_ARG, "%s: q's stride smaller than the heads", kWhat);
+  if ((q_tok_stride | q_batch_stride) & 7) return fail(DTB_ERR_ARG, "%s: strides must be multiples of 8 elements", kWhat);
+  if (!aligned16(q) || !aligned16(out)) return fail(DTB_ERR_ARG, "%s: tensor pointers must be 16-byte aligned", kWhat);
+  if ((rc = check_pool(kWhat, "k_pages", k_pages, pages, page_size, num_kv_heads, head_dim, k_page_stride, k_tok_stride, k_head_stride)) != DTB_OK ||
+      (rc = check_pool(kWhat, "v_pages", v_pages, pages, page_size, num_kv_heads, head_dim, v_page_stride, v_tok_stride, v_head_stride)) != DTB_OK)
+    return rc;
+  if (out_dtype != DTB_F32 && out_dtype != DTB_BF16) return fail(DTB_ERR_ARG, "%s: bad out_dtype %d", kWhat, out_dtype);
+  if (lse_layout != DTB_LSE_BHS && lse_layout != DTB_LSE_BSH) return fail(DTB_ERR_ARG, "%s: bad lse_layout %d", kWhat, lse_layout);
+  if (accumulate && out_dtype != DTB_F32) return fail(DTB_ERR_ARG, "%s: accumulate needs an fp32 state", kWhat);
+  if (!(softmax_scale > 0.f)) return fail(DTB_ERR_ARG, "%s: softmax_scale must be positive", kWhat);
+  if (!scratch || !aligned16(scratch)) return fail(DTB_ERR_ARG, "%s: scratch must be given and 16-byte aligned", kWhat);
+  DeviceInfo* d = nullptr;
+  if ((rc = device_info(&d)) != DTB_OK) return rc;
+  if (seqlen_q == 0 || total_q == 0) return DTB_OK;
+  const PagedPlan plan = plan_paged(nseg, seqlen_q, seqlen_k, num_heads, num_kv_heads, head_dim, d->sm_count);
+  if (scratch_bytes < plan.scratch_bytes)
+    return fail(DTB_ERR_ARG, "%s: scratch of %lld bytes is smaller than the %lld needed", kWhat, static_cast<long long>(scratch_bytes),
+                static_cast<long long>(plan.scratch_bytes));
+
+  dtb::PagedParams p;
+  memset(&p, 0, sizeof(p));
+  p.f.out = out;
+  p.f.lse = lse;
+  p.f.cu_q = cu_seqlens_q;
+  p.f.status = d->status_ptr;
+  p.f.out_tok_stride = q_width;
+  p.f.total_q = total_q;
+  p.f.nseg = nseg;
+  p.f.seqlen_q = seqlen_q;
+  p.f.seqlen_k = seqlen_k;
+  p.f.num_heads = num_heads;
+  p.f.scale_log2 = softmax_scale * 1.4426950408889634f;
+  p.f.out_dtype = out_dtype;
+  p.f.lse_layout = lse_layout;
+  p.f.accumulate = accumulate ? 1 : 0;
+  p.q = static_cast<const uint16_t*>(q);
+  p.q_tok = q_tok_stride;
+  p.q_batch = q_batch_stride;
+  p.seqlens_k = seqlens_k;
+  p.kv_heads = num_kv_heads;
+  p.left = left;
+  p.right = right;
+  p.sinks = left < 0 ? 0 : sinks;             // (all are seen as it is)
+  p.q_start = DTB_QUERIES_LAST;
+  p.splits = 1;
+  p.table = table;
+  p.columns = columns;
+  p.pages = pages;
+  p.page_shift = shift;
+  p.few_rows = plan.few_rows;
+  if ((rc = load_encoder()) != DTB_OK) return rc;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  dtb::PagedMap mk, mv;
+  auto make_maps = [&](int box_rows) {
+    for (dtb::PagedMap* m : {&mk, &mv}) {
+      m->table = table;
+      m->columns = columns;
+      m->pages = pages;
+      m->page_shift = shift;
+      m->box_rows = box_rows;
+      m->dim_shift = head_dim == 64 ? 6 : 7;
+    }
+    p.box_rows = p.key_align = box_rows;
+    const int r = make_page_map(&mk.map, k_pages, head_dim, page_size, k_tok_stride, num_kv_heads, k_head_stride, pages, k_page_stride, box_rows, &p.k_batch_first, "k_pages");
+    return r != DTB_OK ? r : make_page_map(&mv.map, v_pages, head_dim, page_size, v_tok_stride, num_kv_heads, v_head_stride, pages, v_page_stride, box_rows, &p.v_batch_first, "v_pages");
+  };
+  cudaError_t e = cudaSuccess;
+  if (plan.tiles) {
+    // (with a limit to the left runs begin anywhere, and fewer than 16 keys in front of them are cleared)
+    if ((rc = make_maps(left < 0 ? std::min(page_size, 128) : 16)) != DTB_OK) return rc;
+    const bool packed = cu_seqlens_q != nullptr;
+    CUtensorMap tq;
+    if ((rc = make_token_map(&tq, q, q_width, packed ? total_q : seqlen_q, q_tok_stride, packed ? 1 : nseg, q_batch_stride, &p.q_batch_first, "q")) != DTB_OK) return rc;
+    e = head_dim == 64 ? dtb::launch_paged_tiles<64>(tq, mk, mv, p, s) : dtb::launch_paged_tiles<128>(tq, mk, mv, p, s);
+  }
+  if (e == cudaSuccess && (!plan.tiles || (cu_seqlens_q != nullptr && nseg > 1))) {
+    if ((rc = make_maps(std::min(page_size, 64))) != DTB_OK) return rc;
+    e = head_dim == 64 ? dtb::launch_paged_rows<64>(mk, mv, p, plan.rows, scratch, s) : dtb::launch_paged_rows<128>(mk, mv, p, plan.rows, scratch, s);
+  }
+  if (e != cudaSuccess) return fail(DTB_ERR_CUDA, "%s launch failed: %s", kWhat, cudaGetErrorString(e));
   return DTB_OK;
 }
 

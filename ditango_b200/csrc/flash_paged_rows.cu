@@ -1,0 +1,654 @@
+// Attention of few query rows over keys and values in pages: all keys of all sequences dealt evenly to CTAs that stay.
+//
+// A row is a query and one of the heads that share a key head; a block of up to 16, 32 or 64 rows of one key head meets the keys that any row of
+// its sequence sees, [0, first) and [lo, hi), in tiles of 64.  Sequence after sequence, key head after key head, block after block, the tiles
+// are numbered through, W in all, and CTA c of G takes [c W / G, (c + 1) W / G): the lengths stand on the device, and so every CTA works out
+// for itself where its share begins.  Per warp of rows and keys a softmax state (m, l, O) is kept:
+//     S = Q K^T,  m' = max(m, max S) where that grew by more than 2^8, else m,  P = 2^(c (S - m')),
+//     l' = l 2^(c (m - m')) + sum P,  O' = O 2^(c (m - m')) + P V
+// The states of the warps are joined in shared memory.  A block that one CTA has all tiles of is written as it is; the parts of one that several
+// CTAs have go to scratch, and a second launch, set up while this one runs, joins them in the order of their CTAs.
+//
+// HBM-bound: a key and a value are read once for the rows of a block.  Warp 4 loads (TMA, 128-byte swizzle, every lane a page), warps
+// 0-3 compute with mma.sync, because 16 rows fill an instruction of it and a 128-row tile of tcgen05 would be empty for the most part.  With more
+// than 16 rows the warps share the rows out, not the keys, so that what a key costs in shared memory reads stays below what it costs in HBM.
+// P is rounded to bf16 for the product (by 2^-8 of each weight at most, as in the other attention kernels); scores, sums and states are fp32.
+#include "flash_common.cuh"
+#include "flash_paged.cuh"
+
+#include <mutex>
+
+namespace dtb {
+
+namespace {
+
+using namespace flash;
+
+constexpr int kMathWarps = 4;
+constexpr int kThreads = (kMathWarps + 1) * 32;
+constexpr int kKeys = 64;                 // of a tile
+constexpr int kMinTiles = 2;              // of a CTA's share, unless there are fewer
+constexpr int kColumns = 32;              // joined at a time
+constexpr int kPitch = kColumns + 8;      // floats of a row of them in shared memory (rows 8 banks apart)
+
+template <int D, int WM>
+struct Cfg {
+  static constexpr int kRows = 16 * WM;
+  static constexpr int kWN = kMathWarps / WM;                // warps that share a tile's keys
+  static constexpr int kWarpKeys = kKeys / kWN;
+  static constexpr int kSlabs = D / 64;
+  static constexpr int kSlab = kKeys * 128;                  // bytes of 64 channels of a tile
+  static constexpr int kStage = 2 * kSlabs * kSlab;          // K and V
+  static constexpr int kStages = D == 64 ? 6 : 3;
+  static constexpr int kJoin = kWN * kRows * kPitch * 4;
+  static constexpr int kBytes = 1024 + kStages * kStage + kJoin + kWN * kRows * 8 + 2 * kStages * 8 + 64;
+  static_assert(2 * (kBytes + 1024) <= 228 * 1024, "two CTAs to an SM");
+};
+
+// Where a CTA's share begins, and what there is in all; a CTA's is read by the launch that joins.
+struct alignas(16) Share {
+  int64_t first, all;        // its first tile, and all there are
+  int seg, unit, tile;       // sequence, (key head, row block) of it, tile of that
+  int tiles;                 // of each unit of the sequence
+  int ctas;                  // that have a share
+  int pad[3];
+};
+
+// A sequence as its rows' keys are walked.
+struct Seq {
+  WindowSeq w;
+  int blocks;                // of rows, for each key head
+  int first, lo, hi;         // keys that any row sees: [0, first) and [lo, hi)
+  int lead;                  // tiles of the former
+  int tiles;                 // in all, 1 where there is no key: the block's rows are written all the same
+
+  __device__ __forceinline__ int begin(int tile) const { return tile < lead ? tile * kKeys : lo + (tile - lead) * kKeys; }
+};
+
+template <int R>
+__device__ __forceinline__ Seq make_seq(const PagedParams& p, int seg) {
+  Seq s;
+  s.w = paged_seq(p, seg);
+  if (s.w.q_len > p.few_rows) s.w.q_len = 0;
+  s.blocks = (s.w.q_len * (p.f.num_heads / p.kv_heads) + R - 1) / R;
+  const WindowSpan a = window_span(s.w, 0), z = window_span(s.w, max(s.w.q_len - 1, 0));
+  s.first = z.first;
+  s.hi = z.hi;
+  s.lo = max(a.lo, s.first);
+  const int n = max(s.hi - s.lo, 0);
+  if (n > 0) s.lo &= ~(p.key_align - 1);
+  s.lead = (s.first + kKeys - 1) / kKeys;
+  s.tiles = s.lead + (n > 0 ? (s.hi - s.lo + kKeys - 1) / kKeys : 0);
+  if (s.tiles == 0) s.tiles = 1;
+  return s;
+}
+
+// A block's rows and what they see together.
+struct Block {
+  int kv_head, row0, rows;
+  int first, lo, hi;
+
+  // of the tile that begins at key a: the keys that some row sees, [from, to)
+  __device__ __forceinline__ void seen(int a, bool lead, int& from, int& to) const {
+    from = lead ? a : max(a, lo);
+    to = min(a + kKeys, lead ? first : hi);
+  }
+};
+
+template <int R>
+__device__ __forceinline__ Block make_block(const PagedParams& p, const Seq& s, int unit) {
+  Block b;
+  const int group = p.f.num_heads / p.kv_heads;
+  b.kv_head = unit / s.blocks;
+  b.row0 = unit % s.blocks * R;
+  b.rows = min(R, s.w.q_len * group - b.row0);
+  const WindowSpan a = window_span(s.w, b.row0 / group), z = window_span(s.w, (b.row0 + b.rows - 1) / group);
+  b.first = z.first;
+  b.lo = max(a.lo, z.first);
+  b.hi = z.hi;
+  return b;
+}
+
+__device__ __forceinline__ int64_t share_begin(int c, int64_t all, int ctas) { return c * all / ctas; }
+__device__ __forceinline__ int share_of(int64_t tile, int64_t all, int ctas) { return static_cast<int>(((tile + 1) * ctas - 1) / all); }
+
+__device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+// d += a b: 16 x 16 (rows x k) by 16 x 8
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float quad_max(float v) {
+  v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
+  return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+}
+__device__ __forceinline__ float quad_sum(float v) {
+  v += __shfl_xor_sync(0xffffffffu, v, 1);
+  return v + __shfl_xor_sync(0xffffffffu, v, 2);
+}
+// The exponent's reference for a running maximum: 0 while no key has been seen, so that -inf - ref stays -inf.
+__device__ __forceinline__ float reference(float m) { return m == -INFINITY ? 0.f : m; }
+
+__device__ __forceinline__ void math_warps_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+
+// Four columns of a finished row: normalised, merged with the state in memory where the launch accumulates, stored.  `write_lse`: this thread
+// writes the row's lse; the threads of a row that read it before are all in its warp (`mask`) or behind a barrier.
+template <int D>
+__device__ __forceinline__ void store_row4(const PagedParams& p, int seg, const WindowSeq& s, int i, int head, int col, float4 acc, float m, float l,
+                                           bool write_lse, uint32_t mask) {
+  const int64_t tok = p.f.cu_q != nullptr ? static_cast<int64_t>(s.q_begin) + i : static_cast<int64_t>(seg) * p.f.seqlen_q + i;
+  const int64_t li = lse_index(p.f, seg, head, i, tok), oi = tok * p.f.out_tok_stride + static_cast<int64_t>(head) * D + col;
+  const bool empty = l == 0.f;                    // no key seen: nothing to write over a state  (a NaN among the scores is not empty)
+  const bool keep = empty && p.f.accumulate != 0;
+  float lse_out = -INFINITY;
+  if (!keep) {
+    float w_new = 0.f, w_old = 0.f;
+    if (!empty) merge_weights(p.f.accumulate != 0, p.f.accumulate ? p.f.lse[li] : -INFINITY, (m * p.f.scale_log2 + log2f(l)) * kLn2, l, w_new, w_old, lse_out);
+    acc.x *= w_new;
+    acc.y *= w_new;
+    acc.z *= w_new;
+    acc.w *= w_new;
+    if (p.f.out_dtype == 0) {
+      float4* dst = reinterpret_cast<float4*>(static_cast<float*>(p.f.out) + oi);
+      if (w_old != 0.f) {
+        const float4 old = *dst;
+        acc.x = fmaf(old.x, w_old, acc.x);
+        acc.y = fmaf(old.y, w_old, acc.y);
+        acc.z = fmaf(old.z, w_old, acc.z);
+        acc.w = fmaf(old.w, w_old, acc.w);
+      }
+      *dst = acc;
+    } else {
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.f.out) + oi) = make_uint2(pack_bf16x2(acc.x, acc.y), pack_bf16x2(acc.z, acc.w));
+    }
+  }
+  __syncwarp(mask);
+  if (write_lse && !keep) p.f.lse[li] = lse_out;
+}
+
+// The scratch of a launch: shares, then the states' (m, l) and values, two of each CTA (of the first block of its share, and of the last).
+template <int D, int R>
+struct Scratch {
+  Share* shares;
+  float2* ml;
+  float* o;
+  __host__ __device__ Scratch(void* base, int ctas) {
+    shares = static_cast<Share*>(base);
+    ml = reinterpret_cast<float2*>(shares + ctas);
+    o = reinterpret_cast<float*>(ml + 2 * static_cast<int64_t>(ctas) * R);
+  }
+};
+
+}  // namespace
+
+template <int D, int WM>
+__global__ void __launch_bounds__(kThreads, 2)
+flash_paged_rows_kernel(const __grid_constant__ PagedMap tm_k, const __grid_constant__ PagedMap tm_v, const __grid_constant__ PagedParams p, void* scratch) {
+  using C = Cfg<D, WM>;
+  constexpr int R = C::kRows, WN = C::kWN, KW = C::kWarpKeys;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023u);
+  float* s_join = reinterpret_cast<float*>(smem + C::kStages * C::kStage);            // [warp of keys][row][kPitch]
+  float2* s_ml = reinterpret_cast<float2*>(s_join + C::kJoin / 4);                     // [warp of keys][row]
+  uint64_t* full = reinterpret_cast<uint64_t*>(s_ml + WN * R);
+  uint64_t* empty = full + C::kStages;
+  __shared__ long long s_sum[kThreads / 32];
+  __shared__ Share s_share;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Scratch<D, R> sc(scratch, gridDim.x);
+
+  grid_launch_dependents();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < C::kStages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], kMathWarps);
+    }
+    fence_mbar_init();
+    s_share.ctas = 0;
+  }
+  if (warp == kMathWarps && lane == 0) {
+    prefetch_tmap(&tm_k);
+    prefetch_tmap(&tm_v);
+  }
+  // ------------------------------------------------------------------ this CTA's share
+  const int per = (p.f.nseg + kThreads - 1) / kThreads, seg0 = min(static_cast<int>(threadIdx.x) * per, p.f.nseg), seg1 = min(seg0 + per, p.f.nseg);
+  auto weight = [&](const Seq& s) { return static_cast<long long>(s.blocks) * p.kv_heads * s.tiles; };
+  long long sum = 0;
+  for (int i = seg0; i < seg1; ++i) sum += weight(make_seq<R>(p, i));
+  long long upto = sum;
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) {
+    const long long u = __shfl_up_sync(0xffffffffu, upto, d);
+    if (lane >= d) upto += u;
+  }
+  if (lane == 31) s_sum[warp] = upto;
+  // CTA-uniform view of the status word: a CTA that starts after a failure elsewhere does no work.
+  if (__syncthreads_or(*reinterpret_cast<volatile int*>(p.f.status) != 0)) return;
+  long long at = upto - sum, all = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) at += s_sum[w];
+    all += s_sum[w];
+  }
+  const long long most = all / kMinTiles;
+  const int ctas = static_cast<int>(most < 1 ? (all > 0) : most < gridDim.x ? most : gridDim.x);
+  const int cta = blockIdx.x;
+  if (cta >= ctas) {
+    if (cta == 0 && threadIdx.x == 0) sc.shares[0].ctas = 0;
+    return;
+  }
+  const long long begin = share_begin(cta, all, ctas), end = share_begin(cta + 1, all, ctas);
+  if (begin >= at && begin < at + sum) {
+    for (int i = seg0; i < seg1; ++i) {
+      const Seq s = make_seq<R>(p, i);
+      if (begin < at + weight(s)) {
+        Share& w = s_share;
+        w.first = begin;
+        w.all = all;
+        w.seg = i;
+        w.unit = static_cast<int>((begin - at) / s.tiles);
+        w.tile = static_cast<int>((begin - at) % s.tiles);
+        w.tiles = s.tiles;
+        w.ctas = ctas;
+        sc.shares[cta] = w;
+        break;
+      }
+      at += weight(s);
+    }
+  }
+  __syncthreads();
+
+  int seg = s_share.seg, unit = s_share.unit, tile = s_share.tile;
+  long long left = end - begin;             // tiles
+  int stage = 0;
+  uint32_t use = 0;                         // parity of the ring's round
+  Seq s = make_seq<R>(p, seg);
+  bool first_block = true;
+  auto next_block = [&](int to) {
+    left -= to - tile;
+    tile = 0;
+    first_block = false;
+    if (++unit == s.blocks * p.kv_heads && left > 0) {
+      unit = 0;
+      do s = make_seq<R>(p, ++seg); while (s.blocks == 0);
+    }
+  };
+
+  if (warp == kMathWarps) {
+    // ---------------------------------------------------------------- loads: a lane per box of tokens
+    bool ok = true, wrapped = false;
+    const int box = p.box_rows, boxes = kKeys / box;
+    while (ok && left > 0) {
+      const Block b = make_block<R>(p, s, unit);
+      const int to = static_cast<int>(min(static_cast<long long>(s.tiles), tile + left));
+      const int32_t* row = p.table + static_cast<int64_t>(seg) * p.columns;
+      for (int t = tile; t < to; ++t) {
+        const int a = s.begin(t);
+        int from, upto_key;
+        b.seen(a, t < s.lead, from, upto_key);
+        if (from >= upto_key) continue;
+        const int key = a + lane * box, j = key >> p.page_shift, n = (upto_key - a + box - 1) / box;       // boxes that hold a key of the tile
+        int page = -1;
+        if (lane < boxes && lane < n && j < p.columns) page = row[j];
+        if (page < 0 || page >= p.pages) page = p.pages;         // filled with zeros
+        if (wrapped && !warp_wait_or_abort(&empty[stage], use ^ 1, p.f.status, 62)) {
+          ok = false;
+          break;
+        }
+        if (lane == 0) mbar_expect_tx(&full[stage], n * box * 128 * 2 * C::kSlabs);
+        __syncwarp();
+        if (lane < n) {
+          uint8_t* dst = smem + stage * C::kStage + lane * box * 128;
+          const int in_page = key & ((1 << p.page_shift) - 1);
+          const int ka = p.k_batch_first ? b.kv_head : in_page, kb = p.k_batch_first ? in_page : b.kv_head;
+          const int va = p.v_batch_first ? b.kv_head : in_page, vb = p.v_batch_first ? in_page : b.kv_head;
+#pragma unroll
+          for (int x = 0; x < C::kSlabs; ++x) tma_load_4d(dst + x * C::kSlab, &tm_k.map, &full[stage], x * 64, ka, kb, page);
+#pragma unroll
+          for (int x = 0; x < C::kSlabs; ++x) tma_load_4d(dst + (C::kSlabs + x) * C::kSlab, &tm_v.map, &full[stage], x * 64, va, vb, page);
+        }
+        if (++stage == C::kStages) {
+          stage = 0;
+          use ^= 1;
+          wrapped = true;
+        }
+      }
+      next_block(to);
+    }
+  } else {
+    // ---------------------------------------------------------------- scores, weights, products
+    const int wm = warp / WN, wn = warp % WN;
+    const int group = p.f.num_heads / p.kv_heads;
+    const float c = p.f.scale_log2;
+    bool ok = true;             // after a wait that gave up, the blocks are walked to their barriers and nothing more is stored
+    while (left > 0) {
+      const Block b = make_block<R>(p, s, unit);
+      const int to = static_cast<int>(min(static_cast<long long>(s.tiles), tile + left));
+      // this thread's rows lane / 4 and lane / 4 + 8 of the warp's 16; rows that there are not see what the last one sees
+      int end_first[2], from_w[2], to_w[2];
+      uint32_t qf[D / 16][4];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int r = 16 * wm + (lane >> 2) + 8 * h, row = b.row0 + min(r, b.rows - 1);
+        const int i = row / group, g = row % group;
+        const WindowSpan w = window_span(s.w, i);
+        end_first[h] = w.first;
+        from_w[h] = w.lo;
+        to_w[h] = w.hi;
+        const uint16_t* src = r < b.rows ? p.q + window_offset(p, seg, static_cast<int64_t>(s.w.q_begin) + i, p.q_tok, p.q_batch) + static_cast<int64_t>(b.kv_head * group + g) * D : nullptr;
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+          for (int half = 0; half < 2; ++half)
+            qf[k][h + 2 * half] = src != nullptr ? *reinterpret_cast<const uint32_t*>(src + 16 * k + 8 * half + 2 * (lane & 3)) : 0u;
+      }
+      float o[D / 8][4];
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[i][k] = 0.f;
+      float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+      for (int t = tile; t < to; ++t) {
+        const int a = s.begin(t);
+        const bool lead = t < s.lead;
+        int from, upto_key;
+        b.seen(a, lead, from, upto_key);
+        if (from >= upto_key) continue;
+        ok = ok && warp_wait_or_abort(&full[stage], use, p.f.status, 61);
+        if (ok) {
+          const int key0 = wn * KW;               // of the tile, the warp's first
+          const uint32_t ks = smem_u32(smem + stage * C::kStage), vs = ks + C::kSlabs * C::kSlab;
+          const bool ragged = from > a || upto_key < a + kKeys;
+          if (ragged) {
+            // values of keys that no row sees may be anything, and 0 times that is not 0
+            for (int u = lane; u < KW * C::kSlabs * 8; u += 32) {
+              const int row = key0 + u / (C::kSlabs * 8), piece = u % (C::kSlabs * 8);
+              if (a + row < from || a + row >= upto_key)
+                *reinterpret_cast<uint4*>(smem + stage * C::kStage + (C::kSlabs + piece / 8) * C::kSlab + row * 128 + piece % 8 * 16) = make_uint4(0u, 0u, 0u, 0u);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+          }
+          float sr[KW / 8][4];
+#pragma unroll
+          for (int n = 0; n < KW / 16; ++n) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sr[2 * n][e] = sr[2 * n + 1][e] = 0.f;
+            const int row = key0 + n * 16 + ((lane >> 4) << 3) + (lane & 7);
+            const uint32_t at_row = ks + row * 128;
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k) {
+              uint32_t f[4];
+              ldmatrix4(at_row + (k >> 2) * C::kSlab + ((((2 * k + ((lane >> 3) & 1)) & 7) ^ (row & 7)) << 4), f);
+              mma16816(sr[2 * n], qf[k], f[0], f[1]);
+              mma16816(sr[2 * n + 1], qf[k], f[2], f[3]);
+            }
+          }
+          // columns of the warp's keys that the rows see, [c0, c1)
+          int c0[2], c1[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            c0[h] = lead ? 0 : from_w[h] - a - key0;
+            c1[h] = (lead ? end_first[h] : to_w[h]) - a - key0;
+          }
+          if (__any_sync(0xffffffffu, max(c0[0], c0[1]) > 0 || min(c1[0], c1[1]) < KW)) {
+#pragma unroll
+            for (int n = 0; n < KW / 8; ++n)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int h = e >> 1, x = n * 8 + 2 * (lane & 3) + (e & 1);
+                if (x < c0[h] || x >= c1[h]) sr[n][e] = -INFINITY;
+              }
+          }
+          float mx[2];
+          bool grows = false;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float v = fmaxf(sr[0][2 * h], sr[0][2 * h + 1]);
+#pragma unroll
+            for (int n = 1; n < KW / 8; ++n) v = max3(v, sr[n][2 * h], sr[n][2 * h + 1]);
+            mx[h] = fmaxf(m[h], quad_max(v));
+            grows = grows || (mx[h] - m[h]) * c > kRescaleThreshold;       // (from -inf without end; -inf - -inf is not)
+          }
+          if (__any_sync(0xffffffffu, grows)) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float f = m[h] == mx[h] ? 1.f : ex2((m[h] - mx[h]) * c);
+              m[h] = mx[h];
+              l[h] *= f;
+#pragma unroll
+              for (int i = 0; i < D / 8; ++i) {
+                o[i][2 * h] *= f;
+                o[i][2 * h + 1] *= f;
+              }
+            }
+          }
+          const float ref[2] = {reference(m[0]) * c, reference(m[1]) * c};
+#pragma unroll
+          for (int n = 0; n < KW / 8; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              sr[n][e] = ex2(fmaf(sr[n][e], c, -ref[e >> 1]));
+              l[e >> 1] += sr[n][e];
+            }
+#pragma unroll
+          for (int n = 0; n < KW / 16; ++n) {
+            const uint32_t w[4] = {pack_bf16x2(sr[2 * n][0], sr[2 * n][1]), pack_bf16x2(sr[2 * n][2], sr[2 * n][3]),
+                                   pack_bf16x2(sr[2 * n + 1][0], sr[2 * n + 1][1]), pack_bf16x2(sr[2 * n + 1][2], sr[2 * n + 1][3])};
+            const int row = key0 + n * 16 + (((lane >> 3) & 1) << 3) + (lane & 7);
+            const uint32_t at_row = vs + row * 128;
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d) {
+              uint32_t f[4];
+              ldmatrix4_trans(at_row + (d >> 2) * C::kSlab + ((((2 * d + (lane >> 4)) & 7) ^ (row & 7)) << 4), f);
+              mma16816(o[2 * d], w, f[0], f[1]);
+              mma16816(o[2 * d + 1], w, f[2], f[3]);
+            }
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&empty[stage]);
+        }
+        if (++stage == C::kStages) {
+          stage = 0;
+          use ^= 1;
+        }
+      }
+      // join the warps that shared the keys, 32 columns at a time
+      const bool whole = tile == 0 && to == s.tiles;
+      const int slot = 2 * cta + (first_block ? 0 : 1);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float row_sum = quad_sum(l[h]);
+        if ((lane & 3) == 0) s_ml[wn * R + 16 * wm + (lane >> 2) + 8 * h] = make_float2(m[h], row_sum);
+      }
+#pragma unroll
+      for (int x = 0; x < D / kColumns; ++x) {
+#pragma unroll
+        for (int i = 0; i < kColumns / 8; ++i)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            *reinterpret_cast<float2*>(s_join + (wn * R + 16 * wm + (lane >> 2) + 8 * h) * kPitch + 8 * i + 2 * (lane & 3)) =
+                make_float2(o[x * (kColumns / 8) + i][2 * h], o[x * (kColumns / 8) + i][2 * h + 1]);
+        math_warps_sync();
+#pragma unroll 1
+        for (int u0 = 0; u0 < b.rows * (kColumns / 4); u0 += kMathWarps * 32) {
+          const int u = u0 + static_cast<int>(threadIdx.x), r = u / (kColumns / 4), col = u % (kColumns / 4) * 4;
+          const bool there = r < b.rows && ok;
+          const uint32_t mask = __ballot_sync(0xffffffffu, there);
+          if (!there) continue;
+          float mm = -INFINITY;
+#pragma unroll
+          for (int w = 0; w < WN; ++w) mm = fmaxf(mm, s_ml[w * R + r].x);
+          const float ref = reference(mm);
+          float ll = 0.f;
+          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int w = 0; w < WN; ++w) {
+            const float2 ml = s_ml[w * R + r];
+            const float f = ex2((ml.x - ref) * c);
+            const float4 v = *reinterpret_cast<const float4*>(s_join + (w * R + r) * kPitch + col);
+            ll = fmaf(ml.y, f, ll);
+            acc.x = fmaf(v.x, f, acc.x);
+            acc.y = fmaf(v.y, f, acc.y);
+            acc.z = fmaf(v.z, f, acc.z);
+            acc.w = fmaf(v.w, f, acc.w);
+          }
+          const bool last = x == D / kColumns - 1 && col == 0;
+          if (whole) {
+            const int row = b.row0 + r;
+            store_row4<D>(p, seg, s.w, row / group, b.kv_head * group + row % group, x * kColumns + col, acc, mm, ll, last, mask);
+          } else {
+            *reinterpret_cast<float4*>(sc.o + (static_cast<int64_t>(slot) * R + r) * D + x * kColumns + col) = acc;
+            if (last) sc.ml[static_cast<int64_t>(slot) * R + r] = make_float2(mm, ll);
+          }
+        }
+        math_warps_sync();
+      }
+      next_block(to);
+    }
+  }
+  if (*reinterpret_cast<volatile int*>(p.f.status) != 0) __nanosleep(1000000);   // let copies in flight land
+}
+
+// Joins the parts of a block that several CTAs worked on.  grid: (boundaries between two CTAs' shares, rows in fours); the first boundary
+// inside a block is the one that counts.  A warp per row, four warps per row where there are many parts.
+template <int D, int R>
+__global__ void __launch_bounds__(128) flash_paged_join_kernel(const __grid_constant__ PagedParams p, void* scratch) {
+  constexpr int kLaneCols = D / 32;
+  __shared__ float s_acc[4][D];
+  __shared__ float2 s_ml[4];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int cta = blockIdx.x + 1;
+  grid_dependency_wait();
+  if (*reinterpret_cast<volatile int*>(p.f.status) != 0) return;
+  const Scratch<D, R> sc(scratch, gridDim.x + 1);
+  const int ctas = sc.shares[0].ctas;
+  if (cta >= ctas) return;
+  const Share w = sc.shares[cta];
+  if (w.tile == 0) return;                                     // the block before ends with the share before
+  const int64_t begin = w.first - w.tile, end = begin + w.tiles;
+  const int c0 = share_of(begin, w.all, ctas), c1 = share_of(end - 1, w.all, ctas);
+  if (c0 != cta - 1) return;
+  const Seq s = make_seq<R>(p, w.seg);
+  const Block b = make_block<R>(p, s, w.unit);
+  const int group = p.f.num_heads / p.kv_heads, n = c1 - c0 + 1;
+  const float c = p.f.scale_log2;
+  // (only the first of them can have begun with another block)
+  auto slot_of = [&](int i) { return 2 * static_cast<int64_t>(c0 + i) + (i == 0 && share_begin(c0, w.all, ctas) < begin ? 1 : 0); };
+  const bool alone = n <= 8;                                   // a row to each warp
+  const int parts = alone ? 1 : 4, part = alone ? 0 : warp;
+  for (int r = blockIdx.y * 4 + (alone ? warp : 0), rounds = alone ? 1 : 4; rounds > 0; --rounds, ++r) {
+    if (r >= b.rows) return;                                   // (all warps of a row together)
+    float mm = -INFINITY, ll = 0.f, acc[kLaneCols] = {};
+    for (int i = lane; i < n; i += 32) mm = fmaxf(mm, sc.ml[slot_of(i) * R + r].x);
+#pragma unroll
+    for (int d = 16; d > 0; d /= 2) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, d));
+    const float ref = reference(mm);
+#pragma unroll 8
+    for (int i = part; i < n; i += parts) {
+      const int64_t slot = slot_of(i) * R + r;
+      const float2 ml = sc.ml[slot];
+      const float f = ex2((ml.x - ref) * c);
+      ll = fmaf(ml.y, f, ll);
+      const float* src = sc.o + slot * D + lane * kLaneCols;
+      float v[kLaneCols];
+      if constexpr (D == 128) {
+        const float4 q = *reinterpret_cast<const float4*>(src);
+        v[0] = q.x, v[1] = q.y, v[2] = q.z, v[3] = q.w;
+      } else {
+        const float2 q = *reinterpret_cast<const float2*>(src);
+        v[0] = q.x, v[1] = q.y;
+      }
+#pragma unroll
+      for (int k = 0; k < kLaneCols; ++k) acc[k] = fmaf(v[k], f, acc[k]);
+    }
+    if (!alone) {
+#pragma unroll
+      for (int k = 0; k < kLaneCols; ++k) s_acc[warp][lane * kLaneCols + k] = acc[k];
+      if (lane == 0) s_ml[warp] = make_float2(mm, ll);
+      __syncthreads();
+    }
+    // the row's columns, four to a lane
+    if (alone) {
+#pragma unroll
+      for (int k = 0; k < kLaneCols; ++k) s_acc[warp][lane * kLaneCols + k] = acc[k];
+      __syncwarp();
+    } else if (warp == 0) {
+      ll = 0.f;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) ll += s_ml[q].y;
+    }
+    if (alone || warp == 0) {
+      const int row = b.row0 + r;
+      if (lane < D / 4) {
+        float4 a = *reinterpret_cast<const float4*>(&s_acc[alone ? warp : 0][lane * 4]);
+        if (!alone) {
+#pragma unroll
+          for (int q = 1; q < 4; ++q) {
+            const float4 v = *reinterpret_cast<const float4*>(&s_acc[q][lane * 4]);
+            a.x += v.x;
+            a.y += v.y;
+            a.z += v.z;
+            a.w += v.w;
+          }
+        }
+        store_row4<D>(p, w.seg, s.w, row / group, b.kv_head * group + row % group, lane * 4, a, mm, ll, lane == 0, D == 128 ? 0xffffffffu : 0xffffu);
+      }
+    }
+    if (!alone) __syncthreads();
+  }
+}
+
+PagedRowsPlan plan_paged_rows(int rows_of_a_head, int head_dim, int sm_count) {
+  PagedRowsPlan plan;
+  plan.rows = rows_of_a_head <= 16 ? 16 : rows_of_a_head <= 32 ? 32 : 64;
+  plan.ctas = 2 * sm_count;
+  plan.scratch_bytes = plan.ctas * (static_cast<int64_t>(sizeof(Share)) + 2 * plan.rows * (8 + head_dim * 4));
+  return plan;
+}
+
+namespace {
+
+template <int D, int WM>
+cudaError_t launch_rows(const PagedMap& tk, const PagedMap& tv, const PagedParams& p, const PagedRowsPlan& plan, void* scratch, cudaStream_t stream) {
+  using C = Cfg<D, WM>;
+  static bool configured[64] = {};
+  static std::mutex mu;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  {
+    std::lock_guard<std::mutex> lk(mu);
+    if (!configured[dev & 63]) {
+      e = cudaFuncSetAttribute(flash_paged_rows_kernel<D, WM>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kBytes);
+      if (e != cudaSuccess) return e;
+      configured[dev & 63] = true;
+    }
+  }
+  flash_paged_rows_kernel<D, WM><<<plan.ctas, kThreads, C::kBytes, stream>>>(tk, tv, p, scratch);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  return launch_attention_kernel(flash_paged_join_kernel<D, 16 * WM>, dim3(plan.ctas - 1, 4 * WM), 128, 0, stream, true, p, scratch);
+}
+
+}  // namespace
+
+template <int D>
+cudaError_t launch_paged_rows(const PagedMap& tk, const PagedMap& tv, const PagedParams& p, const PagedRowsPlan& plan, void* scratch, cudaStream_t stream) {
+  if (plan.rows == 16) return launch_rows<D, 1>(tk, tv, p, plan, scratch, stream);
+  if (plan.rows == 32) return launch_rows<D, 2>(tk, tv, p, plan, scratch, stream);
+  return launch_rows<D, 4>(tk, tv, p, plan, scratch, stream);
+}
+
+template cudaError_t launch_paged_rows<64>(const PagedMap&, const PagedMap&, const PagedParams&, const PagedRowsPlan&, void*, cudaStream_t);
+template cudaError_t launch_paged_rows<128>(const PagedMap&, const PagedMap&, const PagedParams&, const PagedRowsPlan&, void*, cudaStream_t);
+
+}  // namespace dtb

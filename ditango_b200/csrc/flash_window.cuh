@@ -63,6 +63,9 @@ __device__ __forceinline__ WindowSeq window_seq(const WindowParams& p, int seg) 
   return s;
 }
 
+// Of what number of keys a run that is walked begins at a multiple.  (Dense keys: anywhere.)
+__device__ __forceinline__ int key_align(const WindowParams&) { return 1; }
+
 // Keys that query i sees: [0, first) and [lo, hi), first <= lo <= hi.  A key at position j is seen from position x when
 // j <= x + right and (j >= x - left or j < sinks).
 struct WindowSpan {

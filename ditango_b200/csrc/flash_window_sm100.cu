@@ -37,6 +37,7 @@
 // With few blocks their keys are split into parts of as many tiles each, which are attended like blocks of their own and merged by the
 // state merge's kernel behind this one (24 heads of 128, 64 queries, window 4096: 66 -> 26 us in six parts).
 #include "flash_common.cuh"
+#include "flash_paged.cuh"
 #include "flash_window.cuh"
 
 #include <mutex>
@@ -76,7 +77,7 @@ struct Cfg {
   // barriers: q_full[QB][2], q_empty[QB], kv_full[S], kv_empty[S], s_full[NB], p_lo[NB], p_hi[NB], pv_done[2], o_final[2],
   // o_free[2], ml_full[2], ml_empty[2], work_full[W], work_empty[W], v_tail[T], claim
   static constexpr int kBars = 3 * kQBufs + 2 * kStages + 3 * kSBufs + 10 + 2 * kWork + kTails + 1;
-  static constexpr int kSmemBytes = 1024 + (kQBufs * kQT + kStages) * kTileBytes + kStageOut + kQT * kBM * 8 + kWork * 64 + D * 4 + 16 +
+  static constexpr int kSmemBytes = 1024 + (kQBufs * kQT + kStages) * kTileBytes + kStageOut + kQT * kBM * 8 + kWork * 80 + D * 4 + 16 +
                                     kBars * 8 + 16;
   static constexpr uint32_t kTmemCols = 512;
   static constexpr uint32_t kColS = 0;                    // + buffer * 128
@@ -88,17 +89,20 @@ struct Cfg {
 
 // The key tiles of a block's rows and the order in which its units meet them.
 struct Walk {
-  int lo, win;        // the window's first key and length
+  int lo, win;        // the window's first key and length; with pages it may begin `front` keys, fewer than 16, before the first one seen
+  int front;
   int first;          // first tokens
   int N, n;           // tiles of the window, window steps of a Q tile: N, or N - 1 where Q tile 1 is a tile ahead
   int steps;          // steps in all; 0: nothing to see (such a block only the loader meets), -1: no more blocks
 
   // for the rows i0 to i1
-  __device__ __forceinline__ void plan(int from, int to, int sinks, int k_end, int k_floor, int i0, int i1) {
+  __device__ __forceinline__ void plan(int from, int to, int sinks, int k_end, int k_floor, int i0, int i1, int align) {
     auto span = [&](int i) { return window_span(from, to, sinks, k_end, k_floor, i); };
     const WindowSpan a = span(i0), z = span(i1);
     first = z.first;
     lo = max(a.lo, min(k_floor, z.hi));
+    front = z.hi > lo ? lo & (align - 1) : 0;
+    lo -= front;
     win = max(z.hi - lo, 0);
     N = (win + kBN - 1) / kBN;
     n = N;
@@ -126,7 +130,7 @@ struct Item {
   int from, to, sinks;           // of its sequence, see WindowSeq
   int k_end, k_floor;            // see window_span
 };
-static_assert(sizeof(Item) == 64, "shared-memory layout");
+static_assert(sizeof(Item) <= 80, "shared-memory layout");
 
 // Bits [a, b) of a word, as far as they lie in it.
 __device__ __forceinline__ uint32_t run_of_bits(int a, int b) {
@@ -255,11 +259,12 @@ __device__ __forceinline__ bool claim_answer(const void* response16, int& x, int
 
 }  // namespace
 
-// grid: (row blocks, heads, sequences x parts)
-template <int D>
+// grid: (row blocks, heads, sequences x parts).  Keys and values dense (CUtensorMap, WindowParams) or in pages (PagedMap, PagedParams): the two
+// differ in how a sequence and a tile's rows are found.
+template <int D, class Map, class Params>
 __global__ void __launch_bounds__(kThreads, 1)
-flash_window_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
-                    const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ WindowParams p) {
+flash_window_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ Map tm_k,
+                    const __grid_constant__ Map tm_v, const __grid_constant__ Params p) {
   using C = Cfg<D>;
   constexpr int NB = C::kSBufs;
   extern __shared__ uint8_t smem_raw[];
@@ -372,7 +377,7 @@ flash_window_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
           w.seg = seg;
           w.q0 = bx * (kQT * kBM);
           const WindowSeq s = window_seq(p, seg);
-          w.q_begin = p.f.cu_q != nullptr ? s.q_begin : seg * p.f.seqlen_q + part * static_cast<int>(p.f.total_q);
+          w.q_begin = (p.f.cu_q != nullptr ? s.q_begin : seg * p.f.seqlen_q) + part * static_cast<int>(p.f.total_q);
           w.q_len = s.q_len;
           w.from = s.from;
           w.to = s.to;
@@ -382,7 +387,7 @@ flash_window_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
           asked = false;
           if (w.q0 < w.q_len) {
             const int i1 = min(w.q0 + kQT * kBM, w.q_len) - 1;
-            w.walk.plan(w.from, w.to, w.sinks, w.k_end, w.k_floor, w.q0, i1);
+            w.walk.plan(w.from, w.to, w.sinks, w.k_end, w.k_floor, w.q0, i1, key_align(p));
             if (p.splits > 1) {
               // as many tiles to each part, the first tokens to the last one
               const int begin = w.walk.lo, end = begin + w.walk.win;
@@ -392,7 +397,7 @@ flash_window_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
                 w.k_end = min(w.k_floor + keys, end);
                 w.sinks = 0;
               }
-              w.walk.plan(w.from, w.to, w.sinks, w.k_end, w.k_floor, w.q0, i1);
+              w.walk.plan(w.from, w.to, w.sinks, w.k_end, w.k_floor, w.q0, i1, key_align(p));
             }
             const Walk walk = w.walk;
             const int n_units = 2 * walk.steps;
@@ -406,7 +411,7 @@ flash_window_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
               const int kv_head = by / (p.f.num_heads / p.kv_heads);
               const int batch = p.f.cu_q != nullptr ? 0 : seg;
               int k_tile = -1, v_tile = -1;
-              auto load_kv = [&](const CUtensorMap* tm, int tile, int batch_first) {
+              auto load_kv = [&](const auto* tm, int tile, int batch_first) {
                 const int stage = it % C::kStages;
                 const int round = it / C::kStages;
                 ++it;
@@ -425,17 +430,19 @@ flash_window_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
                 if (walk.tile_of(u) == v_tile) return true;
                 v_tile = walk.tile_of(u);
                 if (!load_kv(&tm_v, v_tile, p.v_batch_first)) return false;
-                const int keys = walk.valid(v_tile);
-                if ((keys & 15) == 0) return true;
-                // What lies behind the tile's last key in its step of 16 is cleared.  (Nobody gives the slot back before that: the
-                // issuer waits for v_tail, so the phase waited for here is the one that this load completes.)
+                const int keys = walk.valid(v_tile), front = u == 0 ? walk.front : 0;
+                if ((keys & 15) == 0 && front == 0) return true;
+                // What lies behind the tile's last key in its step of 16, and before its first one, is cleared.  (Nobody gives the slot back
+                // before that: the issuer waits for v_tail, so the phase waited for here is the one that this load completes.)
                 const int stage = (it - 1) % C::kStages;
                 if (!wait_or_abort(&sh.kv_full[stage], ((it - 1) / C::kStages) & 1, p.f.status, 12)) return false;
 #pragma unroll 1
                 for (int x = 0; x < C::kSlabs; ++x) {
                   uint8_t* behind = sh.s_kv + stage * C::kTileBytes + x * kSlabBytes + keys * 128;     // whole rows of 128 bytes: the swizzle stays inside
 #pragma unroll 1
-                  for (int i = 0; i < (16 - (keys & 15)) * 8; ++i) *reinterpret_cast<uint4*>(behind + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+                  for (int i = 0; i < (-keys & 15) * 8; ++i) *reinterpret_cast<uint4*>(behind + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll 1
+                  for (int i = 0; i < front * 8; ++i) *reinterpret_cast<uint4*>(sh.s_kv + stage * C::kTileBytes + x * kSlabBytes + i * 16) = make_uint4(0u, 0u, 0u, 0u);
                 }
                 fence_proxy_async_smem();                     // the MMA reads shared memory through the asynchronous proxy
                 mbar_arrive(&sh.v_tail[tails++ % kTails]);
@@ -568,10 +575,11 @@ flash_window_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
           auto next_v = [&](int u) {
             if (!next_kv(v_stage, 23)) return false;
             v_steps = kBN / 16;
-            if (u != u_window && u != u_first) return true;
-            const int keys = u == u_window ? walk.valid(walk.N - 1) : walk.valid(walk.N + walk.steps - walk.n - 1);
+            const bool front = u == 0 && walk.front > 0;
+            if (u != u_window && u != u_first && !front) return true;
+            const int keys = u == u_window ? walk.valid(walk.N - 1) : u == u_first ? walk.valid(walk.N + walk.steps - walk.n - 1) : kBN;
             v_steps = (keys + 15) >> 4;
-            if ((keys & 15) == 0) return true;
+            if ((keys & 15) == 0 && !front) return true;
             const int n = tails++;
             return wait_or_abort(&sh.v_tail[n % kTails], (n / kTails) & 1, p.f.status, 28);
           };
@@ -886,11 +894,12 @@ flash_window_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
   }
 }
 
-template <int D>
-cudaError_t launch_window_tiles(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const WindowParams& p, cudaStream_t stream) {
+template <int D, class Map, class Params>
+static cudaError_t launch_tiles(const CUtensorMap& tq, const Map& tk, const Map& tv, const Params& p, cudaStream_t stream) {
   using C = Cfg<D>;
   static bool configured[64] = {};
   static std::mutex mu;
+  const auto kernel = flash_window_kernel<D, Map, Params>;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
@@ -899,19 +908,30 @@ cudaError_t launch_window_tiles(const CUtensorMap& tq, const CUtensorMap& tk, co
     if (!configured[dev & 63]) {
       // the register hand-over waits for good unless the kernel starts with what it was computed for
       cudaFuncAttributes fa;
-      e = cudaFuncGetAttributes(&fa, flash_window_kernel<D>);
+      e = cudaFuncGetAttributes(&fa, kernel);
       if (e == cudaSuccess && fa.numRegs != kRegsLaunch) e = cudaErrorInvalidKernelImage;
-      if (e == cudaSuccess) e = cudaFuncSetAttribute(flash_window_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
+      if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
       if (e != cudaSuccess) return e;
       configured[dev & 63] = true;
     }
   }
   const dim3 grid((p.f.seqlen_q + kQT * kBM - 1) / (kQT * kBM), p.f.num_heads, p.f.nseg * p.splits);
-  flash_window_kernel<D><<<grid, kThreads, C::kSmemBytes, stream>>>(tq, tk, tv, p);
+  kernel<<<grid, kThreads, C::kSmemBytes, stream>>>(tq, tk, tv, p);
   return cudaGetLastError();
+}
+
+template <int D>
+cudaError_t launch_window_tiles(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const WindowParams& p, cudaStream_t stream) {
+  return launch_tiles<D>(tq, tk, tv, p, stream);
+}
+template <int D>
+cudaError_t launch_paged_tiles(const CUtensorMap& tq, const PagedMap& tk, const PagedMap& tv, const PagedParams& p, cudaStream_t stream) {
+  return launch_tiles<D>(tq, tk, tv, p, stream);
 }
 
 template cudaError_t launch_window_tiles<64>(const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, const WindowParams&, cudaStream_t);
 template cudaError_t launch_window_tiles<128>(const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, const WindowParams&, cudaStream_t);
+template cudaError_t launch_paged_tiles<64>(const CUtensorMap&, const PagedMap&, const PagedMap&, const PagedParams&, cudaStream_t);
+template cudaError_t launch_paged_tiles<128>(const CUtensorMap&, const PagedMap&, const PagedMap&, const PagedParams&, cudaStream_t);
 
 }  // namespace dtb

@@ -326,6 +326,230 @@ def flash_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, left: int
     return out, lse
 
 
+class PagePlan(NamedTuple):
+    """What extend_pages found: `slots` [tokens] of the new tokens, `cu_seqlens` [streams + 1] among them, `seqlens` and `free_count` as they are
+    now, and `missing` [1], 0 unless nothing was taken.  All int32 on the device."""
+    slots: torch.Tensor
+    cu_seqlens: torch.Tensor
+    seqlens: torch.Tensor
+    free_count: torch.Tensor
+    missing: torch.Tensor
+
+
+class PageRelease(NamedTuple):
+    """The table, the streams' lengths and the number of free pages after release_pages."""
+    table: torch.Tensor
+    seqlens: torch.Tensor
+    free_count: torch.Tensor
+
+
+def _page_args(table, free, free_count, page_size, *per_stream):
+    """Checks what the tables' two directions are given; returns (streams, columns, pages)."""
+    for x in (table, free, free_count, *per_stream):
+        if x.dtype != torch.int32 or not x.is_contiguous():
+            raise _capi.ExtensionError("tables, lengths and pages are contiguous int32 tensors")
+    if table.dim() != 2 or free.dim() != 1 or free_count.numel() != 1 or any(x.numel() != table.shape[0] for x in per_stream):
+        raise _capi.ExtensionError("a table is [streams, columns], with a number per stream; free pages are a list and their count")
+    if not 0 < page_size < 1 << 31:
+        raise _capi.ExtensionError("a page size is a power of two from 16 to 2^20")
+    return (*table.shape, free.numel())
+
+
+def extend_pages(table: torch.Tensor, seqlens: torch.Tensor, new_lens: torch.Tensor, free: torch.Tensor, free_count: torch.Tensor, page_size: int,
+                 tokens: int) -> PagePlan:
+    """Room in pages for new_lens [streams] tokens more behind the seqlens [streams] that each stream has.
+
+    table [streams, columns] holds the streams' pages; entries for new ones are written in place.  The first free_count [1] of `free` are the
+    numbers of pages that nobody holds, the last of those is taken first, and `free` has one entry per page of the pool.  `tokens`, known to
+    the host, is the number of rows that the new keys and values come in: new_lens add up to it or less, and slots behind the last token
+    are -1 (as is that of a token on a page that release_pages took from inside its stream).  All or nothing: with too few free pages `missing` says how many, with streams that outgrow their row or `tokens` it is -1, and then the
+    table and the numbers stay as they are.  The results are new tensors, for the next step; one launch, no host round trip."""
+    streams, columns, pages = _page_args(table, free, free_count, page_size, seqlens, new_lens)
+    if not 0 <= tokens < (1 << 31) - 4:
+        raise _capi.ExtensionError("tokens is a number of rows")
+    stream = _launch_stream(table, seqlens, new_lens, free, free_count)
+    if streams == 0:
+        raise _capi.ExtensionError("a table without streams")
+    # (one allocation; slots begin it and so are 16-byte aligned)
+    slots, cu, lens, count, missing = _empty((tokens + 2 * streams + 3,), torch.int32, table.device).split((tokens, streams + 1, streams, 1, 1))
+    rc = _capi.load().dtb_extend_pages(
+        table.data_ptr(), seqlens.data_ptr(), new_lens.data_ptr(), free.data_ptr(), free_count.data_ptr(), streams, columns, pages, page_size,
+        slots.data_ptr(), tokens, cu.data_ptr(), lens.data_ptr(), count.data_ptr(), missing.data_ptr(), stream)
+    if rc:
+        _capi.check(rc, "dtb_extend_pages")
+    LaunchLog.count += 1
+    return PagePlan(slots, cu, lens, count, missing)
+
+
+def release_pages(table: torch.Tensor, seqlens: torch.Tensor, free: torch.Tensor, free_count: torch.Tensor, begin: torch.Tensor, end: torch.Tensor,
+                  page_size: int, *, out_table: Optional[torch.Tensor] = None) -> PageRelease:
+    """Gives back the pages of each stream whose tokens all lie in [begin, end) [streams]: what a window has left behind (begin: the first tokens
+    that stay), a stream that is over (0 and its length or more), or its newest tokens, where end is its length or more; it is then
+    begin tokens long.  Their entries become -1, in place unless `out_table` takes the table as it is then; `free` gets them behind the others.  The
+    numbers are new tensors; one launch."""
+    streams, columns, pages = _page_args(table, free, free_count, page_size, seqlens, begin, end)
+    if out_table is None:
+        out_table = table
+    elif out_table.dtype != torch.int32 or out_table.shape != table.shape or not out_table.is_contiguous():
+        raise _capi.ExtensionError("out_table is a contiguous int32 tensor of the table's shape")
+    stream = _launch_stream(table, out_table, seqlens, free, free_count, begin, end)
+    if streams == 0:
+        raise _capi.ExtensionError("a table without streams")
+    lens, count = _empty((streams + 1,), torch.int32, table.device).split((streams, 1))
+    rc = _capi.load().dtb_release_pages(
+        table.data_ptr(), out_table.data_ptr(), seqlens.data_ptr(), begin.data_ptr(), end.data_ptr(), free.data_ptr(), free_count.data_ptr(),
+        streams, columns, pages, page_size, lens.data_ptr(), count.data_ptr(), stream)
+    if rc:
+        _capi.check(rc, "dtb_release_pages")
+    LaunchLog.count += 1
+    return PageRelease(out_table, lens, count)
+
+
+def _pool(x: torch.Tensor, shape) -> Tuple[int, int, int]:
+    """(page, token, head) strides of k_pages or v_pages [pages, P, heads, D]; that of an axis of length 1, which nothing steps along, is given as if it
+    lay behind the others."""
+    if x.dtype != torch.bfloat16 or x.shape != shape or x.dim() != 4 or x.stride(-1) != 1:
+        raise _capi.ExtensionError("pages are bfloat16 [pages, tokens, heads, D] with contiguous channels, of keys as of values")
+    page, tok, head, _ = x.stride()
+    pages, P, heads, D = shape
+    if heads == 1:
+        head = max(tok * P, D)
+    if pages == 1:
+        page = max(tok * P, head * heads)
+    return page, tok, head
+
+
+def write_pages(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, slots: torch.Tensor):
+    """Keys and values k, v [..,Hk,D] bf16 of new tokens, any token stride, into the slots [tokens] (extend_pages) of k_pages and v_pages
+    [pages, P, Hk, D], any strides.  A token whose slot is -1, or none of the pool's, is left out; slots are to differ from one another.
+    One launch."""
+    stream = _launch_stream(k, v, k_pages, v_pages, slots)
+    shape = k_pages.shape
+    k_strides, v_strides = _pool(k_pages, shape), _pool(v_pages, shape)
+    pages, P, Hk, D = shape
+    if k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16 or k.shape != v.shape or k.dim() < 3 or k.shape[-2:] != shape[-2:]:
+        raise _capi.ExtensionError("k and v are bfloat16 [..,Hk,D] with the pages' heads")
+    tokens = k.numel() // (Hk * D)
+    if slots.dtype != torch.int32 or slots.numel() != tokens or not slots.is_contiguous():
+        raise _capi.ExtensionError("slots are contiguous int32, one per token")
+    if tokens == 0:
+        return
+    rc = _capi.load().dtb_write_pages(
+        k.data_ptr(), v.data_ptr(), _flat_tok_stride(k), _flat_tok_stride(v), tokens, slots.data_ptr(), k_pages.data_ptr(), *k_strides,
+        v_pages.data_ptr(), *v_strides, pages, P, Hk, D, stream)
+    if rc:
+        _capi.check(rc, "dtb_write_pages")
+    LaunchLog.count += 1
+
+
+def _flat_tok_stride(x: torch.Tensor) -> int:
+    """_tok_stride where the axes of one token, one head do not count."""
+    if x.is_contiguous():
+        return x.shape[-1] * x.shape[-2]
+    if x.shape[-2] == 1 and x.stride(-1) == 1:
+        x = x.as_strided(x.shape, (*x.stride()[:-2], x.shape[-1], 1))
+    if x.numel() == x.shape[-1] * x.shape[-2]:
+        x = x.as_strided(x.shape, (*(x.shape[-1] * x.shape[-2],) * (x.dim() - 2), *x.stride()[-2:]))
+    return _tok_stride(x)
+
+
+_PAGED_SCRATCH = {}       # (device, sequences, lengths, heads, D) -> bytes that flash_paged needs
+
+
+def flash_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, seqlens_k: torch.Tensor, *, left: int = -1,
+                right: int = -1, sinks: int = 0, cu_seqlens_q: Optional[torch.Tensor] = None, max_seqlen_q: Optional[int] = None,
+                max_seqlen_k: Optional[int] = None, out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None,
+                accumulate: bool = False, out_dtype: torch.dtype = torch.float32, lse_layout: int = LSE_BHS,
+                softmax_scale: Optional[float] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Attention state of the newest tokens of sequences over their keys and values in pages: flash_window with a table.
+
+    k_pages, v_pages [pages, P, Hk, D] bf16, any strides that are multiples of 8; table int32 [B, columns], entry j of a row is the page of the
+    sequence's tokens [j P, (j + 1) P); seqlens_k int32 [B] keys of each, those of the queries included (write_pages goes before this).  The last
+    query is at the last key's position; the query at position x sees key j when j <= x + right and (j >= x - left or j < sinks); -1
+    means no limit (right=0: causal; -1: all tokens of a chunk see one another).
+
+    Dense: q [B,Sq,H,D] bf16.  Packed: q [T,H,D] with cu_seqlens_q int32 [B + 1] on the device, up to max_seqlen_q (known to the host, T if not
+    given) queries each; rows behind the last sequence are left as they are.  Hk divides H.  max_seqlen_k is about the longest sequence's
+    length, if the host knows it: kernels are chosen by it, results do not depend on it.
+
+    Returns (out, lse) as flash_window does, mergeable with its states and flash_partial's; with accumulate=True the state is merged into the given
+    fp32 (out, lse) in place.  A row that sees no key has out 0 and lse -inf.  Entries of the table behind a sequence's last page or for pages that no
+    query sees may be anything; where one that a query sees is not a page of the pool, its keys and values are 0.  Keys and values that
+    no query near by (in its 256) sees may hold anything, the others must be finite.  Scratch comes from the allocator of the current stream."""
+    stream = _launch_stream(q, k_pages, v_pages, table, seqlens_k, cu_seqlens_q, out, lse)
+    if not (-1 <= left <= _FAR and -1 <= right <= _FAR and 0 <= sinks <= _FAR):
+        raise _capi.ExtensionError("left, right and sinks are within 2^30")
+    shape, pshape = q.shape, k_pages.shape
+    if q.dtype != torch.bfloat16:
+        raise _capi.ExtensionError("q must be bfloat16")
+    k_strides, v_strides = _pool(k_pages, pshape), _pool(v_pages, pshape)
+    pages, P, Hk, D = pshape
+    packed = cu_seqlens_q is not None
+    if len(shape) != (3 if packed else 4) or shape[-1] != D:
+        raise _capi.ExtensionError("q is [B,S,H,D], packed [T,H,D], with the pages' channels")
+    if table.dtype != torch.int32 or table.dim() != 2 or not table.is_contiguous():
+        raise _capi.ExtensionError("table is contiguous int32 [sequences, columns]")
+    nseg, columns = table.shape
+    if seqlens_k.dtype != torch.int32 or seqlens_k.numel() != nseg or not seqlens_k.is_contiguous():
+        raise _capi.ExtensionError("seqlens_k is contiguous int32 with one length per sequence")
+    if packed:
+        T, H, _ = shape
+        sq = min(T, int(max_seqlen_q)) if max_seqlen_q is not None else T
+        if cu_seqlens_q.dtype != torch.int32 or not cu_seqlens_q.is_contiguous() or cu_seqlens_q.numel() != nseg + 1:
+            raise _capi.ExtensionError("cu_seqlens_q must be contiguous int32, one more than sequences")
+        lse_shape = (H, T) if lse_layout == LSE_BHS else (T, H)
+    else:
+        batch, sq, H, _ = shape
+        if batch != nseg:
+            raise _capi.ExtensionError("q and the table must have one batch size")
+        T = nseg * sq
+        lse_shape = (nseg, H, sq) if lse_layout == LSE_BHS else (nseg, sq, H)
+    sk = min(columns * P, _FAR - 1)
+    if max_seqlen_k is not None:
+        sk = max(0, min(sk, int(max_seqlen_k)))
+    if accumulate and (out is None or lse is None or out.dtype != torch.float32):
+        raise _capi.ExtensionError("accumulate needs an existing fp32 (out, lse) state")
+    if out is None:
+        if out_dtype not in _VALUES:
+            raise _capi.ExtensionError("out must be float32 or bfloat16")
+        out = _empty_like(q, out_dtype)
+    elif out.shape != shape or not out.is_contiguous() or out.dtype not in _VALUES:
+        raise _capi.ExtensionError("out must be contiguous float32 or bfloat16 of q's shape")
+    if lse is None:
+        lse = _empty(lse_shape, torch.float32, q.device)
+    elif tuple(lse.shape) != lse_shape or not lse.is_contiguous() or lse.dtype != torch.float32:
+        raise _capi.ExtensionError(f"lse must be a contiguous fp32 tensor of shape {lse_shape}")
+    if q.numel() == 0 or sq <= 0:
+        return out, lse
+    lib = _capi.load()
+    key = (q.get_device(), nseg, sq, sk, H, Hk, D)
+    need = _PAGED_SCRATCH.get(key)
+    if need is None:
+        need = lib.dtb_flash_paged_scratch_bytes(nseg, sq, sk, H, Hk, D)
+        if need < 0:
+            _capi.check(need, "dtb_flash_paged_scratch_bytes")
+        if len(_PAGED_SCRATCH) >= 4096:
+            _PAGED_SCRATCH.clear()
+        _PAGED_SCRATCH[key] = need
+    scratch = _empty((need,), torch.uint8, q.device)
+    ev = None
+    if LaunchLog.events is not None:
+        ev = (torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True))
+        ev[0].record()
+    rc = lib.dtb_flash_paged(
+        q.data_ptr(), *_strides(q, shape), k_pages.data_ptr(), *k_strides, v_pages.data_ptr(), *v_strides, pages, P, table.data_ptr(), columns,
+        seqlens_k.data_ptr(), cu_seqlens_q.data_ptr() if packed else None, out.data_ptr(), _VALUES[out.dtype], lse.data_ptr(), lse_layout, accumulate,
+        nseg, sq, sk, T, H, Hk, D, D ** -0.5 if softmax_scale is None else softmax_scale, left, right, sinks, scratch.data_ptr(), need, stream)
+    if rc:
+        _capi.check(rc, "dtb_flash_paged")
+    LaunchLog.count += 2
+    if ev is not None:
+        ev[1].record()
+        span = sk if left < 0 or right < 0 else min(sk, left + right + 1 + sinks)      # upper bound of a row's keys
+        LaunchLog.events.append((ev[0], ev[1], 4.0 * T * H * span * D))
+    return out, lse
+
+
 class QuantizedRows(NamedTuple):
     """Values of a state in 8 bits: codes [..,H,D] (int8 or float8_e4m3fn) and one exponent byte b per row [..,H]; a value is
     code * 2^(b - 127).  b = 255 marks a row with an infinity or a NaN, which reads back as NaN."""

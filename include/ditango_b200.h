@@ -190,6 +190,62 @@ DTB_API int64_t dtb_flash_window_scratch_bytes(int nseg, int seqlen_q, int seqle
                                                int left, int right, int sinks);
 
 /*
+ * Keys and values of sequences that grow, in pages.  (The reference has no cache of keys and values.)  A pool holds `pages` pages of
+ * `page_size` tokens, a power of two from 16 to 2^20: k_pages and v_pages, bf16, token t of head h of page n at
+ * n * page_stride + t * tok_stride + h * head_stride, head_dim channels behind it; strides are multiples of 8 elements, pointers 16-byte
+ * aligned.  Slot s is token s % page_size of page s / page_size.  table[b][j], int32 [streams, columns], is the page that holds the tokens
+ * [j * page_size, (j + 1) * page_size) of stream b.  A row of the table has room for fewer than 2^30 tokens, the pool for fewer than 2^31.
+ * free_pages, int32 [pages]: the first *free_count of it are pages that nobody holds, the last of those is taken first.
+ *
+ * dtb_extend_pages: room for new_lens[b] >= 0 tokens behind the seqlens[b] of each stream, for streams in their order.
+ *   table           gets the new pages' numbers; its other entries stay
+ *   slots           [tokens]: the new tokens' slots, stream after stream; -1 behind the last one, and for a token on a page that was given
+ *                   back before (of a stream that was cut short within what a window had left behind)
+ *   cu_seqlens      [streams + 1]: where each stream's new tokens begin among them, and their number
+ *   seqlens_out     [streams], free_count_out: the numbers as they are now (not over seqlens or free_count)
+ *   missing         0; or how many pages there were too few, or -1 where a stream's tokens do not fit its row, all of them not `tokens`, or a
+ *                   number is out of range: then nothing was taken, slots are -1, cu_seqlens 0, the numbers those of before
+ * dtb_release_pages: the pages of stream b whose tokens all lie in [begin[b], end[b]) go to the end of the list, streams and their pages in
+ * order; their entries become -1.  A stream whose end it is (end[b] >= seqlens[b] > begin[b]) is begin[b] tokens long afterwards.
+ *   table_out       the table afterwards, may be `table`
+ *   streams * (columns / 256, rounded up) is at most 262144.
+ * dtb_write_pages: k, v of `tokens` tokens, bf16, token t at t * tok_stride, its heads dense behind it, to the slots of slots[t]; a token whose
+ * slot is -1, or not in the pool, is left out.  Of two tokens with one slot either one may stay, for keys and values each.
+ * All three are one launch.
+ */
+DTB_API int dtb_extend_pages(int32_t* table, const int32_t* seqlens, const int32_t* new_lens, const int32_t* free_pages, const int32_t* free_count,
+                     int streams, int columns, int pages, int page_size, int32_t* slots, int64_t tokens, int32_t* cu_seqlens,
+                     int32_t* seqlens_out, int32_t* free_count_out, int32_t* missing, void* stream);
+DTB_API int dtb_release_pages(const int32_t* table, int32_t* table_out, const int32_t* seqlens, const int32_t* begin, const int32_t* end,
+                     int32_t* free_pages, const int32_t* free_count, int streams, int columns, int pages, int page_size,
+                     int32_t* seqlens_out, int32_t* free_count_out, void* stream);
+DTB_API int dtb_write_pages(const void* k, const void* v, int64_t k_tok_stride, int64_t v_tok_stride, int64_t tokens, const int32_t* slots,
+                     void* k_pages, int64_t k_page_stride, int64_t k_page_tok_stride, int64_t k_head_stride,
+                     void* v_pages, int64_t v_page_stride, int64_t v_page_tok_stride, int64_t v_head_stride,
+                     int pages, int page_size, int num_kv_heads, int head_dim, void* stream);
+
+/*
+ * dtb_flash_window over a pool: attention of each sequence's newest queries, the last at the last key's position, over its seqlens_k[b] keys,
+ * which include their own.  Arguments as there and above;
+ *   table          int32 [nseg, columns]; the rows together have room for fewer than 2^31 tokens.  A page number outside the pool stands for
+ *                  keys and values of 0.
+ *   seqlens_k      int32 [nseg], taken to be at most columns * page_size
+ *   cu_seqlens_q   NULL for a dense batch of seqlen_q queries each, else device int32 [nseg + 1]; rows outside all sequences are left alone
+ *   seqlen_q       the longest sequence's queries (of longer ones the rest is left out); seqlen_k: about the longest sequence's keys, which
+ *                  only the choice of kernels goes by
+ *   scratch        dtb_flash_paged_scratch_bytes(...) bytes, 16-byte aligned, of one call at a time
+ */
+DTB_API int64_t dtb_flash_paged_scratch_bytes(int nseg, int seqlen_q, int seqlen_k, int num_heads, int num_kv_heads, int head_dim);
+DTB_API int dtb_flash_paged(const void* q, int64_t q_tok_stride, int64_t q_batch_stride,
+                     const void* k_pages, int64_t k_page_stride, int64_t k_tok_stride, int64_t k_head_stride,
+                     const void* v_pages, int64_t v_page_stride, int64_t v_tok_stride, int64_t v_head_stride,
+                     int pages, int page_size, const int32_t* table, int columns, const int32_t* seqlens_k, const int32_t* cu_seqlens_q,
+                     void* out, int out_dtype, float* lse, int lse_layout, int accumulate,
+                     int nseg, int seqlen_q, int seqlen_k, int64_t total_q, int num_heads, int num_kv_heads, int head_dim, float softmax_scale,
+                     int left, int right, int sinks, void* scratch, int64_t scratch_bytes, void* stream);
+
+
+/*
  * N-way merge of partial softmax states in one pass over HBM:
  *     lse_out = log sum_i exp(lse_i),   out = sum_i exp(lse_i - lse_out) * out_i
  * Replaces the chains of update_out_and_lse (utils.py:24-84) at core/attention.py:110-116, :144,
