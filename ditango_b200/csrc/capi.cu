@@ -845,19 +845,15 @@ DTB_API int dtb_flash_paged(const void* q, int64_t q_tok_stride, int64_t q_batch
   p.columns = columns;
   p.pages = pages;
   p.page_shift = shift;
-  p.few_rows = plan.few_rows;
+  // Sequences of few and of many queries in one batch take a launch each.  (With rows for more than that, none of them has few, unless there are
+  // rows behind the last one; the kernel of many then takes it.)
+  const bool mixed = plan.tiles && cu_seqlens_q != nullptr && total_q <= static_cast<int64_t>(nseg - 1) * seqlen_q + plan.few_rows;
+  p.few_rows = plan.tiles && !mixed ? -1 : plan.few_rows;
   if ((rc = load_encoder()) != DTB_OK) return rc;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   dtb::PagedMap mk, mv;
   auto make_maps = [&](int box_rows) {
-    for (dtb::PagedMap* m : {&mk, &mv}) {
-      m->table = table;
-      m->columns = columns;
-      m->pages = pages;
-      m->page_shift = shift;
-      m->box_rows = box_rows;
-      m->dim_shift = head_dim == 64 ? 6 : 7;
-    }
+    mk.dim_shift = mv.dim_shift = head_dim == 64 ? 6 : 7;
     p.box_rows = p.key_align = box_rows;
     const int r = make_page_map(&mk.map, k_pages, head_dim, page_size, k_tok_stride, num_kv_heads, k_head_stride, pages, k_page_stride, box_rows, &p.k_batch_first, "k_pages");
     return r != DTB_OK ? r : make_page_map(&mv.map, v_pages, head_dim, page_size, v_tok_stride, num_kv_heads, v_head_stride, pages, v_page_stride, box_rows, &p.v_batch_first, "v_pages");
@@ -871,7 +867,7 @@ DTB_API int dtb_flash_paged(const void* q, int64_t q_tok_stride, int64_t q_batch
     if ((rc = make_token_map(&tq, q, q_width, packed ? total_q : seqlen_q, q_tok_stride, packed ? 1 : nseg, q_batch_stride, &p.q_batch_first, "q")) != DTB_OK) return rc;
     e = head_dim == 64 ? dtb::launch_paged_tiles<64>(tq, mk, mv, p, s) : dtb::launch_paged_tiles<128>(tq, mk, mv, p, s);
   }
-  if (e == cudaSuccess && (!plan.tiles || (cu_seqlens_q != nullptr && nseg > 1))) {
+  if (e == cudaSuccess && (!plan.tiles || mixed)) {
     if ((rc = make_maps(std::min(page_size, 64))) != DTB_OK) return rc;
     e = head_dim == 64 ? dtb::launch_paged_rows<64>(mk, mv, p, plan.rows, scratch, s) : dtb::launch_paged_rows<128>(mk, mv, p, plan.rows, scratch, s);
   }

@@ -8,7 +8,7 @@
 //   warps 8-11   results: O out of tensor memory, normalisation, merge with the state in global memory, stores
 //   warp  12     blocks, their plans, TMA loads; the results of blocks that see no key
 //   warp  13     MMA issuer
-//   warps 14-15  no role
+//   warps 14-15  loads of keys and values in pages; no role where they are dense
 //
 // Key tiles of a block: N that cover the window [lo, hi) of its rows, the first one beginning at the first key that any of them sees, then
 // the tiles that hold the first tokens.  The rows of Q tile 1 are 128 further on than those of Q tile 0, and so are their windows, by
@@ -304,6 +304,7 @@ flash_window_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     }
     for (int i = 0; i < kTails; ++i) mbar_init(&sh.v_tail[i], 1);
     mbar_init(sh.claim, 1);
+    init_loads(p);
     fence_mbar_init();
   }
   if (warp == kMmaWarp + 1 && lane < D / 4) {
@@ -340,8 +341,10 @@ flash_window_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
 
   if (warp >= kTmaWarp) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kRegsOther));
-    if (aborted || warp > kMmaWarp) {
+    if (aborted) {
       // fall through to the tear-down
+    } else if (warp > kMmaWarp) {
+      serve_loads<D>(p, warp - kMmaWarp - 1);
     } else if (warp == kTmaWarp) {
       // ------------------------------------------------------------ blocks and TMA loads
       const Shared<D> sh(smem + opaque_zero());
@@ -479,6 +482,7 @@ flash_window_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         bulk_store_wait();               // the zeros have been read
       }
       __syncwarp();
+      if (lane == 0) end_loads(p);
     } else {
       // ------------------------------------------------------------ MMA issuer
       const Shared<D> sh(smem + opaque_zero());
