@@ -755,7 +755,7 @@ static PagedPlan plan_paged(int64_t nseg, int64_t seqlen_q, int64_t seqlen_k, in
   const int64_t group = num_heads / kv_heads;
   plan.few_rows = static_cast<int>(std::max<int64_t>(128 / group, 1));
   plan.tiles = seqlen_q > plan.few_rows;
-  plan.rows = dtb::plan_paged_rows(static_cast<int>(std::min<int64_t>(std::min<int64_t>(seqlen_q, plan.few_rows) * group, 64)), head_dim, sm_count);
+  plan.rows = dtb::plan_paged_rows(std::min<int64_t>(seqlen_q, plan.few_rows) * group, seqlen_k, kv_heads, nseg, head_dim, sm_count);
   plan.scratch_bytes = plan.rows.scratch_bytes;
   return plan;
 }

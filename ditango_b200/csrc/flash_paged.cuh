@@ -139,7 +139,8 @@ struct PagedRowsPlan {
   int ctas;                // at most
   int64_t scratch_bytes;
 };
-PagedRowsPlan plan_paged_rows(int rows_of_a_head, int head_dim, int sm_count);
+// (rows of a key head's longest sequence; `keys` of the longest sequence, about: more CTAs than that needs would not be used)
+PagedRowsPlan plan_paged_rows(int64_t rows_of_a_head, int64_t keys, int64_t kv_heads, int64_t nseg, int head_dim, int sm_count);
 template <int D>
 cudaError_t launch_paged_rows(const PagedMap& tm_k, const PagedMap& tm_v, const PagedParams& p, const PagedRowsPlan& plan, void* scratch, cudaStream_t stream);
 

@@ -1,9 +1,9 @@
 // Attention of few query rows over keys and values in pages: all keys of all sequences dealt evenly to CTAs that stay.
 //
 // A row is a query and one of the heads that share a key head; a block of up to 16, 32 or 64 rows of one key head meets the keys that any row of
-// its sequence sees, [0, first) and [lo, hi), in tiles of 64.  Sequence after sequence, key head after key head, block after block, the tiles
-// are numbered through, W in all, and CTA c of G takes [c W / G, (c + 1) W / G): the lengths stand on the device, and so every CTA works out
-// for itself where its share begins.  Per warp of rows and keys a softmax state (m, l, O) is kept:
+// its sequence sees, [0, first) and [lo, hi), in tiles of 64.  Sequence after sequence, key head after key head, block after block, places
+// are numbered through, one per tile and a few in front of each block for what that costs, and each CTA takes as many of them as any other: the
+// lengths stand on the device, and so every CTA works out for itself where its share begins.  Per warp of rows and keys a softmax state (m, l, O) is kept:
 //     S = Q K^T,  m' = max(m, max S) where that grew by more than 2^8, else m,  P = 2^(c (S - m')),
 //     l' = l 2^(c (m - m')) + sum P,  O' = O 2^(c (m - m')) + P V
 // The states of the warps are joined in shared memory.  A block that one CTA has all tiles of is written as it is; the parts of one that several
@@ -27,7 +27,8 @@ using namespace flash;
 constexpr int kMathWarps = 4;
 constexpr int kThreads = (kMathWarps + 1) * 32;
 constexpr int kKeys = 64;                 // of a tile
-constexpr int kMinTiles = 2;              // of a CTA's share, unless there are fewer
+constexpr int kBlockCost = 2;             // places in front of a block's tiles
+constexpr int kMinPlaces = 2;             // of a CTA's share, unless there are fewer
 constexpr int kColumns = 32;              // joined at a time
 constexpr int kPitch = kColumns + 8;      // floats of a row of them in shared memory (rows 8 banks apart)
 
@@ -45,13 +46,11 @@ struct Cfg {
   static_assert(2 * (kBytes + 1024) <= 228 * 1024, "two CTAs to an SM");
 };
 
-// Where a CTA's share begins, and what there is in all; a CTA's is read by the launch that joins.
-struct alignas(16) Share {
-  int64_t first, all;        // its first tile, and all there are
-  int seg, unit, tile;       // sequence, (key head, row block) of it, tile of that
-  int tiles;                 // of each unit of the sequence
-  int ctas;                  // that have a share
-  int pad[3];
+// What the launch that joins has to know of the boundary in front of a CTA's share.
+struct alignas(16) Join {
+  int parts;                 // of the block that the boundary is the first one in; 0: in none, or not the first
+  int cta, late;             // that has the first part; whether that was not the first block of its share
+  int seg, q_begin, kv_head, row0, rows;
 };
 
 // A sequence as its rows' keys are walked.
@@ -61,6 +60,7 @@ struct Seq {
   int first, lo, hi;         // keys that any row sees: [0, first) and [lo, hi)
   int lead;                  // tiles of the former
   int tiles;                 // in all, 1 where there is no key: the block's rows are written all the same
+  int group;                 // query heads of a key head
 
   __device__ __forceinline__ int begin(int tile) const { return tile < lead ? tile * kKeys : lo + (tile - lead) * kKeys; }
 };
@@ -70,7 +70,8 @@ __device__ __forceinline__ Seq make_seq(const PagedParams& p, int seg) {
   Seq s;
   s.w = paged_seq(p, seg);
   if (s.w.q_len > p.few_rows) s.w.q_len = 0;
-  s.blocks = (s.w.q_len * (p.f.num_heads / p.kv_heads) + R - 1) / R;
+  s.group = p.f.num_heads / p.kv_heads;
+  s.blocks = (s.w.q_len * s.group + R - 1) / R;
   const WindowSpan a = window_span(s.w, 0), z = window_span(s.w, max(s.w.q_len - 1, 0));
   s.first = z.first;
   s.hi = z.hi;
@@ -98,19 +99,56 @@ struct Block {
 template <int R>
 __device__ __forceinline__ Block make_block(const PagedParams& p, const Seq& s, int unit) {
   Block b;
-  const int group = p.f.num_heads / p.kv_heads;
   b.kv_head = unit / s.blocks;
-  b.row0 = unit % s.blocks * R;
-  b.rows = min(R, s.w.q_len * group - b.row0);
-  const WindowSpan a = window_span(s.w, b.row0 / group), z = window_span(s.w, (b.row0 + b.rows - 1) / group);
+  b.row0 = (unit - b.kv_head * s.blocks) * R;
+  b.rows = min(R, s.w.q_len * s.group - b.row0);
+  const WindowSpan a = window_span(s.w, b.row0 / s.group), z = window_span(s.w, (b.row0 + b.rows - 1) / s.group);
   b.first = z.first;
   b.lo = max(a.lo, z.first);
   b.hi = z.hi;
   return b;
 }
 
-__device__ __forceinline__ int64_t share_begin(int c, int64_t all, int ctas) { return c * all / ctas; }
-__device__ __forceinline__ int share_of(int64_t tile, int64_t all, int ctas) { return static_cast<int>(((tile + 1) * ctas - 1) / all); }
+// Shares: the first `longer` CTAs have `size` + 1 places, the others `size`.  (Divisions in 32 bits where they do: they are a fifth as long.)
+__device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
+  return ((a | b) >> 31) == 0 ? static_cast<int64_t>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b)) : a / b;
+}
+struct Shares {
+  int64_t all, size;
+  int ctas, longer;
+
+  __device__ __forceinline__ Shares(int64_t places, int most) {
+    all = places;
+    const int64_t n = places / kMinPlaces;
+    ctas = static_cast<int>(n < 1 ? (places > 0) : n < most ? n : most);
+    size = ctas > 0 ? divide(places, ctas) : 0;
+    longer = static_cast<int>(places - size * ctas);
+  }
+  __device__ __forceinline__ int64_t begin(int c) const { return c * size + min(c, longer); }
+  __device__ __forceinline__ int of(int64_t place) const {
+    const int64_t first = longer * (size + 1);
+    return static_cast<int>(place < first ? divide(place, size + 1) : longer + divide(place - first, size));
+  }
+};
+
+// Places of a sequence's block, and the tiles that lie in front of one of them.
+__device__ __forceinline__ int places_of(const Seq& s) { return s.tiles + kBlockCost; }
+__device__ __forceinline__ int tiles_before(int place) { return max(place - kBlockCost, 0); }
+
+// The record of the boundary in front of CTA `cta`, whose share begins at `place` of the block.
+__device__ __forceinline__ Join make_join(const Shares& sh, const Seq& s, const Block& b, int seg, int cta, int place) {
+  Join j = {0, 0, 0, seg, s.w.q_begin, b.kv_head, b.row0, b.rows};
+  if (tiles_before(place) > 0) {
+    const int64_t begin = sh.begin(cta) - place;
+    const int c0 = sh.of(begin + kBlockCost), c1 = sh.of(begin + places_of(s) - 1);      // that have its first tile, and its last
+    if (c0 == cta - 1) {
+      j.parts = c1 - c0 + 1;
+      j.cta = c0;
+      j.late = sh.begin(c0) < begin;
+    }
+  }
+  return j;
+}
 
 __device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
@@ -121,7 +159,7 @@ __device__ __forceinline__ void ldmatrix4_trans(uint32_t addr, uint32_t (&r)[4])
 }
 // d += a b: 16 x 16 (rows x k) by 16 x 8
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -142,9 +180,9 @@ __device__ __forceinline__ void math_warps_sync() { asm volatile("bar.sync 1, 12
 // Four columns of a finished row: normalised, merged with the state in memory where the launch accumulates, stored.  `write_lse`: this thread
 // writes the row's lse; the threads of a row that read it before are all in its warp (`mask`) or behind a barrier.
 template <int D>
-__device__ __forceinline__ void store_row4(const PagedParams& p, int seg, const WindowSeq& s, int i, int head, int col, float4 acc, float m, float l,
+__device__ __forceinline__ void store_row4(const PagedParams& p, int seg, int q_begin, int i, int head, int col, float4 acc, float m, float l,
                                            bool write_lse, uint32_t mask) {
-  const int64_t tok = p.f.cu_q != nullptr ? static_cast<int64_t>(s.q_begin) + i : static_cast<int64_t>(seg) * p.f.seqlen_q + i;
+  const int64_t tok = p.f.cu_q != nullptr ? static_cast<int64_t>(q_begin) + i : static_cast<int64_t>(seg) * p.f.seqlen_q + i;
   const int64_t li = lse_index(p.f, seg, head, i, tok), oi = tok * p.f.out_tok_stride + static_cast<int64_t>(head) * D + col;
   const bool empty = l == 0.f;                    // no key seen: nothing to write over a state  (a NaN among the scores is not empty)
   const bool keep = empty && p.f.accumulate != 0;
@@ -174,15 +212,15 @@ __device__ __forceinline__ void store_row4(const PagedParams& p, int seg, const 
   if (write_lse && !keep) p.f.lse[li] = lse_out;
 }
 
-// The scratch of a launch: shares, then the states' (m, l) and values, two of each CTA (of the first block of its share, and of the last).
+// The scratch of a launch: records, then the states' (m, l) and values, two of each CTA (of the first block of its share, and of the last).
 template <int D, int R>
 struct Scratch {
-  Share* shares;
+  Join* joins;
   float2* ml;
   float* o;
   __host__ __device__ Scratch(void* base, int ctas) {
-    shares = static_cast<Share*>(base);
-    ml = reinterpret_cast<float2*>(shares + ctas);
+    joins = static_cast<Join*>(base);
+    ml = reinterpret_cast<float2*>(joins + ctas);
     o = reinterpret_cast<float*>(ml + 2 * static_cast<int64_t>(ctas) * R);
   }
 };
@@ -201,7 +239,8 @@ flash_paged_rows_kernel(const __grid_constant__ PagedMap tm_k, const __grid_cons
   uint64_t* full = reinterpret_cast<uint64_t*>(s_ml + WN * R);
   uint64_t* empty = full + C::kStages;
   __shared__ long long s_sum[kThreads / 32];
-  __shared__ Share s_share;
+  __shared__ Seq s_seq;                     // the share's first sequence, ...
+  __shared__ int s_seg, s_unit, s_place;    // ... (key head, row block) of that, and place of the block
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Scratch<D, R> sc(scratch, gridDim.x);
 
@@ -212,7 +251,6 @@ flash_paged_rows_kernel(const __grid_constant__ PagedMap tm_k, const __grid_cons
       mbar_init(&empty[i], kMathWarps);
     }
     fence_mbar_init();
-    s_share.ctas = 0;
   }
   if (warp == kMathWarps && lane == 0) {
     prefetch_tmap(&tm_k);
@@ -220,9 +258,10 @@ flash_paged_rows_kernel(const __grid_constant__ PagedMap tm_k, const __grid_cons
   }
   // ------------------------------------------------------------------ this CTA's share
   const int per = (p.f.nseg + kThreads - 1) / kThreads, seg0 = min(static_cast<int>(threadIdx.x) * per, p.f.nseg), seg1 = min(seg0 + per, p.f.nseg);
-  auto weight = [&](const Seq& s) { return static_cast<long long>(s.blocks) * p.kv_heads * s.tiles; };
+  auto places = [&](const Seq& s) { return static_cast<long long>(s.blocks) * p.kv_heads * places_of(s); };
   long long sum = 0;
-  for (int i = seg0; i < seg1; ++i) sum += weight(make_seq<R>(p, i));
+  Seq s;
+  for (int i = seg0; i < seg1; ++i) sum += places(s = make_seq<R>(p, i));
   long long upto = sum;
 #pragma unroll
   for (int d = 1; d < 32; d *= 2) {
@@ -238,43 +277,39 @@ flash_paged_rows_kernel(const __grid_constant__ PagedMap tm_k, const __grid_cons
     if (w < warp) at += s_sum[w];
     all += s_sum[w];
   }
-  const long long most = all / kMinTiles;
-  const int ctas = static_cast<int>(most < 1 ? (all > 0) : most < gridDim.x ? most : gridDim.x);
+  const Shares shares(all, gridDim.x);
   const int cta = blockIdx.x;
-  if (cta >= ctas) {
-    if (cta == 0 && threadIdx.x == 0) sc.shares[0].ctas = 0;
+  if (cta >= shares.ctas) {
+    if (threadIdx.x == 0) sc.joins[cta].parts = 0;
     return;
   }
-  const long long begin = share_begin(cta, all, ctas), end = share_begin(cta + 1, all, ctas);
+  const long long begin = shares.begin(cta);
   if (begin >= at && begin < at + sum) {
     for (int i = seg0; i < seg1; ++i) {
-      const Seq s = make_seq<R>(p, i);
-      if (begin < at + weight(s)) {
-        Share& w = s_share;
-        w.first = begin;
-        w.all = all;
-        w.seg = i;
-        w.unit = static_cast<int>((begin - at) / s.tiles);
-        w.tile = static_cast<int>((begin - at) % s.tiles);
-        w.tiles = s.tiles;
-        w.ctas = ctas;
-        sc.shares[cta] = w;
+      if (per > 1) s = make_seq<R>(p, i);
+      if (begin < at + places(s)) {
+        s_seq = s;
+        s_seg = i;
+        s_unit = static_cast<int>(divide(begin - at, places_of(s)));
+        s_place = static_cast<int>(begin - at - static_cast<long long>(s_unit) * places_of(s));
         break;
       }
-      at += weight(s);
+      at += places(s);
     }
   }
   __syncthreads();
 
-  int seg = s_share.seg, unit = s_share.unit, tile = s_share.tile;
-  long long left = end - begin;             // tiles
+  int seg = s_seg, unit = s_unit, place = s_place;
+  long long left = shares.begin(cta + 1) - begin;             // places
   int stage = 0;
   uint32_t use = 0;                         // parity of the ring's round
-  Seq s = make_seq<R>(p, seg);
+  s = s_seq;
   bool first_block = true;
-  auto next_block = [&](int to) {
-    left -= to - tile;
-    tile = 0;
+  // the block's tiles that are this CTA's: up to, not with, this one
+  auto last_tile = [&]() { return tiles_before(static_cast<int>(min(static_cast<long long>(places_of(s)), place + left))); };
+  auto next_block = [&]() {
+    left -= min(static_cast<long long>(places_of(s) - place), left);
+    place = 0;
     first_block = false;
     if (++unit == s.blocks * p.kv_heads && left > 0) {
       unit = 0;
@@ -288,7 +323,7 @@ flash_paged_rows_kernel(const __grid_constant__ PagedMap tm_k, const __grid_cons
     const int box = p.box_rows, boxes = kKeys / box;
     while (ok && left > 0) {
       const Block b = make_block<R>(p, s, unit);
-      const int to = static_cast<int>(min(static_cast<long long>(s.tiles), tile + left));
+      const int tile = tiles_before(place), to = last_tile();
       const int32_t* row = p.table + static_cast<int64_t>(seg) * p.columns;
       for (int t = tile; t < to; ++t) {
         const int a = s.begin(t);
@@ -321,17 +356,21 @@ flash_paged_rows_kernel(const __grid_constant__ PagedMap tm_k, const __grid_cons
           wrapped = true;
         }
       }
-      next_block(to);
+      next_block();
     }
   } else {
     // ---------------------------------------------------------------- scores, weights, products
     const int wm = warp / WN, wn = warp % WN;
-    const int group = p.f.num_heads / p.kv_heads;
     const float c = p.f.scale_log2;
+    if (threadIdx.x == 0) sc.joins[cta] = make_join(shares, s, make_block<R>(p, s, unit), seg, cta, place);
     bool ok = true;             // after a wait that gave up, the blocks are walked to their barriers and nothing more is stored
     while (left > 0) {
+      const int tile = tiles_before(place), to = last_tile(), group = s.group;
+      if (tile == to) {                         // places in front of a block that the next CTA begins with
+        next_block();
+        continue;
+      }
       const Block b = make_block<R>(p, s, unit);
-      const int to = static_cast<int>(min(static_cast<long long>(s.tiles), tile + left));
       // this thread's rows lane / 4 and lane / 4 + 8 of the warp's 16; rows that there are not see what the last one sees
       int end_first[2], from_w[2], to_w[2];
       uint32_t qf[D / 16][4];
@@ -377,17 +416,20 @@ flash_paged_rows_kernel(const __grid_constant__ PagedMap tm_k, const __grid_cons
             fence_proxy_async_smem();
             __syncwarp();
           }
+          // (all keys for 16 channels before the next 16: as many chains of products as the warp has keys to feed them)
           float sr[KW / 8][4];
 #pragma unroll
-          for (int n = 0; n < KW / 16; ++n) {
+          for (int n = 0; n < KW / 8; ++n)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sr[2 * n][e] = sr[2 * n + 1][e] = 0.f;
-            const int row = key0 + n * 16 + ((lane >> 4) << 3) + (lane & 7);
-            const uint32_t at_row = ks + row * 128;
+            for (int e = 0; e < 4; ++e) sr[n][e] = 0.f;
+          const uint32_t k_row = ks + (key0 + ((lane >> 4) << 3) + (lane & 7)) * 128;
 #pragma unroll
-            for (int k = 0; k < D / 16; ++k) {
+          for (int k = 0; k < D / 16; ++k) {
+            const uint32_t piece = (k >> 2) * C::kSlab + ((((2 * k + ((lane >> 3) & 1)) & 7) ^ (lane & 7)) << 4);
+#pragma unroll
+            for (int n = 0; n < KW / 16; ++n) {
               uint32_t f[4];
-              ldmatrix4(at_row + (k >> 2) * C::kSlab + ((((2 * k + ((lane >> 3) & 1)) & 7) ^ (row & 7)) << 4), f);
+              ldmatrix4(k_row + n * 16 * 128 + piece, f);
               mma16816(sr[2 * n], qf[k], f[0], f[1]);
               mma16816(sr[2 * n + 1], qf[k], f[2], f[3]);
             }
@@ -504,7 +546,7 @@ flash_paged_rows_kernel(const __grid_constant__ PagedMap tm_k, const __grid_cons
           const bool last = x == D / kColumns - 1 && col == 0;
           if (whole) {
             const int row = b.row0 + r;
-            store_row4<D>(p, seg, s.w, row / group, b.kv_head * group + row % group, x * kColumns + col, acc, mm, ll, last, mask);
+            store_row4<D>(p, seg, s.w.q_begin, row / group, b.kv_head * group + row % group, x * kColumns + col, acc, mm, ll, last, mask);
           } else {
             *reinterpret_cast<float4*>(sc.o + (static_cast<int64_t>(slot) * R + r) * D + x * kColumns + col) = acc;
             if (last) sc.ml[static_cast<int64_t>(slot) * R + r] = make_float2(mm, ll);
@@ -512,106 +554,98 @@ flash_paged_rows_kernel(const __grid_constant__ PagedMap tm_k, const __grid_cons
         }
         math_warps_sync();
       }
-      next_block(to);
+      next_block();
     }
   }
   if (*reinterpret_cast<volatile int*>(p.f.status) != 0) __nanosleep(1000000);   // let copies in flight land
 }
 
-// Joins the parts of a block that several CTAs worked on.  grid: (boundaries between two CTAs' shares, rows in fours); the first boundary
-// inside a block is the one that counts.  A warp per row, four warps per row where there are many parts.
+// Joins the parts of a block that several CTAs worked on.  grid: (boundaries between two CTAs' shares, 16); the first boundary inside a block
+// is the one that counts.  The four warps share a row's parts, a lane has D / 32 columns.
 template <int D, int R>
 __global__ void __launch_bounds__(128) flash_paged_join_kernel(const __grid_constant__ PagedParams p, void* scratch) {
-  constexpr int kLaneCols = D / 32;
+  constexpr int kCols = D / 32;
   __shared__ float s_acc[4][D];
-  __shared__ float2 s_ml[4];
+  __shared__ float s_sum[4];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int cta = blockIdx.x + 1;
-  grid_dependency_wait();
-  if (*reinterpret_cast<volatile int*>(p.f.status) != 0) return;
   const Scratch<D, R> sc(scratch, gridDim.x + 1);
-  const int ctas = sc.shares[0].ctas;
-  if (cta >= ctas) return;
-  const Share w = sc.shares[cta];
-  if (w.tile == 0) return;                                     // the block before ends with the share before
-  const int64_t begin = w.first - w.tile, end = begin + w.tiles;
-  const int c0 = share_of(begin, w.all, ctas), c1 = share_of(end - 1, w.all, ctas);
-  if (c0 != cta - 1) return;
-  const Seq s = make_seq<R>(p, w.seg);
-  const Block b = make_block<R>(p, s, w.unit);
-  const int group = p.f.num_heads / p.kv_heads, n = c1 - c0 + 1;
+  const int group = p.f.num_heads / p.kv_heads;
   const float c = p.f.scale_log2;
-  // (only the first of them can have begun with another block)
-  auto slot_of = [&](int i) { return 2 * static_cast<int64_t>(c0 + i) + (i == 0 && share_begin(c0, w.all, ctas) < begin ? 1 : 0); };
-  const bool alone = n <= 8;                                   // a row to each warp
-  const int parts = alone ? 1 : 4, part = alone ? 0 : warp;
-  for (int r = blockIdx.y * 4 + (alone ? warp : 0), rounds = alone ? 1 : 4; rounds > 0; --rounds, ++r) {
-    if (r >= b.rows) return;                                   // (all warps of a row together)
-    float mm = -INFINITY, ll = 0.f, acc[kLaneCols] = {};
-    for (int i = lane; i < n; i += 32) mm = fmaxf(mm, sc.ml[slot_of(i) * R + r].x);
+  grid_dependency_wait();
+  const int status = *reinterpret_cast<volatile int*>(p.f.status);
+  const Join j = sc.joins[blockIdx.x + 1];
+  if (status != 0) return;
+  auto slot_of = [&](int i) { return static_cast<int64_t>(2 * (j.cta + i) + (i == 0 ? j.late : 0)) * R; };
+  for (int r = blockIdx.y; j.parts > 0 && r < j.rows; r += gridDim.y) {
+    float mm = -INFINITY;
+    for (int i = lane; i < j.parts; i += 32) mm = fmaxf(mm, sc.ml[slot_of(i) + r].x);
+    float sum = 0.f, acc[kCols] = {};
+    constexpr int kAhead = 8;
+    for (int i0 = 0; i0 < j.parts; i0 += 4 * kAhead) {
+      float2 ml[kAhead];
+      float v[kAhead][kCols];
 #pragma unroll
-    for (int d = 16; d > 0; d /= 2) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, d));
-    const float ref = reference(mm);
-#pragma unroll 8
-    for (int i = part; i < n; i += parts) {
-      const int64_t slot = slot_of(i) * R + r;
-      const float2 ml = sc.ml[slot];
-      const float f = ex2((ml.x - ref) * c);
-      ll = fmaf(ml.y, f, ll);
-      const float* src = sc.o + slot * D + lane * kLaneCols;
-      float v[kLaneCols];
-      if constexpr (D == 128) {
-        const float4 q = *reinterpret_cast<const float4*>(src);
-        v[0] = q.x, v[1] = q.y, v[2] = q.z, v[3] = q.w;
-      } else {
-        const float2 q = *reinterpret_cast<const float2*>(src);
-        v[0] = q.x, v[1] = q.y;
-      }
+      for (int u = 0; u < kAhead; ++u) {
+        const int i = i0 + 4 * u + warp;
+        ml[u] = make_float2(-INFINITY, 0.f);
 #pragma unroll
-      for (int k = 0; k < kLaneCols; ++k) acc[k] = fmaf(v[k], f, acc[k]);
-    }
-    if (!alone) {
-#pragma unroll
-      for (int k = 0; k < kLaneCols; ++k) s_acc[warp][lane * kLaneCols + k] = acc[k];
-      if (lane == 0) s_ml[warp] = make_float2(mm, ll);
-      __syncthreads();
-    }
-    // the row's columns, four to a lane
-    if (alone) {
-#pragma unroll
-      for (int k = 0; k < kLaneCols; ++k) s_acc[warp][lane * kLaneCols + k] = acc[k];
-      __syncwarp();
-    } else if (warp == 0) {
-      ll = 0.f;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) ll += s_ml[q].y;
-    }
-    if (alone || warp == 0) {
-      const int row = b.row0 + r;
-      if (lane < D / 4) {
-        float4 a = *reinterpret_cast<const float4*>(&s_acc[alone ? warp : 0][lane * 4]);
-        if (!alone) {
-#pragma unroll
-          for (int q = 1; q < 4; ++q) {
-            const float4 v = *reinterpret_cast<const float4*>(&s_acc[q][lane * 4]);
-            a.x += v.x;
-            a.y += v.y;
-            a.z += v.z;
-            a.w += v.w;
+        for (int k = 0; k < kCols; ++k) v[u][k] = 0.f;
+        if (i < j.parts) {
+          const int64_t at = slot_of(i) + r;
+          ml[u] = sc.ml[at];
+          const float* src = sc.o + at * D + lane * kCols;
+          if constexpr (D == 128) {
+            const float4 q = *reinterpret_cast<const float4*>(src);
+            v[u][0] = q.x, v[u][1] = q.y, v[u][2] = q.z, v[u][3] = q.w;
+          } else {
+            const float2 q = *reinterpret_cast<const float2*>(src);
+            v[u][0] = q.x, v[u][1] = q.y;
           }
         }
-        store_row4<D>(p, w.seg, s.w, row / group, b.kv_head * group + row % group, lane * 4, a, mm, ll, lane == 0, D == 128 ? 0xffffffffu : 0xffffu);
+      }
+      if (i0 == 0) {
+#pragma unroll
+        for (int d = 16; d > 0; d /= 2) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, d));
+      }
+      const float ref = reference(mm);
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const float f = ex2((ml[u].x - ref) * c);
+        sum = fmaf(ml[u].y, f, sum);
+#pragma unroll
+        for (int k = 0; k < kCols; ++k) acc[k] = fmaf(v[u][k], f, acc[k]);
       }
     }
-    if (!alone) __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kCols; ++k) s_acc[warp][lane * kCols + k] = acc[k];
+    if (lane == 0) s_sum[warp] = sum;
+    __syncthreads();
+    if (warp == 0 && lane < D / 4) {
+      float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+      float l = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float4 v = *reinterpret_cast<const float4*>(&s_acc[w][lane * 4]);
+        a.x += v.x;
+        a.y += v.y;
+        a.z += v.z;
+        a.w += v.w;
+        l += s_sum[w];
+      }
+      const int row = j.row0 + r;
+      store_row4<D>(p, j.seg, j.q_begin, row / group, j.kv_head * group + row % group, lane * 4, a, mm, l, lane == 0, D == 128 ? 0xffffffffu : 0xffffu);
+    }
+    __syncthreads();
   }
 }
 
-PagedRowsPlan plan_paged_rows(int rows_of_a_head, int head_dim, int sm_count) {
+PagedRowsPlan plan_paged_rows(int64_t rows_of_a_head, int64_t keys, int64_t kv_heads, int64_t nseg, int head_dim, int sm_count) {
   PagedRowsPlan plan;
   plan.rows = rows_of_a_head <= 16 ? 16 : rows_of_a_head <= 32 ? 32 : 64;
-  plan.ctas = 2 * sm_count;
-  plan.scratch_bytes = plan.ctas * (static_cast<int64_t>(sizeof(Share)) + 2 * plan.rows * (8 + head_dim * 4));
+  const int64_t places = (rows_of_a_head + plan.rows - 1) / plan.rows * kv_heads * nseg * (keys / kKeys + 2 + kBlockCost);
+  const int64_t resident = 2 * sm_count, useful = places / kMinPlaces;
+  plan.ctas = static_cast<int>(useful < 2 ? 2 : useful < resident ? useful : resident);
+  plan.scratch_bytes = plan.ctas * (static_cast<int64_t>(sizeof(Join)) + 2 * plan.rows * (8 + head_dim * 4));
   return plan;
 }
 
@@ -636,7 +670,7 @@ cudaError_t launch_rows(const PagedMap& tk, const PagedMap& tv, const PagedParam
   flash_paged_rows_kernel<D, WM><<<plan.ctas, kThreads, C::kBytes, stream>>>(tk, tv, p, scratch);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  return launch_attention_kernel(flash_paged_join_kernel<D, 16 * WM>, dim3(plan.ctas - 1, 4 * WM), 128, 0, stream, true, p, scratch);
+  return launch_attention_kernel(flash_paged_join_kernel<D, 16 * WM>, dim3(plan.ctas - 1, 16), 128, 0, stream, true, p, scratch);
 }
 
 }  // namespace

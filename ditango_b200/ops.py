@@ -470,7 +470,7 @@ def flash_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, t
 
     Dense: q [B,Sq,H,D] bf16.  Packed: q [T,H,D] with cu_seqlens_q int32 [B + 1] on the device, up to max_seqlen_q (known to the host, T if not
     given) queries each; rows behind the last sequence are left as they are.  Hk divides H.  max_seqlen_k is about the longest sequence's
-    length, if the host knows it: kernels are chosen by it, results do not depend on it.
+    length, if the host knows it: kernels and numbers of CTAs are chosen by it, and results depend on it by roundings alone.
 
     Returns (out, lse) as flash_window does, mergeable with its states and flash_partial's; with accumulate=True the state is merged into the given
     fp32 (out, lse) in place.  A row that sees no key has out 0 and lse -inf.  Entries of the table behind a sequence's last page or for pages that no

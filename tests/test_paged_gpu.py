@@ -287,8 +287,10 @@ def test_dense_queries_and_both_layouts_of_lse(n, D):
     cache = _Cache(lens, 2, D, 32, seed=2)
     q = _rand((4 * n, 6, D), 52)
     out, lse = _attend(cache, q, [n] * 4, right=0, packed=False)
-    again, bhs = ops.flash_paged(q.cuda().view(4, n, 6, D), cache.k_pages, cache.v_pages, cache.table, cache.seqlens, right=0, max_seqlen_k=77)
+    again, bhs = ops.flash_paged(q.cuda().view(4, n, 6, D), cache.k_pages, cache.v_pages, cache.table, cache.seqlens, right=0)
     assert torch.equal(bhs, lse.transpose(1, 2)) and torch.equal(again, out)
+    for hint in (1, 77, 10 ** 6):              # (about the longest length: other numbers of CTAs, and so other roundings)
+        _attend(cache, q, [n] * 4, right=0, packed=False, max_seqlen_k=hint)
     fused = torch.randn(4, n, 3, 6, D, device="cuda").to(torch.bfloat16)
     fused[:, :, 1] = q.cuda().view(4, n, 6, D)
     view, _ = ops.flash_paged(fused[:, :, 1], cache.k_pages, cache.v_pages, cache.table, cache.seqlens, right=0)

@@ -11,7 +11,7 @@ import subprocess
 
 import pytest
 
-from tests.test_flash_issuer_cpu import CSRC, _block
+from tests.test_flash_issuer_cpu import CSRC
 
 SOURCE = r"""
 #include <algorithm>
@@ -35,7 +35,8 @@ struct PagedParams : WindowParams { int columns, pages, page_shift, box_rows, ke
 %(span)s
 %(paged)s
 constexpr int kKeys = 64;
-constexpr int kMinTiles = %(min_tiles)s;
+%(constants)s
+struct Join { int parts, cta, late, seg, q_begin, kv_head, row0, rows; };
 %(walk)s
 constexpr int R = %(rows)d;
 int main(int argc, char** argv) {
@@ -49,33 +50,35 @@ int main(int argc, char** argv) {
   std::vector<int32_t> cu(1, 0), lens;
   for (int b = 0; b < n; ++b) { cu.push_back(cu.back() + a[9 + 2 * b]); lens.push_back(a[10 + 2 * b]); p.f.seqlen_q = max(p.f.seqlen_q, a[9 + 2 * b]); p.columns = max(p.columns, (a[10 + 2 * b] >> p.page_shift) + 1); }
   p.f.cu_q = cu.data(); p.seqlens_k = lens.data(); p.f.nseg = n;
-  auto weight = [&](const Seq& s) { return (long long)s.blocks * p.kv_heads * s.tiles; };
+  auto places = [&](const Seq& s) { return (long long)s.blocks * p.kv_heads * places_of(s); };
   long long all = 0;
-  for (int i = 0; i < n; ++i) all += weight(make_seq<R>(p, i));
-  const long long most = all / kMinTiles;
-  const int ctas = int(most < 1 ? (all > 0) : most < most_ctas ? most : most_ctas);
+  for (int i = 0; i < n; ++i) all += places(make_seq<R>(p, i));
+  const Shares sh(all, most_ctas);
+  const int ctas = sh.ctas;
+  CHECK(sh.begin(0) == 0 && sh.begin(ctas) == all && ctas <= most_ctas && (ctas > 0) == (all > 0));
   // (sequence, unit) -> [(CTA, slot, first tile, last tile)]
   std::map<std::pair<int, int>, std::vector<std::tuple<int, int, int, int>>> parts;
-  std::map<int, std::tuple<long long, int, int, int, int>> shares;
+  std::vector<Join> joins(max(ctas, 1));
   for (int c = 0; c < ctas; ++c) {
-    const long long begin = share_begin(c, all, ctas), end = share_begin(c + 1, all, ctas);
+    const long long begin = sh.begin(c), end = sh.begin(c + 1);
     CHECK(begin < end);
-    for (long long x : {begin, end - 1}) CHECK(share_of(x, all, ctas) == c);
+    for (long long x : {begin, end - 1}) CHECK(sh.of(x) == c);
     long long at = 0;
-    int seg = 0, unit = 0, tile = 0;
+    int seg = 0, unit = 0, place = 0;
     for (;; ++seg) {
       const Seq s = make_seq<R>(p, seg);
-      if (begin < at + weight(s)) { unit = int((begin - at) / s.tiles); tile = int((begin - at) %% s.tiles); shares[c] = {begin, seg, unit, tile, s.tiles}; break; }
-      at += weight(s);
+      if (begin < at + places(s)) { unit = int(divide(begin - at, places_of(s))); place = int(begin - at - (long long)unit * places_of(s)); break; }
+      at += places(s);
     }
     long long left = end - begin;
     Seq s = make_seq<R>(p, seg);
+    joins[c] = make_join(sh, s, make_block<R>(p, s, unit), seg, c, place);
     bool first_block = true;
     while (left > 0) {
       CHECK(seg < n && unit < s.blocks * p.kv_heads);
-      const int to = int(min((long long)s.tiles, tile + left));
-      parts[{seg, unit}].push_back({c, 2 * c + (first_block ? 0 : 1), tile, to});
-      left -= to - tile; tile = 0; first_block = false;
+      const int tile = tiles_before(place), to = tiles_before(int(min((long long)places_of(s), place + left)));
+      if (tile < to) parts[{seg, unit}].push_back({c, 2 * c + (first_block ? 0 : 1), tile, to});
+      left -= min((long long)(places_of(s) - place), left); place = 0; first_block = false;
       if (++unit == s.blocks * p.kv_heads && left > 0) { unit = 0; do s = make_seq<R>(p, ++seg); while (s.blocks == 0); }
     }
   }
@@ -124,17 +127,18 @@ int main(int argc, char** argv) {
   // the joins
   std::set<std::pair<int, int>> joined;
   for (int c = 1; c < ctas; ++c) {
-    auto [first, seg, unit, tile, tiles] = shares[c];
-    if (tile == 0) continue;
-    const long long begin = first - tile, end = begin + tiles;
-    const int c0 = share_of(begin, all, ctas), c1 = share_of(end - 1, all, ctas);
-    if (c0 != c - 1) continue;
-    CHECK(joined.insert({seg, unit}).second);
-    const auto& list = parts.at({seg, unit});
-    CHECK(int(list.size()) == c1 - c0 + 1);
-    for (int i = 0; i < int(list.size()); ++i) {
-      const int slot = 2 * (c0 + i) + (i == 0 && share_begin(c0, all, ctas) < begin ? 1 : 0);
-      CHECK(std::get<0>(list[i]) == c0 + i && std::get<1>(list[i]) == slot && slot < 2 * most_ctas);
+    const Join& j = joins[c];
+    if (j.parts == 0) continue;
+    const Seq s = make_seq<R>(p, j.seg);
+    const int unit = j.kv_head * s.blocks + j.row0 / R;
+    const Block b = make_block<R>(p, s, unit);
+    CHECK(b.kv_head == j.kv_head && b.row0 == j.row0 && b.rows == j.rows && j.q_begin == cu[j.seg]);
+    CHECK(joined.insert({j.seg, unit}).second);
+    const auto& list = parts.at({j.seg, unit});
+    CHECK(j.parts >= 2 && int(list.size()) == j.parts);
+    for (int i = 0; i < j.parts; ++i) {
+      const int slot = 2 * (j.cta + i) + (i == 0 ? j.late : 0);
+      CHECK(std::get<0>(list[i]) == j.cta + i && std::get<1>(list[i]) == slot && slot < 2 * most_ctas);
     }
   }
   long long whole = 0;
@@ -158,7 +162,7 @@ def replay(tmp_path_factory):
         span=window[window.index("struct WindowSpan"):window.index("// Element offset")],
         paged=paged[paged.index("__device__ __forceinline__ int paged_keys"):paged.index("__device__ __forceinline__ WindowSeq window_seq(const PagedParams")],
         walk=kernel[kernel.index("struct Seq {"):kernel.index("__device__ __forceinline__ void ldmatrix4(")],
-        min_tiles=re.search(r"constexpr int kMinTiles = (\d+);", kernel).group(1))
+        constants="\n".join(re.findall(r"^constexpr int k(?:BlockCost|MinPlaces) = [^;]*;", kernel, re.M)))
     built = {}
     for rows in (16, 32, 64):
         d = tmp_path_factory.mktemp("shares")
@@ -195,5 +199,5 @@ def test_shares_cover_every_key_of_every_row_once(replay, rows, seed):
 
 def test_one_long_sequence_goes_to_all(replay):
     assert replay(16, 1, 296, 8, 1, -1, 0, 0, 6, 16, 1, 100000) == 296
-    assert replay(16, 1, 296, 8, 8, -1, 0, 0, 4, 16, 1, 63) == 4
+    assert replay(16, 1, 296, 8, 8, -1, 0, 0, 4, 16, 1, 63) <= 12
     assert replay(16, 1, 296, 8, 1, -1, 0, 0, 4, 16, 1, 0) == 1
