@@ -473,18 +473,28 @@ flash_paged_rows_kernel(const __grid_constant__ PagedMap tm_k, const __grid_cons
               }
             }
           }
-          const float ref[2] = {reference(m[0]) * c, reference(m[1]) * c};
+          // P, a pair of columns of a row at a time
+          uint32_t pr[KW / 8][2];
 #pragma unroll
-          for (int n = 0; n < KW / 8; ++n)
+          for (int h = 0; h < 2; ++h) {
+            const float ref = -reference(m[h]) * c;
+            const uint64_t c2 = pack2(c, c), ref2 = pack2(ref, ref);
+            uint64_t sum2 = pack2(l[h], 0.f);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              sr[n][e] = ex2(fmaf(sr[n][e], c, -ref[e >> 1]));
-              l[e >> 1] += sr[n][e];
+            for (int n = 0; n < KW / 8; ++n) {
+              const uint64_t w2 = exp2_mufu2(fma2(pack2(sr[n][2 * h], sr[n][2 * h + 1]), c2, ref2));
+              sum2 = add2(sum2, w2);
+              float w0, w1;
+              unpack2(w2, w0, w1);
+              pr[n][h] = pack_bf16x2(w0, w1);
             }
+            float s0, s1;
+            unpack2(sum2, s0, s1);
+            l[h] = s0 + s1;
+          }
 #pragma unroll
           for (int n = 0; n < KW / 16; ++n) {
-            const uint32_t w[4] = {pack_bf16x2(sr[2 * n][0], sr[2 * n][1]), pack_bf16x2(sr[2 * n][2], sr[2 * n][3]),
-                                   pack_bf16x2(sr[2 * n + 1][0], sr[2 * n + 1][1]), pack_bf16x2(sr[2 * n + 1][2], sr[2 * n + 1][3])};
+            const uint32_t w[4] = {pr[2 * n][0], pr[2 * n][1], pr[2 * n + 1][0], pr[2 * n + 1][1]};
             const int row = key0 + n * 16 + (((lane >> 3) & 1) << 3) + (lane & 7);
             const uint32_t at_row = vs + row * 128;
 #pragma unroll
@@ -561,7 +571,7 @@ flash_paged_rows_kernel(const __grid_constant__ PagedMap tm_k, const __grid_cons
 }
 
 // Joins the parts of a block that several CTAs worked on.  grid: (boundaries between two CTAs' shares, 16); the first boundary inside a block
-// is the one that counts.  The four warps share a row's parts, a lane has D / 32 columns.
+// is the one that counts.  A lane has D / 32 columns; the four warps have a row each, or share the parts of one where there are many.
 template <int D, int R>
 __global__ void __launch_bounds__(128) flash_paged_join_kernel(const __grid_constant__ PagedParams p, void* scratch) {
   constexpr int kCols = D / 32;
@@ -576,40 +586,39 @@ __global__ void __launch_bounds__(128) flash_paged_join_kernel(const __grid_cons
   const Join j = sc.joins[blockIdx.x + 1];
   if (status != 0) return;
   auto slot_of = [&](int i) { return static_cast<int64_t>(2 * (j.cta + i) + (i == 0 ? j.late : 0)) * R; };
-  for (int r = blockIdx.y; j.parts > 0 && r < j.rows; r += gridDim.y) {
-    float mm = -INFINITY;
+  if (j.parts == 0) return;
+  const int per_row = j.parts <= 16 ? 1 : 4;                                // warps
+  const int part = warp % per_row, step = 4 / per_row;                      // ... and rows of a CTA at a time
+  for (int r0 = blockIdx.y * step; r0 < j.rows; r0 += gridDim.y * step) {
+    const int r = min(r0 + warp / per_row, j.rows - 1);                     // (a warp without a row does the last one once more)
+    float mm = -INFINITY, sum = 0.f, acc[kCols] = {};
     for (int i = lane; i < j.parts; i += 32) mm = fmaxf(mm, sc.ml[slot_of(i) + r].x);
-    float sum = 0.f, acc[kCols] = {};
     constexpr int kAhead = 8;
-    for (int i0 = 0; i0 < j.parts; i0 += 4 * kAhead) {
+    for (int i0 = part; i0 < j.parts; i0 += per_row * kAhead) {
+      // (all reads are under way before one is used)
       float2 ml[kAhead];
       float v[kAhead][kCols];
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
-        const int i = i0 + 4 * u + warp;
-        ml[u] = make_float2(-INFINITY, 0.f);
-#pragma unroll
-        for (int k = 0; k < kCols; ++k) v[u][k] = 0.f;
-        if (i < j.parts) {
-          const int64_t at = slot_of(i) + r;
-          ml[u] = sc.ml[at];
-          const float* src = sc.o + at * D + lane * kCols;
-          if constexpr (D == 128) {
-            const float4 q = *reinterpret_cast<const float4*>(src);
-            v[u][0] = q.x, v[u][1] = q.y, v[u][2] = q.z, v[u][3] = q.w;
-          } else {
-            const float2 q = *reinterpret_cast<const float2*>(src);
-            v[u][0] = q.x, v[u][1] = q.y;
-          }
+        const int64_t at = slot_of(min(i0 + per_row * u, j.parts - 1)) + r;
+        ml[u] = sc.ml[at];
+        const float* src = sc.o + at * D + lane * kCols;
+        if constexpr (D == 128) {
+          const float4 q = *reinterpret_cast<const float4*>(src);
+          v[u][0] = q.x, v[u][1] = q.y, v[u][2] = q.z, v[u][3] = q.w;
+        } else {
+          const float2 q = *reinterpret_cast<const float2*>(src);
+          v[u][0] = q.x, v[u][1] = q.y;
         }
       }
-      if (i0 == 0) {
+      if (i0 == part) {
 #pragma unroll
         for (int d = 16; d > 0; d /= 2) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, d));
       }
       const float ref = reference(mm);
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
+        if (i0 + per_row * u >= j.parts) break;
         const float f = ex2((ml[u].x - ref) * c);
         sum = fmaf(ml[u].y, f, sum);
 #pragma unroll
@@ -620,11 +629,10 @@ __global__ void __launch_bounds__(128) flash_paged_join_kernel(const __grid_cons
     for (int k = 0; k < kCols; ++k) s_acc[warp][lane * kCols + k] = acc[k];
     if (lane == 0) s_sum[warp] = sum;
     __syncthreads();
-    if (warp == 0 && lane < D / 4) {
+    if (r0 + warp / per_row < j.rows && part == 0 && lane < D / 4) {
       float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
       float l = 0.f;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
+      for (int w = warp; w < warp + per_row; ++w) {
         const float4 v = *reinterpret_cast<const float4*>(&s_acc[w][lane * 4]);
         a.x += v.x;
         a.y += v.y;
