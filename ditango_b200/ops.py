@@ -343,16 +343,20 @@ class PageRelease(NamedTuple):
     free_count: torch.Tensor
 
 
-def _page_args(table, free, free_count, page_size, *per_stream):
-    """Checks what the tables' two directions are given; returns (streams, columns, pages)."""
-    for x in (table, free, free_count, *per_stream):
-        if x.dtype != torch.int32 or not x.is_contiguous():
-            raise _capi.ExtensionError("tables, lengths and pages are contiguous int32 tensors")
-    if table.dim() != 2 or free.dim() != 1 or free_count.numel() != 1 or any(x.numel() != table.shape[0] for x in per_stream):
+def _page_args(table, free, free_count, page_size, a, b, c):
+    """Checks what the tables' two directions are given, a, b and c (or None) with a number per stream; returns (streams, columns, pages)."""
+    i32 = torch.int32
+    if not (table.dtype is i32 and free.dtype is i32 and free_count.dtype is i32 and a.dtype is i32 and b.dtype is i32 and (c is None or c.dtype is i32) and
+            table.is_contiguous() and free.is_contiguous() and a.is_contiguous() and b.is_contiguous() and (c is None or c.is_contiguous())):
+        raise _capi.ExtensionError("tables, lengths and pages are contiguous int32 tensors")
+    shape = table.shape
+    if len(shape) != 2 or free.dim() != 1 or free_count.numel() != 1 or not (a.numel() == b.numel() == shape[0] and (c is None or c.numel() == shape[0])):
         raise _capi.ExtensionError("a table is [streams, columns], with a number per stream; free pages are a list and their count")
+    if shape[0] == 0:
+        raise _capi.ExtensionError("a table without streams")
     if not 0 < page_size < 1 << 31:
         raise _capi.ExtensionError("a page size is a power of two from 16 to 2^20")
-    return (*table.shape, free.numel())
+    return shape[0], shape[1], free.numel()
 
 
 def extend_pages(table: torch.Tensor, seqlens: torch.Tensor, new_lens: torch.Tensor, free: torch.Tensor, free_count: torch.Tensor, page_size: int,
@@ -364,21 +368,24 @@ def extend_pages(table: torch.Tensor, seqlens: torch.Tensor, new_lens: torch.Ten
     the host, is the number of rows that the new keys and values come in: new_lens add up to it or less, and slots behind the last token
     are -1 (as is that of a token on a page that release_pages took from inside its stream).  All or nothing: with too few free pages `missing` says how many, with streams that outgrow their row or `tokens` it is -1, and then the
     table and the numbers stay as they are.  The results are new tensors, for the next step; one launch, no host round trip."""
-    streams, columns, pages = _page_args(table, free, free_count, page_size, seqlens, new_lens)
+    streams, columns, pages = _page_args(table, free, free_count, page_size, seqlens, new_lens, None)
     if not 0 <= tokens < (1 << 31) - 4:
         raise _capi.ExtensionError("tokens is a number of rows")
     stream = _launch_stream(table, seqlens, new_lens, free, free_count)
-    if streams == 0:
-        raise _capi.ExtensionError("a table without streams")
     # (one allocation; slots begin it and so are 16-byte aligned)
-    slots, cu, lens, count, missing = _empty((tokens + 2 * streams + 3,), torch.int32, table.device).split((tokens, streams + 1, streams, 1, 1))
+    results = _empty((tokens + 2 * streams + 3,), torch.int32, table.device)
+    slots = results.data_ptr()
+    cu = slots + 4 * tokens
+    lens = cu + 4 * streams + 4
+    count = lens + 4 * streams
     rc = _capi.load().dtb_extend_pages(
         table.data_ptr(), seqlens.data_ptr(), new_lens.data_ptr(), free.data_ptr(), free_count.data_ptr(), streams, columns, pages, page_size,
-        slots.data_ptr(), tokens, cu.data_ptr(), lens.data_ptr(), count.data_ptr(), missing.data_ptr(), stream)
+        slots, tokens, cu, lens, count, count + 4, stream)
     if rc:
         _capi.check(rc, "dtb_extend_pages")
     LaunchLog.count += 1
-    return PagePlan(slots, cu, lens, count, missing)
+    # (results are whole numbers: nothing is lost by parts that autograd does not know as views, and they are made in half the time)
+    return PagePlan(*torch.unsafe_split_with_sizes(results, (tokens, streams + 1, streams, 1, 1)))
 
 
 def release_pages(table: torch.Tensor, seqlens: torch.Tensor, free: torch.Tensor, free_count: torch.Tensor, begin: torch.Tensor, end: torch.Tensor,
@@ -390,33 +397,37 @@ def release_pages(table: torch.Tensor, seqlens: torch.Tensor, free: torch.Tensor
     streams, columns, pages = _page_args(table, free, free_count, page_size, seqlens, begin, end)
     if out_table is None:
         out_table = table
-    elif out_table.dtype != torch.int32 or out_table.shape != table.shape or not out_table.is_contiguous():
+    elif out_table.dtype is not torch.int32 or out_table.shape != table.shape or not out_table.is_contiguous():
         raise _capi.ExtensionError("out_table is a contiguous int32 tensor of the table's shape")
     stream = _launch_stream(table, out_table, seqlens, free, free_count, begin, end)
-    if streams == 0:
-        raise _capi.ExtensionError("a table without streams")
-    lens, count = _empty((streams + 1,), torch.int32, table.device).split((streams, 1))
+    results = _empty((streams + 1,), torch.int32, table.device)
+    lens = results.data_ptr()
     rc = _capi.load().dtb_release_pages(
         table.data_ptr(), out_table.data_ptr(), seqlens.data_ptr(), begin.data_ptr(), end.data_ptr(), free.data_ptr(), free_count.data_ptr(),
-        streams, columns, pages, page_size, lens.data_ptr(), count.data_ptr(), stream)
+        streams, columns, pages, page_size, lens, lens + 4 * streams, stream)
     if rc:
         _capi.check(rc, "dtb_release_pages")
     LaunchLog.count += 1
-    return PageRelease(out_table, lens, count)
+    return PageRelease(out_table, *torch.unsafe_split_with_sizes(results, (streams, 1)))
 
 
-def _pool(x: torch.Tensor, shape) -> Tuple[int, int, int]:
-    """(page, token, head) strides of k_pages or v_pages [pages, P, heads, D]; that of an axis of length 1, which nothing steps along, is given as if it
-    lay behind the others."""
-    if x.dtype != torch.bfloat16 or x.shape != shape or x.dim() != 4 or x.stride(-1) != 1:
+def _pools(k: torch.Tensor, v: torch.Tensor):
+    """Shape [pages, P, heads, D] of k_pages and v_pages, and the (page, token, head) strides of each; that of an axis of length 1, which nothing steps
+    along, is given as if it lay behind the others."""
+    shape, k_strides, v_strides = k.shape, k.stride(), v.stride()
+    if not (k.dtype is v.dtype is torch.bfloat16 and len(shape) == 4 and v.shape == shape and k_strides[3] == v_strides[3] == 1):
         raise _capi.ExtensionError("pages are bfloat16 [pages, tokens, heads, D] with contiguous channels, of keys as of values")
-    page, tok, head, _ = x.stride()
+    if shape[0] > 1 and shape[2] > 1:
+        return shape, k_strides[:3], v_strides[:3]
     pages, P, heads, D = shape
-    if heads == 1:
-        head = max(tok * P, D)
-    if pages == 1:
-        page = max(tok * P, head * heads)
-    return page, tok, head
+    both = []
+    for page, tok, head, _ in (k_strides, v_strides):
+        if heads == 1:
+            head = max(tok * P, D)
+        if pages == 1:
+            page = max(tok * P, head * heads)
+        both.append((page, tok, head))
+    return shape, *both
 
 
 def write_pages(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, slots: torch.Tensor):
@@ -424,13 +435,15 @@ def write_pages(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages
     [pages, P, Hk, D], any strides.  A token whose slot is -1, or none of the pool's, is left out; slots are to differ from one another.
     One launch."""
     stream = _launch_stream(k, v, k_pages, v_pages, slots)
-    shape = k_pages.shape
-    k_strides, v_strides = _pool(k_pages, shape), _pool(v_pages, shape)
+    shape, k_strides, v_strides = _pools(k_pages, v_pages)
     pages, P, Hk, D = shape
-    if k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16 or k.shape != v.shape or k.dim() < 3 or k.shape[-2:] != shape[-2:]:
+    kshape = k.shape
+    if not (k.dtype is v.dtype is torch.bfloat16 and len(kshape) >= 3 and v.shape == kshape and kshape[-1] == D and kshape[-2] == Hk):
         raise _capi.ExtensionError("k and v are bfloat16 [..,Hk,D] with the pages' heads")
+    if Hk * D == 0:
+        return
     tokens = k.numel() // (Hk * D)
-    if slots.dtype != torch.int32 or slots.numel() != tokens or not slots.is_contiguous():
+    if slots.dtype is not torch.int32 or slots.numel() != tokens or not slots.is_contiguous():
         raise _capi.ExtensionError("slots are contiguous int32, one per token")
     if tokens == 0:
         return
@@ -479,23 +492,21 @@ def flash_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, t
     stream = _launch_stream(q, k_pages, v_pages, table, seqlens_k, cu_seqlens_q, out, lse)
     if not (-1 <= left <= _FAR and -1 <= right <= _FAR and 0 <= sinks <= _FAR):
         raise _capi.ExtensionError("left, right and sinks are within 2^30")
-    shape, pshape = q.shape, k_pages.shape
-    if q.dtype != torch.bfloat16:
-        raise _capi.ExtensionError("q must be bfloat16")
-    k_strides, v_strides = _pool(k_pages, pshape), _pool(v_pages, pshape)
-    pages, P, Hk, D = pshape
+    shape = q.shape
+    (pages, P, Hk, D), k_strides, v_strides = _pools(k_pages, v_pages)
     packed = cu_seqlens_q is not None
-    if len(shape) != (3 if packed else 4) or shape[-1] != D:
-        raise _capi.ExtensionError("q is [B,S,H,D], packed [T,H,D], with the pages' channels")
-    if table.dtype != torch.int32 or table.dim() != 2 or not table.is_contiguous():
+    if q.dtype is not torch.bfloat16 or len(shape) != (3 if packed else 4) or shape[-1] != D:
+        raise _capi.ExtensionError("q is bfloat16 [B,S,H,D], packed [T,H,D], with the pages' channels")
+    tshape = table.shape
+    if table.dtype is not torch.int32 or len(tshape) != 2 or not table.is_contiguous():
         raise _capi.ExtensionError("table is contiguous int32 [sequences, columns]")
-    nseg, columns = table.shape
-    if seqlens_k.dtype != torch.int32 or seqlens_k.numel() != nseg or not seqlens_k.is_contiguous():
+    nseg, columns = tshape
+    if seqlens_k.dtype is not torch.int32 or seqlens_k.numel() != nseg or not seqlens_k.is_contiguous():
         raise _capi.ExtensionError("seqlens_k is contiguous int32 with one length per sequence")
     if packed:
         T, H, _ = shape
         sq = min(T, int(max_seqlen_q)) if max_seqlen_q is not None else T
-        if cu_seqlens_q.dtype != torch.int32 or not cu_seqlens_q.is_contiguous() or cu_seqlens_q.numel() != nseg + 1:
+        if cu_seqlens_q.dtype is not torch.int32 or not cu_seqlens_q.is_contiguous() or cu_seqlens_q.numel() != nseg + 1:
             raise _capi.ExtensionError("cu_seqlens_q must be contiguous int32, one more than sequences")
         lse_shape = (H, T) if lse_layout == LSE_BHS else (T, H)
     else:
@@ -519,7 +530,7 @@ def flash_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, t
         lse = _empty(lse_shape, torch.float32, q.device)
     elif tuple(lse.shape) != lse_shape or not lse.is_contiguous() or lse.dtype != torch.float32:
         raise _capi.ExtensionError(f"lse must be a contiguous fp32 tensor of shape {lse_shape}")
-    if q.numel() == 0 or sq <= 0:
+    if T * H * D == 0 or sq <= 0:
         return out, lse
     lib = _capi.load()
     key = (q.get_device(), nseg, sq, sk, H, Hk, D)
@@ -531,13 +542,14 @@ def flash_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, t
         if len(_PAGED_SCRATCH) >= 4096:
             _PAGED_SCRATCH.clear()
         _PAGED_SCRATCH[key] = need
-    scratch = _empty((need,), torch.uint8, q.device)
+    scratch = torch.empty_strided((need,), (1,), dtype=torch.uint8, device=q.device)
+    q_strides = (H * D, 0 if packed else sq * H * D) if q.is_contiguous() else _strides(q, shape)
     ev = None
     if LaunchLog.events is not None:
         ev = (torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True))
         ev[0].record()
     rc = lib.dtb_flash_paged(
-        q.data_ptr(), *_strides(q, shape), k_pages.data_ptr(), *k_strides, v_pages.data_ptr(), *v_strides, pages, P, table.data_ptr(), columns,
+        q.data_ptr(), *q_strides, k_pages.data_ptr(), *k_strides, v_pages.data_ptr(), *v_strides, pages, P, table.data_ptr(), columns,
         seqlens_k.data_ptr(), cu_seqlens_q.data_ptr() if packed else None, out.data_ptr(), _VALUES[out.dtype], lse.data_ptr(), lse_layout, accumulate,
         nseg, sq, sk, T, H, Hk, D, D ** -0.5 if softmax_scale is None else softmax_scale, left, right, sinks, scratch.data_ptr(), need, stream)
     if rc:
