@@ -89,7 +89,7 @@ def load():
         [c_void_p, c_int64, c_int64] + pool * 2 + [c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int] +
         [c_int, c_int, c_int, c_int64, c_int, c_int, c_int, c_float, c_int, c_int, c_int, c_void_p, c_int64, c_void_p])
     lib.dtb_flash_paged_scratch_bytes.restype = c_int64
-    lib.dtb_flash_paged_scratch_bytes.argtypes = [c_int] * 6
+    lib.dtb_flash_paged_scratch_bytes.argtypes = [c_int, c_int, c_int, c_int64, c_int, c_int, c_int]
     lib.dtb_merge_states.restype = c_int
     lib.dtb_merge_states.argtypes = [
         c_int, POINTER(c_void_p), POINTER(c_int), POINTER(c_void_p), POINTER(c_int),

@@ -745,18 +745,28 @@ DTB_API int dtb_write_pages(const void* k, const void* v, int64_t k_tok_stride, 
 
 // Which kernels a launch over pages takes.
 struct PagedPlan {
-  int few_rows;                  // sequences with at most this many queries go to the kernel of few rows; -1: none do
+  int few_rows;                  // sequences with at most this many queries go to the kernel of few rows
   bool tiles;                    // there may be others
   dtb::PagedRowsPlan rows;
+  int states;                    // of parts, at most; 0: the kernel of tiles splits no keys
+  int64_t tile_bytes;            // of scratch, in front of that of the kernel of few rows
   int64_t scratch_bytes;
 };
-static PagedPlan plan_paged(int64_t nseg, int64_t seqlen_q, int64_t seqlen_k, int64_t num_heads, int64_t kv_heads, int head_dim, int sm_count) {
+static PagedPlan plan_paged(int64_t nseg, int64_t seqlen_q, int64_t seqlen_k, int64_t total_q, int64_t num_heads, int64_t kv_heads, int head_dim, int sm_count) {
   PagedPlan plan = {};
   const int64_t group = num_heads / kv_heads;
   plan.few_rows = static_cast<int>(std::max<int64_t>(128 / group, 1));
   plan.tiles = seqlen_q > plan.few_rows;
   plan.rows = dtb::plan_paged_rows(std::min<int64_t>(seqlen_q, plan.few_rows) * group, seqlen_k, kv_heads, nseg, head_dim, sm_count);
-  plan.scratch_bytes = plan.rows.scratch_bytes;
+  if (plan.tiles) {
+    // Of sequences of one number of queries the blocks are known: with a round of them for each sequence the one that walks furthest has no more
+    // than its share, and with a last round that is nearly full nothing is split.  (The launch that joins takes 5 us.)
+    const int64_t blocks = (seqlen_q + 255) / 256 * num_heads * nseg, rounds = (blocks + sm_count - 1) / sm_count;
+    const bool may = total_q != nseg * seqlen_q || blocks <= sm_count * nseg || static_cast<double>(rounds * sm_count) > 1.15 * static_cast<double>(blocks);
+    plan.states = may && seqlen_k > 256 ? 2 * sm_count : 0;
+    plan.tile_bytes = plan.states * (256ll * (head_dim + 1) * 4) + plan.states / 2 * static_cast<int64_t>(sizeof(dtb::TileJoin));
+  }
+  plan.scratch_bytes = plan.tile_bytes + plan.rows.scratch_bytes;
   return plan;
 }
 
@@ -769,12 +779,12 @@ static int check_paged_shape(const char* what, int nseg, int seqlen_q, int seqle
   return DTB_OK;
 }
 
-DTB_API int64_t dtb_flash_paged_scratch_bytes(int nseg, int seqlen_q, int seqlen_k, int num_heads, int num_kv_heads, int head_dim) {
+DTB_API int64_t dtb_flash_paged_scratch_bytes(int nseg, int seqlen_q, int seqlen_k, int64_t total_q, int num_heads, int num_kv_heads, int head_dim) {
   int rc = check_paged_shape("dtb_flash_paged_scratch_bytes", nseg, seqlen_q, seqlen_k, num_heads, num_kv_heads, head_dim);
   if (rc != DTB_OK) return rc;
   DeviceInfo* d = nullptr;
   if ((rc = device_info(&d)) != DTB_OK) return rc;
-  return plan_paged(nseg, seqlen_q, seqlen_k, num_heads, num_kv_heads, head_dim, d->sm_count).scratch_bytes;
+  return plan_paged(nseg, seqlen_q, seqlen_k, total_q, num_heads, num_kv_heads, head_dim, d->sm_count).scratch_bytes;
 }
 
 DTB_API int dtb_flash_paged(const void* q, int64_t q_tok_stride, int64_t q_batch_stride,
@@ -810,7 +820,7 @@ DTB_API int dtb_flash_paged(const void* q, int64_t q_tok_stride, int64_t q_batch
   DeviceInfo* d = nullptr;
   if ((rc = device_info(&d)) != DTB_OK) return rc;
   if (seqlen_q == 0 || total_q == 0) return DTB_OK;
-  const PagedPlan plan = plan_paged(nseg, seqlen_q, seqlen_k, num_heads, num_kv_heads, head_dim, d->sm_count);
+  const PagedPlan plan = plan_paged(nseg, seqlen_q, seqlen_k, total_q, num_heads, num_kv_heads, head_dim, d->sm_count);
   if (scratch_bytes < plan.scratch_bytes)
     return fail(DTB_ERR_ARG, "%s: scratch of %lld bytes is smaller than the %lld needed", kWhat, static_cast<long long>(scratch_bytes),
                 static_cast<long long>(plan.scratch_bytes));
@@ -865,11 +875,30 @@ DTB_API int dtb_flash_paged(const void* q, int64_t q_tok_stride, int64_t q_batch
     const bool packed = cu_seqlens_q != nullptr;
     CUtensorMap tq;
     if ((rc = make_token_map(&tq, q, q_width, packed ? total_q : seqlen_q, q_tok_stride, packed ? 1 : nseg, q_batch_stride, &p.q_batch_first, "q")) != DTB_OK) return rc;
+    // blocks of 256 rows: as many as fit the rows that there are, and room for the parts
+    const int64_t per_seq = (seqlen_q + 255) / 256, in_rows = total_q / 256 + nseg;
+    p.planned = nseg <= dtb::kPlanSeqs && in_rows * num_heads < dtb::kPlanBlocks;
+    const int64_t blocks = p.planned ? std::min(nseg * per_seq, in_rows) * num_heads + plan.states : nseg * per_seq * num_heads;
+    if (blocks >= (1ll << 31)) return fail(DTB_ERR_ARG, "%s: too many blocks of rows", kWhat);
+    p.blocks = static_cast<int>(blocks);
+    p.ctas = d->sm_count;
+    p.most_states = p.planned ? plan.states : 0;
+    p.parts = p.f;
+    p.parts.out = scratch;
+    p.parts.lse = static_cast<float*>(scratch) + plan.states * 256ll * head_dim;
+    p.joins = reinterpret_cast<dtb::TileJoin*>(p.parts.lse + plan.states * 256ll);
+    p.parts.out_dtype = DTB_F32;
+    p.parts.out_tok_stride = head_dim;
+    p.parts.num_heads = 1;
+    p.parts.lse_layout = DTB_LSE_BSH;
+    p.parts.accumulate = 0;
     e = head_dim == 64 ? dtb::launch_paged_tiles<64>(tq, mk, mv, p, s) : dtb::launch_paged_tiles<128>(tq, mk, mv, p, s);
+    if (e == cudaSuccess && p.most_states > 0) e = head_dim == 64 ? dtb::launch_tile_join<64>(p, s) : dtb::launch_tile_join<128>(p, s);
   }
   if (e == cudaSuccess && (!plan.tiles || mixed)) {
     if ((rc = make_maps(std::min(page_size, 64))) != DTB_OK) return rc;
-    e = head_dim == 64 ? dtb::launch_paged_rows<64>(mk, mv, p, plan.rows, scratch, s) : dtb::launch_paged_rows<128>(mk, mv, p, plan.rows, scratch, s);
+    void* rows_scratch = static_cast<uint8_t*>(scratch) + plan.tile_bytes;
+    e = head_dim == 64 ? dtb::launch_paged_rows<64>(mk, mv, p, plan.rows, rows_scratch, s) : dtb::launch_paged_rows<128>(mk, mv, p, plan.rows, rows_scratch, s);
   }
   if (e != cudaSuccess) return fail(DTB_ERR_CUDA, "%s launch failed: %s", kWhat, cudaGetErrorString(e));
   return DTB_OK;

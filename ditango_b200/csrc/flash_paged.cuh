@@ -15,6 +15,19 @@ struct PagedParams : WindowParams {    // (k, v, their strides, cu_k and k_start
   int box_rows;                        // tokens of a tile that one load fetches; divides a page, so that no load crosses one
   int key_align;                       // runs of keys are walked from a multiple of this
   int few_rows;                        // the kernel of few rows takes the sequences with at most this many queries, that of many the others
+  // of the kernel of tiles:
+  int planned;                         // whether plan_blocks orders them; 0: row block, head, sequence, the first of them changing fastest
+  int blocks;                          // of the grid
+  int ctas;                            // that run at once
+  int most_states;                     // of parts, or 0: keys are not split
+  FlashParams parts;                   // where those go, 256 rows each, ...
+  struct TileJoin* joins;              // ... and the blocks they are of, for the launch that joins them: [most_states / 2]
+};
+
+// A block whose keys were split.
+struct alignas(16) TileJoin {
+  int seg, head, q0, rows;             // rows 0: no block
+  int q_begin, state, parts, pad;      // its first part's state, and how many there are
 };
 
 // A tensor map of the pool [channel, token, head, page] (head before token where heads are nearer to one another), with what its loads go by.
@@ -129,9 +142,223 @@ __device__ __forceinline__ void serve_loads(const PagedParams& p, int which) {
   }
 }
 
+// The blocks of 256 rows of one head that the kernel of tiles takes, in the order in which its CTAs claim them: the sequences with the longest
+// walks over keys first, so that short ones fill the end; of a sequence one head after another, whose row blocks read the same keys,
+// the end whose rows see more keys first.  Where blocks are fewer than CTAs, or the last round
+// of them is far from full, keys are split:
+//   - less work than a block of the longest kind for every CTA: all of it into parts of about an even share,
+//   - a last round that wastes more than 15 %: the blocks of the last half a round in two.
+// Every CTA plans for itself, from lengths that stand on the device; batches of more sequences than there is room for are not planned.
+// (us, one launch after another: a HunyuanVideo frame with a window, 2.4 rounds of blocks, 438 -> 409; chunks and tokens mixed 898 -> 860; 200 queries of
+// 32 heads against 60000 keys 852 -> 255; two CogVideoX frames, which are not split, 643 -> 650.)
+constexpr int kPlanSeqs = 256;
+constexpr int kPlanBlocks = 1 << 22;     // sums of them are exact in fp32
+constexpr int kPlanThreads = 512;
+constexpr int kBlockSteps = 5;           // what a block costs beside its steps of 128 keys, in such steps
+struct TilePlan {
+  int seqs, blocks, splits;              // sequences, 0: as the grid says; places of blocks and parts; blocks that are split
+  uint16_t seq[kPlanSeqs];               // in their order
+  uint16_t parts[kPlanSeqs];             // of each of a sequence's blocks from `whole` on
+  int row_blocks[kPlanSeqs];             // of each head; negative: the last one first
+  int whole[kPlanSeqs];
+  int first[kPlanSeqs], first_split[kPlanSeqs], first_state[kPlanSeqs];      // places, split blocks and states in front of it
+};
+__device__ __forceinline__ TilePlan& tile_plan() {
+  __shared__ TilePlan plan;
+  return plan;
+}
+
+// The row block that a sequence's block i, counted through its heads, is.
+__device__ __forceinline__ int row_block_of(const TilePlan& plan, int seq, int i) {
+  const int n = plan.row_blocks[seq];
+  return n > 0 ? i % n : -n - 1 - i % -n;
+}
+
+// Steps of 128 keys that the rows i0 to i1 walk.
+__device__ __forceinline__ int block_steps(const WindowSeq& s, int i0, int i1) {
+  const WindowSpan a = window_span(s, i0), z = window_span(s, i1);
+  const int lo = max(a.lo, min(s.sinks, z.hi));
+  return (max(z.hi - lo, 0) + 127) / 128 + (z.first + 127) / 128;
+}
+
+// Sum over the 512 threads, and over those before this one.
+__device__ __forceinline__ float plan_sum(float v, float& before) {
+  __shared__ float s_warp[kPlanThreads / 32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float upto = v;
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) {
+    const float u = __shfl_up_sync(0xffffffffu, upto, d);
+    if (lane >= d) upto += u;
+  }
+  __syncthreads();
+  if (lane == 31) s_warp[warp] = upto;
+  __syncthreads();
+  float all = 0.f;
+  before = upto - v;
+#pragma unroll
+  for (int w = 0; w < kPlanThreads / 32; ++w) {
+    if (w < warp) before += s_warp[w];
+    all += s_warp[w];
+  }
+  return all;
+}
+
+__device__ __forceinline__ void plan_blocks(const WindowParams&) {}
+// By all threads.  (Sums are of whole numbers below 2^24 or of estimates: fp32 does.)
+__device__ __forceinline__ void plan_blocks(const PagedParams& p) {
+  TilePlan& plan = tile_plan();
+  const int n = p.f.nseg, t = threadIdx.x;
+  grid_launch_dependents();              // (the launch that joins)
+  if (!p.planned) {
+    if (t == 0) plan.seqs = 0;
+    return;
+  }
+  __shared__ int s_steps[kPlanSeqs];
+  int blocks = 0, longest = 0, q_len = 0;
+  bool rising = false;                   // the last rows walk further than the first
+  float steps = 0.f;                     // of a block, on average
+  if (t < n) {
+    const WindowSeq s = window_seq(p, t);
+    q_len = s.q_len;
+    blocks = (q_len + 255) / 256;
+    if (blocks > 0) {
+      const int a = block_steps(s, 0, min(q_len, 256) - 1), z = block_steps(s, (blocks - 1) * 256, q_len - 1);
+      longest = max(max(a, z), 1);
+      rising = z > a;
+      steps = 0.5f * (a + z);
+    }
+    s_steps[t] = longest;
+  }
+  __syncthreads();
+  int rank = 0;
+  if (t < n) {
+    for (int i = 0; i < n; ++i) rank += s_steps[i] > longest || (s_steps[i] == longest && i < t);
+    plan.seq[rank] = static_cast<uint16_t>(t);
+    plan.row_blocks[rank] = rising ? -blocks : blocks;
+    plan.first[rank] = longest;
+    plan.whole[rank] = __float_as_int(steps);
+  }
+  __syncthreads();
+  if (t < n) {
+    blocks = abs(plan.row_blocks[t]);
+    longest = plan.first[t];
+    steps = __int_as_float(plan.whole[t]);
+  }
+  const int top = max(plan.first[0], 0) + kBlockSteps;
+  const int mine = t < n ? blocks * p.f.num_heads : 0;
+  const float each = steps + kBlockSteps;
+  float blocks_before, work_before, x;
+  const float all = plan_sum(static_cast<float>(mine), blocks_before), work = plan_sum(mine * each, work_before);
+  const float share = work / p.ctas;
+  int parts = 1, whole = mine;
+  if (p.most_states > 0 && share < top) {
+    float size = fmaxf(1.15f * share, 6.f);
+    for (int round = 0; round < 8; ++round, size *= 1.4f) {
+      parts = mine > 0 ? max(1, min(min(static_cast<int>(ceilf(longest / size)), longest / 2), 255)) : 1;
+      if (plan_sum(parts > 1 ? static_cast<float>(mine) * parts : 0.f, x) <= p.most_states) break;
+      parts = 1;
+    }
+    whole = parts > 1 ? 0 : mine;
+  } else if (p.most_states > 0 && all > p.ctas && ceilf(all / p.ctas) * p.ctas > 1.15f * all) {
+    parts = longest + kBlockSteps > 0.5f * top && longest >= 4 ? 2 : 1;
+    if (parts > 1) whole = max(0, min(mine, static_cast<int>(ceilf((work - 0.5f * top * p.ctas - work_before) / each))));
+    if (plan_sum(parts > 1 ? 2.f * (mine - whole) : 0.f, x) > p.most_states) whole = mine;
+  }
+  if (whole == mine) parts = 1;
+  const int split = mine - whole;
+  float split_before, state_before, first_before;
+  const float splits = plan_sum(static_cast<float>(split), split_before);
+  plan_sum(static_cast<float>(split) * parts, state_before);
+  const float places = plan_sum(static_cast<float>(whole + split * parts), first_before);
+  if (t < n) {
+    plan.parts[t] = static_cast<uint16_t>(parts);
+    plan.whole[t] = whole;
+    plan.first[t] = static_cast<int>(first_before);
+    plan.first_split[t] = static_cast<int>(split_before);
+    plan.first_state[t] = static_cast<int>(state_before);
+  }
+  if (t == 0) {
+    plan.seqs = n;
+    plan.blocks = static_cast<int>(places);
+    plan.splits = static_cast<int>(splits);
+  }
+  __syncthreads();
+  // one CTA leaves what the launch that joins has to know
+  if (blockIdx.x == 0 && p.most_states > 0) {
+    for (int i = t; i < p.most_states / 2; i += kPlanThreads) {
+      TileJoin j = {0, 0, 0, 0, 0, 0, 0, 0};
+      if (i < plan.splits) {
+        int b = 0;
+        while (b + 1 < n && plan.first_split[b + 1] <= i) ++b;
+        const int k = i - plan.first_split[b], block = plan.whole[b] + k;
+        const WindowSeq s = window_seq(p, plan.seq[b]);
+        j.seg = plan.seq[b];
+        j.head = block / abs(plan.row_blocks[b]);
+        j.q0 = row_block_of(plan, b, block) * 256;
+        j.rows = min(256, s.q_len - j.q0);
+        j.q_begin = s.q_begin;
+        j.state = plan.first_state[b] + k * plan.parts[b];
+        j.parts = plan.parts[b];
+      }
+      p.joins[i] = j;
+    }
+  }
+}
+
+__device__ __forceinline__ void place_block(const PagedParams& p, int& bx, int& by, int& bz, int& splits, int& state) {
+  const TilePlan& plan = tile_plan();
+  int i = bx;
+  splits = 1;
+  state = -1;
+  if (plan.seqs == 0) {
+    const int row_blocks = (p.f.seqlen_q + 255) / 256;
+    bx = i % row_blocks;
+    by = i / row_blocks % p.f.num_heads;
+    bz = i / row_blocks / p.f.num_heads;
+    return;
+  }
+  if (i >= plan.blocks) {              // (the grid has room for more than there may be)
+    bx = 1 << 22;
+    by = bz = 0;
+    return;
+  }
+  int lo = 0, hi = plan.seqs;          // the last sequence that begins at or before it
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (plan.first[mid] <= i) lo = mid; else hi = mid;
+  }
+  // (sequences without blocks begin where the next one does, behind the others: there is none with blocks behind them)
+  i -= plan.first[lo];
+  int part = 0;
+  if (i >= plan.whole[lo]) {
+    const int k = i - plan.whole[lo];
+    splits = plan.parts[lo];
+    part = k % splits;
+    i = plan.whole[lo] + k / splits;
+    if (splits > 1) state = plan.first_state[lo] + k;
+  }
+  by = i / abs(plan.row_blocks[lo]);
+  bx = row_block_of(plan, lo, i);
+  bz = plan.seq[lo] * splits + part;
+}
+template <class Item>
+__device__ __forceinline__ void place_results(const PagedParams&, Item& w, int state) {
+  if (state < 0) return;
+  w.part = 1;
+  w.head = 0;
+  w.q_begin = state * 256 - w.q0;
+}
+template <class Item>
+__device__ __forceinline__ bool is_part(const PagedParams&, const Item& w) { return w.part != 0; }
+__device__ __forceinline__ const FlashParams& parts_of(const PagedParams& p) { return p.parts; }
+
 // Tiles of 128: q [heads * D, tokens, batch] as for the dense kernel.
 template <int D>
 cudaError_t launch_paged_tiles(const CUtensorMap& tm_q, const PagedMap& tm_k, const PagedMap& tm_v, const PagedParams& p, cudaStream_t stream);
+// ... and, behind that launch, the join of the parts of blocks whose keys it split.
+template <int D>
+cudaError_t launch_tile_join(const PagedParams& p, cudaStream_t stream);
 
 // Few rows: blocks of 16, 32 or 64.  Scratch holds the states of sequences that more than one CTA works on.
 struct PagedRowsPlan {

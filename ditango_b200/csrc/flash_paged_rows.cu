@@ -647,6 +647,68 @@ __global__ void __launch_bounds__(128) flash_paged_join_kernel(const __grid_cons
   }
 }
 
+// Joins the parts of blocks whose keys the kernel of tiles split: normalised values and lse of each, 256 rows apart.  grid: (blocks, CTAs to a block's rows),
+// a warp per row.
+template <int D>
+__global__ void __launch_bounds__(256) flash_tile_join_kernel(const __grid_constant__ PagedParams p) {
+  constexpr int kCols = D / 32, kAhead = 8;
+  __shared__ float s_row[8][D];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  grid_dependency_wait();
+  const int status = *reinterpret_cast<volatile int*>(p.f.status);
+  const TileJoin j = p.joins[blockIdx.x];
+  if (status != 0) return;
+  for (int r = blockIdx.y * 8 + warp; r < j.rows; r += gridDim.y * 8) {
+    const float* o = static_cast<const float*>(p.parts.out) + (static_cast<int64_t>(j.state) * 256 + r) * D + lane * kCols;
+    const float* lse = p.parts.lse + static_cast<int64_t>(j.state) * 256 + r;
+    float top = -INFINITY, sum = 0.f, acc[kCols] = {};
+    for (int i = lane; i < j.parts; i += 32) top = fmaxf(top, lse[i * 256]);
+    for (int i0 = 0; i0 < j.parts; i0 += kAhead) {
+      // (all reads are under way before one is used)
+      float l[kAhead], v[kAhead][kCols];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int64_t i = min(i0 + u, j.parts - 1);
+        l[u] = lse[i * 256];
+        if constexpr (D == 128) {
+          const float4 q = *reinterpret_cast<const float4*>(o + i * 256 * D);
+          v[u][0] = q.x, v[u][1] = q.y, v[u][2] = q.z, v[u][3] = q.w;
+        } else {
+          const float2 q = *reinterpret_cast<const float2*>(o + i * 256 * D);
+          v[u][0] = q.x, v[u][1] = q.y;
+        }
+      }
+      if (i0 == 0) {
+#pragma unroll
+        for (int d = 16; d > 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+      }
+      const float ref = reference(top);
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        if (i0 + u >= j.parts) break;
+        const float f = __expf(l[u] - ref);
+        sum += f;
+#pragma unroll
+        for (int k = 0; k < kCols; ++k) acc[k] = fmaf(v[u][k], f, acc[k]);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kCols; ++k) s_row[warp][lane * kCols + k] = acc[k];
+    __syncwarp();
+    if (lane < D / 4)          // (the maximum in units of raw scores, as store_row4 takes it)
+      store_row4<D>(p, j.seg, j.q_begin, j.q0 + r, j.head, lane * 4, *reinterpret_cast<const float4*>(&s_row[warp][lane * 4]),
+                    top / (p.f.scale_log2 * kLn2), sum, lane == 0, D == 128 ? 0xffffffffu : 0xffffu);
+    __syncwarp();
+  }
+}
+
+template <int D>
+cudaError_t launch_tile_join(const PagedParams& p, cudaStream_t stream) {
+  return launch_attention_kernel(flash_tile_join_kernel<D>, dim3(p.most_states / 2, 8), 256, 0, stream, true, p);
+}
+template cudaError_t launch_tile_join<64>(const PagedParams&, cudaStream_t);
+template cudaError_t launch_tile_join<128>(const PagedParams&, cudaStream_t);
+
 PagedRowsPlan plan_paged_rows(int64_t rows_of_a_head, int64_t keys, int64_t kv_heads, int64_t nseg, int head_dim, int sm_count) {
   PagedRowsPlan plan;
   plan.rows = rows_of_a_head <= 16 ? 16 : rows_of_a_head <= 32 ? 32 : 64;

@@ -65,6 +65,14 @@ __device__ __forceinline__ WindowSeq window_seq(const WindowParams& p, int seg) 
 
 // Of what number of keys a run that is walked begins at a multiple.  (Dense keys: anywhere.)
 __device__ __forceinline__ int key_align(const WindowParams&) { return 1; }
+// Which block a CTA's place in the grid stands for: row block, head, sequence x parts, and the parts that its keys are split into.
+__device__ __forceinline__ void place_block(const WindowParams&, int&, int&, int&, int&, int&) {}
+// A block's results go to p.f, whichever part of its keys it has.
+template <class Item>
+__device__ __forceinline__ void place_results(const WindowParams&, Item&, int) {}
+template <class Item>
+__device__ __forceinline__ constexpr bool is_part(const WindowParams&, const Item&) { return false; }
+__device__ __forceinline__ const FlashParams& parts_of(const WindowParams& p) { return p.f; }
 
 // Keys that query i sees: [0, first) and [lo, hi), first <= lo <= hi.  A key at position j is seen from position x when
 // j <= x + right and (j >= x - left or j < sinks).

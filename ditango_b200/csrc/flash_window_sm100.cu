@@ -129,6 +129,7 @@ struct Item {
   int q_begin, q_len;            // where its sequence begins in the results, and its length
   int from, to, sinks;           // of its sequence, see WindowSeq
   int k_end, k_floor;            // see window_span
+  int part;                      // 1: a part's state, which a launch behind this one joins with the others
 };
 static_assert(sizeof(Item) <= 80, "shared-memory layout");
 
@@ -259,7 +260,7 @@ __device__ __forceinline__ bool claim_answer(const void* response16, int& x, int
 
 }  // namespace
 
-// grid: (row blocks, heads, sequences x parts).  Keys and values dense (CUtensorMap, WindowParams) or in pages (PagedMap, PagedParams): the two
+// grid: (row blocks, heads, sequences x parts); in pages as plan_blocks deals them out.  Keys and values dense (CUtensorMap, WindowParams) or in pages (PagedMap, PagedParams): the two
 // differ in how a sequence and a tile's rows are found.
 template <int D, class Map, class Params>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -307,6 +308,7 @@ flash_window_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     init_loads(p);
     fence_mbar_init();
   }
+  plan_blocks(p);
   if (warp == kMmaWarp + 1 && lane < D / 4) {
     reinterpret_cast<uint4*>(sh.s_zero)[lane] = make_uint4(0u, 0u, 0u, 0u);
     fence_proxy_async_smem();
@@ -358,7 +360,7 @@ flash_window_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         int published = 0;
         uint32_t claims = 0;
         bool live = true, asked = false;
-        int bx = blockIdx.x, by = blockIdx.y, bz = blockIdx.z;
+        int bx = blockIdx.x, by = blockIdx.y, bz = blockIdx.z, splits = p.splits, state = -1;
         auto ask = [&]() {
           fence_proxy_async_smem();            // the answer before this one has been read
           mbar_expect_tx(sh.claim, 16);
@@ -375,7 +377,8 @@ flash_window_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         };
         for (;;) {
           Item w;
-          const int seg = bz / p.splits, part = bz % p.splits;
+          place_block(p, bx, by, bz, splits, state);
+          const int seg = bz / splits, part = bz % splits;
           w.head = by;
           w.seg = seg;
           w.q0 = bx * (kQT * kBM);
@@ -387,17 +390,20 @@ flash_window_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
           w.sinks = s.sinks;
           w.k_end = s.k_len;
           w.k_floor = s.sinks;
+          w.part = 0;
+          place_results(p, w, state);
           asked = false;
           if (w.q0 < w.q_len) {
             const int i1 = min(w.q0 + kQT * kBM, w.q_len) - 1;
             w.walk.plan(w.from, w.to, w.sinks, w.k_end, w.k_floor, w.q0, i1, key_align(p));
-            if (p.splits > 1) {
+            if (splits > 1) {
               // as many tiles to each part, the first tokens to the last one
               const int begin = w.walk.lo, end = begin + w.walk.win;
-              const int keys = (w.walk.N + (w.walk.first + kBN - 1) / kBN + p.splits - 1) / p.splits * kBN;
-              w.k_floor = min(begin + part * keys, end);
-              if (part + 1 < p.splits) {
-                w.k_end = min(w.k_floor + keys, end);
+              const int keys = (w.walk.N + (w.walk.first + kBN - 1) / kBN + splits - 1) / splits * kBN;
+              // (the first tile may begin in front of the window's keys)
+              w.k_floor = max(min(begin + part * keys, end), w.k_floor);
+              if (part + 1 < splits) {
+                w.k_end = min(begin + (part + 1) * keys, end);
                 w.sinks = 0;
               }
               w.walk.plan(w.from, w.to, w.sinks, w.k_end, w.k_floor, w.q0, i1, key_align(p));
@@ -407,7 +413,7 @@ flash_window_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
             if (n_units == 0) {
               // The other roles do not meet it.  (The issuer asks for the block behind the one under way before it ends that one: with
               // a run of such blocks in between, more than there are slots, each role would wait for another.)
-              write_none<D>(p.f, w, sh.s_zero);
+              write_none<D>(is_part(p, w) ? parts_of(p) : p.f, w, sh.s_zero);
             } else {
               if (!publish(w)) break;
               const int qb = items % C::kQBufs, q_round = items / C::kQBufs;
@@ -670,8 +676,52 @@ flash_window_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       for (int slot; (slot = fetch_warp(sh)) >= 0;) {
         const int q0 = sh.s_work[slot].q0, head = sh.s_work[slot].head, seg = sh.s_work[slot].seg;
         const int q_begin = sh.s_work[slot].q_begin, q_len = sh.s_work[slot].q_len;
+        const bool part = is_part(p, sh.s_work[slot]);
         give_back(sh, slot);
         bool ok = true;
+        if (part) {
+          // a part's state: fp32, 256 rows one after another, nothing to fold into
+#pragma unroll 1
+          for (int tile = 0; ok && tile < kQT; ++tile) {
+            ok = warp_wait_or_abort(&sh.ml_full[tile], item_use, p.f.status, 42);
+            if (!ok) break;
+            const float2 ml = sh.s_ml[tile * kBM + quarter * 32 + lane];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.ml_empty[tile]);
+            ok = warp_wait_or_abort(&sh.o_final[tile], item_use, p.f.status, 41);
+            if (!ok) break;
+            tc_fence_after();
+            const int64_t row0 = static_cast<int64_t>(q_begin) + q0 + tile * kBM + quarter * 32;
+            const FlashParams& f = parts_of(p);
+            const float w = ml.y != 0.f ? 1.f / ml.y : 0.f;
+            f.lse[row0 + lane] = ml.y != 0.f ? (ml.x * c + log2f(ml.y)) * kLn2 : -INFINITY;
+            float* dst = static_cast<float*>(f.out) + row0 * D;
+#pragma unroll 1
+            for (int q = 0; q < D / 32; ++q) {
+              uint32_t orow[32];
+              tmem_ld32(lane_base + C::kColO + tile * D + q * 32, orow);
+              tmem_wait_ld<32>(orow);
+              if (q == D / 32 - 1) {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.o_free[tile]);
+              }
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                *reinterpret_cast<float4*>(stage + lane * 128 + ((i ^ (lane & 7)) << 4)) =
+                    make_float4(__uint_as_float(orow[4 * i]) * w, __uint_as_float(orow[4 * i + 1]) * w, __uint_as_float(orow[4 * i + 2]) * w,
+                                __uint_as_float(orow[4 * i + 3]) * w);
+              __syncwarp();
+#pragma unroll 1
+              for (int r = lane >> 3; r < 32; r += 4)
+                *reinterpret_cast<float4*>(dst + r * D + q * 32 + (lane & 7) * 4) = *reinterpret_cast<const float4*>(stage + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+              __syncwarp();
+            }
+          }
+          if (!ok) break;
+          item_use ^= 1;
+          continue;
+        }
 #pragma unroll 1
         for (int tile = 0; ok && tile < kQT; ++tile) {
           const uint32_t o_taddr = lane_base + C::kColO + tile * D;
@@ -898,6 +948,9 @@ flash_window_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
   }
 }
 
+static dim3 tile_grid(const WindowParams& p) { return dim3((p.f.seqlen_q + kQT * kBM - 1) / (kQT * kBM), p.f.num_heads, p.f.nseg * p.splits); }
+static dim3 tile_grid(const PagedParams& p) { return dim3(p.blocks); }
+
 template <int D, class Map, class Params>
 static cudaError_t launch_tiles(const CUtensorMap& tq, const Map& tk, const Map& tv, const Params& p, cudaStream_t stream) {
   using C = Cfg<D>;
@@ -919,8 +972,7 @@ static cudaError_t launch_tiles(const CUtensorMap& tq, const Map& tk, const Map&
       configured[dev & 63] = true;
     }
   }
-  const dim3 grid((p.f.seqlen_q + kQT * kBM - 1) / (kQT * kBM), p.f.num_heads, p.f.nseg * p.splits);
-  kernel<<<grid, kThreads, C::kSmemBytes, stream>>>(tq, tk, tv, p);
+  kernel<<<tile_grid(p), kThreads, C::kSmemBytes, stream>>>(tq, tk, tv, p);
   return cudaGetLastError();
 }
 

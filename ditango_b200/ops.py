@@ -533,10 +533,10 @@ def flash_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, t
     if T * H * D == 0 or sq <= 0:
         return out, lse
     lib = _capi.load()
-    key = (q.get_device(), nseg, sq, sk, H, Hk, D)
+    key = (q.get_device(), nseg, sq, sk, T, H, Hk, D)
     need = _PAGED_SCRATCH.get(key)
     if need is None:
-        need = lib.dtb_flash_paged_scratch_bytes(nseg, sq, sk, H, Hk, D)
+        need = lib.dtb_flash_paged_scratch_bytes(nseg, sq, sk, T, H, Hk, D)
         if need < 0:
             _capi.check(need, "dtb_flash_paged_scratch_bytes")
         if len(_PAGED_SCRATCH) >= 4096:

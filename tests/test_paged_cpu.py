@@ -67,7 +67,7 @@ def test_flash_refuses(args, word):
     assert _flash(lib, **args) == -1 and word in lib.dtb_last_error().decode()
 
 
-@pytest.mark.parametrize("args,word", [((0, 9, 9, 2, 2, 64), "nseg"), ((1, -1, 9, 2, 2, 64), "length"), ((1, 9, 9, 3, 2, 64), "heads"), ((1, 9, 9, 2, 2, 32), "head_dim")])
+@pytest.mark.parametrize("args,word", [((0, 9, 9, 9, 2, 2, 64), "nseg"), ((1, -1, 9, 9, 2, 2, 64), "length"), ((1, 9, 9, 9, 3, 2, 64), "heads"), ((1, 9, 9, 9, 2, 2, 32), "head_dim")])
 def test_flash_scratch_refuses(args, word):
     lib = _lib()
     assert lib.dtb_flash_paged_scratch_bytes(*args) == -1 and word in lib.dtb_last_error().decode()

@@ -279,6 +279,44 @@ def test_chunks_match_the_definition(new, lens, H, Hk, P, left, right, sinks, D)
     _attend(cache, _rand((sum(new), H, D), 51), new, left=left, right=right, sinks=sinks, out_dtype=dtype)
 
 
+# few blocks against many keys (all split), a last round of blocks that is mostly empty (some split), both among short sequences, more sequences
+# than blocks are planned for, lengths that a plan has to order
+SPLITS = [([300], [6000], 2, 1, -1, 0, 0), ([140, 1, 600], [9000, 4000, 700], 2, 2, -1, 0, 0), ([129], [5000], 1, 1, 900, 0, 70), ([1000], [1200], 40, 1, -1, -1, 0),
+          ([700, 300, 900], [800, 4000, 900], 24, 1, -1, 0, 0), ([600], [2500], 60, 1, 500, 100, 30), ([200, 1, 130] * 100, [220, 90, 140] * 100, 2, 2, -1, 0, 0),
+          ([130, 260, 0, 513] * 5, [140, 3000, 77, 1500] * 5, 2, 1, -1, 10, 0), ([129] * 3, [0, 5, 4000], 4, 4, -1, 0, 0)]
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("new,lens,H,Hk,left,right,sinks", SPLITS)
+def test_blocks_whose_keys_are_split(new, lens, H, Hk, left, right, sinks, D):
+    """(129 rows and more of a key head to each query head: the kernel of few rows takes up to 128 / (H / Hk) queries)"""
+    cache = _Cache(lens, Hk, D, 64, seed=9)
+    q = _rand((sum(new), H, D), 61)
+    _attend(cache, q, new, left=left, right=right, sinks=sinks, out_dtype=torch.bfloat16 if H % 4 else torch.float32)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_split_blocks_fold_into_a_state(D):
+    from ditango_b200 import ops
+    new, lens, H = [200, 140], [5000, 300], 4
+    cache = _Cache(lens, 2, D, 16, seed=10)
+    T = sum(new) + 3
+    q = _rand((T, H, D), 62)
+    old_k, old_v = _rand((40, 2, D), 63), _rand((40, 2, D), 64)
+    out, lse = ops.flash_window(q[None].cuda(), old_k[None].cuda(), old_v[None].cuda())
+    out, lse = out[0].contiguous(), lse[0].contiguous()
+    before = out.clone(), lse.clone()
+    cu = [0, 200, 340]
+    ops.flash_paged(q.cuda(), cache.k_pages, cache.v_pages, cache.table, cache.seqlens, left=2000, right=0, sinks=9, cu_seqlens_q=_i(cu), max_seqlen_q=200, out=out, lse=lse,
+                    accumulate=True)
+    assert torch.equal(out[340:], before[0][340:]) and torch.equal(lse[:, 340:], before[1][:, 340:])
+    for b, n in enumerate(new):
+        seen = torch.cat([torch.ones(n, 40, dtype=torch.bool), _visible(n, lens[b], 2000, 0, 9, lens[b] - n, 0)], 1)
+        want, want_lse, spread = _exact(q[cu[b]:cu[b + 1]], torch.cat([old_k, cache.k[b]]), torch.cat([old_v, cache.v[b]]), seen)
+        _check(out[cu[b]:cu[b + 1]], lse.t()[cu[b]:cu[b + 1]], want, want_lse, 1.01 * spread)
+    assert ops.read_status() == 0
+
+
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("n", [1, 5, 70, 300])
 def test_dense_queries_and_both_layouts_of_lse(n, D):
