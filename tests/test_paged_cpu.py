@@ -88,3 +88,17 @@ def test_tensors_on_the_cpu_and_of_other_types_are_refused():
                  lambda: ops.write_pages(k, k, pages, pages, torch.zeros(5, dtype=torch.int32)), lambda: ops.flash_paged(q, pages, pages, table, i)):
         with pytest.raises(ExtensionError):
             call()
+
+
+@pytest.mark.parametrize("args", [dict(page_size=24), dict(page_size=8), dict(layers=0), dict(head_dim=96), dict(left=-2), dict(sinks=-1), dict(max_tokens=0)])
+def test_stream_cache_refuses(args):
+    from ditango_b200.core.stream_cache import StreamCache
+    with pytest.raises(ValueError):
+        StreamCache(**{**dict(layers=1, streams=1, num_pages=1, kv_heads=1, head_dim=64, max_tokens=10, device="cpu"), **args})
+
+
+def test_stream_cache_has_no_fallback():
+    from ditango_b200._capi import ExtensionError
+    from ditango_b200.core.stream_cache import StreamCache
+    with pytest.raises(ExtensionError):
+        StreamCache(1, 1, 1, 1, 64, 10, device="cpu")
