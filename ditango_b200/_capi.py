@@ -23,7 +23,7 @@ EXPORTS = (
     "dtb_peek_status_async", "dtb_post_status",
     "dtb_ipc_export_mem", "dtb_ipc_open_mem", "dtb_ipc_close_mem", "dtb_peer_copy_async",
     "dtb_flash_fwd", "dtb_flash_fwd_ex", "dtb_flash_window", "dtb_flash_window_scratch_bytes",
-    "dtb_extend_pages", "dtb_release_pages", "dtb_write_pages", "dtb_flash_paged", "dtb_flash_paged_scratch_bytes", "dtb_merge_states", "dtb_merge_rows", "dtb_quantize_rows",
+    "dtb_extend_pages", "dtb_release_pages", "dtb_write_pages", "dtb_flash_paged", "dtb_flash_paged_launches", "dtb_flash_paged_scratch_bytes", "dtb_merge_states", "dtb_merge_rows", "dtb_quantize_rows",
     "dtb_dequantize_rows", "dtb_copy_chunks",
     "dtb_norm_rope", "dtb_norm_rope_grid", "dtb_norm_rope_grid_scratch_bytes", "dtb_norm_rope_grid_backward", "dtb_ln_modulate", "dtb_gate_add", "dtb_drift_scratch_bytes", "dtb_drift_accumulate",
     "dtb_drift_noalloc_max_elements", "dtb_drift_accumulate_noalloc",
@@ -88,6 +88,8 @@ def load():
     lib.dtb_flash_paged.argtypes = (
         [c_void_p, c_int64, c_int64] + pool * 2 + [c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int] +
         [c_int, c_int, c_int, c_int64, c_int, c_int, c_int, c_float, c_int, c_int, c_int, c_void_p, c_int64, c_void_p])
+    lib.dtb_flash_paged_launches.restype = c_int
+    lib.dtb_flash_paged_launches.argtypes = [c_int, c_int, c_int, c_int64, c_int, c_int, c_int, c_int]
     lib.dtb_flash_paged_scratch_bytes.restype = c_int64
     lib.dtb_flash_paged_scratch_bytes.argtypes = [c_int, c_int, c_int, c_int64, c_int, c_int, c_int]
     lib.dtb_merge_states.restype = c_int

@@ -787,6 +787,28 @@ DTB_API int64_t dtb_flash_paged_scratch_bytes(int nseg, int seqlen_q, int seqlen
   return plan_paged(nseg, seqlen_q, seqlen_k, total_q, num_heads, num_kv_heads, head_dim, d->sm_count).scratch_bytes;
 }
 
+// Sequences of few and of many queries in one batch take a launch each.  (With rows for more than that, none of them has few, unless there are
+// rows behind the last one; the kernel of many then takes it.)
+static bool paged_mixed(const PagedPlan& plan, bool packed, int64_t nseg, int64_t seqlen_q, int64_t total_q) {
+  return plan.tiles && packed && total_q <= (nseg - 1) * seqlen_q + plan.few_rows;
+}
+static bool paged_planned(int64_t nseg, int64_t total_q, int64_t num_heads) {
+  return nseg <= dtb::kPlanSeqs && (total_q / 256 + nseg) * num_heads < dtb::kPlanBlocks;
+}
+
+DTB_API int dtb_flash_paged_launches(int nseg, int seqlen_q, int seqlen_k, int64_t total_q, int packed, int num_heads, int num_kv_heads, int head_dim) {
+  int rc = check_paged_shape("dtb_flash_paged_launches", nseg, seqlen_q, seqlen_k, num_heads, num_kv_heads, head_dim);
+  if (rc != DTB_OK) return rc;
+  DeviceInfo* d = nullptr;
+  if ((rc = device_info(&d)) != DTB_OK) return rc;
+  if (seqlen_q == 0 || total_q == 0) return 0;
+  const PagedPlan plan = plan_paged(nseg, seqlen_q, seqlen_k, total_q, num_heads, num_kv_heads, head_dim, d->sm_count);
+  int n = 0;
+  if (plan.tiles) n += plan.states > 0 && paged_planned(nseg, total_q, num_heads) ? 2 : 1;
+  if (!plan.tiles || paged_mixed(plan, packed != 0, nseg, seqlen_q, total_q)) n += 2;
+  return n;
+}
+
 DTB_API int dtb_flash_paged(const void* q, int64_t q_tok_stride, int64_t q_batch_stride,
                             const void* k_pages, int64_t k_page_stride, int64_t k_tok_stride, int64_t k_head_stride,
                             const void* v_pages, int64_t v_page_stride, int64_t v_tok_stride, int64_t v_head_stride,
@@ -855,9 +877,7 @@ DTB_API int dtb_flash_paged(const void* q, int64_t q_tok_stride, int64_t q_batch
   p.columns = columns;
   p.pages = pages;
   p.page_shift = shift;
-  // Sequences of few and of many queries in one batch take a launch each.  (With rows for more than that, none of them has few, unless there are
-  // rows behind the last one; the kernel of many then takes it.)
-  const bool mixed = plan.tiles && cu_seqlens_q != nullptr && total_q <= static_cast<int64_t>(nseg - 1) * seqlen_q + plan.few_rows;
+  const bool mixed = paged_mixed(plan, cu_seqlens_q != nullptr, nseg, seqlen_q, total_q);
   p.few_rows = plan.tiles && !mixed ? -1 : plan.few_rows;
   if ((rc = load_encoder()) != DTB_OK) return rc;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -877,7 +897,7 @@ DTB_API int dtb_flash_paged(const void* q, int64_t q_tok_stride, int64_t q_batch
     if ((rc = make_token_map(&tq, q, q_width, packed ? total_q : seqlen_q, q_tok_stride, packed ? 1 : nseg, q_batch_stride, &p.q_batch_first, "q")) != DTB_OK) return rc;
     // blocks of 256 rows: as many as fit the rows that there are, and room for the parts
     const int64_t per_seq = (seqlen_q + 255) / 256, in_rows = total_q / 256 + nseg;
-    p.planned = nseg <= dtb::kPlanSeqs && in_rows * num_heads < dtb::kPlanBlocks;
+    p.planned = paged_planned(nseg, total_q, num_heads);
     const int64_t blocks = p.planned ? std::min(nseg * per_seq, in_rows) * num_heads + plan.states : nseg * per_seq * num_heads;
     if (blocks >= (1ll << 31)) return fail(DTB_ERR_ARG, "%s: too many blocks of rows", kWhat);
     p.blocks = static_cast<int>(blocks);

@@ -44,9 +44,14 @@ __device__ __forceinline__ int paged_keys(const PagedParams& p, int seg) { retur
 // The tile kernel's view of a sequence.  Its keys are numbered through all sequences, seg * columns * P + j.
 __device__ __forceinline__ WindowSeq paged_seq(const PagedParams& p, int seg) {
   WindowSeq s;
-  s.q_begin = p.f.cu_q != nullptr ? p.f.cu_q[seg] : 0;
-  s.q_len = p.f.cu_q != nullptr ? p.f.cu_q[seg + 1] - s.q_begin : p.f.seqlen_q;
-  s.q_len = max(min(s.q_len, p.f.seqlen_q), 0);
+  s.q_begin = 0;
+  s.q_len = p.f.seqlen_q;
+  if (p.f.cu_q != nullptr) {
+    // (what offsets say beyond the rows that there are is not followed)
+    const int total = static_cast<int>(p.f.total_q);
+    s.q_begin = min(max(p.f.cu_q[seg], 0), total);
+    s.q_len = max(min(min(max(p.f.cu_q[seg + 1], 0), total) - s.q_begin, p.f.seqlen_q), 0);
+  }
   s.k_begin = seg * (p.columns << p.page_shift);
   s.k_len = paged_keys(p, seg);
   const int64_t x = static_cast<int64_t>(s.k_len) - s.q_len;

@@ -240,6 +240,7 @@ flash_paged_rows_kernel(const __grid_constant__ PagedMap tm_k, const __grid_cons
   uint64_t* empty = full + C::kStages;
   __shared__ long long s_sum[kThreads / 32];
   __shared__ Seq s_seq;                     // the share's first sequence, ...
+  __shared__ Seq s_seqs[kThreads / 32];     // the one that each warp is at: in registers it would have others spilled
   __shared__ int s_seg, s_unit, s_place;    // ... (key head, row block) of that, and place of the block
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Scratch<D, R> sc(scratch, gridDim.x);
@@ -260,8 +261,8 @@ flash_paged_rows_kernel(const __grid_constant__ PagedMap tm_k, const __grid_cons
   const int per = (p.f.nseg + kThreads - 1) / kThreads, seg0 = min(static_cast<int>(threadIdx.x) * per, p.f.nseg), seg1 = min(seg0 + per, p.f.nseg);
   auto places = [&](const Seq& s) { return static_cast<long long>(s.blocks) * p.kv_heads * places_of(s); };
   long long sum = 0;
-  Seq s;
-  for (int i = seg0; i < seg1; ++i) sum += places(s = make_seq<R>(p, i));
+  Seq own;
+  for (int i = seg0; i < seg1; ++i) sum += places(own = make_seq<R>(p, i));
   long long upto = sum;
 #pragma unroll
   for (int d = 1; d < 32; d *= 2) {
@@ -286,15 +287,15 @@ flash_paged_rows_kernel(const __grid_constant__ PagedMap tm_k, const __grid_cons
   const long long begin = shares.begin(cta);
   if (begin >= at && begin < at + sum) {
     for (int i = seg0; i < seg1; ++i) {
-      if (per > 1) s = make_seq<R>(p, i);
-      if (begin < at + places(s)) {
-        s_seq = s;
+      if (per > 1) own = make_seq<R>(p, i);
+      if (begin < at + places(own)) {
+        s_seq = own;
         s_seg = i;
-        s_unit = static_cast<int>(divide(begin - at, places_of(s)));
-        s_place = static_cast<int>(begin - at - static_cast<long long>(s_unit) * places_of(s));
+        s_unit = static_cast<int>(divide(begin - at, places_of(own)));
+        s_place = static_cast<int>(begin - at - static_cast<long long>(s_unit) * places_of(own));
         break;
       }
-      at += places(s);
+      at += places(own);
     }
   }
   __syncthreads();
@@ -303,7 +304,9 @@ flash_paged_rows_kernel(const __grid_constant__ PagedMap tm_k, const __grid_cons
   long long left = shares.begin(cta + 1) - begin;             // places
   int stage = 0;
   uint32_t use = 0;                         // parity of the ring's round
-  s = s_seq;
+  Seq& s = s_seqs[warp];
+  if (lane == 0) s = s_seq;
+  __syncwarp();
   bool first_block = true;
   // the block's tiles that are this CTA's: up to, not with, this one
   auto last_tile = [&]() { return tiles_before(static_cast<int>(min(static_cast<long long>(places_of(s)), place + left))); };
@@ -313,7 +316,11 @@ flash_paged_rows_kernel(const __grid_constant__ PagedMap tm_k, const __grid_cons
     first_block = false;
     if (++unit == s.blocks * p.kv_heads && left > 0) {
       unit = 0;
-      do s = make_seq<R>(p, ++seg); while (s.blocks == 0);
+      Seq next;
+      do next = make_seq<R>(p, ++seg); while (next.blocks == 0);
+      __syncwarp();
+      if (lane == 0) s = next;
+      __syncwarp();
     }
   };
 

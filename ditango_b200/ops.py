@@ -466,7 +466,7 @@ def _flat_tok_stride(x: torch.Tensor) -> int:
     return _tok_stride(x)
 
 
-_PAGED_SCRATCH = {}       # (device, sequences, lengths, heads, D) -> bytes that flash_paged needs
+_PAGED_PLANS = {}         # (device, sequences, lengths, heads, D, packed) -> (bytes that flash_paged needs, its launches)
 
 
 def flash_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, seqlens_k: torch.Tensor, *, left: int = -1,
@@ -533,15 +533,16 @@ def flash_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, t
     if T * H * D == 0 or sq <= 0:
         return out, lse
     lib = _capi.load()
-    key = (q.get_device(), nseg, sq, sk, T, H, Hk, D)
-    need = _PAGED_SCRATCH.get(key)
-    if need is None:
-        need = lib.dtb_flash_paged_scratch_bytes(nseg, sq, sk, T, H, Hk, D)
-        if need < 0:
-            _capi.check(need, "dtb_flash_paged_scratch_bytes")
-        if len(_PAGED_SCRATCH) >= 4096:
-            _PAGED_SCRATCH.clear()
-        _PAGED_SCRATCH[key] = need
+    key = (q.get_device(), nseg, sq, sk, T, H, Hk, D, packed)
+    plan = _PAGED_PLANS.get(key)
+    if plan is None:
+        plan = lib.dtb_flash_paged_scratch_bytes(nseg, sq, sk, T, H, Hk, D), lib.dtb_flash_paged_launches(nseg, sq, sk, T, packed, H, Hk, D)
+        if min(plan) < 0:
+            _capi.check(min(plan), "dtb_flash_paged")
+        if len(_PAGED_PLANS) >= 4096:
+            _PAGED_PLANS.clear()
+        _PAGED_PLANS[key] = plan
+    need, launches = plan
     scratch = torch.empty_strided((need,), (1,), dtype=torch.uint8, device=q.device)
     q_strides = (H * D, 0 if packed else sq * H * D) if q.is_contiguous() else _strides(q, shape)
     ev = None
@@ -554,7 +555,7 @@ def flash_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, t
         nseg, sq, sk, T, H, Hk, D, D ** -0.5 if softmax_scale is None else softmax_scale, left, right, sinks, scratch.data_ptr(), need, stream)
     if rc:
         _capi.check(rc, "dtb_flash_paged")
-    LaunchLog.count += 2
+    LaunchLog.count += launches
     if ev is not None:
         ev[1].record()
         span = sk if left < 0 or right < 0 else min(sk, left + right + 1 + sinks)      # upper bound of a row's keys

@@ -236,6 +236,8 @@ DTB_API int dtb_write_pages(const void* k, const void* v, int64_t k_tok_stride, 
  *   scratch        dtb_flash_paged_scratch_bytes(...) bytes, 16-byte aligned, of one call at a time
  */
 DTB_API int64_t dtb_flash_paged_scratch_bytes(int nseg, int seqlen_q, int seqlen_k, int64_t total_q, int num_heads, int num_kv_heads, int head_dim);
+/* Kernels that such a call launches (packed: whether cu_seqlens_q is given), for accounting. */
+DTB_API int dtb_flash_paged_launches(int nseg, int seqlen_q, int seqlen_k, int64_t total_q, int packed, int num_heads, int num_kv_heads, int head_dim);
 DTB_API int dtb_flash_paged(const void* q, int64_t q_tok_stride, int64_t q_batch_stride,
                      const void* k_pages, int64_t k_page_stride, int64_t k_tok_stride, int64_t k_head_stride,
                      const void* v_pages, int64_t v_page_stride, int64_t v_tok_stride, int64_t v_head_stride,

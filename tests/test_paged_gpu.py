@@ -493,6 +493,55 @@ def test_a_step_in_a_graph(n):
     assert lens.tolist() == total and ops.read_status() == 0
 
 
+@pytest.mark.parametrize("n", [1, 300])
+def test_a_posted_status_keeps_results_from_being_written(n):
+    from ditango_b200 import ops
+    cache = _Cache([2000, 333], 2, 64, 16, seed=11)
+    q = _rand((2 * n, 4, 64), 65).cuda()
+    out, lse = torch.full((2 * n, 4, 64), 7.0, device="cuda"), torch.full((4, 2 * n), 7.0, device="cuda")
+    kw = dict(right=0, cu_seqlens_q=_i([0, n, 2 * n]), max_seqlen_q=n)
+    torch.cuda.synchronize()
+    ops.post_status(5)
+    ops.flash_paged(q, cache.k_pages, cache.v_pages, cache.table, cache.seqlens, out=out, lse=lse, **kw)
+    assert ops.read_status() == 5 and (out == 7).all() and (lse == 7).all()
+    _attend(cache, q.cpu(), [n, n], right=0)
+
+
+@pytest.mark.parametrize("n", [2, 200])
+def test_offsets_beyond_the_rows_are_not_followed(n):
+    """Offsets of the queries that end behind the rows, begin before them or fall: nothing outside the rows is read or written."""
+    from ditango_b200 import ops
+    cache = _Cache([500, 400, 300], 1, 64, 16, seed=12)
+    guard = torch.full((n + 40, 2, 64), 7.0, device="cuda")
+    lse_guard = torch.full((n + 40, 2), 7.0, device="cuda")
+    q = _rand((n, 2, 64), 66).cuda()
+    for cu in ([0, n // 2, n + 30, n + 60], [-20, n, n, n], [n, 0, n // 2, 2 * n], [2 ** 31 - 1, -2 ** 31, n, n]):
+        guard.fill_(7.0)
+        lse_guard.fill_(7.0)
+        ops.flash_paged(q, cache.k_pages, cache.v_pages, cache.table, cache.seqlens, right=0, cu_seqlens_q=_i(cu), max_seqlen_q=n, out=guard[20:20 + n], lse=lse_guard[20:20 + n],
+                        lse_layout=ops.LSE_BSH)
+        assert ops.read_status() == 0
+        for x in (guard, lse_guard):
+            assert (x[:20] == 7).all() and (x[20 + n:] == 7).all()
+
+
+def test_launches_are_counted():
+    from torch.profiler import ProfilerActivity, profile
+    from ditango_b200 import ops
+    cache = _Cache([3000, 40], 2, 64, 16, seed=13)
+    for new in ([1, 1], [300, 1], [300, 300]):
+        q = _rand((sum(new), 4, 64), 67).cuda()
+        kw = dict(right=0, cu_seqlens_q=_i([0, new[0], sum(new)]), max_seqlen_q=max(new))
+        ops.flash_paged(q, cache.k_pages, cache.v_pages, cache.table, cache.seqlens, **kw)
+        torch.cuda.synchronize()
+        before = ops.LaunchLog.count
+        with profile(activities=[ProfilerActivity.CUDA]) as prof:
+            ops.flash_paged(q, cache.k_pages, cache.v_pages, cache.table, cache.seqlens, **kw)
+            torch.cuda.synchronize()
+        kernels = [e for e in prof.events() if "flash_" in e.name]
+        assert len(kernels) == ops.LaunchLog.count - before
+
+
 def test_other_devices_and_types_are_refused():
     from ditango_b200 import ops
     from ditango_b200._capi import ExtensionError

@@ -28,7 +28,7 @@ SOURCE = r"""
 using std::max; using std::min;
 #define CHECK(x) do { if (!(x)) { std::printf("failed: %%s, line %%d\n", #x, __LINE__); std::exit(1); } } while (0)
 constexpr int kQueriesLast = INT32_MIN;
-struct FlashParams { const int32_t *cu_q, *cu_k; int seqlen_q, seqlen_k, num_heads, nseg; };
+struct FlashParams { const int32_t *cu_q, *cu_k; int seqlen_q, seqlen_k, num_heads, nseg; int64_t total_q; };
 struct WindowParams { FlashParams f; const int32_t* seqlens_k; int kv_heads, left, right, sinks, q_start, k_start; };
 struct PagedParams : WindowParams { int columns, pages, page_shift, box_rows, key_align, few_rows; };
 %(seq)s
@@ -49,7 +49,7 @@ int main(int argc, char** argv) {
   p.box_rows = p.key_align = min(1 << p.page_shift, 64);
   std::vector<int32_t> cu(1, 0), lens;
   for (int b = 0; b < n; ++b) { cu.push_back(cu.back() + a[9 + 2 * b]); lens.push_back(a[10 + 2 * b]); p.f.seqlen_q = max(p.f.seqlen_q, a[9 + 2 * b]); p.columns = max(p.columns, (a[10 + 2 * b] >> p.page_shift) + 1); }
-  p.f.cu_q = cu.data(); p.seqlens_k = lens.data(); p.f.nseg = n;
+  p.f.cu_q = cu.data(); p.f.total_q = cu.back(); p.seqlens_k = lens.data(); p.f.nseg = n;
   auto places = [&](const Seq& s) { return (long long)s.blocks * p.kv_heads * places_of(s); };
   long long all = 0;
   for (int i = 0; i < n; ++i) all += places(make_seq<R>(p, i));
