@@ -166,6 +166,25 @@ int make_page_map(CUtensorMap* tm, const void* base, int64_t head_dim, int64_t p
   return DTB_OK;
 }
 
+// 4-D bf16 view of queries [channel, head, token, batch], a token's heads dense, for boxes of 64 channels x `pack` heads x 128 / pack tokens.
+int make_query_map(CUtensorMap* tm, const void* base, int64_t head_dim, int64_t heads, int64_t tokens, int64_t tok_stride, int64_t batch, int64_t batch_stride,
+                   int pack, int* batch_first) {
+  const bool swap = batch > 1 && batch_stride < tok_stride;
+  const int64_t inner = swap ? batch : tokens, outer = swap ? tokens : batch;
+  const int64_t inner_stride = swap ? batch_stride : tok_stride, outer_stride = swap ? tok_stride : batch > 1 ? batch_stride : tok_stride;
+  cuuint64_t gdim[4] = {static_cast<cuuint64_t>(head_dim), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(outer)};
+  cuuint64_t gstride[3] = {static_cast<cuuint64_t>(head_dim) * 2, static_cast<cuuint64_t>(inner_stride) * 2, static_cast<cuuint64_t>(outer_stride) * 2};
+  const cuuint32_t rows = 128 / static_cast<cuuint32_t>(pack);
+  cuuint32_t box[4] = {64, static_cast<cuuint32_t>(pack), swap ? 1u : rows, swap ? rows : 1u};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult r = g_encode(tm, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), gdim, gstride, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  *batch_first = swap ? 1 : 0;
+  if (r != CUDA_SUCCESS) return fail(DTB_ERR_CUDA, "cuTensorMapEncodeTiled(q) failed with CUresult %d", static_cast<int>(r));
+  return DTB_OK;
+}
+
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // Encoded tensor maps, kept per (base pointer, rows, width, pitch, box rows).  The attention path calls
@@ -747,6 +766,7 @@ DTB_API int dtb_write_pages(const void* k, const void* v, int64_t k_tok_stride, 
 struct PagedPlan {
   int few_rows;                  // sequences with at most this many queries go to the kernel of few rows
   bool tiles;                    // there may be others
+  int pack_shift;                // that many heads of a key head (their logarithm) share the tiles of 128 rows
   dtb::PagedRowsPlan rows;
   int states;                    // of parts, at most; 0: the kernel of tiles splits no keys
   int64_t tile_bytes;            // of scratch, in front of that of the kernel of few rows
@@ -755,13 +775,18 @@ struct PagedPlan {
 static PagedPlan plan_paged(int64_t nseg, int64_t seqlen_q, int64_t seqlen_k, int64_t total_q, int64_t num_heads, int64_t kv_heads, int head_dim, int sm_count) {
   PagedPlan plan = {};
   const int64_t group = num_heads / kv_heads;
-  plan.few_rows = static_cast<int>(std::max<int64_t>(128 / group, 1));
+  // Up to 64 rows of a key head are a block of the kernel of few rows, which reads keys at the rate of HBM; for more, tiles of 256 rows take as long for a key
+  // as one of its blocks.  Batches some of whose sequences have up to twice that stay in one launch.  (us: 10 queries of 16 heads each against 4236 keys of
+  // three sequences 69 in that kernel, 29 in tiles; 15 queries and 1 of two sequences, 8 heads, 11396 keys of 128 43, and 57 in both kernels.)
+  const bool few = seqlen_q * group <= 128 && total_q != nseg * seqlen_q;
+  plan.few_rows = static_cast<int>(std::max<int64_t>((few ? 128 : 64) / group, 1));
+  while (plan.pack_shift < 7 && group % (2ll << plan.pack_shift) == 0) ++plan.pack_shift;
   plan.tiles = seqlen_q > plan.few_rows;
   plan.rows = dtb::plan_paged_rows(std::min<int64_t>(seqlen_q, plan.few_rows) * group, seqlen_k, kv_heads, nseg, head_dim, sm_count);
   if (plan.tiles) {
     // Of sequences of one number of queries the blocks are known: with a round of them for each sequence the one that walks furthest has no more
     // than its share, and with a last round that is nearly full nothing is split.  (The launch that joins takes 5 us.)
-    const int64_t blocks = (seqlen_q + 255) / 256 * num_heads * nseg, rounds = (blocks + sm_count - 1) / sm_count;
+    const int64_t blocks = ((seqlen_q << plan.pack_shift) + 255) / 256 * (num_heads >> plan.pack_shift) * nseg, rounds = (blocks + sm_count - 1) / sm_count;
     const bool may = total_q != nseg * seqlen_q || blocks <= sm_count * nseg || static_cast<double>(rounds * sm_count) > 1.15 * static_cast<double>(blocks);
     plan.states = may && seqlen_k > 256 ? 2 * sm_count : 0;
     plan.tile_bytes = plan.states * (256ll * (head_dim + 1) * 4) + plan.states / 2 * static_cast<int64_t>(sizeof(dtb::TileJoin));
@@ -792,8 +817,12 @@ DTB_API int64_t dtb_flash_paged_scratch_bytes(int nseg, int seqlen_q, int seqlen
 static bool paged_mixed(const PagedPlan& plan, bool packed, int64_t nseg, int64_t seqlen_q, int64_t total_q) {
   return plan.tiles && packed && total_q <= (nseg - 1) * seqlen_q + plan.few_rows;
 }
-static bool paged_planned(int64_t nseg, int64_t total_q, int64_t num_heads) {
-  return nseg <= dtb::kPlanSeqs && (total_q / 256 + nseg) * num_heads < dtb::kPlanBlocks;
+// Blocks of 256 rows, as many as fit the rows that there are.
+static int64_t paged_blocks(const PagedPlan& plan, int64_t nseg, int64_t total_q, int64_t num_heads) {
+  return ((total_q << plan.pack_shift) / 256 + nseg) * (num_heads >> plan.pack_shift);
+}
+static bool paged_planned(const PagedPlan& plan, int64_t nseg, int64_t total_q, int64_t num_heads) {
+  return nseg <= dtb::kPlanSeqs && paged_blocks(plan, nseg, total_q, num_heads) < dtb::kPlanBlocks;
 }
 
 DTB_API int dtb_flash_paged_launches(int nseg, int seqlen_q, int seqlen_k, int64_t total_q, int packed, int num_heads, int num_kv_heads, int head_dim) {
@@ -804,7 +833,7 @@ DTB_API int dtb_flash_paged_launches(int nseg, int seqlen_q, int seqlen_k, int64
   if (seqlen_q == 0 || total_q == 0) return 0;
   const PagedPlan plan = plan_paged(nseg, seqlen_q, seqlen_k, total_q, num_heads, num_kv_heads, head_dim, d->sm_count);
   int n = 0;
-  if (plan.tiles) n += plan.states > 0 && paged_planned(nseg, total_q, num_heads) ? 2 : 1;
+  if (plan.tiles) n += plan.states > 0 && paged_planned(plan, nseg, total_q, num_heads) ? 2 : 1;
   if (!plan.tiles || paged_mixed(plan, packed != 0, nseg, seqlen_q, total_q)) n += 2;
   return n;
 }
@@ -823,7 +852,7 @@ DTB_API int dtb_flash_paged(const void* q, int64_t q_tok_stride, int64_t q_batch
   if ((rc = check_table(kWhat, nseg, columns, pages, shift)) != DTB_OK) return rc;
   if ((static_cast<int64_t>(nseg) * columns << shift) >= (1ll << 31)) return fail(DTB_ERR_ARG, "%s: the table's %d rows have room for 2^31 tokens or more", kWhat, nseg);
   if (!q || !out || !lse || !table || !seqlens_k) return fail(DTB_ERR_ARG, "%s: null tensor pointer", kWhat);
-  if (total_q < 0 || total_q >= (1ll << 31)) return fail(DTB_ERR_ARG, "%s: too many tokens", kWhat);
+  if (total_q < 0 || total_q >= (1ll << 31) || total_q * num_heads >= (1ll << 31)) return fail(DTB_ERR_ARG, "%s: too many tokens", kWhat);
   if (cu_seqlens_q == nullptr && static_cast<int64_t>(nseg) * seqlen_q != total_q) return fail(DTB_ERR_ARG, "%s: total tokens are not nseg*seqlen", kWhat);
   constexpr int kFar = 1 << 30;
   if (left < -1 || right < -1 || sinks < 0 || left > kFar || right > kFar || sinks > kFar) return fail(DTB_ERR_ARG, "%s: window (%d, %d) or sinks %d out of range", kWhat, left, right, sinks);
@@ -879,6 +908,7 @@ DTB_API int dtb_flash_paged(const void* q, int64_t q_tok_stride, int64_t q_batch
   p.page_shift = shift;
   const bool mixed = paged_mixed(plan, cu_seqlens_q != nullptr, nseg, seqlen_q, total_q);
   p.few_rows = plan.tiles && !mixed ? -1 : plan.few_rows;
+  p.real = p.f;
   if ((rc = load_encoder()) != DTB_OK) return rc;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   dtb::PagedMap mk, mv;
@@ -893,27 +923,31 @@ DTB_API int dtb_flash_paged(const void* q, int64_t q_tok_stride, int64_t q_batch
     // (with a limit to the left runs begin anywhere, and fewer than 16 keys in front of them are cleared)
     if ((rc = make_maps(left < 0 ? std::min(page_size, 128) : 16)) != DTB_OK) return rc;
     const bool packed = cu_seqlens_q != nullptr;
-    CUtensorMap tq;
-    if ((rc = make_token_map(&tq, q, q_width, packed ? total_q : seqlen_q, q_tok_stride, packed ? 1 : nseg, q_batch_stride, &p.q_batch_first, "q")) != DTB_OK) return rc;
-    // blocks of 256 rows: as many as fit the rows that there are, and room for the parts
-    const int64_t per_seq = (seqlen_q + 255) / 256, in_rows = total_q / 256 + nseg;
-    p.planned = paged_planned(nseg, total_q, num_heads);
-    const int64_t blocks = p.planned ? std::min(nseg * per_seq, in_rows) * num_heads + plan.states : nseg * per_seq * num_heads;
+    dtb::PagedParams t = p;
+    dtb::QueryMap tq;
+    tq.dim_shift = mk.dim_shift;
+    tq.pack_shift = t.pack_shift = plan.pack_shift;
+    if ((rc = make_query_map(&tq.map, q, head_dim, num_heads, packed ? total_q : seqlen_q, q_tok_stride, packed ? 1 : nseg, q_batch_stride, 1 << plan.pack_shift,
+                             &t.q_batch_first)) != DTB_OK) return rc;
+    t.f.num_heads = num_heads >> plan.pack_shift;
+    t.f.seqlen_q = seqlen_q << plan.pack_shift;
+    t.f.total_q = total_q << plan.pack_shift;
+    // the grid: places for the blocks and for the parts
+    t.planned = paged_planned(plan, nseg, total_q, num_heads);
+    const int64_t per_seq = (static_cast<int64_t>(t.f.seqlen_q) + 255) / 256 * nseg * t.f.num_heads;
+    const int64_t blocks = t.planned ? std::min(per_seq, paged_blocks(plan, nseg, total_q, num_heads)) + plan.states : per_seq;
     if (blocks >= (1ll << 31)) return fail(DTB_ERR_ARG, "%s: too many blocks of rows", kWhat);
-    p.blocks = static_cast<int>(blocks);
-    p.ctas = d->sm_count;
-    p.most_states = p.planned ? plan.states : 0;
-    p.parts = p.f;
-    p.parts.out = scratch;
-    p.parts.lse = static_cast<float*>(scratch) + plan.states * 256ll * head_dim;
-    p.joins = reinterpret_cast<dtb::TileJoin*>(p.parts.lse + plan.states * 256ll);
-    p.parts.out_dtype = DTB_F32;
-    p.parts.out_tok_stride = head_dim;
-    p.parts.num_heads = 1;
-    p.parts.lse_layout = DTB_LSE_BSH;
-    p.parts.accumulate = 0;
-    e = head_dim == 64 ? dtb::launch_paged_tiles<64>(tq, mk, mv, p, s) : dtb::launch_paged_tiles<128>(tq, mk, mv, p, s);
-    if (e == cudaSuccess && p.most_states > 0) e = head_dim == 64 ? dtb::launch_tile_join<64>(p, s) : dtb::launch_tile_join<128>(p, s);
+    t.blocks = static_cast<int>(blocks);
+    t.ctas = d->sm_count;
+    t.most_states = t.planned ? plan.states : 0;
+    t.parts.out = scratch;
+    t.parts.lse = static_cast<float*>(scratch) + plan.states * 256ll * head_dim;
+    t.joins = reinterpret_cast<dtb::TileJoin*>(t.parts.lse + plan.states * 256ll);
+    e = head_dim == 64 ? dtb::launch_paged_tiles<64>(tq, mk, mv, t, s) : dtb::launch_paged_tiles<128>(tq, mk, mv, t, s);
+    if (e == cudaSuccess && t.most_states > 0) {
+      t.f = t.real;
+      e = head_dim == 64 ? dtb::launch_tile_join<64>(t, s) : dtb::launch_tile_join<128>(t, s);
+    }
   }
   if (e == cudaSuccess && (!plan.tiles || mixed)) {
     if ((rc = make_maps(std::min(page_size, 64))) != DTB_OK) return rc;

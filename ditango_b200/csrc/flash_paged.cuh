@@ -9,7 +9,11 @@
 
 namespace dtb {
 
+// The kernel of tiles takes the rows of 1 << pack_shift query heads that share a key head as those of one: row r of a sequence is query
+// r >> pack_shift and head (r & ((1 << pack_shift) - 1)) of them.  Its f.num_heads, f.seqlen_q and f.total_q count so; `real` does not.
 struct PagedParams : WindowParams {    // (k, v, their strides, cu_k and k_start are not used; seqlens_k is given always)
+  int pack_shift;
+  FlashParams real;
   const int32_t* table;                // [sequences, columns]
   int columns, pages, page_shift;
   int box_rows;                        // tokens of a tile that one load fetches; divides a page, so that no load crosses one
@@ -41,16 +45,17 @@ __device__ __forceinline__ int key_align(const PagedParams& p) { return p.key_al
 
 __device__ __forceinline__ int paged_keys(const PagedParams& p, int seg) { return max(min(p.seqlens_k[seg], p.columns << p.page_shift), 0); }
 
-// The tile kernel's view of a sequence.  Its keys are numbered through all sequences, seg * columns * P + j.
+// A sequence.  Its keys are numbered through all sequences, seg * columns * P + j.
 __device__ __forceinline__ WindowSeq paged_seq(const PagedParams& p, int seg) {
   WindowSeq s;
+  const int longest = p.f.seqlen_q >> p.pack_shift;
   s.q_begin = 0;
-  s.q_len = p.f.seqlen_q;
+  s.q_len = longest;
   if (p.f.cu_q != nullptr) {
     // (what offsets say beyond the rows that there are is not followed)
-    const int total = static_cast<int>(p.f.total_q);
+    const int total = static_cast<int>(p.f.total_q >> p.pack_shift);
     s.q_begin = min(max(p.f.cu_q[seg], 0), total);
-    s.q_len = max(min(min(max(p.f.cu_q[seg + 1], 0), total) - s.q_begin, p.f.seqlen_q), 0);
+    s.q_len = max(min(min(max(p.f.cu_q[seg + 1], 0), total) - s.q_begin, longest), 0);
   }
   s.k_begin = seg * (p.columns << p.page_shift);
   s.k_len = paged_keys(p, seg);
@@ -63,8 +68,11 @@ __device__ __forceinline__ WindowSeq paged_seq(const PagedParams& p, int seg) {
 __device__ __forceinline__ WindowSeq window_seq(const PagedParams& p, int seg) {
   WindowSeq s = paged_seq(p, seg);
   if (s.q_len <= p.few_rows) s.q_len = 0;
+  s.q_begin <<= p.pack_shift;
+  s.q_len <<= p.pack_shift;
   return s;
 }
+__device__ __forceinline__ int row_shift(const PagedParams& p) { return p.pack_shift; }
 
 __device__ __forceinline__ void tma_load_4d(void* smem_dst, const CUtensorMap* m, uint64_t* bar, int x, int a, int b, int page) {
   asm volatile(
@@ -74,6 +82,18 @@ __device__ __forceinline__ void tma_load_4d(void* smem_dst, const CUtensorMap* m
 }
 
 __device__ __forceinline__ void prefetch_tmap(const PagedMap* m) { prefetch_tmap(&m->map); }
+
+// A tensor map of the queries [channel, head, token, batch] (batch before token where that has the smaller stride); a box is 64 channels of
+// the rows of a tile, that is, of 1 << pack_shift heads of 128 >> pack_shift tokens.
+struct alignas(64) QueryMap {
+  CUtensorMap map;
+  int dim_shift, pack_shift;
+};
+__device__ __forceinline__ void prefetch_tmap(const QueryMap* m) { prefetch_tmap(&m->map); }
+__device__ __forceinline__ void tma_load_token(void* smem_dst, const QueryMap* m, uint64_t* bar, int x, int row, int batch, int batch_first) {
+  const int token = row >> m->pack_shift;
+  tma_load_4d(smem_dst, &m->map, bar, x & ((1 << m->dim_shift) - 1), (x >> m->dim_shift) << m->pack_shift, batch_first ? batch : token, batch_first ? token : batch);
+}
 
 // Loads of tiles over pages.  The thread that walks a block's tiles asks for them, and two warps that have no other role look the pages up and
 // issue the loads, a lane to each 64 channels of a box.  (One thread that does all of it is what bounds a launch: 16 loads of 2 KB and 8
@@ -179,7 +199,7 @@ __device__ __forceinline__ int row_block_of(const TilePlan& plan, int seq, int i
   return n > 0 ? i % n : -n - 1 - i % -n;
 }
 
-// Steps of 128 keys that the rows i0 to i1 walk.
+// Steps of 128 keys that the queries i0 to i1 walk.
 __device__ __forceinline__ int block_steps(const WindowSeq& s, int i0, int i1) {
   const WindowSpan a = window_span(s, i0), z = window_span(s, i1);
   const int lo = max(a.lo, min(s.sinks, z.hi));
@@ -228,7 +248,7 @@ __device__ __forceinline__ void plan_blocks(const PagedParams& p) {
     q_len = s.q_len;
     blocks = (q_len + 255) / 256;
     if (blocks > 0) {
-      const int a = block_steps(s, 0, min(q_len, 256) - 1), z = block_steps(s, (blocks - 1) * 256, q_len - 1);
+      const int a = block_steps(s, 0, (min(q_len, 256) - 1) >> p.pack_shift), z = block_steps(s, ((blocks - 1) * 256) >> p.pack_shift, (q_len - 1) >> p.pack_shift);
       longest = max(max(a, z), 1);
       rising = z > a;
       steps = 0.5f * (a + z);
@@ -354,14 +374,137 @@ __device__ __forceinline__ void place_results(const PagedParams&, Item& w, int s
   w.head = 0;
   w.q_begin = state * 256 - w.q0;
 }
-template <class Item>
-__device__ __forceinline__ bool is_part(const PagedParams&, const Item& w) { return w.part != 0; }
-__device__ __forceinline__ const FlashParams& parts_of(const PagedParams& p) { return p.parts; }
 
-// Tiles of 128: q [heads * D, tokens, batch] as for the dense kernel.
+// Where row R of a head (of the tile kernel's, counted through all sequences' rows) is in the results.
+struct RowPlace {
+  const FlashParams& f;
+  int shift, head0;                    // first of the heads that share rows
+
+  __device__ __forceinline__ RowPlace(const PagedParams& p, int head) : f(p.real), shift(p.pack_shift), head0(head << p.pack_shift) {}
+  __device__ __forceinline__ int head(int64_t R) const { return head0 + (static_cast<int>(R) & ((1 << shift) - 1)); }
+  template <int D>
+  __device__ __forceinline__ int64_t out(int64_t R) const { return (R >> shift) * f.out_tok_stride + static_cast<int64_t>(head(R)) * D; }
+  // `row` of its sequence
+  __device__ __forceinline__ int64_t lse(int64_t R, int seg, int row) const { return flash::lse_index(f, seg, head(R), row >> shift, R >> shift); }
+};
+
+// The results of a block that sees no key, by one thread, as the dense kernel's write_none.
+struct PagedResults {
+  const PagedParams& p;
+};
+template <class Item>
+__device__ __forceinline__ PagedResults results_at(const PagedParams& p, const Item&) { return PagedResults{p}; }
+template <int D, class Item>
+__device__ __forceinline__ void write_none(const PagedResults& r, const Item& w, const uint8_t* zeros) {
+  const PagedParams& p = r.p;
+  const RowPlace at(p, w.head);
+  if (w.part == 0 && p.f.accumulate) return;
+  const int size = p.f.out_dtype == 0 ? 4 : 2;
+#pragma unroll 1
+  for (int i = w.q0; i < min(w.q0 + 256, w.q_len); ++i) {
+    const int64_t R = static_cast<int64_t>(w.q_begin) + i;
+    if (w.part != 0) {
+      p.parts.lse[R] = -INFINITY;
+      bulk_store(static_cast<float*>(p.parts.out) + R * D, zeros, D * 4);
+    } else {
+      p.f.lse[at.lse(R, w.seg, i)] = -INFINITY;
+      bulk_store(static_cast<uint8_t*>(p.f.out) + at.out<D>(R) * size, zeros, D * size);
+    }
+  }
+  bulk_store_commit();
+}
+
+// The results of a warp's 32 rows, from row `pos` of the sequence: normalised, merged with the state in memory where the launch accumulates,
+// stored; a part's state is fp32, 256 rows one after another.  `ready` waits for the rows and gives this lane's reference and sum,
+// `read` says that O is not needed any more.  Rows go through shared memory (4 KB of the warp's, 16-byte pieces XOR-swizzled by row), so
+// that 8 lanes write 128 contiguous bytes.
+template <int D, class Ready, class Read>
+__device__ __forceinline__ bool paged_results(const PagedParams& p, bool part, int seg, int head, int pos, int q_begin, int q_len, uint32_t o_taddr, uint8_t* stage,
+                                              const Ready& ready, const Read& read) {
+  using namespace flash;
+  const int lane = threadIdx.x & 31, r0 = lane >> 3, piece = lane & 7, rows = q_len - pos;
+  const int64_t R0 = static_cast<int64_t>(q_begin) + pos;
+  const RowPlace at(p, head);
+  const float c = p.f.scale_log2;
+  const bool accumulate = !part && p.f.accumulate != 0;
+  const int64_t li = part ? R0 + lane : at.lse(R0 + lane, seg, pos + lane);
+  float* lse = part ? p.parts.lse : p.f.lse;
+  float lse_old = -INFINITY;
+  if (accumulate && lane < rows) lse_old = lse[li];     // under way while the rows are still being computed
+  float2 ml;
+  if (!ready(ml)) return false;
+  // a row that has seen no key is an empty state, and leaves a state that it is folded into as it is (a NaN among its scores is not that)
+  float w_new = 0.f, w_old = lse_old != -INFINITY ? 1.f : 0.f, lse_out = lse_old;
+  if (ml.y != 0.f) merge_weights(accumulate, lse_old, (ml.x * c + log2f(ml.y)) * kLn2, ml.y, w_new, w_old, lse_out);
+  if (lane < rows) lse[li] = lse_out;
+  if (!part && p.f.out_dtype != 0) {
+    uint16_t* dst = static_cast<uint16_t*>(p.f.out) + piece * 8;
+#pragma unroll 1
+    for (int x = 0; x < D / 64; ++x) {
+      uint32_t row[32];
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        uint32_t v[32];
+        tmem_ld32(o_taddr + x * 64 + q * 32, v);
+        tmem_wait_ld<32>(v);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) row[q * 16 + i] = pack_bf16x2(__uint_as_float(v[2 * i]) * w_new, __uint_as_float(v[2 * i + 1]) * w_new);
+      }
+      if (x == D / 64 - 1) read();
+      if (rows <= 0) continue;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        *reinterpret_cast<uint4*>(stage + lane * 128 + ((i ^ (lane & 7)) << 4)) = make_uint4(row[4 * i], row[4 * i + 1], row[4 * i + 2], row[4 * i + 3]);
+      __syncwarp();
+#pragma unroll
+      for (int it = 0; it < 8; ++it) {
+        const int r = it * 4 + r0;
+        const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 128 + ((piece ^ (r & 7)) << 4));
+        if (r < rows) *reinterpret_cast<uint4*>(dst + at.out<D>(R0 + r) + x * 64) = v;
+      }
+      __syncwarp();        // the stage is written again for the next columns
+    }
+    return true;
+  }
+  float* dst = static_cast<float*>(part ? p.parts.out : p.f.out) + piece * 4;
+#pragma unroll 1
+  for (int q = 0; q < D / 32; ++q) {
+    uint32_t row[32];
+    tmem_ld32(o_taddr + q * 32, row);
+    tmem_wait_ld<32>(row);
+    if (q == D / 32 - 1) read();
+    if (rows <= 0) continue;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      *reinterpret_cast<float4*>(stage + lane * 128 + ((i ^ (lane & 7)) << 4)) =
+          make_float4(__uint_as_float(row[4 * i]) * w_new, __uint_as_float(row[4 * i + 1]) * w_new, __uint_as_float(row[4 * i + 2]) * w_new,
+                      __uint_as_float(row[4 * i + 3]) * w_new);
+    __syncwarp();
+#pragma unroll
+    for (int it = 0; it < 8; ++it) {
+      const int r = it * 4 + r0;
+      float4 v = *reinterpret_cast<const float4*>(stage + r * 128 + ((piece ^ (r & 7)) << 4));
+      float4* to = reinterpret_cast<float4*>(dst + (part ? (R0 + r) * D : at.out<D>(R0 + r)) + q * 32);
+      if (accumulate) {
+        const float wo = __shfl_sync(0xffffffffu, w_old, r);
+        if (r < rows && wo != 0.f) {
+          const float4 old = *to;
+          v.x = fmaf(old.x, wo, v.x);
+          v.y = fmaf(old.y, wo, v.y);
+          v.z = fmaf(old.z, wo, v.z);
+          v.w = fmaf(old.w, wo, v.w);
+        }
+      }
+      if (r < rows) *to = v;
+    }
+    __syncwarp();
+  }
+  return true;
+}
+
 template <int D>
-cudaError_t launch_paged_tiles(const CUtensorMap& tm_q, const PagedMap& tm_k, const PagedMap& tm_v, const PagedParams& p, cudaStream_t stream);
-// ... and, behind that launch, the join of the parts of blocks whose keys it split.
+cudaError_t launch_paged_tiles(const QueryMap& tm_q, const PagedMap& tm_k, const PagedMap& tm_v, const PagedParams& p, cudaStream_t stream);
+// ... and, behind that launch, the join of the parts of blocks whose keys it split (with p.f as it is in p.real).
 template <int D>
 cudaError_t launch_tile_join(const PagedParams& p, cudaStream_t stream);
 

@@ -703,7 +703,8 @@ __global__ void __launch_bounds__(256) flash_tile_join_kernel(const __grid_const
     for (int k = 0; k < kCols; ++k) s_row[warp][lane * kCols + k] = acc[k];
     __syncwarp();
     if (lane < D / 4)          // (the maximum in units of raw scores, as store_row4 takes it)
-      store_row4<D>(p, j.seg, j.q_begin, j.q0 + r, j.head, lane * 4, *reinterpret_cast<const float4*>(&s_row[warp][lane * 4]),
+      store_row4<D>(p, j.seg, j.q_begin >> p.pack_shift, (j.q0 + r) >> p.pack_shift, (j.head << p.pack_shift) + ((j.q0 + r) & ((1 << p.pack_shift) - 1)), lane * 4,
+                    *reinterpret_cast<const float4*>(&s_row[warp][lane * 4]),
                     top / (p.f.scale_log2 * kLn2), sum, lane == 0, D == 128 ? 0xffffffffu : 0xffffu);
     __syncwarp();
   }

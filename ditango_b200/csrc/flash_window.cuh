@@ -67,12 +67,12 @@ __device__ __forceinline__ WindowSeq window_seq(const WindowParams& p, int seg) 
 __device__ __forceinline__ int key_align(const WindowParams&) { return 1; }
 // Which block a CTA's place in the grid stands for: row block, head, sequence x parts, and the parts that its keys are split into.
 __device__ __forceinline__ void place_block(const WindowParams&, int&, int&, int&, int&, int&) {}
-// A block's results go to p.f, whichever part of its keys it has.
+// Rows are queries (here: times 1 << 0 heads), and where a block's results go, whichever part of its keys it has.
+__device__ __forceinline__ constexpr int row_shift(const WindowParams&) { return 0; }
 template <class Item>
 __device__ __forceinline__ void place_results(const WindowParams&, Item&, int) {}
 template <class Item>
-__device__ __forceinline__ constexpr bool is_part(const WindowParams&, const Item&) { return false; }
-__device__ __forceinline__ const FlashParams& parts_of(const WindowParams& p) { return p.f; }
+__device__ __forceinline__ const FlashParams& results_at(const WindowParams& p, const Item&) { return p.f; }
 
 // Keys that query i sees: [0, first) and [lo, hi), first <= lo <= hi.  A key at position j is seen from position x when
 // j <= x + right and (j >= x - left or j < sinks).

@@ -41,6 +41,7 @@
 #include "flash_window.cuh"
 
 #include <mutex>
+#include <type_traits>
 
 namespace dtb {
 
@@ -96,8 +97,8 @@ struct Walk {
   int steps;          // steps in all; 0: nothing to see (such a block only the loader meets), -1: no more blocks
 
   // for the rows i0 to i1
-  __device__ __forceinline__ void plan(int from, int to, int sinks, int k_end, int k_floor, int i0, int i1, int align) {
-    auto span = [&](int i) { return window_span(from, to, sinks, k_end, k_floor, i); };
+  __device__ __forceinline__ void plan(int from, int to, int sinks, int k_end, int k_floor, int i0, int i1, int align, int shift) {
+    auto span = [&](int i) { return window_span(from, to, sinks, k_end, k_floor, i >> shift); };
     const WindowSpan a = span(i0), z = span(i1);
     first = z.first;
     lo = max(a.lo, min(k_floor, z.hi));
@@ -262,9 +263,9 @@ __device__ __forceinline__ bool claim_answer(const void* response16, int& x, int
 
 // grid: (row blocks, heads, sequences x parts); in pages as plan_blocks deals them out.  Keys and values dense (CUtensorMap, WindowParams) or in pages (PagedMap, PagedParams): the two
 // differ in how a sequence and a tile's rows are found.
-template <int D, class Map, class Params>
+template <int D, class QMap, class Map, class Params>
 __global__ void __launch_bounds__(kThreads, 1)
-flash_window_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ Map tm_k,
+flash_window_kernel(const __grid_constant__ QMap tm_q, const __grid_constant__ Map tm_k,
                     const __grid_constant__ Map tm_v, const __grid_constant__ Params p) {
   using C = Cfg<D>;
   constexpr int NB = C::kSBufs;
@@ -395,7 +396,7 @@ flash_window_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
           asked = false;
           if (w.q0 < w.q_len) {
             const int i1 = min(w.q0 + kQT * kBM, w.q_len) - 1;
-            w.walk.plan(w.from, w.to, w.sinks, w.k_end, w.k_floor, w.q0, i1, key_align(p));
+            w.walk.plan(w.from, w.to, w.sinks, w.k_end, w.k_floor, w.q0, i1, key_align(p), row_shift(p));
             if (splits > 1) {
               // as many tiles to each part, the first tokens to the last one
               const int begin = w.walk.lo, end = begin + w.walk.win;
@@ -406,14 +407,14 @@ flash_window_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
                 w.k_end = min(begin + (part + 1) * keys, end);
                 w.sinks = 0;
               }
-              w.walk.plan(w.from, w.to, w.sinks, w.k_end, w.k_floor, w.q0, i1, key_align(p));
+              w.walk.plan(w.from, w.to, w.sinks, w.k_end, w.k_floor, w.q0, i1, key_align(p), row_shift(p));
             }
             const Walk walk = w.walk;
             const int n_units = 2 * walk.steps;
             if (n_units == 0) {
               // The other roles do not meet it.  (The issuer asks for the block behind the one under way before it ends that one: with
               // a run of such blocks in between, more than there are slots, each role would wait for another.)
-              write_none<D>(is_part(p, w) ? parts_of(p) : p.f, w, sh.s_zero);
+              write_none<D>(results_at(p, w), w, sh.s_zero);
             } else {
               if (!publish(w)) break;
               const int qb = items % C::kQBufs, q_round = items / C::kQBufs;
@@ -676,110 +677,84 @@ flash_window_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       for (int slot; (slot = fetch_warp(sh)) >= 0;) {
         const int q0 = sh.s_work[slot].q0, head = sh.s_work[slot].head, seg = sh.s_work[slot].seg;
         const int q_begin = sh.s_work[slot].q_begin, q_len = sh.s_work[slot].q_len;
-        const bool part = is_part(p, sh.s_work[slot]);
+        const int part = sh.s_work[slot].part;
         give_back(sh, slot);
         bool ok = true;
-        if (part) {
-          // a part's state: fp32, 256 rows one after another, nothing to fold into
+        if constexpr (std::is_same<Params, PagedParams>::value) {
+          for (int tile = 0; ok && tile < kQT; ++tile)
+            ok = paged_results<D>(p, part != 0, seg, head, q0 + tile * kBM + quarter * 32, q_begin, q_len, lane_base + C::kColO + tile * D, stage, [&](float2& ml) {
+              if (!warp_wait_or_abort(&sh.ml_full[tile], item_use, p.f.status, 42)) return false;
+              ml = sh.s_ml[tile * kBM + quarter * 32 + lane];
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&sh.ml_empty[tile]);
+              if (!warp_wait_or_abort(&sh.o_final[tile], item_use, p.f.status, 41)) return false;
+              tc_fence_after();
+              return true;
+            }, [&]() {
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&sh.o_free[tile]);
+            });
+        } else {
 #pragma unroll 1
           for (int tile = 0; ok && tile < kQT; ++tile) {
+            const uint32_t o_taddr = lane_base + C::kColO + tile * D;
+            const int warp_pos = q0 + tile * kBM + quarter * 32;      // position of the warp's first row
+            const int rows = q_len - warp_pos;
+            const int64_t tok0 = static_cast<int64_t>(q_begin) + warp_pos;
+            const int64_t li = lse_index(p.f, seg, head, warp_pos + lane, tok0 + lane);
+            const int64_t col = static_cast<int64_t>(head) * D;
+            float lse_old = -INFINITY;
+            if (accumulate && lane < rows) lse_old = p.f.lse[li];     // under way while the rows are still being computed
             ok = warp_wait_or_abort(&sh.ml_full[tile], item_use, p.f.status, 42);
             if (!ok) break;
             const float2 ml = sh.s_ml[tile * kBM + quarter * 32 + lane];
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.ml_empty[tile]);
+            // a row that has seen no key is an empty state, and leaves a state that it is folded into as it is (a NaN among its scores is not that)
+            float w_new = 0.f, w_old = lse_old != -INFINITY ? 1.f : 0.f, lse_out = lse_old;
+            if (ml.y != 0.f) merge_weights(accumulate, lse_old, (ml.x * c + log2f(ml.y)) * kLn2, ml.y, w_new, w_old, lse_out);
             ok = warp_wait_or_abort(&sh.o_final[tile], item_use, p.f.status, 41);
             if (!ok) break;
             tc_fence_after();
-            const int64_t row0 = static_cast<int64_t>(q_begin) + q0 + tile * kBM + quarter * 32;
-            const FlashParams& f = parts_of(p);
-            const float w = ml.y != 0.f ? 1.f / ml.y : 0.f;
-            f.lse[row0 + lane] = ml.y != 0.f ? (ml.x * c + log2f(ml.y)) * kLn2 : -INFINITY;
-            float* dst = static_cast<float*>(f.out) + row0 * D;
+            if (lane < rows) p.f.lse[li] = lse_out;
+            auto o_read = [&]() {
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&sh.o_free[tile]);
+            };
+            if (p.f.out_dtype != 0) {
+              // bf16: 64 columns at a time, rounded as they are read, so that the next block's products do not wait long for O.  (A block of
+              // 25 steps, D = 64 and 128: 35.5 and 55.0 us; 36.6 and 54.8 with 32 fp32 columns staged at a time, 36.5 and 56.0 with
+              // every lane storing its row from registers.)
+              uint16_t* dst = static_cast<uint16_t*>(p.f.out) + tok0 * p.f.out_tok_stride + col;
 #pragma unroll 1
+              for (int x = 0; x < D / 64; ++x) {
+                uint32_t orow[32];
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                  uint32_t v[32];
+                  tmem_ld32(o_taddr + x * 64 + q * 32, v);
+                  tmem_wait_ld<32>(v);
+#pragma unroll
+                  for (int i = 0; i < 16; ++i)
+                    orow[q * 16 + i] = pack_bf16x2(__uint_as_float(v[2 * i]) * w_new, __uint_as_float(v[2 * i + 1]) * w_new);
+                }
+                if (x == D / 64 - 1) o_read();
+                if (rows > 0) store_rows64_bf16(stage, dst + x * 64, p.f.out_tok_stride, rows, orow);
+              }
+              continue;
+            }
+#pragma unroll
             for (int q = 0; q < D / 32; ++q) {
               uint32_t orow[32];
-              tmem_ld32(lane_base + C::kColO + tile * D + q * 32, orow);
+              tmem_ld32(o_taddr + q * 32, orow);
               tmem_wait_ld<32>(orow);
-              if (q == D / 32 - 1) {
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sh.o_free[tile]);
-              }
-#pragma unroll
-              for (int i = 0; i < 8; ++i)
-                *reinterpret_cast<float4*>(stage + lane * 128 + ((i ^ (lane & 7)) << 4)) =
-                    make_float4(__uint_as_float(orow[4 * i]) * w, __uint_as_float(orow[4 * i + 1]) * w, __uint_as_float(orow[4 * i + 2]) * w,
-                                __uint_as_float(orow[4 * i + 3]) * w);
-              __syncwarp();
-#pragma unroll 1
-              for (int r = lane >> 3; r < 32; r += 4)
-                *reinterpret_cast<float4*>(dst + r * D + q * 32 + (lane & 7) * 4) = *reinterpret_cast<const float4*>(stage + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
-              __syncwarp();
+              if (q == D / 32 - 1) o_read();
+              OldRows old;
+              if (accumulate) load_old_rows32(p.f, tok0, rows, col + q * 32, old);
+              if (rows > 0) store_rows32(p.f, stage, tok0, rows, col + q * 32, orow, old, w_new, w_old);
             }
-          }
-          if (!ok) break;
-          item_use ^= 1;
-          continue;
-        }
-#pragma unroll 1
-        for (int tile = 0; ok && tile < kQT; ++tile) {
-          const uint32_t o_taddr = lane_base + C::kColO + tile * D;
-          const int warp_pos = q0 + tile * kBM + quarter * 32;      // position of the warp's first row
-          const int rows = q_len - warp_pos;
-          const int64_t tok0 = static_cast<int64_t>(q_begin) + warp_pos;
-          const int64_t li = lse_index(p.f, seg, head, warp_pos + lane, tok0 + lane);
-          const int64_t col = static_cast<int64_t>(head) * D;
-          float lse_old = -INFINITY;
-          if (accumulate && lane < rows) lse_old = p.f.lse[li];     // under way while the rows are still being computed
-          ok = warp_wait_or_abort(&sh.ml_full[tile], item_use, p.f.status, 42);
-          if (!ok) break;
-          const float2 ml = sh.s_ml[tile * kBM + quarter * 32 + lane];
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sh.ml_empty[tile]);
-          // a row that has seen no key is an empty state, and leaves a state that it is folded into as it is (a NaN among its scores is not that)
-          float w_new = 0.f, w_old = lse_old != -INFINITY ? 1.f : 0.f, lse_out = lse_old;
-          if (ml.y != 0.f) merge_weights(accumulate, lse_old, (ml.x * c + log2f(ml.y)) * kLn2, ml.y, w_new, w_old, lse_out);
-          ok = warp_wait_or_abort(&sh.o_final[tile], item_use, p.f.status, 41);
-          if (!ok) break;
-          tc_fence_after();
-          if (lane < rows) p.f.lse[li] = lse_out;
-          auto o_read = [&]() {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.o_free[tile]);
-          };
-          if (p.f.out_dtype != 0) {
-            // bf16: 64 columns at a time, rounded as they are read, so that the next block's products do not wait long for O.  (A block of
-            // 25 steps, D = 64 and 128: 35.5 and 55.0 us; 36.6 and 54.8 with 32 fp32 columns staged at a time, 36.5 and 56.0 with
-            // every lane storing its row from registers.)
-            uint16_t* dst = static_cast<uint16_t*>(p.f.out) + tok0 * p.f.out_tok_stride + col;
-#pragma unroll 1
-            for (int x = 0; x < D / 64; ++x) {
-              uint32_t orow[32];
-#pragma unroll
-              for (int q = 0; q < 2; ++q) {
-                uint32_t v[32];
-                tmem_ld32(o_taddr + x * 64 + q * 32, v);
-                tmem_wait_ld<32>(v);
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                  orow[q * 16 + i] = pack_bf16x2(__uint_as_float(v[2 * i]) * w_new, __uint_as_float(v[2 * i + 1]) * w_new);
-              }
-              if (x == D / 64 - 1) o_read();
-              if (rows > 0) store_rows64_bf16(stage, dst + x * 64, p.f.out_tok_stride, rows, orow);
-            }
-            continue;
-          }
-#pragma unroll
-          for (int q = 0; q < D / 32; ++q) {
-            uint32_t orow[32];
-            tmem_ld32(o_taddr + q * 32, orow);
-            tmem_wait_ld<32>(orow);
-            if (q == D / 32 - 1) o_read();
-            OldRows old;
-            if (accumulate) load_old_rows32(p.f, tok0, rows, col + q * 32, old);
-            if (rows > 0) store_rows32(p.f, stage, tok0, rows, col + q * 32, orow, old, w_new, w_old);
           }
         }
         if (!ok) break;
@@ -810,7 +785,7 @@ flash_window_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
           left = w.walk.steps;
           window = w.walk.n;
           // (a row behind the last one sees what the last one sees)
-          const WindowSpan span = window_span(w.from, w.to, w.sinks, w.k_end, w.k_floor, min(w.q0 + tile * kBM + quarter * 32 + lane, w.q_len - 1));
+          const WindowSpan span = window_span(w.from, w.to, w.sinks, w.k_end, w.k_floor, min(w.q0 + tile * kBM + quarter * 32 + lane, w.q_len - 1) >> row_shift(p));
           const int base = w.walk.lo + ((w.walk.N - window) & tile) * kBN;
           c0 = span.lo - base;
           c1 = span.hi - base;
@@ -951,12 +926,12 @@ flash_window_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
 static dim3 tile_grid(const WindowParams& p) { return dim3((p.f.seqlen_q + kQT * kBM - 1) / (kQT * kBM), p.f.num_heads, p.f.nseg * p.splits); }
 static dim3 tile_grid(const PagedParams& p) { return dim3(p.blocks); }
 
-template <int D, class Map, class Params>
-static cudaError_t launch_tiles(const CUtensorMap& tq, const Map& tk, const Map& tv, const Params& p, cudaStream_t stream) {
+template <int D, class QMap, class Map, class Params>
+static cudaError_t launch_tiles(const QMap& tq, const Map& tk, const Map& tv, const Params& p, cudaStream_t stream) {
   using C = Cfg<D>;
   static bool configured[64] = {};
   static std::mutex mu;
-  const auto kernel = flash_window_kernel<D, Map, Params>;
+  const auto kernel = flash_window_kernel<D, QMap, Map, Params>;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
@@ -981,13 +956,13 @@ cudaError_t launch_window_tiles(const CUtensorMap& tq, const CUtensorMap& tk, co
   return launch_tiles<D>(tq, tk, tv, p, stream);
 }
 template <int D>
-cudaError_t launch_paged_tiles(const CUtensorMap& tq, const PagedMap& tk, const PagedMap& tv, const PagedParams& p, cudaStream_t stream) {
+cudaError_t launch_paged_tiles(const QueryMap& tq, const PagedMap& tk, const PagedMap& tv, const PagedParams& p, cudaStream_t stream) {
   return launch_tiles<D>(tq, tk, tv, p, stream);
 }
 
 template cudaError_t launch_window_tiles<64>(const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, const WindowParams&, cudaStream_t);
 template cudaError_t launch_window_tiles<128>(const CUtensorMap&, const CUtensorMap&, const CUtensorMap&, const WindowParams&, cudaStream_t);
-template cudaError_t launch_paged_tiles<64>(const CUtensorMap&, const PagedMap&, const PagedMap&, const PagedParams&, cudaStream_t);
-template cudaError_t launch_paged_tiles<128>(const CUtensorMap&, const PagedMap&, const PagedMap&, const PagedParams&, cudaStream_t);
+template cudaError_t launch_paged_tiles<64>(const QueryMap&, const PagedMap&, const PagedMap&, const PagedParams&, cudaStream_t);
+template cudaError_t launch_paged_tiles<128>(const QueryMap&, const PagedMap&, const PagedMap&, const PagedParams&, cudaStream_t);
 
 }  // namespace dtb

@@ -289,10 +289,27 @@ SPLITS = [([300], [6000], 2, 1, -1, 0, 0), ([140, 1, 600], [9000, 4000, 700], 2,
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("new,lens,H,Hk,left,right,sinks", SPLITS)
 def test_blocks_whose_keys_are_split(new, lens, H, Hk, left, right, sinks, D):
-    """(129 rows and more of a key head to each query head: the kernel of few rows takes up to 128 / (H / Hk) queries)"""
+    """(the kernel of few rows takes up to 64 / (H / Hk) queries)"""
     cache = _Cache(lens, Hk, D, 64, seed=9)
     q = _rand((sum(new), H, D), 61)
     _attend(cache, q, new, left=left, right=right, sinks=sinks, out_dtype=torch.bfloat16 if H % 4 else torch.float32)
+
+
+# heads that share the rows of a tile: powers of two of them, and the power of two in other numbers; tokens around the ends of blocks
+SHARED = [([65], [700], 8, 8), ([33, 40], [500, 41], 16, 8), ([9, 17, 100, 1], [300, 17, 1000, 5], 16, 2), ([3, 70], [400, 300], 48, 2), ([2, 3], [129, 700], 64, 1),
+          ([1, 2, 5], [60, 2, 900], 128, 1), ([30], [2000], 12, 1), ([64, 65, 31], [64, 400, 333], 24, 6), ([40, 200], [40, 777], 5, 1), ([129], [1500], 6, 2)]
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("left,right,sinks", [(-1, 0, 0), (-1, -1, 0), (90, 20, 33), (3, 0, 0)])
+@pytest.mark.parametrize("packed", [True, False])
+@pytest.mark.parametrize("new,lens,H,Hk", SHARED)
+def test_heads_that_share_tiles(new, lens, H, Hk, packed, left, right, sinks, D):
+    if not packed:
+        new = [max(new)] * len(new)
+    cache = _Cache(lens, Hk, D, 32, layout="token" if H % 3 else "head", seed=14)
+    dtype = torch.bfloat16 if (H + left) % 2 else torch.float32
+    _attend(cache, _rand((sum(new), H, D), 68), new, left=left, right=right, sinks=sinks, packed=packed, out_dtype=dtype)
 
 
 @pytest.mark.parametrize("D", [64, 128])

@@ -30,7 +30,7 @@ using std::max; using std::min;
 constexpr int kQueriesLast = INT32_MIN;
 struct FlashParams { const int32_t *cu_q, *cu_k; int seqlen_q, seqlen_k, num_heads, nseg; int64_t total_q; };
 struct WindowParams { FlashParams f; const int32_t* seqlens_k; int kv_heads, left, right, sinks, q_start, k_start; };
-struct PagedParams : WindowParams { int columns, pages, page_shift, box_rows, key_align, few_rows; };
+struct PagedParams : WindowParams { int pack_shift = 0, columns, pages, page_shift, box_rows, key_align, few_rows; };
 %(seq)s
 %(span)s
 %(paged)s
