@@ -834,7 +834,7 @@ DTB_API int dtb_flash_paged_launches(int nseg, int seqlen_q, int seqlen_k, int64
   const PagedPlan plan = plan_paged(nseg, seqlen_q, seqlen_k, total_q, num_heads, num_kv_heads, head_dim, d->sm_count);
   int n = 0;
   if (plan.tiles) n += plan.states > 0 && paged_planned(plan, nseg, total_q, num_heads) ? 2 : 1;
-  if (!plan.tiles || paged_mixed(plan, packed != 0, nseg, seqlen_q, total_q)) n += 2;
+  if (!plan.tiles || paged_mixed(plan, packed != 0, nseg, seqlen_q, total_q)) n += plan.rows.cluster > 0 ? 1 : 2;
   return n;
 }
 
@@ -867,12 +867,12 @@ DTB_API int dtb_flash_paged(const void* q, int64_t q_tok_stride, int64_t q_batch
   if (lse_layout != DTB_LSE_BHS && lse_layout != DTB_LSE_BSH) return fail(DTB_ERR_ARG, "%s: bad lse_layout %d", kWhat, lse_layout);
   if (accumulate && out_dtype != DTB_F32) return fail(DTB_ERR_ARG, "%s: accumulate needs an fp32 state", kWhat);
   if (!(softmax_scale > 0.f)) return fail(DTB_ERR_ARG, "%s: softmax_scale must be positive", kWhat);
-  if (!scratch || !aligned16(scratch)) return fail(DTB_ERR_ARG, "%s: scratch must be given and 16-byte aligned", kWhat);
+  if (!aligned16(scratch)) return fail(DTB_ERR_ARG, "%s: scratch must be 16-byte aligned", kWhat);
   DeviceInfo* d = nullptr;
   if ((rc = device_info(&d)) != DTB_OK) return rc;
   if (seqlen_q == 0 || total_q == 0) return DTB_OK;
   const PagedPlan plan = plan_paged(nseg, seqlen_q, seqlen_k, total_q, num_heads, num_kv_heads, head_dim, d->sm_count);
-  if (scratch_bytes < plan.scratch_bytes)
+  if (scratch_bytes < plan.scratch_bytes || (!scratch && plan.scratch_bytes))
     return fail(DTB_ERR_ARG, "%s: scratch of %lld bytes is smaller than the %lld needed", kWhat, static_cast<long long>(scratch_bytes),
                 static_cast<long long>(plan.scratch_bytes));
 

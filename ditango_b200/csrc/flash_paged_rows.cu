@@ -8,6 +8,8 @@
 //     l' = l 2^(c (m - m')) + sum P,  O' = O 2^(c (m - m')) + P V
 // The states of the warps are joined in shared memory.  A block that one CTA has all tiles of is written as it is; the parts of one that several
 // CTAs have go to scratch, and a second launch, set up while this one runs, joins them in the order of their CTAs.
+// Small batches take one launch: a cluster of up to 8 CTAs to each block, which share its tiles out and join their states through distributed
+// shared memory, and nothing to add up beforehand.
 //
 // HBM-bound: a key and a value are read once for the rows of a block.  Warp 4 loads (TMA, 128-byte swizzle, every lane a page), warps
 // 0-3 compute with mma.sync, because 16 rows fill an instruction of it and a 128-row tile of tcgen05 would be empty for the most part.  With more
@@ -16,6 +18,9 @@
 #include "flash_common.cuh"
 #include "flash_paged.cuh"
 
+#include <cooperative_groups.h>
+
+#include <algorithm>
 #include <mutex>
 
 namespace dtb {
@@ -30,6 +35,7 @@ constexpr int kKeys = 64;                 // of a tile
 constexpr int kBlockCost = 2;             // places in front of a block's tiles
 constexpr int kMinPlaces = 2;             // of a CTA's share, unless there are fewer
 constexpr int kColumns = 32;              // joined at a time
+constexpr int kMostCluster = 8;
 constexpr int kPitch = kColumns + 8;      // floats of a row of them in shared memory (rows 8 banks apart)
 
 template <int D, int WM>
@@ -227,15 +233,21 @@ struct Scratch {
 
 }  // namespace
 
-template <int D, int WM>
+// grid: the CTAs that share all places out; with kCluster (row blocks x key heads x sequences) clusters, a row block of each sequence's `row_blocks`.
+template <int D, int WM, bool kCluster>
 __global__ void __launch_bounds__(kThreads, 2)
-flash_paged_rows_kernel(const __grid_constant__ PagedMap tm_k, const __grid_constant__ PagedMap tm_v, const __grid_constant__ PagedParams p, void* scratch) {
+flash_paged_rows_kernel(const __grid_constant__ PagedMap tm_k, const __grid_constant__ PagedMap tm_v, const __grid_constant__ PagedParams p, void* scratch,
+                        int row_blocks) {
+  namespace cg = cooperative_groups;
   using C = Cfg<D, WM>;
   constexpr int R = C::kRows, WN = C::kWN, KW = C::kWarpKeys;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023u);
   float* s_join = reinterpret_cast<float*>(smem + C::kStages * C::kStage);            // [warp of keys][row][kPitch]
   float2* s_ml = reinterpret_cast<float2*>(s_join + C::kJoin / 4);                     // [warp of keys][row]
+  float* s_state = reinterpret_cast<float*>(smem);                                     // of a cluster's CTA: O [row][D], (m, l) [row], over the ring
+  float2* s_state_ml = reinterpret_cast<float2*>(s_state + R * D);
+  static_assert(R * (D * 4 + 8) <= C::kStages * C::kStage, "states take the ring's place");
   uint64_t* full = reinterpret_cast<uint64_t*>(s_ml + WN * R);
   uint64_t* empty = full + C::kStages;
   __shared__ long long s_sum[kThreads / 32];
@@ -258,55 +270,77 @@ flash_paged_rows_kernel(const __grid_constant__ PagedMap tm_k, const __grid_cons
     prefetch_tmap(&tm_v);
   }
   // ------------------------------------------------------------------ this CTA's share
-  const int per = (p.f.nseg + kThreads - 1) / kThreads, seg0 = min(static_cast<int>(threadIdx.x) * per, p.f.nseg), seg1 = min(seg0 + per, p.f.nseg);
-  auto places = [&](const Seq& s) { return static_cast<long long>(s.blocks) * p.kv_heads * places_of(s); };
-  long long sum = 0;
-  Seq own;
-  for (int i = seg0; i < seg1; ++i) sum += places(own = make_seq<R>(p, i));
-  long long upto = sum;
-#pragma unroll
-  for (int d = 1; d < 32; d *= 2) {
-    const long long u = __shfl_up_sync(0xffffffffu, upto, d);
-    if (lane >= d) upto += u;
-  }
-  if (lane == 31) s_sum[warp] = upto;
-  // CTA-uniform view of the status word: a CTA that starts after a failure elsewhere does no work.
-  if (__syncthreads_or(*reinterpret_cast<volatile int*>(p.f.status) != 0)) return;
-  long long at = upto - sum, all = 0;
-#pragma unroll
-  for (int w = 0; w < kThreads / 32; ++w) {
-    if (w < warp) at += s_sum[w];
-    all += s_sum[w];
-  }
-  const Shares shares(all, gridDim.x);
+  int seg, unit, place;
+  long long left;                           // places
   const int cta = blockIdx.x;
-  if (cta >= shares.ctas) {
-    if (threadIdx.x == 0) sc.joins[cta].parts = 0;
-    return;
-  }
-  const long long begin = shares.begin(cta);
-  if (begin >= at && begin < at + sum) {
-    for (int i = seg0; i < seg1; ++i) {
-      if (per > 1) own = make_seq<R>(p, i);
-      if (begin < at + places(own)) {
-        s_seq = own;
-        s_seg = i;
-        s_unit = static_cast<int>(divide(begin - at, places_of(own)));
-        s_place = static_cast<int>(begin - at - static_cast<long long>(s_unit) * places_of(own));
-        break;
-      }
-      at += places(own);
+  Seq& s = s_seqs[warp];
+  if constexpr (kCluster) {
+    // (Nobody leaves here after a failure elsewhere: the others of its cluster wait for it.  Its waits end at once.)
+    const int ranks = static_cast<int>(cg::this_cluster().num_blocks()), rank = static_cast<int>(cg::this_cluster().block_rank());
+    int id = cta / ranks;
+    const int block = id % row_blocks;
+    id /= row_blocks;
+    seg = id / p.kv_heads;
+    const Seq own = make_seq<R>(p, seg);
+    if (block >= own.blocks) return;        // all CTAs of the cluster
+    unit = (id - seg * p.kv_heads) * own.blocks + block;
+    const int t0 = static_cast<int>(static_cast<int64_t>(own.tiles) * rank / ranks), t1 = static_cast<int>(static_cast<int64_t>(own.tiles) * (rank + 1) / ranks);
+    place = t0 + kBlockCost;
+    left = t1 - t0;
+    if (lane == 0) s = own;
+    __syncthreads();                        // the barriers are there
+  } else {
+    const int per = (p.f.nseg + kThreads - 1) / kThreads, seg0 = min(static_cast<int>(threadIdx.x) * per, p.f.nseg), seg1 = min(seg0 + per, p.f.nseg);
+    auto places = [&](const Seq& s) { return static_cast<long long>(s.blocks) * p.kv_heads * places_of(s); };
+    long long sum = 0;
+    Seq own;
+    for (int i = seg0; i < seg1; ++i) sum += places(own = make_seq<R>(p, i));
+    long long upto = sum;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      const long long u = __shfl_up_sync(0xffffffffu, upto, d);
+      if (lane >= d) upto += u;
     }
+    if (lane == 31) s_sum[warp] = upto;
+    // CTA-uniform view of the status word: a CTA that starts after a failure elsewhere does no work.
+    if (__syncthreads_or(*reinterpret_cast<volatile int*>(p.f.status) != 0)) return;
+    long long at = upto - sum, all = 0;
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) {
+      if (w < warp) at += s_sum[w];
+      all += s_sum[w];
+    }
+    const Shares shares(all, gridDim.x);
+    if (cta >= shares.ctas) {
+      if (threadIdx.x == 0) sc.joins[cta].parts = 0;
+      return;
+    }
+    const long long begin = shares.begin(cta);
+    if (begin >= at && begin < at + sum) {
+      for (int i = seg0; i < seg1; ++i) {
+        if (per > 1) own = make_seq<R>(p, i);
+        if (begin < at + places(own)) {
+          s_seq = own;
+          s_seg = i;
+          s_unit = static_cast<int>(divide(begin - at, places_of(own)));
+          s_place = static_cast<int>(begin - at - static_cast<long long>(s_unit) * places_of(own));
+          break;
+        }
+        at += places(own);
+      }
+    }
+    __syncthreads();
+    seg = s_seg;
+    unit = s_unit;
+    place = s_place;
+    left = shares.begin(cta + 1) - begin;
+    if (lane == 0) s = s_seq;
+    __syncwarp();
+    if (threadIdx.x == 0) sc.joins[cta] = make_join(shares, s, make_block<R>(p, s, unit), seg, cta, place);
   }
-  __syncthreads();
-
-  int seg = s_seg, unit = s_unit, place = s_place;
-  long long left = shares.begin(cta + 1) - begin;             // places
+  const int unit0 = unit;
   int stage = 0;
   uint32_t use = 0;                         // parity of the ring's round
-  Seq& s = s_seqs[warp];
-  if (lane == 0) s = s_seq;
-  __syncwarp();
   bool first_block = true;
   // the block's tiles that are this CTA's: up to, not with, this one
   auto last_tile = [&]() { return tiles_before(static_cast<int>(min(static_cast<long long>(places_of(s)), place + left))); };
@@ -369,11 +403,10 @@ flash_paged_rows_kernel(const __grid_constant__ PagedMap tm_k, const __grid_cons
     // ---------------------------------------------------------------- scores, weights, products
     const int wm = warp / WN, wn = warp % WN;
     const float c = p.f.scale_log2;
-    if (threadIdx.x == 0) sc.joins[cta] = make_join(shares, s, make_block<R>(p, s, unit), seg, cta, place);
     bool ok = true;             // after a wait that gave up, the blocks are walked to their barriers and nothing more is stored
-    while (left > 0) {
+    for (bool once = kCluster; once || left > 0; once = false) {
       const int tile = tiles_before(place), to = last_tile(), group = s.group;
-      if (tile == to) {                         // places in front of a block that the next CTA begins with
+      if (!kCluster && tile == to) {                         // places in front of a block that the next CTA begins with
         next_block();
         continue;
       }
@@ -521,7 +554,7 @@ flash_paged_rows_kernel(const __grid_constant__ PagedMap tm_k, const __grid_cons
         }
       }
       // join the warps that shared the keys, 32 columns at a time
-      const bool whole = tile == 0 && to == s.tiles;
+      const bool whole = !kCluster && tile == 0 && to == s.tiles;
       const int slot = 2 * cta + (first_block ? 0 : 1);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -564,6 +597,9 @@ flash_paged_rows_kernel(const __grid_constant__ PagedMap tm_k, const __grid_cons
           if (whole) {
             const int row = b.row0 + r;
             store_row4<D>(p, seg, s.w.q_begin, row / group, b.kv_head * group + row % group, x * kColumns + col, acc, mm, ll, last, mask);
+          } else if (kCluster) {
+            *reinterpret_cast<float4*>(s_state + r * D + x * kColumns + col) = acc;
+            if (last) s_state_ml[r] = make_float2(mm, ll);
           } else {
             *reinterpret_cast<float4*>(sc.o + (static_cast<int64_t>(slot) * R + r) * D + x * kColumns + col) = acc;
             if (last) sc.ml[static_cast<int64_t>(slot) * R + r] = make_float2(mm, ll);
@@ -575,6 +611,49 @@ flash_paged_rows_kernel(const __grid_constant__ PagedMap tm_k, const __grid_cons
     }
   }
   if (*reinterpret_cast<volatile int*>(p.f.status) != 0) __nanosleep(1000000);   // let copies in flight land
+  if constexpr (kCluster) {
+    // the CTAs' states, four columns of a row per thread, the rows dealt out over the cluster
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    const int ranks = static_cast<int>(cluster.num_blocks());
+    const Block b = make_block<R>(p, s, unit0);
+    const float c = p.f.scale_log2;
+    const bool stores = *reinterpret_cast<volatile int*>(p.f.status) == 0;
+    for (int u = static_cast<int>(cluster.block_rank()) * kThreads + threadIdx.x; u < b.rows * (D / 4); u += ranks * kThreads) {
+      const int r = u / (D / 4), col = u % (D / 4) * 4;
+      // (all reads of the other CTAs' memory are under way before one is used)
+      float2 ml[kMostCluster];
+      float4 v[kMostCluster];
+#pragma unroll
+      for (int i = 0; i < kMostCluster; ++i) {
+        ml[i] = make_float2(-INFINITY, 0.f);
+        v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (i < ranks) {
+          ml[i] = cluster.map_shared_rank(s_state_ml, i)[r];
+          v[i] = *reinterpret_cast<const float4*>(cluster.map_shared_rank(s_state, i) + r * D + col);
+        }
+      }
+      float mm = -INFINITY, ll = 0.f;
+#pragma unroll
+      for (int i = 0; i < kMostCluster; ++i) mm = fmaxf(mm, ml[i].x);
+      const float ref = reference(mm);
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < kMostCluster; ++i) {
+        const float f = ex2((ml[i].x - ref) * c);
+        ll = fmaf(ml[i].y, f, ll);
+        acc.x = fmaf(v[i].x, f, acc.x);
+        acc.y = fmaf(v[i].y, f, acc.y);
+        acc.z = fmaf(v[i].z, f, acc.z);
+        acc.w = fmaf(v[i].w, f, acc.w);
+      }
+      const int row = b.row0 + r;
+      if (stores)
+        store_row4<D>(p, seg, s.w.q_begin, row / s.group, b.kv_head * s.group + row % s.group, col, acc, mm, ll, col == 0,
+                      D == 128 ? 0xffffffffu : 0xffffu << (lane & 16));
+    }
+    cluster.sync();                         // nobody leaves while its shared memory is read
+  }
 }
 
 // Joins the parts of a block that several CTAs worked on.  grid: (boundaries between two CTAs' shares, 16); the first boundary inside a block
@@ -717,11 +796,33 @@ cudaError_t launch_tile_join(const PagedParams& p, cudaStream_t stream) {
 template cudaError_t launch_tile_join<64>(const PagedParams&, cudaStream_t);
 template cudaError_t launch_tile_join<128>(const PagedParams&, cudaStream_t);
 
+// A cluster to each block, or all blocks shared out: what is expected to finish first, where all CTAs of the clusters can run at once.  A CTA alone on
+// its SM takes 0.47 us for a tile at D = 64 and 0.62 at D = 128; sharing out and joining take 5 us, and lengths that the host does not know
+// are taken to be half of the longest on average.  us, clusters / shared out, sequences of one length:
+//   keys                              200        1500        4000        8000        16000       32000       64000
+//   1 x 8 heads over 1 of 64       5.8/7.6    6.8/8.6     9.1/8.6    12.7/9.8    20.4/11.5   35.0/15.9   64.2/18.1
+//   1 x 32 over 8 of 64            6.1/8.3    6.9/9.4     9.1/11.6   13.0/13.4   21.5/15.8   36.7/22.7   66.9/33.2
+//   4 x 32 over 8 of 64            6.3/9.2    7.5/12.7   11.2/16.4   17.1/22.6   26.7/32.6   45.5/53.0   83.7/93.6
+//   1 x 32 over 8 of 128           7.0/9.2    7.8/10.6   11.0/13.1   16.7/16.3   27.3/23.1   47.5/33.3   87.4/52.1
+//   1 x 24 over 24 of 128          7.1/10.0   8.6/13.9   14.8/20.9   21.8/28.2   35.6/42.8   62.2/70.2    116/128
+//   3 x 8 over 2 of 128            6.9/9.2    7.9/10.3   10.9/11.7   16.2/14.5   27.5/20.6   47.4/28.1   87.4/42.7
 PagedRowsPlan plan_paged_rows(int64_t rows_of_a_head, int64_t keys, int64_t kv_heads, int64_t nseg, int head_dim, int sm_count) {
-  PagedRowsPlan plan;
+  PagedRowsPlan plan = {};
   plan.rows = rows_of_a_head <= 16 ? 16 : rows_of_a_head <= 32 ? 32 : 64;
-  const int64_t places = (rows_of_a_head + plan.rows - 1) / plan.rows * kv_heads * nseg * (keys / kKeys + 2 + kBlockCost);
-  const int64_t resident = 2 * sm_count, useful = places / kMinPlaces;
+  const int64_t resident = 2 * sm_count, tiles = keys / kKeys + 1;
+  plan.row_blocks = static_cast<int>((rows_of_a_head + plan.rows - 1) / plan.rows);
+  const int64_t units = plan.row_blocks * kv_heads * nseg;
+  int ranks = kMostCluster;
+  while (ranks > 1 && (units * ranks > resident || tiles < 2 * ranks)) ranks /= 2;
+  const double tile = head_dim == 64 ? 0.47 : 0.62, hbm = static_cast<double>(units * tiles) * kKeys * head_dim * 4 / 6.6e6;
+  const double alone = 5.6 + std::max(tile * ((tiles + ranks - 1) / ranks), hbm);
+  const double shared = 10.5 + 1.1 * (nseg > 1 ? 0.5 : 1.) * std::max(tile * units * (tiles + kBlockCost) / resident, hbm);
+  if (units * ranks <= resident && alone < shared) {
+    plan.cluster = ranks;
+    plan.ctas = static_cast<int>(units * ranks);
+    return plan;
+  }
+  const int64_t useful = units * (tiles + 1 + kBlockCost) / kMinPlaces;
   plan.ctas = static_cast<int>(useful < 2 ? 2 : useful < resident ? useful : resident);
   plan.scratch_bytes = plan.ctas * (static_cast<int64_t>(sizeof(Join)) + 2 * plan.rows * (8 + head_dim * 4));
   return plan;
@@ -729,9 +830,10 @@ PagedRowsPlan plan_paged_rows(int64_t rows_of_a_head, int64_t keys, int64_t kv_h
 
 namespace {
 
-template <int D, int WM>
+template <int D, int WM, bool kCluster>
 cudaError_t launch_rows(const PagedMap& tk, const PagedMap& tv, const PagedParams& p, const PagedRowsPlan& plan, void* scratch, cudaStream_t stream) {
   using C = Cfg<D, WM>;
+  const auto kernel = flash_paged_rows_kernel<D, WM, kCluster>;
   static bool configured[64] = {};
   static std::mutex mu;
   int dev = 0;
@@ -740,15 +842,33 @@ cudaError_t launch_rows(const PagedMap& tk, const PagedMap& tv, const PagedParam
   {
     std::lock_guard<std::mutex> lk(mu);
     if (!configured[dev & 63]) {
-      e = cudaFuncSetAttribute(flash_paged_rows_kernel<D, WM>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kBytes);
+      e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kBytes);
       if (e != cudaSuccess) return e;
       configured[dev & 63] = true;
     }
   }
-  flash_paged_rows_kernel<D, WM><<<plan.ctas, kThreads, C::kBytes, stream>>>(tk, tv, p, scratch);
+  if constexpr (kCluster) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(plan.ctas);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = C::kBytes;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = plan.cluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, tk, tv, p, scratch, plan.row_blocks);
+  }
+  kernel<<<plan.ctas, kThreads, C::kBytes, stream>>>(tk, tv, p, scratch, plan.row_blocks);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   return launch_attention_kernel(flash_paged_join_kernel<D, 16 * WM>, dim3(plan.ctas - 1, 16), 128, 0, stream, true, p, scratch);
+}
+template <int D, int WM>
+cudaError_t launch_rows(const PagedMap& tk, const PagedMap& tv, const PagedParams& p, const PagedRowsPlan& plan, void* scratch, cudaStream_t stream) {
+  return plan.cluster > 0 ? launch_rows<D, WM, true>(tk, tv, p, plan, scratch, stream) : launch_rows<D, WM, false>(tk, tv, p, plan, scratch, stream);
 }
 
 }  // namespace

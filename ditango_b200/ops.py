@@ -518,6 +518,8 @@ def flash_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, t
     sk = min(columns * P, _FAR - 1)
     if max_seqlen_k is not None:
         sk = max(0, min(sk, int(max_seqlen_k)))
+    if left >= 0:
+        sk = min(sk, left + sq + sinks)          # (the keys that a sequence's queries see together)
     if accumulate and (out is None or lse is None or out.dtype != torch.float32):
         raise _capi.ExtensionError("accumulate needs an existing fp32 (out, lse) state")
     if out is None:
@@ -543,7 +545,7 @@ def flash_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, t
             _PAGED_PLANS.clear()
         _PAGED_PLANS[key] = plan
     need, launches = plan
-    scratch = torch.empty_strided((need,), (1,), dtype=torch.uint8, device=q.device)
+    scratch = torch.empty_strided((need,), (1,), dtype=torch.uint8, device=q.device) if need else None
     q_strides = (H * D, 0 if packed else sq * H * D) if q.is_contiguous() else _strides(q, shape)
     ev = None
     if LaunchLog.events is not None:
@@ -552,7 +554,7 @@ def flash_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, t
     rc = lib.dtb_flash_paged(
         q.data_ptr(), *q_strides, k_pages.data_ptr(), *k_strides, v_pages.data_ptr(), *v_strides, pages, P, table.data_ptr(), columns,
         seqlens_k.data_ptr(), cu_seqlens_q.data_ptr() if packed else None, out.data_ptr(), _VALUES[out.dtype], lse.data_ptr(), lse_layout, accumulate,
-        nseg, sq, sk, T, H, Hk, D, D ** -0.5 if softmax_scale is None else softmax_scale, left, right, sinks, scratch.data_ptr(), need, stream)
+        nseg, sq, sk, T, H, Hk, D, D ** -0.5 if softmax_scale is None else softmax_scale, left, right, sinks, None if scratch is None else scratch.data_ptr(), need, stream)
     if rc:
         _capi.check(rc, "dtb_flash_paged")
     LaunchLog.count += launches

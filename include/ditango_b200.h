@@ -231,9 +231,9 @@ DTB_API int dtb_write_pages(const void* k, const void* v, int64_t k_tok_stride, 
  *                  keys and values of 0.
  *   seqlens_k      int32 [nseg], taken to be at most columns * page_size
  *   cu_seqlens_q   NULL for a dense batch of seqlen_q queries each, else device int32 [nseg + 1]; rows outside all sequences are left alone
- *   seqlen_q       the longest sequence's queries (of longer ones the rest is left out); seqlen_k: about the longest sequence's keys, which
- *                  only the choice of kernels goes by
- *   scratch        dtb_flash_paged_scratch_bytes(...) bytes, 16-byte aligned, of one call at a time
+ *   seqlen_q       the longest sequence's queries (of longer ones the rest is left out); seqlen_k: about the most keys that a
+ *                  sequence's queries see together, which only the choice of kernels goes by
+ *   scratch        dtb_flash_paged_scratch_bytes(...) bytes, 16-byte aligned, of one call at a time; may be NULL for 0 bytes
  */
 DTB_API int64_t dtb_flash_paged_scratch_bytes(int nseg, int seqlen_q, int seqlen_k, int64_t total_q, int num_heads, int num_kv_heads, int head_dim);
 /* Kernels that such a call launches (packed: whether cu_seqlens_q is given), for accounting. */

@@ -61,7 +61,7 @@ def test_write_refuses(args, word):
     (dict(table=None), "null"), (dict(lens=None), "null"), (dict(lse=None), "null"), (dict(kp=None), "null"), (dict(tq=21), "total"), (dict(left=-2), "window"), (dict(right=2 ** 30 + 1), "window"),
     (dict(sinks=-1), "sinks"), (dict(qt=128), "stride"), (dict(qb=128), "stride"), (dict(qt=388), "multiples of 8"), (dict(q=24), "aligned"), (dict(vp=24), "aligned"),
     (dict(ks=(4096, 192, 60)), "multiples of 8"), (dict(vs=(4096, 128, 64)), "lie over"), (dict(odt=2), "out_dtype"), (dict(lay=2), "lse_layout"), (dict(acc=1, odt=1), "accumulate"),
-    (dict(scale=0.0), "scale"), (dict(scale=float("nan")), "scale"), (dict(scratch=None), "scratch"), (dict(scratch=24), "scratch")])
+    (dict(scale=0.0), "scale"), (dict(scale=float("nan")), "scale"), (dict(scratch=24), "scratch")])
 def test_flash_refuses(args, word):
     lib = _lib()
     assert _flash(lib, **args) == -1 and word in lib.dtb_last_error().decode()
