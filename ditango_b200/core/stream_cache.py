@@ -27,6 +27,12 @@ class StreamCache:
             raise ValueError(f"page_size is a power of two from 16, not {page_size}")
         if min(layers, streams, num_pages, kv_heads, max_tokens) < 1 or head_dim not in (64, 128) or left < -1 or sinks < 0:
             raise ValueError("sizes are positive, head_dim is 64 or 128, left is -1 or more and sinks 0 or more")
+        columns = -(-max_tokens // page_size)
+        room = columns * page_size
+        if (page_size > 1 << 20 or room >= 1 << 30 or max(streams * room, num_pages * page_size) >= 1 << 31 or max(left, sinks) > 1 << 30 or
+                streams > 16384 or streams * -(-columns // 256) > 1 << 18):
+            raise ValueError("pages hold up to 2^20 tokens, a stream fewer than 2^30, all streams and all pages fewer than 2^31 each; up to 16384 streams, "
+                             "and 2^18 runs of 256 pages in their table")
         device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
         if device.type != "cuda":
             raise ExtensionError("ditango_b200 kernels take CUDA tensors only")
@@ -34,8 +40,7 @@ class StreamCache:
         self.left, self.sinks = left, sinks
         # the tokens of a page's head one after another: what attention reads of it is one run of memory
         self.pages = torch.empty(layers, 2, num_pages, kv_heads, page_size, head_dim, dtype=torch.bfloat16, device=device)
-        columns = -(-max_tokens // page_size)
-        self.max_tokens = columns * page_size
+        self.max_tokens = room
 
         def ints(*shape, fill=0):
             return torch.full(shape, fill, dtype=torch.int32, device=device)

@@ -11,6 +11,8 @@ namespace dtb {
 
 // The kernel of tiles takes the rows of 1 << pack_shift query heads that share a key head as those of one: row r of a sequence is query
 // r >> pack_shift and head (r & ((1 << pack_shift) - 1)) of them.  Its f.num_heads, f.seqlen_q and f.total_q count so; `real` does not.
+// (A tile of keys is loaded once for these heads, and a few queries of many heads fill its rows.  us, one launch after another, heads apart and together:
+// chunks and tokens mixed, 32 heads over 8, 841 -> 752; 45 queries of 16 heads to a key head against 15369 keys of 15 sequences 821 -> 253.)
 struct PagedParams : WindowParams {    // (k, v, their strides, cu_k and k_start are not used; seqlens_k is given always)
   int pack_shift;
   FlashParams real;
@@ -99,6 +101,8 @@ __device__ __forceinline__ void tma_load_token(void* smem_dst, const QueryMap* m
 // issue the loads, a lane to each 64 channels of a box.  (One thread that does all of it is what bounds a launch: 16 loads of 2 KB and 8
 // look-ups for a tile at D = 128 and pages of 16, which a step of 1.6 us takes two of.)  A request's place in the queue is taken again only
 // when the tile's slot in the ring is, that is, after its loads have landed: there are more places than loads in the ring, and nothing to wait for.
+// (us, from a graph, one thread and two warps: two CogVideoX frames over pages of 64 770 -> 654, as dense keys 637; chunks and tokens over pages of 16
+// mixed 1297 -> 924.)
 constexpr int kLoadPlaces = 16;
 constexpr int kLoadWarps = 2;            // they take requests in turn
 struct LoadRequest {

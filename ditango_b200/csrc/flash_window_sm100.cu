@@ -261,8 +261,8 @@ __device__ __forceinline__ bool claim_answer(const void* response16, int& x, int
 
 }  // namespace
 
-// grid: (row blocks, heads, sequences x parts); in pages as plan_blocks deals them out.  Keys and values dense (CUtensorMap, WindowParams) or in pages (PagedMap, PagedParams): the two
-// differ in how a sequence and a tile's rows are found.
+// grid: (row blocks, heads, sequences x parts); in pages as plan_blocks deals them out.  Keys and values dense (CUtensorMap, WindowParams) or in
+// pages (PagedMap, PagedParams): the two differ in how a sequence and a tile's rows are found.
 template <int D, class QMap, class Map, class Params>
 __global__ void __launch_bounds__(kThreads, 1)
 flash_window_kernel(const __grid_constant__ QMap tm_q, const __grid_constant__ Map tm_k,

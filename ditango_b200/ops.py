@@ -366,8 +366,9 @@ def extend_pages(table: torch.Tensor, seqlens: torch.Tensor, new_lens: torch.Ten
     table [streams, columns] holds the streams' pages; entries for new ones are written in place.  The first free_count [1] of `free` are the
     numbers of pages that nobody holds, the last of those is taken first, and `free` has one entry per page of the pool.  `tokens`, known to
     the host, is the number of rows that the new keys and values come in: new_lens add up to it or less, and slots behind the last token
-    are -1 (as is that of a token on a page that release_pages took from inside its stream).  All or nothing: with too few free pages `missing` says how many, with streams that outgrow their row or `tokens` it is -1, and then the
-    table and the numbers stay as they are.  The results are new tensors, for the next step; one launch, no host round trip."""
+    are -1 (as is that of a token on a page that release_pages took from inside its stream).  All or nothing: with too few free pages `missing`
+    says how many, with streams that outgrow their row or `tokens` it is -1, and then the table and the numbers stay as they are.  The results
+    are new tensors, for the next step; one launch, no host round trip.  Up to 16384 streams."""
     streams, columns, pages = _page_args(table, free, free_count, page_size, seqlens, new_lens, None)
     if not 0 <= tokens < (1 << 31) - 4:
         raise _capi.ExtensionError("tokens is a number of rows")
@@ -483,7 +484,8 @@ def flash_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, t
 
     Dense: q [B,Sq,H,D] bf16.  Packed: q [T,H,D] with cu_seqlens_q int32 [B + 1] on the device, up to max_seqlen_q (known to the host, T if not
     given) queries each; rows behind the last sequence are left as they are.  Hk divides H.  max_seqlen_k is about the longest sequence's
-    length, if the host knows it: kernels and numbers of CTAs are chosen by it, and results depend on it by roundings alone.
+    length, if the host knows it (the room in a row of the table if not): kernels and numbers of CTAs are chosen by it, and results depend on it by
+    roundings alone.
 
     Returns (out, lse) as flash_window does, mergeable with its states and flash_partial's; with accumulate=True the state is merged into the given
     fp32 (out, lse) in place.  A row that sees no key has out 0 and lse -inf.  Entries of the table behind a sequence's last page or for pages that no

@@ -207,10 +207,10 @@ DTB_API int64_t dtb_flash_window_scratch_bytes(int nseg, int seqlen_q, int seqle
  *                   number is out of range: then nothing was taken, slots are -1, cu_seqlens 0, the numbers those of before
  * dtb_release_pages: the pages of stream b whose tokens all lie in [begin[b], end[b]) go to the end of the list, streams and their pages in
  * order; their entries become -1.  A stream whose end it is (end[b] >= seqlens[b] > begin[b]) is begin[b] tokens long afterwards.
- *   table_out       the table afterwards, may be `table`
+ *   table_out       the table afterwards, may be `table`; seqlens_out and free_count_out are not over seqlens or free_count
  *   streams * (columns / 256, rounded up) is at most 262144.
  * dtb_write_pages: k, v of `tokens` tokens, bf16, token t at t * tok_stride, its heads dense behind it, to the slots of slots[t]; a token whose
- * slot is -1, or not in the pool, is left out.  Of two tokens with one slot either one may stay, for keys and values each.
+ * slot is -1, or not in the pool, is left out.  Slots differ from one another; two tokens with one slot leave some of either there.
  * All three are one launch.
  */
 DTB_API int dtb_extend_pages(int32_t* table, const int32_t* seqlens, const int32_t* new_lens, const int32_t* free_pages, const int32_t* free_count,

@@ -90,7 +90,9 @@ def test_tensors_on_the_cpu_and_of_other_types_are_refused():
             call()
 
 
-@pytest.mark.parametrize("args", [dict(page_size=24), dict(page_size=8), dict(layers=0), dict(head_dim=96), dict(left=-2), dict(sinks=-1), dict(max_tokens=0)])
+@pytest.mark.parametrize("args", [dict(page_size=24), dict(page_size=8), dict(layers=0), dict(head_dim=96), dict(left=-2), dict(sinks=-1), dict(max_tokens=0),
+                                  dict(page_size=1 << 21), dict(max_tokens=(1 << 30) - 3), dict(streams=16385), dict(streams=9, max_tokens=1 << 28),
+                                  dict(num_pages=1 << 27), dict(left=(1 << 30) + 1)])
 def test_stream_cache_refuses(args):
     from ditango_b200.core.stream_cache import StreamCache
     with pytest.raises(ValueError):
