@@ -512,7 +512,7 @@ cudaError_t launch_paged_tiles(const QueryMap& tm_q, const PagedMap& tm_k, const
 template <int D>
 cudaError_t launch_tile_join(const PagedParams& p, cudaStream_t stream);
 
-// Few rows: blocks of 16, 32 or 64.  Scratch, where there is a second launch, holds the states of sequences that more than one CTA works on.
+// Few rows: blocks of 16, 32, 48 or 64.  Scratch, where there is a second launch, holds the states of sequences that more than one CTA works on.
 struct PagedRowsPlan {
   int rows;                // of a block
   int row_blocks;          // of the longest sequence, for each key head

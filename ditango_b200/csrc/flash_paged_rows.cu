@@ -1,6 +1,6 @@
 // Attention of few query rows over keys and values in pages: all keys of all sequences dealt evenly to CTAs that stay.
 //
-// A row is a query and one of the heads that share a key head; a block of up to 16, 32 or 64 rows of one key head meets the keys that any row of
+// A row is a query and one of the heads that share a key head; a block of up to 16, 32, 48 or 64 rows of one key head meets the keys that any row of
 // its sequence sees, [0, first) and [lo, hi), in tiles of 64.  Sequence after sequence, key head after key head, block after block, places
 // are numbered through, one per tile and a few in front of each block for what that costs, and each CTA takes as many of them as any other: the
 // lengths stand on the device, and so every CTA works out for itself where its share begins.  Per warp of rows and keys a softmax state (m, l, O) is kept:
@@ -18,7 +18,7 @@
 //
 // us, one launch after another, and keys and values a second: 32 heads over 8 of 128, 24 tokens against 200 to 30000 keys each 107 (5.85 TB/s); a
 // token of 24 heads of 128 against 119056 keys 209; of 32 over 8 of 64 against 1500 keys 7.1.  What a launch takes beside its keys: 2 us until a share is
-// known, 3 until the first tile is there, 3 to 6 for the join.  Five queries of 32 heads over 4 of 64 against seven sequences of 5003 to 20011 keys: 36 us,
+// known, 3 until the first tile is there, 3 to 6 for the join.  Five queries of 32 heads over 4 of 64 against seven sequences of 5003 to 20011 keys: 33 us,
 // bound by those and by the rate of mma.sync on 40 rows.  Two CTAs to an SM: with one the 24 tokens take 142, with three CTAs to two SMs 110.
 #include "flash_common.cuh"
 #include "flash_paged.cuh"
@@ -34,8 +34,6 @@ namespace {
 
 using namespace flash;
 
-constexpr int kMathWarps = 4;
-constexpr int kThreads = (kMathWarps + 1) * 32;
 constexpr int kKeys = 64;                 // of a tile
 constexpr int kBlockCost = 2;             // places in front of a block's tiles
 constexpr int kMinPlaces = 2;             // of a CTA's share, unless there are fewer
@@ -46,6 +44,8 @@ constexpr int kPitch = kColumns + 8;      // floats of a row of them in shared m
 template <int D, int WM>
 struct Cfg {
   static constexpr int kRows = 16 * WM;
+  static constexpr int kMathWarps = WM == 3 ? 3 : 4;
+  static constexpr int kThreads = (kMathWarps + 1) * 32;
   static constexpr int kWN = kMathWarps / WM;                // warps that share a tile's keys
   static constexpr int kWarpKeys = kKeys / kWN;
   static constexpr int kSlabs = D / 64;
@@ -186,7 +186,8 @@ __device__ __forceinline__ float quad_sum(float v) {
 // The exponent's reference for a running maximum: 0 while no key has been seen, so that -inf - ref stays -inf.
 __device__ __forceinline__ float reference(float m) { return m == -INFINITY ? 0.f : m; }
 
-__device__ __forceinline__ void math_warps_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void math_warps_sync() { asm volatile("bar.sync 1, %0;" ::"n"(N) : "memory"); }
 
 // Four columns of a finished row: normalised, merged with the state in memory where the launch accumulates, stored.  `write_lse`: this thread
 // writes the row's lse; the threads of a row that read it before are all in its warp (`mask`) or behind a barrier.
@@ -240,12 +241,12 @@ struct Scratch {
 
 // grid: the CTAs that share all places out; with kCluster (row blocks x key heads x sequences) clusters, a row block of each sequence's `row_blocks`.
 template <int D, int WM, bool kCluster>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(Cfg<D, WM>::kThreads, 2)
 flash_paged_rows_kernel(const __grid_constant__ PagedMap tm_k, const __grid_constant__ PagedMap tm_v, const __grid_constant__ PagedParams p, void* scratch,
                         int row_blocks) {
   namespace cg = cooperative_groups;
   using C = Cfg<D, WM>;
-  constexpr int R = C::kRows, WN = C::kWN, KW = C::kWarpKeys;
+  constexpr int R = C::kRows, WN = C::kWN, KW = C::kWarpKeys, kMathWarps = C::kMathWarps, kThreads = C::kThreads;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023u);
   float* s_join = reinterpret_cast<float*>(smem + C::kStages * C::kStage);            // [warp of keys][row][kPitch]
@@ -574,7 +575,7 @@ flash_paged_rows_kernel(const __grid_constant__ PagedMap tm_k, const __grid_cons
           for (int h = 0; h < 2; ++h)
             *reinterpret_cast<float2*>(s_join + (wn * R + 16 * wm + (lane >> 2) + 8 * h) * kPitch + 8 * i + 2 * (lane & 3)) =
                 make_float2(o[x * (kColumns / 8) + i][2 * h], o[x * (kColumns / 8) + i][2 * h + 1]);
-        math_warps_sync();
+        math_warps_sync<kMathWarps * 32>();
 #pragma unroll 1
         for (int u0 = 0; u0 < b.rows * (kColumns / 4); u0 += kMathWarps * 32) {
           const int u = u0 + static_cast<int>(threadIdx.x), r = u / (kColumns / 4), col = u % (kColumns / 4) * 4;
@@ -610,7 +611,7 @@ flash_paged_rows_kernel(const __grid_constant__ PagedMap tm_k, const __grid_cons
             if (last) sc.ml[static_cast<int64_t>(slot) * R + r] = make_float2(mm, ll);
           }
         }
-        math_warps_sync();
+        math_warps_sync<kMathWarps * 32>();
       }
       next_block();
     }
@@ -813,7 +814,10 @@ template cudaError_t launch_tile_join<128>(const PagedParams&, cudaStream_t);
 //   3 x 8 over 2 of 128            6.9/9.2    7.9/10.3   10.9/11.7   16.2/14.5   27.5/20.6   47.4/28.1   87.4/42.7
 PagedRowsPlan plan_paged_rows(int64_t rows_of_a_head, int64_t keys, int64_t kv_heads, int64_t nseg, int head_dim, int sm_count) {
   PagedRowsPlan plan = {};
-  plan.rows = rows_of_a_head <= 16 ? 16 : rows_of_a_head <= 32 ? 32 : 64;
+  // As few blocks as there can be, and of these the smallest, three warps instead of four.  (us, blocks of 64 and of 48: seven sequences of 5003 to 20011
+  // keys, 32 heads over 4 of 64 / 128, five queries 35.5 / 60.2 and 32.7 / 46.8, eight to twelve 51.6 / 89.3 and 45.6 / 68.9.)
+  const int64_t r = rows_of_a_head;
+  plan.rows = r <= 16 ? 16 : r <= 32 ? 32 : r <= 48 || (r > 64 && r <= 96) ? 48 : 64;
   const int64_t resident = 2 * sm_count, tiles = keys / kKeys + 1;
   plan.row_blocks = static_cast<int>((rows_of_a_head + plan.rows - 1) / plan.rows);
   const int64_t units = plan.row_blocks * kv_heads * nseg;
@@ -855,7 +859,7 @@ cudaError_t launch_rows(const PagedMap& tk, const PagedMap& tv, const PagedParam
   if constexpr (kCluster) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(plan.ctas);
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(C::kThreads);
     cfg.dynamicSmemBytes = C::kBytes;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
@@ -866,7 +870,7 @@ cudaError_t launch_rows(const PagedMap& tk, const PagedMap& tv, const PagedParam
     cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, kernel, tk, tv, p, scratch, plan.row_blocks);
   }
-  kernel<<<plan.ctas, kThreads, C::kBytes, stream>>>(tk, tv, p, scratch, plan.row_blocks);
+  kernel<<<plan.ctas, C::kThreads, C::kBytes, stream>>>(tk, tv, p, scratch, plan.row_blocks);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   return launch_attention_kernel(flash_paged_join_kernel<D, 16 * WM>, dim3(plan.ctas - 1, 16), 128, 0, stream, true, p, scratch);
@@ -882,6 +886,7 @@ template <int D>
 cudaError_t launch_paged_rows(const PagedMap& tk, const PagedMap& tv, const PagedParams& p, const PagedRowsPlan& plan, void* scratch, cudaStream_t stream) {
   if (plan.rows == 16) return launch_rows<D, 1>(tk, tv, p, plan, scratch, stream);
   if (plan.rows == 32) return launch_rows<D, 2>(tk, tv, p, plan, scratch, stream);
+  if (plan.rows == 48) return launch_rows<D, 3>(tk, tv, p, plan, scratch, stream);
   return launch_rows<D, 4>(tk, tv, p, plan, scratch, stream);
 }
 

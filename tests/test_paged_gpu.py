@@ -269,6 +269,19 @@ def test_tokens_match_the_definition(new, lens, H, Hk, P, left, right, sinks, D)
     _attend(cache, _rand((sum(new), H, D), 50), new, left=left, right=right, sinks=sinks, out_dtype=dtype)
 
 
+# rows of a key head from 33 to 96: one block of 48, or two
+ROWS48 = [([5, 2, 0], [900, 70, 9], 16, 2), ([3], [2111], 48, 3), ([33], [1290], 2, 2), ([12, 1, 9], [3000, 64, 500], 8, 1), ([9, 11, 0, 5], [9, 4000, 3, 129], 16, 2),
+          ([24, 17, 2], [1000, 17, 65], 4, 1), ([48, 50, 1], [48, 2000, 700], 3, 3)]
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("left,right,sinks", WINDOWS)
+@pytest.mark.parametrize("new,lens,H,Hk", ROWS48)
+def test_rows_in_blocks_of_48(new, lens, H, Hk, left, right, sinks, D):
+    cache = _Cache(lens, Hk, D, 32, layout=("head", "token", "both")[len(new) % 3], seed=15)
+    _attend(cache, _rand((sum(new) + 1, H, D), 69), new, left=left, right=right, sinks=sinks, out_dtype=torch.bfloat16 if H % 4 else torch.float32)
+
+
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("left,right,sinks", WINDOWS)
 @pytest.mark.parametrize("P", [16, 64, 256])

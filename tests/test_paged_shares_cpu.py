@@ -164,7 +164,7 @@ def replay(tmp_path_factory):
         walk=kernel[kernel.index("struct Seq {"):kernel.index("__device__ __forceinline__ void ldmatrix4(")],
         constants="\n".join(re.findall(r"^constexpr int k(?:BlockCost|MinPlaces) = [^;]*;", kernel, re.M)))
     built = {}
-    for rows in (16, 32, 64):
+    for rows in (16, 32, 48, 64):
         d = tmp_path_factory.mktemp("shares")
         src, exe = str(d / "shares.cpp"), str(d / "shares")
         with open(src, "w") as f:
@@ -180,7 +180,7 @@ def replay(tmp_path_factory):
     return run
 
 
-@pytest.mark.parametrize("rows", [16, 32, 64])
+@pytest.mark.parametrize("rows", [16, 32, 48, 64])
 @pytest.mark.parametrize("seed", range(60))
 def test_shares_cover_every_key_of_every_row_once(replay, rows, seed):
     rng = random.Random(seed)
