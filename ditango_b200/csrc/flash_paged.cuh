@@ -44,6 +44,8 @@ struct alignas(64) PagedMap {
 
 // Runs of keys begin where the loads of a tile can: at a multiple of 16 tokens, or of whole tiles where no window moves them.
 __device__ __forceinline__ int key_align(const PagedParams& p) { return p.key_align; }
+template <class Walk>
+__device__ __forceinline__ int front_of(const PagedParams&, const Walk& w) { return w.front; }
 
 __device__ __forceinline__ int paged_keys(const PagedParams& p, int seg) { return max(min(p.seqlens_k[seg], p.columns << p.page_shift), 0); }
 

@@ -64,7 +64,9 @@ __device__ __forceinline__ WindowSeq window_seq(const WindowParams& p, int seg) 
 }
 
 // Of what number of keys a run that is walked begins at a multiple.  (Dense keys: anywhere.)
-__device__ __forceinline__ int key_align(const WindowParams&) { return 1; }
+__device__ __forceinline__ constexpr int key_align(const WindowParams&) { return 1; }
+template <class Walk>
+__device__ __forceinline__ constexpr int front_of(const WindowParams&, const Walk&) { return 0; }
 // Which block a CTA's place in the grid stands for: row block, head, sequence x parts, and the parts that its keys are split into.
 __device__ __forceinline__ void place_block(const WindowParams&, int&, int&, int&, int&, int&) {}
 // Rows are queries (here: times 1 << 0 heads), and where a block's results go, whichever part of its keys it has.

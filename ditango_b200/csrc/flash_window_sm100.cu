@@ -440,7 +440,7 @@ flash_window_kernel(const __grid_constant__ QMap tm_q, const __grid_constant__ M
                 if (walk.tile_of(u) == v_tile) return true;
                 v_tile = walk.tile_of(u);
                 if (!load_kv(&tm_v, v_tile, p.v_batch_first)) return false;
-                const int keys = walk.valid(v_tile), front = u == 0 ? walk.front : 0;
+                const int keys = walk.valid(v_tile), front = u == 0 ? front_of(p, walk) : 0;
                 if ((keys & 15) == 0 && front == 0) return true;
                 // What lies behind the tile's last key in its step of 16, and before its first one, is cleared.  (Nobody gives the slot back
                 // before that: the issuer waits for v_tail, so the phase waited for here is the one that this load completes.)
@@ -586,7 +586,7 @@ flash_window_kernel(const __grid_constant__ QMap tm_q, const __grid_constant__ M
           auto next_v = [&](int u) {
             if (!next_kv(v_stage, 23)) return false;
             v_steps = kBN / 16;
-            const bool front = u == 0 && walk.front > 0;
+            const bool front = u == 0 && front_of(p, walk) > 0;
             if (u != u_window && u != u_first && !front) return true;
             const int keys = u == u_window ? walk.valid(walk.N - 1) : u == u_first ? walk.valid(walk.N + walk.steps - walk.n - 1) : kBN;
             v_steps = (keys + 15) >> 4;
