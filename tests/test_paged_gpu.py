@@ -473,6 +473,53 @@ def test_results_are_the_same_on_every_run_and_stream():
     assert new and ops.read_status() == 0
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("group", [3, 7, 20, 48, 65, 128, 200])
+def test_any_number_of_heads_to_a_key_head(group, D):
+    for new, lens, Hk in (([2, 1], [300, 1], 2), ([3], [2500], 1), ([1, 5, 0, 2], [64, 1000, 0, 2], 1)):
+        cache = _Cache(lens, Hk, D, 16, seed=16)
+        _attend(cache, _rand((sum(new), group * Hk, D), 70), new, right=0, out_dtype=torch.bfloat16)
+
+
+@pytest.mark.parametrize("hint", [0, 1, 100, 4000, 2 ** 31 - 1])
+@pytest.mark.parametrize("new,lens,H,Hk", [([1], [3000], 8, 1), ([1] * 40, [700] * 39 + [20], 8, 2), ([70], [5000], 2, 2), ([300, 2], [9000, 2], 4, 2)])
+def test_a_wrong_guess_of_the_lengths_does_no_harm(new, lens, H, Hk, hint):
+    cache = _Cache(lens, Hk, 64, 32, seed=19)
+    for left in (-1, 500):
+        _attend(cache, _rand((sum(new), H, 64), 72), new, left=left, right=0, max_seqlen_k=hint)
+
+
+def test_two_graphs_at_once():
+    """(each has scratch of its own)"""
+    from ditango_b200 import ops
+    caches = [_Cache([3000, 40], 2, 64, 16, seed=17), _Cache([9000, 500, 7], 4, 128, 32, seed=18)]
+    graphs, results, expected = [], [], []
+    for cache, new, H in ((caches[0], [1, 1], 8), (caches[1], [5, 200, 2], 8), (caches[1], [1, 1, 1], 32), (caches[0], [300, 20], 4)):
+        q, cu = _rand((sum(new), H, cache.k_pages.shape[-1]), 71).cuda(), _i([sum(new[:i]) for i in range(len(new) + 1)])
+
+        def call():
+            return ops.flash_paged(q, cache.k_pages, cache.v_pages, cache.table, cache.seqlens, right=0, cu_seqlens_q=cu, max_seqlen_q=max(new))
+        expected.append([x.clone() for x in call()])
+        torch.cuda.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            results.append(call())
+        graphs[-1].inputs = q, cu
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(20):
+        for out, lse in results:
+            out.zero_()
+            lse.zero_()
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        assert ops.read_status() == 0
+        for got, want in zip(results, expected):
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
 @pytest.mark.parametrize("n", [1, 4, 300])
 def test_a_step_in_a_graph(n):
     """Pages, writes and attention of one step captured; lengths, tables and tokens of each replay are read from the device."""
