@@ -16,9 +16,9 @@
 // than 16 rows the warps share the rows out, not the keys, so that what a key costs in shared memory reads stays below what it costs in HBM.
 // P is rounded to bf16 for the product (by 2^-8 of each weight at most, as in the other attention kernels); scores, sums and states are fp32.
 //
-// us, one launch after another, and keys and values a second: 32 heads over 8 of 128, 24 tokens against 200 to 30000 keys each 107 (5.85 TB/s); a
+// us, one launch after another, and keys and values a second: 32 heads over 8 of 128, 24 tokens against 200 to 30000 keys each 106 (5.9 TB/s); a
 // token of 24 heads of 128 against 119056 keys 209; of 32 over 8 of 64 against 1500 keys 7.1.  What a launch takes beside its keys: 2 us until a share is
-// known, 3 until the first tile is there, 3 to 6 for the join.  Five queries of 32 heads over 4 of 64 against seven sequences of 5003 to 20011 keys: 33 us,
+// known, 3 until the first tile is there, 2 to 5 for the join.  Five queries of 32 heads over 4 of 64 against seven sequences of 5003 to 20011 keys: 29 us,
 // bound by those and by the rate of mma.sync on 40 rows.  Two CTAs to an SM: with one the 24 tokens take 142, with three CTAs to two SMs 110.
 #include "flash_common.cuh"
 #include "flash_paged.cuh"
@@ -57,9 +57,10 @@ struct Cfg {
   static_assert(2 * (kBytes + 1024) <= 228 * 1024, "two CTAs to an SM");
 };
 
-// What the launch that joins has to know of the boundary in front of a CTA's share.
+// What the launch that joins has to know of a block that several CTAs have parts of.  There is one for each block where the host knows that blocks are
+// fewer than boundaries between shares, else one for each boundary; only the first one inside a block counts.
 struct alignas(16) Join {
-  int parts;                 // of the block that the boundary is the first one in; 0: in none, or not the first
+  int parts;                 // 0: of none
   int cta, late;             // that has the first part; whether that was not the first block of its share
   int seg, q_begin, kv_head, row0, rows;
 };
@@ -240,6 +241,7 @@ struct Scratch {
 }  // namespace
 
 // grid: the CTAs that share all places out; with kCluster (row blocks x key heads x sequences) clusters, a row block of each sequence's `row_blocks`.
+// (Of shares: row_blocks > 0 where joins go by blocks.)
 template <int D, int WM, bool kCluster>
 __global__ void __launch_bounds__(Cfg<D, WM>::kThreads, 2)
 flash_paged_rows_kernel(const __grid_constant__ PagedMap tm_k, const __grid_constant__ PagedMap tm_v, const __grid_constant__ PagedParams p, void* scratch,
@@ -318,7 +320,7 @@ flash_paged_rows_kernel(const __grid_constant__ PagedMap tm_k, const __grid_cons
     }
     const Shares shares(all, gridDim.x);
     if (cta >= shares.ctas) {
-      if (threadIdx.x == 0) sc.joins[cta].parts = 0;
+      if (threadIdx.x == 0 && row_blocks == 0) sc.joins[cta].parts = 0;
       return;
     }
     const long long begin = shares.begin(cta);
@@ -342,7 +344,12 @@ flash_paged_rows_kernel(const __grid_constant__ PagedMap tm_k, const __grid_cons
     left = shares.begin(cta + 1) - begin;
     if (lane == 0) s = s_seq;
     __syncwarp();
-    if (threadIdx.x == 0) sc.joins[cta] = make_join(shares, s, make_block<R>(p, s, unit), seg, cta, place);
+    if (threadIdx.x == 0) {
+      const Block b = make_block<R>(p, s, unit);
+      const Join j = make_join(shares, s, b, seg, cta, place);
+      if (row_blocks == 0) sc.joins[cta] = j;
+      else if (j.parts > 0) sc.joins[(seg * p.kv_heads + b.kv_head) * row_blocks + b.row0 / R] = j;
+    }
   }
   const int unit0 = unit;
   int stage = 0;
@@ -561,6 +568,7 @@ flash_paged_rows_kernel(const __grid_constant__ PagedMap tm_k, const __grid_cons
       }
       // join the warps that shared the keys, 32 columns at a time
       const bool whole = !kCluster && tile == 0 && to == s.tiles;
+      if (whole && row_blocks > 0 && threadIdx.x == 0) sc.joins[(seg * p.kv_heads + b.kv_head) * row_blocks + b.row0 / R].parts = 0;
       const int slot = 2 * cta + (first_block ? 0 : 1);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -662,21 +670,23 @@ flash_paged_rows_kernel(const __grid_constant__ PagedMap tm_k, const __grid_cons
   }
 }
 
-// Joins the parts of a block that several CTAs worked on.  grid: (boundaries between two CTAs' shares, 16); the first boundary inside a block
-// is the one that counts.  A lane has D / 32 columns; the four warps have a row each, or share the parts of one where there are many.
+// Joins the parts of a block that several CTAs worked on.  grid: (blocks, or boundaries between two of `ctas` shares; CTAs to the rows of one).
+// A lane has D / 32 columns; the four warps have a row each, or share the parts of one where there are many.
 template <int D, int R>
-__global__ void __launch_bounds__(128) flash_paged_join_kernel(const __grid_constant__ PagedParams p, void* scratch) {
+__global__ void __launch_bounds__(128) flash_paged_join_kernel(const __grid_constant__ PagedParams p, void* scratch, int ctas, int row_blocks) {
   constexpr int kCols = D / 32;
   __shared__ float s_acc[4][D];
   __shared__ float s_sum[4];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const Scratch<D, R> sc(scratch, gridDim.x + 1);
+  const Scratch<D, R> sc(scratch, ctas);
   const int group = p.f.num_heads / p.kv_heads;
   const float c = p.f.scale_log2;
+  // (a block that its sequence has not is nobody's, and its record nothing)
+  const bool there = row_blocks == 0 || static_cast<int>(blockIdx.x) % row_blocks < make_seq<R>(p, static_cast<int>(blockIdx.x) / row_blocks / p.kv_heads).blocks;
   grid_dependency_wait();
   const int status = *reinterpret_cast<volatile int*>(p.f.status);
-  const Join j = sc.joins[blockIdx.x + 1];
-  if (status != 0) return;
+  const Join j = sc.joins[blockIdx.x + (row_blocks == 0 ? 1 : 0)];
+  if (status != 0 || !there) return;
   auto slot_of = [&](int i) { return static_cast<int64_t>(2 * (j.cta + i) + (i == 0 ? j.late : 0)) * R; };
   if (j.parts == 0) return;
   const int per_row = j.parts <= 16 ? 1 : 4;                                // warps
@@ -870,10 +880,18 @@ cudaError_t launch_rows(const PagedMap& tk, const PagedMap& tv, const PagedParam
     cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, kernel, tk, tv, p, scratch, plan.row_blocks);
   }
-  kernel<<<plan.ctas, C::kThreads, C::kBytes, stream>>>(tk, tv, p, scratch, plan.row_blocks);
+  // Joins by blocks where they are fewer; rows beside one another as far as the launch stays small, for 1000 CTAs of nothing take 0.75 us and the rows of
+  // a CTA 1.5 each.  (us, by boundaries and by blocks: five queries as above 32.5 and 28.7, of one sequence 23.6 and 17.2; 24 tokens 108.5 and 105.5; a
+  // token of 8 heads over one of 64 against 60000 keys, 296 parts of one block, 19.1 and 20.4.)
+  const int64_t units = static_cast<int64_t>(plan.row_blocks) * p.kv_heads * p.f.nseg;
+  const bool by_blocks = units < plan.ctas;
+  const int row_blocks = by_blocks ? plan.row_blocks : 0;
+  const unsigned joins = by_blocks ? static_cast<unsigned>(units) : plan.ctas - 1;
+  const unsigned rows = by_blocks ? static_cast<unsigned>(std::clamp<int64_t>(2048 / units, 4, 16 * WM)) : WM == 1 ? 8 : 16;
+  kernel<<<plan.ctas, C::kThreads, C::kBytes, stream>>>(tk, tv, p, scratch, row_blocks);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  return launch_attention_kernel(flash_paged_join_kernel<D, 16 * WM>, dim3(plan.ctas - 1, 16), 128, 0, stream, true, p, scratch);
+  return launch_attention_kernel(flash_paged_join_kernel<D, 16 * WM>, dim3(joins, rows), 128, 0, stream, true, p, scratch, plan.ctas, row_blocks);
 }
 template <int D, int WM>
 cudaError_t launch_rows(const PagedMap& tk, const PagedMap& tv, const PagedParams& p, const PagedRowsPlan& plan, void* scratch, cudaStream_t stream) {
