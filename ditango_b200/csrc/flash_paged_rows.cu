@@ -379,14 +379,21 @@ flash_paged_rows_kernel(const __grid_constant__ PagedMap tm_k, const __grid_cons
       const Block b = make_block<R>(p, s, unit);
       const int tile = tiles_before(place), to = last_tile();
       const int32_t* row = p.table + static_cast<int64_t>(seg) * p.columns;
+      // This lane's entry for a tile, looked up while the loads of the tile before are issued.  (24 tokens of 32 heads over 8 of 64, pages of 16: 62.3 us
+      // -> 59.1.)
+      auto look_up = [&](int t) {
+        const int j = (s.begin(t) + lane * box) >> p.page_shift;
+        return lane < boxes && j < p.columns ? row[j] : -1;
+      };
+      int entry = tile < to ? look_up(tile) : -1;
       for (int t = tile; t < to; ++t) {
         const int a = s.begin(t);
+        int page = entry;
+        if (t + 1 < to) entry = look_up(t + 1);
         int from, upto_key;
         b.seen(a, t < s.lead, from, upto_key);
         if (from >= upto_key) continue;
-        const int key = a + lane * box, j = key >> p.page_shift, n = (upto_key - a + box - 1) / box;       // boxes that hold a key of the tile
-        int page = -1;
-        if (lane < boxes && lane < n && j < p.columns) page = row[j];
+        const int key = a + lane * box, n = (upto_key - a + box - 1) / box;       // boxes that hold a key of the tile
         if (page < 0 || page >= p.pages) page = p.pages;         // filled with zeros
         if (wrapped && !warp_wait_or_abort(&empty[stage], use ^ 1, p.f.status, 62)) {
           ok = false;
@@ -813,15 +820,18 @@ template cudaError_t launch_tile_join<64>(const PagedParams&, cudaStream_t);
 template cudaError_t launch_tile_join<128>(const PagedParams&, cudaStream_t);
 
 // A cluster to each block, or all blocks shared out: what is expected to finish first, where all CTAs of the clusters can run at once.  A CTA alone on
-// its SM takes 0.47 us for a tile at D = 64 and 0.62 at D = 128; sharing out and joining take 5 us, and lengths that the host does not know
-// are taken to be half of the longest on average.  us, clusters / shared out, sequences of one length:
+// its SM takes 0.47 us for a tile at D = 64 and 0.62 at D = 128, over pages of 16 tokens, whose loads are small, 0.69 and 0.97 (the rule has what lies
+// between); sharing out and joining take 3.5 us, and lengths that the host does not know are taken to be two thirds of the longest on average.  us, clusters /
+// shared out, sequences of one length, pages of 64:
 //   keys                              200        1500        4000        8000        16000       32000       64000
-//   1 x 8 heads over 1 of 64       5.8/7.6    6.8/8.6     9.1/8.6    12.7/9.8    20.4/11.5   35.0/15.9   64.2/18.1
-//   1 x 32 over 8 of 64            6.1/8.3    6.9/9.4     9.1/11.6   13.0/13.4   21.5/15.8   36.7/22.7   66.9/33.2
-//   4 x 32 over 8 of 64            6.3/9.2    7.5/12.7   11.2/16.4   17.1/22.6   26.7/32.6   45.5/53.0   83.7/93.6
-//   1 x 32 over 8 of 128           7.0/9.2    7.8/10.6   11.0/13.1   16.7/16.3   27.3/23.1   47.5/33.3   87.4/52.1
-//   1 x 24 over 24 of 128          7.1/10.0   8.6/13.9   14.8/20.9   21.8/28.2   35.6/42.8   62.2/70.2    116/128
-//   3 x 8 over 2 of 128            6.9/9.2    7.9/10.3   10.9/11.7   16.2/14.5   27.5/20.6   47.4/28.1   87.4/42.7
+//   1 x 8 heads over 1 of 64       6.4/8.1    6.9/8.8     9.1/8.5    13.0/9.0    20.9/10.3   36.2/14.0   67.0/20.3
+//   1 x 32 over 8 of 64            6.4/8.4    6.8/9.0     9.1/9.3    13.1/11.5   22.0/14.0   37.6/20.5   68.9/31.0
+//   4 x 32 over 8 of 64            6.4/8.9    7.7/10.9   11.2/14.3   16.9/20.9   26.2/31.0   44.6/51.5   81.2/92.5
+//   1 x 32 over 8 of 128           7.2/9.3    7.9/10.2   11.1/10.7   16.7/14.3   27.3/21.8   47.0/31.9   86.3/52.1
+//   1 x 24 over 24 of 128          7.4/9.6    8.8/11.7   14.8/18.6   21.9/26.1   35.8/40.6   62.8/69.9    117/128
+//   3 x 8 over 2 of 128            7.2/9.2    7.9/10.0   11.1/10.7   16.2/13.1   27.0/19.1   47.0/26.7   86.1/41.5
+// ... and over pages of 16, at 1500, 4000 and 8000 keys: the second 7.4/9.1, 10.5/9.4, 16.0/12.1, the third 8.1/11.2, 12.5/15.3, 18.3/20.6, the fourth
+// 8.4/10.5, 13.3/10.9, 21.3/14.6.
 PagedRowsPlan plan_paged_rows(int64_t rows_of_a_head, int64_t keys, int64_t kv_heads, int64_t nseg, int head_dim, int sm_count) {
   PagedRowsPlan plan = {};
   // As few blocks as there can be, and of these the smallest, three warps instead of four.  (us, blocks of 64 and of 48: seven sequences of 5003 to 20011
@@ -833,9 +843,9 @@ PagedRowsPlan plan_paged_rows(int64_t rows_of_a_head, int64_t keys, int64_t kv_h
   const int64_t units = plan.row_blocks * kv_heads * nseg;
   int ranks = kMostCluster;
   while (ranks > 1 && (units * ranks > resident || tiles < 2 * ranks)) ranks /= 2;
-  const double tile = head_dim == 64 ? 0.47 : 0.62, hbm = static_cast<double>(units * tiles) * kKeys * head_dim * 4 / 6.6e6;
+  const double tile = head_dim == 64 ? 0.55 : 0.8, hbm = static_cast<double>(units * tiles) * kKeys * head_dim * 4 / 6.6e6;
   const double alone = 5.6 + std::max(tile * ((tiles + ranks - 1) / ranks), hbm);
-  const double shared = 10.5 + 1.1 * (nseg > 1 ? 0.5 : 1.) * std::max(tile * units * (tiles + kBlockCost) / resident, hbm);
+  const double shared = 9. + 1.1 * (nseg > 1 ? 0.65 : 1.) * std::max(tile * units * (tiles + kBlockCost) / resident, hbm);
   if (units * ranks <= resident && alone < shared) {
     plan.cluster = ranks;
     plan.ctas = static_cast<int>(units * ranks);
