@@ -115,19 +115,21 @@ __global__ void __launch_bounds__(kExtendThreads) extend_pages_kernel(const Exte
   __syncthreads();
 
   const int id = blockIdx.x * kExtendThreads + threadIdx.x, threads = gridDim.x * kExtendThreads;
+  // (a step from the last of nearly 2^31 rows would wrap around)
+  auto next = [&](int t, int step) { return t < p.tokens - step ? t + step : p.tokens; };
   if (refused) {
-    for (int64_t t = id; t < p.tokens; t += threads) p.slots[t] = -1;
+    for (int t = id; t < p.tokens; t = next(t, threads)) p.slots[t] = -1;
     return;
   }
-  // four tokens of a thread, which mostly are of one stream  (counted in 64 bits: a step from the last of nearly 2^31 rows ends beyond them)
+  // four tokens of a thread, which mostly are of one stream
   const int n_tokens = static_cast<int>(t_all), mask = (1 << p.page_shift) - 1;
-  for (int64_t t0 = 4 * id; t0 < p.tokens; t0 += 4 * threads) {
+  for (int t0 = 4 * id; t0 < p.tokens; t0 = next(t0, 4 * threads)) {
     int slot[4] = {-1, -1, -1, -1};
     if (t0 < n_tokens) {
-      int b = last_not_above(s_cu, p.streams, static_cast<int>(t0));
+      int b = last_not_above(s_cu, p.streams, t0);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int t = static_cast<int>(t0) + i;
+        const int t = t0 + i;
         if (t < n_tokens) {
           while (t >= s_cu[b + 1]) ++b;
           const int len = s_len[b], x = len + t - s_cu[b], j = x >> p.page_shift, first = pages_of(len, p.page_shift);
