@@ -187,6 +187,10 @@ __device__ __forceinline__ float quad_sum(float v) {
 // The exponent's reference for a running maximum: 0 while no key has been seen, so that -inf - ref stays -inf.
 __device__ __forceinline__ float reference(float m) { return m == -INFINITY ? 0.f : m; }
 
+// (m, l) of a row whose state was not formed, because a wait gave up: a sum of weights is not negative.
+__device__ __forceinline__ float2 lost_state() { return make_float2(0.f, -1.f); }
+__device__ __forceinline__ bool is_lost(float l) { return l < 0.f; }
+
 template <int N>
 __device__ __forceinline__ void math_warps_sync() { asm volatile("bar.sync 1, %0;" ::"n"(N) : "memory"); }
 
@@ -281,6 +285,7 @@ flash_paged_rows_kernel(const __grid_constant__ PagedMap tm_k, const __grid_cons
   int seg, unit, place;
   long long left;                           // places
   const int cta = blockIdx.x;
+  bool ok = true;                           // after a wait that gave up, the blocks are walked to their barriers and no result is stored
   Seq& s = s_seqs[warp];
   if constexpr (kCluster) {
     // (Nobody leaves here after a failure elsewhere: the others of its cluster wait for it.  Its waits end at once.)
@@ -310,8 +315,9 @@ flash_paged_rows_kernel(const __grid_constant__ PagedMap tm_k, const __grid_cons
       if (lane >= d) upto += u;
     }
     if (lane == 31) s_sum[warp] = upto;
-    // CTA-uniform view of the status word: a CTA that starts after a failure elsewhere does no work.
-    if (__syncthreads_or(*reinterpret_cast<volatile int*>(p.f.status) != 0)) return;
+    // CTA-uniform view of the status word: a CTA that starts after a failure elsewhere walks its blocks as after one of its own.  (It does not just leave: the
+    // launch behind this one follows the records, and the word may be clear again by then.)
+    if (__syncthreads_or(*reinterpret_cast<volatile int*>(p.f.status) != 0)) ok = false;
     long long at = upto - sum, all = 0;
 #pragma unroll
     for (int w = 0; w < kThreads / 32; ++w) {
@@ -373,7 +379,7 @@ flash_paged_rows_kernel(const __grid_constant__ PagedMap tm_k, const __grid_cons
 
   if (warp == kMathWarps) {
     // ---------------------------------------------------------------- loads: a lane per box of tokens
-    bool ok = true, wrapped = false;
+    bool wrapped = false;
     const int box = p.box_rows, boxes = kKeys / box;
     while (ok && left > 0) {
       const Block b = make_block<R>(p, s, unit);
@@ -423,7 +429,6 @@ flash_paged_rows_kernel(const __grid_constant__ PagedMap tm_k, const __grid_cons
     // ---------------------------------------------------------------- scores, weights, products
     const int wm = warp / WN, wn = warp % WN;
     const float c = p.f.scale_log2;
-    bool ok = true;             // after a wait that gave up, the blocks are walked to their barriers and nothing more is stored
     for (bool once = kCluster; once || left > 0; once = false) {
       const int tile = tiles_before(place), to = last_tile(), group = s.group;
       if (!kCluster && tile == to) {                         // places in front of a block that the next CTA begins with
@@ -580,7 +585,7 @@ flash_paged_rows_kernel(const __grid_constant__ PagedMap tm_k, const __grid_cons
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const float row_sum = quad_sum(l[h]);
-        if ((lane & 3) == 0) s_ml[wn * R + 16 * wm + (lane >> 2) + 8 * h] = make_float2(m[h], row_sum);
+        if ((lane & 3) == 0) s_ml[wn * R + 16 * wm + (lane >> 2) + 8 * h] = ok ? make_float2(m[h], row_sum) : lost_state();
       }
 #pragma unroll
       for (int x = 0; x < D / kColumns; ++x) {
@@ -594,21 +599,26 @@ flash_paged_rows_kernel(const __grid_constant__ PagedMap tm_k, const __grid_cons
 #pragma unroll 1
         for (int u0 = 0; u0 < b.rows * (kColumns / 4); u0 += kMathWarps * 32) {
           const int u = u0 + static_cast<int>(threadIdx.x), r = u / (kColumns / 4), col = u % (kColumns / 4) * 4;
-          const bool there = r < b.rows && ok;
+          float2 ml[WN];                      // (of rows that there are not too: r is below R)
+#pragma unroll
+          for (int w = 0; w < WN; ++w) ml[w] = s_ml[w * R + r];
+          float mm = -INFINITY, least = 0.f;
+#pragma unroll
+          for (int w = 0; w < WN; ++w) {
+            mm = fmaxf(mm, ml[w].x);
+            least = fminf(least, ml[w].y);
+          }
+          const bool lost = is_lost(least), there = r < b.rows && !(whole && lost);
           const uint32_t mask = __ballot_sync(0xffffffffu, there);
           if (!there) continue;
-          float mm = -INFINITY;
-#pragma unroll
-          for (int w = 0; w < WN; ++w) mm = fmaxf(mm, s_ml[w * R + r].x);
           const float ref = reference(mm);
           float ll = 0.f;
           float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
           for (int w = 0; w < WN; ++w) {
-            const float2 ml = s_ml[w * R + r];
-            const float f = ex2((ml.x - ref) * c);
+            const float f = ex2((ml[w].x - ref) * c);
             const float4 v = *reinterpret_cast<const float4*>(s_join + (w * R + r) * kPitch + col);
-            ll = fmaf(ml.y, f, ll);
+            ll = fmaf(ml[w].y, f, ll);
             acc.x = fmaf(v.x, f, acc.x);
             acc.y = fmaf(v.y, f, acc.y);
             acc.z = fmaf(v.z, f, acc.z);
@@ -620,10 +630,10 @@ flash_paged_rows_kernel(const __grid_constant__ PagedMap tm_k, const __grid_cons
             store_row4<D>(p, seg, s.w.q_begin, row / group, b.kv_head * group + row % group, x * kColumns + col, acc, mm, ll, last, mask);
           } else if (kCluster) {
             *reinterpret_cast<float4*>(s_state + r * D + x * kColumns + col) = acc;
-            if (last) s_state_ml[r] = make_float2(mm, ll);
+            if (last) s_state_ml[r] = lost ? lost_state() : make_float2(mm, ll);
           } else {
             *reinterpret_cast<float4*>(sc.o + (static_cast<int64_t>(slot) * R + r) * D + x * kColumns + col) = acc;
-            if (last) sc.ml[static_cast<int64_t>(slot) * R + r] = make_float2(mm, ll);
+            if (last) sc.ml[static_cast<int64_t>(slot) * R + r] = lost ? lost_state() : make_float2(mm, ll);
           }
         }
         math_warps_sync<kMathWarps * 32>();
@@ -655,8 +665,12 @@ flash_paged_rows_kernel(const __grid_constant__ PagedMap tm_k, const __grid_cons
         }
       }
       float mm = -INFINITY, ll = 0.f;
+      float least = 0.f;
 #pragma unroll
-      for (int i = 0; i < kMostCluster; ++i) mm = fmaxf(mm, ml[i].x);
+      for (int i = 0; i < kMostCluster; ++i) {
+        mm = fmaxf(mm, ml[i].x);
+        least = fminf(least, ml[i].y);
+      }
       const float ref = reference(mm);
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
@@ -669,7 +683,7 @@ flash_paged_rows_kernel(const __grid_constant__ PagedMap tm_k, const __grid_cons
         acc.w = fmaf(v[i].w, f, acc.w);
       }
       const int row = b.row0 + r;
-      if (stores)
+      if (stores && !is_lost(least))
         store_row4<D>(p, seg, s.w.q_begin, row / s.group, b.kv_head * s.group + row % s.group, col, acc, mm, ll, col == 0,
                       D == 128 ? 0xffffffffu : 0xffffu << (lane & 16));
     }
@@ -701,7 +715,12 @@ __global__ void __launch_bounds__(128) flash_paged_join_kernel(const __grid_cons
   for (int r0 = blockIdx.y * step; r0 < j.rows; r0 += gridDim.y * step) {
     const int r = min(r0 + warp / per_row, j.rows - 1);                     // (a warp without a row does the last one once more)
     float mm = -INFINITY, sum = 0.f, acc[kCols] = {};
-    for (int i = lane; i < j.parts; i += 32) mm = fmaxf(mm, sc.ml[slot_of(i) + r].x);
+    bool lost = false;
+    for (int i = lane; i < j.parts; i += 32) {
+      const float2 ml = sc.ml[slot_of(i) + r];
+      mm = fmaxf(mm, ml.x);
+      lost = lost || is_lost(ml.y);
+    }
     constexpr int kAhead = 8;
     for (int i0 = part; i0 < j.parts; i0 += per_row * kAhead) {
       // (all reads are under way before one is used)
@@ -723,6 +742,7 @@ __global__ void __launch_bounds__(128) flash_paged_join_kernel(const __grid_cons
       if (i0 == part) {
 #pragma unroll
         for (int d = 16; d > 0; d /= 2) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, d));
+        lost = __any_sync(0xffffffffu, lost);
       }
       const float ref = reference(mm);
 #pragma unroll
@@ -738,7 +758,7 @@ __global__ void __launch_bounds__(128) flash_paged_join_kernel(const __grid_cons
     for (int k = 0; k < kCols; ++k) s_acc[warp][lane * kCols + k] = acc[k];
     if (lane == 0) s_sum[warp] = sum;
     __syncthreads();
-    if (r0 + warp / per_row < j.rows && part == 0 && lane < D / 4) {
+    if (r0 + warp / per_row < j.rows && part == 0 && lane < D / 4 && !lost) {
       float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
       float l = 0.f;
       for (int w = warp; w < warp + per_row; ++w) {

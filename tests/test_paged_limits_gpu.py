@@ -31,3 +31,23 @@ def test_rows_up_to_the_largest_number(free):
         assert (missing.item(), left.item(), out.tolist(), cu.tolist()) == (2, 1, [16, 0], [0, 0, 0])
     for part in rows.split(1 << 28):
         assert bool((part == -1).all())
+
+
+@pytest.mark.parametrize("accumulate", [False, True])
+@pytest.mark.parametrize("lens,n", [([2000, 333], 1), ([60000], 1), ([9000, 40, 3000], 9), ([5000], 1000), ([20000, 100], 300)])
+def test_after_a_failure_nothing_is_stored_until_the_word_is_clear(lens, n, accumulate):
+    """By every kernel: clusters, shares, tiles, tiles whose keys are split, and the launches that join."""
+    from ditango_b200 import ops
+    from tests.test_flash_window_gpu import _rand
+    from tests.test_paged_gpu import _attend, _Cache
+    cache = _Cache(lens, 2, 64, 16, seed=21)
+    T = n * len(lens)
+    q = _rand((T, 8, 64), 66).cuda()
+    out, lse = torch.full((T, 8, 64), 7.0, device="cuda"), torch.full((8, T), 7.0, device="cuda")
+    kw = dict(right=0, cu_seqlens_q=_i([n * i for i in range(len(lens) + 1)]), max_seqlen_q=n, accumulate=accumulate)
+    torch.cuda.synchronize()
+    ops.post_status(5)
+    for _ in range(3):
+        ops.flash_paged(q, cache.k_pages, cache.v_pages, cache.table, cache.seqlens, out=out, lse=lse, **kw)
+    assert ops.read_status() == 5 and bool((out == 7).all()) and bool((lse == 7).all())
+    _attend(cache, q.cpu(), [n] * len(lens), right=0)
