@@ -85,6 +85,10 @@ __device__ __forceinline__ void tma_load_4d(void* smem_dst, const CUtensorMap* m
       : "memory");
 }
 
+__device__ __forceinline__ void st_relaxed16(void* to, int a, int b, int c, int d) {
+  asm volatile("st.relaxed.gpu.global.v4.s32 [%0], {%1, %2, %3, %4};" ::"l"(to), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
 __device__ __forceinline__ void prefetch_tmap(const PagedMap* m) { prefetch_tmap(&m->map); }
 
 // A tensor map of the queries [channel, head, token, batch] (batch before token where that has the smaller stride); a box is 64 channels of
@@ -315,13 +319,17 @@ __device__ __forceinline__ void plan_blocks(const PagedParams& p) {
     plan.splits = static_cast<int>(splits);
   }
   __syncthreads();
-  // one CTA leaves what the launch that joins has to know
-  if (blockIdx.x == 0 && p.most_states > 0) {
+  // Every CTA leaves what the launch that joins has to know, all of them the same: none is sure to start, since a CTA that runs may take over the block of one
+  // that has not begun, whichever that is.
+  if (p.most_states > 0) {
     for (int i = t; i < p.most_states / 2; i += kPlanThreads) {
       TileJoin j = {0, 0, 0, 0, 0, 0, 0, 0};
       if (i < plan.splits) {
-        int b = 0;
-        while (b + 1 < n && plan.first_split[b + 1] <= i) ++b;
+        int b = 0, end = n;
+        while (end - b > 1) {
+          const int mid = (b + end) >> 1;
+          if (plan.first_split[mid] <= i) b = mid; else end = mid;
+        }
         const int k = i - plan.first_split[b], block = plan.whole[b] + k;
         const WindowSeq s = window_seq(p, plan.seq[b]);
         j.seg = plan.seq[b];
@@ -332,7 +340,8 @@ __device__ __forceinline__ void plan_blocks(const PagedParams& p) {
         j.state = plan.first_state[b] + k * plan.parts[b];
         j.parts = plan.parts[b];
       }
-      p.joins[i] = j;
+      st_relaxed16(&p.joins[i].seg, j.seg, j.head, j.q0, j.rows);
+      st_relaxed16(&p.joins[i].q_begin, j.q_begin, j.state, j.parts, 0);
     }
   }
 }

@@ -75,6 +75,8 @@ DTB_API int dtb_read_status(void* stream);
  * dtb_post_status lets the host set the word (code > 0), ordered on `stream`: a watchdog that learnt
  * on the host that a peer rank is gone uses it to make kernels in flight give up their waits (they
  * poll the word) and to stop later launches, instead of letting each wait run to its limit.
+ *
+ * The word is one per device: cleared while launches are in flight on other streams, it leaves what those store not valid, and unreported.
  */
 DTB_API int dtb_peek_status_async(int* host_word, void* stream);
 DTB_API int dtb_post_status(int code, void* stream);
