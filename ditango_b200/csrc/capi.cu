@@ -932,12 +932,11 @@ DTB_API int dtb_flash_paged(const void* q, int64_t q_tok_stride, int64_t q_batch
     t.f.num_heads = num_heads >> plan.pack_shift;
     t.f.seqlen_q = seqlen_q << plan.pack_shift;
     t.f.total_q = total_q << plan.pack_shift;
-    // the grid: places for the blocks and for the parts
+    // the grid: places for the blocks and for the parts, or CTAs that share the blocks out
     t.planned = paged_planned(plan, nseg, total_q, num_heads);
     const int64_t per_seq = (static_cast<int64_t>(t.f.seqlen_q) + 255) / 256 * nseg * t.f.num_heads;
-    const int64_t blocks = t.planned ? std::min(per_seq, paged_blocks(plan, nseg, total_q, num_heads)) + plan.states : per_seq;
-    if (blocks >= (1ll << 31)) return fail(DTB_ERR_ARG, "%s: too many blocks of rows", kWhat);
-    t.blocks = static_cast<int>(blocks);
+    const int64_t blocks = std::min(per_seq, paged_blocks(plan, nseg, total_q, num_heads));
+    t.blocks = static_cast<int>(t.planned ? blocks + plan.states : std::min<int64_t>(blocks, d->sm_count));
     t.ctas = d->sm_count;
     t.most_states = t.planned ? plan.states : 0;
     t.parts.out = scratch;

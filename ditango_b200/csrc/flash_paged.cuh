@@ -22,7 +22,7 @@ struct PagedParams : WindowParams {    // (k, v, their strides, cu_k and k_start
   int key_align;                       // runs of keys are walked from a multiple of this
   int few_rows;                        // the kernel of few rows takes the sequences with at most this many queries, that of many the others
   // of the kernel of tiles:
-  int planned;                         // whether plan_blocks orders them; 0: row block, head, sequence, the first of them changing fastest
+  int planned;                         // whether plan_blocks orders them; 0: as they come, row block, head, sequence, the first of them changing fastest
   int blocks;                          // of the grid
   int ctas;                            // that run at once
   int most_states;                     // of parts, or 0: keys are not split
@@ -183,20 +183,25 @@ __device__ __forceinline__ void serve_loads(const PagedParams& p, int which) {
 // of them is far from full, keys are split:
 //   - less work than a block of the longest kind for every CTA: all of it into parts of about an even share,
 //   - a last round that wastes more than 15 %: the blocks of the last half a round in two.
-// Every CTA plans for itself, from lengths that stand on the device; batches of more sequences than there is room for are not planned.
-// (us, one launch after another: a HunyuanVideo frame with a window, 2.4 rounds of blocks, 438 -> 409; chunks and tokens mixed 898 -> 860; 200 queries of
-// 32 heads against 60000 keys 852 -> 255; two CogVideoX frames, which are not split, 643 -> 650.)
+// Every CTA plans for itself, from lengths that stand on the device.
+// Batches of more sequences than there is room for are taken as they come, and no keys are split: of each round of as many blocks as CTAs every CTA has one,
+// the next place's in the next round (for sequences alike a place would always be the same row block).  (The host knows the longest sequence's blocks alone;
+// a grid with as many for each, claimed one by one, is mostly blocks that there are not.  us, that and this: 300 streams, a prompt of 8192 and tokens, 32
+// heads over 8 of 128, 2100 and 862; 16384 streams, 2000 rows and tokens, heads of 64, 20485 and 1808; 400 chunks of 200 rows 1845 and 1692.)
 constexpr int kPlanSeqs = 256;
 constexpr int kPlanBlocks = 1 << 22;     // sums of them are exact in fp32
 constexpr int kPlanThreads = 512;
 constexpr int kBlockSteps = 5;           // what a block costs beside its steps of 128 keys, in such steps
 struct TilePlan {
-  int seqs, blocks, splits;              // sequences, 0: as the grid says; places of blocks and parts; blocks that are split
+  int seqs, blocks, splits;              // sequences; places of blocks and parts; blocks that are split
   uint16_t seq[kPlanSeqs];               // in their order
   uint16_t parts[kPlanSeqs];             // of each of a sequence's blocks from `whole` on
   int row_blocks[kPlanSeqs];             // of each head; negative: the last one first
   int whole[kPlanSeqs];
   int first[kPlanSeqs], first_split[kPlanSeqs], first_state[kPlanSeqs];      // places, split blocks and states in front of it
+  // ... or, of sequences as they come:
+  int before[kPlanThreads];              // blocks in front of each thread's run of sequences
+  int round, turn;                       // blocks of the rounds before, and this CTA's place in this one, of the thread that walks the blocks
 };
 __device__ __forceinline__ TilePlan& tile_plan() {
   __shared__ TilePlan plan;
@@ -217,19 +222,20 @@ __device__ __forceinline__ int block_steps(const WindowSeq& s, int i0, int i1) {
 }
 
 // Sum over the 512 threads, and over those before this one.
-__device__ __forceinline__ float plan_sum(float v, float& before) {
-  __shared__ float s_warp[kPlanThreads / 32];
+template <class T>
+__device__ __forceinline__ T plan_sum(T v, T& before) {
+  __shared__ T s_warp[kPlanThreads / 32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  float upto = v;
+  T upto = v;
 #pragma unroll
   for (int d = 1; d < 32; d *= 2) {
-    const float u = __shfl_up_sync(0xffffffffu, upto, d);
+    const T u = __shfl_up_sync(0xffffffffu, upto, d);
     if (lane >= d) upto += u;
   }
   __syncthreads();
   if (lane == 31) s_warp[warp] = upto;
   __syncthreads();
-  float all = 0.f;
+  T all = 0;
   before = upto - v;
 #pragma unroll
   for (int w = 0; w < kPlanThreads / 32; ++w) {
@@ -239,6 +245,10 @@ __device__ __forceinline__ float plan_sum(float v, float& before) {
   return all;
 }
 
+// Threads have runs of that many sequences, and a sequence that many blocks, where they are taken as they come.
+__device__ __forceinline__ int run_of_sequences(const PagedParams& p) { return (p.f.nseg + kPlanThreads - 1) / kPlanThreads; }
+__device__ __forceinline__ int row_blocks_of(const PagedParams& p, int seg) { return (window_seq(p, seg).q_len + 255) / 256; }
+
 __device__ __forceinline__ void plan_blocks(const WindowParams&) {}
 // By all threads.  (Sums are of whole numbers below 2^24 or of estimates: fp32 does.)
 __device__ __forceinline__ void plan_blocks(const PagedParams& p) {
@@ -246,7 +256,16 @@ __device__ __forceinline__ void plan_blocks(const PagedParams& p) {
   const int n = p.f.nseg, t = threadIdx.x;
   grid_launch_dependents();              // (the launch that joins)
   if (!p.planned) {
-    if (t == 0) plan.seqs = 0;
+    const int per = run_of_sequences(p), b0 = min(t * per, n), b1 = min(b0 + per, n);
+    int mine = 0, before;
+    for (int b = b0; b < b1; ++b) mine += row_blocks_of(p, b) * p.f.num_heads;      // (fewer than rows, which 31 bits hold)
+    const int all = plan_sum(mine, before);
+    plan.before[t] = before;
+    if (t == 0) {
+      plan.blocks = all;
+      plan.round = 0;
+      plan.turn = static_cast<int>(blockIdx.x);
+    }
     return;
   }
   __shared__ int s_steps[kPlanSeqs];
@@ -351,16 +370,26 @@ __device__ __forceinline__ void place_block(const PagedParams& p, int& bx, int& 
   int i = bx;
   splits = 1;
   state = -1;
-  if (plan.seqs == 0) {
-    const int row_blocks = (p.f.seqlen_q + 255) / 256;
-    bx = i % row_blocks;
-    by = i / row_blocks % p.f.num_heads;
-    bz = i / row_blocks / p.f.num_heads;
-    return;
-  }
   if (i >= plan.blocks) {              // (the grid has room for more than there may be)
     bx = 1 << 22;
     by = bz = 0;
+    return;
+  }
+  if (!p.planned) {
+    int lo = 0, hi = kPlanThreads;     // the last run that begins at or before it
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (plan.before[mid] <= i) lo = mid; else hi = mid;
+    }
+    i -= plan.before[lo];
+    bz = lo * run_of_sequences(p);
+    int row_blocks = row_blocks_of(p, bz);
+    while (i >= row_blocks * p.f.num_heads && bz + 1 < p.f.nseg) {
+      i -= row_blocks * p.f.num_heads;
+      row_blocks = row_blocks_of(p, ++bz);
+    }
+    by = i / row_blocks;
+    bx = i % row_blocks;
     return;
   }
   int lo = 0, hi = plan.seqs;          // the last sequence that begins at or before it
@@ -381,6 +410,16 @@ __device__ __forceinline__ void place_block(const PagedParams& p, int& bx, int& 
   by = i / abs(plan.row_blocks[lo]);
   bx = row_block_of(plan, lo, i);
   bz = plan.seq[lo] * splits + part;
+}
+__device__ __forceinline__ bool claims_blocks(const PagedParams& p) { return p.planned != 0; }
+__device__ __forceinline__ bool next_place(const PagedParams&, int& bx) {
+  TilePlan& plan = tile_plan();
+  const int ctas = static_cast<int>(gridDim.x);
+  if (plan.blocks - plan.round <= ctas) return false;
+  plan.round += ctas;
+  if (++plan.turn == ctas) plan.turn = 0;
+  bx = plan.round + plan.turn;
+  return bx < plan.blocks;               // (it is the last round)
 }
 template <class Item>
 __device__ __forceinline__ void place_results(const PagedParams&, Item& w, int state) {

@@ -69,6 +69,9 @@ template <class Walk>
 __device__ __forceinline__ constexpr int front_of(const WindowParams&, const Walk&) { return 0; }
 // Which block a CTA's place in the grid stands for: row block, head, sequence x parts, and the parts that its keys are split into.
 __device__ __forceinline__ void place_block(const WindowParams&, int&, int&, int&, int&, int&) {}
+// Whether a CTA that is done with a block claims one of the grid's that has not started; else next_place says which place is its next, if any.
+__device__ __forceinline__ constexpr bool claims_blocks(const WindowParams&) { return true; }
+__device__ __forceinline__ constexpr bool next_place(const WindowParams&, int&) { return false; }
 // Rows are queries (here: times 1 << 0 heads), and where a block's results go, whichever part of its keys it has.
 __device__ __forceinline__ constexpr int row_shift(const WindowParams&) { return 0; }
 template <class Item>

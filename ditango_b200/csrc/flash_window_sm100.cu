@@ -363,10 +363,11 @@ flash_window_kernel(const __grid_constant__ QMap tm_q, const __grid_constant__ M
         bool live = true, asked = false;
         int bx = blockIdx.x, by = blockIdx.y, bz = blockIdx.z, splits = p.splits, state = -1;
         auto ask = [&]() {
+          asked = true;
+          if (!claims_blocks(p)) return;
           fence_proxy_async_smem();            // the answer before this one has been read
           mbar_expect_tx(sh.claim, 16);
           claim_request(sh.s_claim, sh.claim);
-          asked = true;
         };
         auto publish = [&](const Item& w) {
           const int slot = published % kWork, round = published / kWork;
@@ -478,9 +479,15 @@ flash_window_kernel(const __grid_constant__ QMap tm_q, const __grid_constant__ M
             }
           }
           if (!asked) ask();
-          if (!wait_or_abort(sh.claim, claims & 1, p.f.status, 15)) break;
-          ++claims;
-          if (!claim_answer(sh.s_claim, bx, by, bz)) {
+          bool more;
+          if (claims_blocks(p)) {
+            if (!wait_or_abort(sh.claim, claims & 1, p.f.status, 15)) break;
+            ++claims;
+            more = claim_answer(sh.s_claim, bx, by, bz);
+          } else {
+            more = next_place(p, bx);
+          }
+          if (!more) {
             w.walk.steps = -1;
             publish(w);
             break;

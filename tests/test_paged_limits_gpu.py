@@ -51,3 +51,50 @@ def test_after_a_failure_nothing_is_stored_until_the_word_is_clear(lens, n, accu
         ops.flash_paged(q, cache.k_pages, cache.v_pages, cache.table, cache.seqlens, out=out, lse=lse, **kw)
     assert ops.read_status() == 5 and bool((out == 7).all()) and bool((lse == 7).all())
     _attend(cache, q.cpu(), [n] * len(lens), right=0)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("left,right,sinks", [(-1, 0, 0), (-1, -1, 0), (300, 20, 33)])
+@pytest.mark.parametrize("hints", [True, False])
+@pytest.mark.parametrize("new,lens", [([1500] + [1] * 299, [2000] + [70] * 299), ([2] * 150 + [0, 900] + [1] * 150, [50] * 150 + [0, 900] + [1] * 150), ([40] * 260, [100] * 260)])
+def test_a_long_chunk_among_hundreds_of_streams(new, lens, hints, left, right, sinks, D):
+    from tests.test_flash_window_gpu import _rand
+    from tests.test_paged_gpu import _attend, _Cache
+    cache = _Cache(lens, 2, D, 16, seed=22)
+    q = _rand((sum(new), 8, D), 71)
+    _attend(cache, q, new, left=left, right=right, sinks=sinks, **({} if hints else dict(max_seqlen_q=None)))
+
+
+def test_as_many_streams_as_there_can_be_and_a_chunk_of_any_length():
+    """Rows of one sequence times sequences are more than 2^31; the rows that there are, are not."""
+    from ditango_b200 import ops
+    streams, T, H, D, P = 65535, 262145, 32, 64, 16
+    g = torch.Generator(device="cuda").manual_seed(4)
+    q = torch.randn(T, H, D, device="cuda", generator=g).to(torch.bfloat16)
+    k_pages, v_pages = (torch.randn(8, P, H, D, device="cuda", generator=g).to(torch.bfloat16) for _ in range(2))
+    at = 40000                                            # the stream with all but one of the others' rows
+    new = torch.ones(streams, dtype=torch.int64)
+    new[at] = T - streams + 1
+    table = (torch.arange(streams, dtype=torch.int32, device="cuda") % 8)[:, None].contiguous()
+    lens = (torch.arange(streams, dtype=torch.int32, device="cuda") % 5 + 1).contiguous()
+    lens[at] = 16
+    cu = torch.zeros(streams + 1, dtype=torch.int32)
+    cu[1:] = new.cumsum(0)
+    for right in (-1, 0):
+        out, lse = ops.flash_paged(q, k_pages, v_pages, table, lens, right=right, cu_seqlens_q=cu.cuda(), lse_layout=ops.LSE_BSH)
+        assert ops.read_status() == 0
+        owner = torch.repeat_interleave(torch.arange(streams, device="cuda"), new.cuda())
+        i = torch.arange(T, device="cuda") - cu.cuda()[owner]
+        x = lens[owner] - new.cuda()[owner] + i
+        for a in range(0, T, 1 << 15):
+            rows = slice(a, min(a + (1 << 15), T))
+            k, v = (pages.float()[owner[rows] % 8] for pages in (k_pages, v_pages))                      # [rows, P, H, D]
+            j = torch.arange(P, device="cuda")
+            seen = (j < lens[owner[rows], None]) & (torch.ones_like(x[rows, None], dtype=torch.bool) if right < 0 else j <= x[rows, None])
+            s = torch.einsum("thd,tphd->thp", q[rows].float(), k).masked_fill(~seen[:, None], float("-inf")) / 8
+            top = torch.logsumexp(s, -1)
+            w = torch.where(top[..., None] == float("-inf"), 0.0, (s - top[..., None]).exp())
+            want, spread = torch.einsum("thp,tphd->thd", w, v), torch.einsum("thp,tphd->thd", w, v.abs())
+            assert bool(((out[rows] - want).abs() <= (2.0 ** -8 + 3e-4) * spread + 1e-6).all())
+            assert torch.equal(top == float("-inf"), lse[rows] == float("-inf"))
+            assert bool(((lse[rows] - top).abs()[top > float("-inf")] <= 2e-4).all())

@@ -69,11 +69,17 @@ int main(int argc, char** argv) {
   std::memset(joins.data(), 0x7f, joins.size() * sizeof(TileJoin));
   t.joins = joins.data();
   const int grid = t.blocks;
-  launch_block(cta % grid, grid, kPlanThreads, [&] { plan_blocks(t); });
+  CHECK(t.planned == (nseg <= kPlanSeqs) && (t.planned || (grid <= 148 && t.most_states == 0)));
   // who is placed where
   std::map<std::tuple<int, int, int>, std::vector<Item>> blocks;      // (sequence, head of the tiles, first row) -> its parts
   std::set<int> states;
-  for (int place = 0; place < grid; ++place) {
+  int empty = 0;
+  // one CTA's plan for all places of the grid, or each CTA's own places
+  for (int c = t.planned ? cta % grid : 0, end = t.planned ? c + 1 : grid; c < end; ++c) {
+   launch_block(c, grid, kPlanThreads, [&] { plan_blocks(t); });
+   CHECK(claims_blocks(t) == (t.planned != 0));
+   for (int place = t.planned ? 0 : c;; ++place) {
+    if (t.planned && place == grid) break;
     int bx = place, by = 0, bz = 0, splits = t.splits, state = -1;
     bool asked = true;
     const PagedParams& p = t;
@@ -84,8 +90,17 @@ int main(int argc, char** argv) {
       auto& parts = blocks[{seg, by, w.q0}];
       parts.push_back(w);
       CHECK(int(parts.size()) <= splits);
+    } else {
+      ++empty;
     }
+    if (!t.planned) {
+      if (!next_place(t, place)) break;
+      --place;
+    }
+   }
   }
+  // (a CTA without a block of its own begins at none)
+  CHECK(t.planned || empty <= grid);
   const int group = num_heads / num_kv_heads, pack = 1 << t.pack_shift;
   size_t count = 0, split = 0;
   for (int b = 0; b < nseg; ++b) {
@@ -110,7 +125,7 @@ int main(int argc, char** argv) {
         } else {
           CHECK(parts[0].q_begin == cu[b] * pack && parts[0].part == 0);
         }
-        if (head != 0) continue;
+        if (head != 0 || nseg > 1000) continue;
         for (int i = q0; i < min(q0 + 256, n * pack); i += 37) {
           const int x = lens[b] - n + (i >> t.pack_shift);
           std::vector<int> times(lens[b] + 1, 0);
@@ -160,6 +175,16 @@ def test_every_block_is_placed_once_and_its_parts_are_joined(program, new, lens,
     assert count > 0
 
 
+@pytest.mark.parametrize("new,lens", [([200, 1, 130] * 100, [220, 90, 140] * 100), ([8192] + [1] * 299, [9000] + [500] * 299), ([1] * 299 + [5000], [500] * 299 + [5000]),
+                                      ([0] * 600 + [700, 0, 0, 300] + [0] * 600, [40] * 600 + [800, 3, 0, 300] + [40] * 600), ([70] * 257, [100] * 257),
+                                      ([1] * 8000 + [20000] + [1] * 8383, [3] * 16384)])
+@pytest.mark.parametrize("heads", [(4, 1), (6, 6)])
+def test_more_sequences_than_are_planned(program, new, lens, heads):
+    for window in WINDOWS[:1] if len(new) > 2000 else WINDOWS:
+        count, split, grid = map(int, output(program, 0, *heads, *window, len(new), *[x for pair in zip(new, lens) for x in pair]).split())
+        assert count > 0 and split == 0 and grid <= 148
+
+
 def test_records_of_split_blocks_come_from_any_of_the_ctas(program):
     assert len({output(program, cta, 32, 32, -1, -1, 0, 1, 200, 60000) for cta in range(0, 64, 4)}) == 1
     assert int(output(program, 3, 32, 32, -1, -1, 0, 1, 200, 60000).split()[1]) == 32
@@ -169,7 +194,7 @@ def test_records_of_split_blocks_come_from_any_of_the_ctas(program):
 def test_batches_at_random(program, seed):
     rng = random.Random(seed)
     heads = rng.choice(((1, 1), (4, 4), (8, 1), (6, 2), (8, 2), (7, 1)))
-    n = rng.choice((1, 2, 7, 40, 256))
+    n = rng.choice((1, 2, 7, 40, 256, 257, 700))
     most = rng.choice((20, 300, 1500)) if n < 40 else 300
     pairs = [x for _ in range(n) for x in (rng.choice((0, 1, rng.randrange(most), rng.randrange(most))), rng.choice((0, rng.randrange(100), rng.randrange(6000))))]
     output(program, rng.randrange(200), *heads, *rng.choice(WINDOWS), n, *pairs)
