@@ -54,16 +54,17 @@ __device__ __forceinline__ WindowSeq paged_seq(const PagedParams& p, int seg) {
   WindowSeq s;
   const int longest = p.f.seqlen_q >> p.pack_shift;
   s.q_begin = 0;
-  s.q_len = longest;
+  int rows = longest;
   if (p.f.cu_q != nullptr) {
     // (what offsets say beyond the rows that there are is not followed)
     const int total = static_cast<int>(p.f.total_q >> p.pack_shift);
     s.q_begin = min(max(p.f.cu_q[seg], 0), total);
-    s.q_len = max(min(min(max(p.f.cu_q[seg + 1], 0), total) - s.q_begin, longest), 0);
+    rows = max(min(max(p.f.cu_q[seg + 1], 0), total) - s.q_begin, 0);
   }
+  s.q_len = min(rows, longest);          // (the rows that are kept stay where they are: the last one of all is at the last key)
   s.k_begin = seg * (p.columns << p.page_shift);
   s.k_len = paged_keys(p, seg);
-  const int64_t x = static_cast<int64_t>(s.k_len) - s.q_len;
+  const int64_t x = static_cast<int64_t>(s.k_len) - rows;
   s.from = p.left < 0 ? -kFar : clamp_position(x - p.left);
   s.to = p.right < 0 ? kFar : clamp_position(x + p.right + 1);
   s.sinks = max(min(p.sinks, s.k_len), 0);

@@ -483,7 +483,7 @@ def flash_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, t
     means no limit (right=0: causal; -1: all tokens of a chunk see one another).
 
     Dense: q [B,Sq,H,D] bf16.  Packed: q [T,H,D] with cu_seqlens_q int32 [B + 1] on the device, up to max_seqlen_q (known to the host, T if not
-    given) queries each; rows behind the last sequence are left as they are.  Hk divides H.  max_seqlen_k is about the longest sequence's
+    given) queries each; rows behind the last sequence, and behind the first max_seqlen_q of one, are left as they are.  Hk divides H.  max_seqlen_k is about the longest sequence's
     length, if the host knows it (the room in a row of the table if not): kernels and numbers of CTAs are chosen by it, and results depend on it by
     roundings alone.
 

@@ -233,7 +233,7 @@ DTB_API int dtb_write_pages(const void* k, const void* v, int64_t k_tok_stride, 
  *                  keys and values of 0.
  *   seqlens_k      int32 [nseg], taken to be at most columns * page_size
  *   cu_seqlens_q   NULL for a dense batch of seqlen_q queries each, else device int32 [nseg + 1]; rows outside all sequences are left alone
- *   seqlen_q       the longest sequence's queries (of longer ones the rest is left out); seqlen_k: about the most keys that a
+ *   seqlen_q       the longest sequence's queries (of longer ones the first seqlen_q are attended, from their positions); seqlen_k: about the most keys that a
  *                  sequence's queries see together, which only the choice of kernels goes by
  *   scratch        dtb_flash_paged_scratch_bytes(...) bytes, 16-byte aligned, of one call at a time; may be NULL for 0 bytes
  */

@@ -98,3 +98,31 @@ def test_as_many_streams_as_there_can_be_and_a_chunk_of_any_length():
             assert bool(((out[rows] - want).abs() <= (2.0 ** -8 + 3e-4) * spread + 1e-6).all())
             assert torch.equal(top == float("-inf"), lse[rows] == float("-inf"))
             assert bool(((lse[rows] - top).abs()[top > float("-inf")] <= 2e-4).all())
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("left,right,sinks", [(-1, 0, 0), (50, 7, 20), (-1, -1, 0)])
+@pytest.mark.parametrize("most", [1, 3, 40, 150, 300])
+def test_of_sequences_longer_than_said_the_first_rows_are_as_they_were(most, left, right, sinks, D):
+    from ditango_b200 import ops
+    from tests.test_flash_window_gpu import _rand
+    from tests.test_paged_gpu import _Cache
+    new, lens = [400, 2, 170], [900, 60, 200]
+    cache = _Cache(lens, 2, D, 16, seed=23)
+    q = _rand((sum(new), 4, D), 72).cuda()
+    cu = [0, 400, 402, 572]
+    call = lambda **kw: ops.flash_paged(q, cache.k_pages, cache.v_pages, cache.table, cache.seqlens, left=left, right=right, sinks=sinks, cu_seqlens_q=_i(cu),
+                                        lse_layout=ops.LSE_BSH, **kw)
+    whole, whole_lse = call()
+    out, lse = torch.full_like(whole, 7.0), torch.full_like(whole_lse, 7.0)
+    call(out=out, lse=lse, max_seqlen_q=most)
+    assert ops.read_status() == 0
+    for b, n in enumerate(new):
+        kept = min(n, most)
+        a, z = cu[b] + kept, cu[b + 1]
+        assert bool((out[a:z] == 7).all()) and bool((lse[a:z] == 7).all())
+        # (another kernel may have them: two results, each off by 2^-8 of its weights and 1e-4 for the scores)
+        rows = slice(cu[b], a)
+        assert bool((out[rows] - whole[rows]).abs().max() <= 2 * (2.0 ** -8 + 2e-4) * max(1.0, cache.v[b].abs().max().item()))
+        same = (lse[rows] == whole_lse[rows]) | ((lse[rows] - whole_lse[rows]).abs() <= 2e-4)
+        assert bool(same.all())

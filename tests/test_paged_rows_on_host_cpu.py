@@ -83,6 +83,7 @@ int main(int, char** argv) {
     lens.push_back(rnd(5) ? rnd(900) : rnd(3));
     p.f.seqlen_q = max(p.f.seqlen_q, cu[b + 1] - cu[b]);
   }
+  if (std::atoi(argv[3])) p.f.seqlen_q = max(1, p.f.seqlen_q / 2);          // of longer sequences the rest is left out
   const int T = cu.back(), extra = rnd(3);
   if (T == 0) { std::printf("0 0 0\n"); return 0; }
   const int windows[][3] = {{-1, -1, 0}, {-1, 0, 0}, {0, 0, 3}, {100, 0, 40}, {150, 7, 0}}, w = rnd(5);
@@ -155,10 +156,12 @@ int main(int, char** argv) {
       written += written_rows;
     }
   }
-  // (each row was looked at once, and those behind the last one are as they were)
+  // (each row was looked at once, and those left out and behind the last one are as they were)
+  int b = 0;
   for (int t = 0; t < T + extra; ++t)
     for (int h = 0; h < H; ++h) {
-      const float want = t < T ? 9.f : 7.f;
+      while (b < n && t >= cu[b + 1]) ++b;
+      const float want = b < n && t - cu[b] < p.f.seqlen_q ? 9.f : 7.f;
       CHECK(lse[p.f.lse_layout == 1 ? t * H + h : h * (T + extra) + t] == want);
       for (int d = 0; d < D; ++d) CHECK(out[(t * H + h) * D + d] == want);
     }
@@ -190,6 +193,12 @@ def programs(tmp_path_factory):
 def test_a_launch_that_joins_follows_what_this_one_left(programs, size, trouble):
     written = kept = joined = 0
     for seed in range(12):
-        a, b, c = map(int, output(programs[size], seed, trouble).split())
+        a, b, c = map(int, output(programs[size], seed, trouble, 0).split())
         written, kept, joined = written + a, kept + b, joined + c
     assert written > 0 and joined > 0 and (kept > 0) == (trouble > 0)
+
+
+@pytest.mark.parametrize("size", SIZES)
+def test_rows_that_are_kept_of_a_longer_sequence_stay_at_their_positions(programs, size):
+    for seed in range(12):
+        output(programs[size], seed, 0, 1)
