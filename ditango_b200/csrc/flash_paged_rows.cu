@@ -288,7 +288,8 @@ flash_paged_rows_kernel(const __grid_constant__ PagedMap tm_k, const __grid_cons
   bool ok = true;                           // after a wait that gave up, the blocks are walked to their barriers and no result is stored
   Seq& s = s_seqs[warp];
   if constexpr (kCluster) {
-    // (Nobody leaves here after a failure elsewhere: the others of its cluster wait for it.  Its waits end at once.)
+    // (Nobody leaves here after a failure elsewhere: the others of its cluster wait for it.  Rows are lost by it all the same.)
+    const int word = *reinterpret_cast<volatile int*>(p.f.status);
     const int ranks = static_cast<int>(cg::this_cluster().num_blocks()), rank = static_cast<int>(cg::this_cluster().block_rank());
     int id = cta / ranks;
     const int block = id % row_blocks;
@@ -301,7 +302,7 @@ flash_paged_rows_kernel(const __grid_constant__ PagedMap tm_k, const __grid_cons
     place = t0 + kBlockCost;
     left = t1 - t0;
     if (lane == 0) s = own;
-    __syncthreads();                        // the barriers are there
+    if (__syncthreads_or(word != 0)) ok = false;      // the barriers are there
   } else {
     const int per = (p.f.nseg + kThreads - 1) / kThreads, seg0 = min(static_cast<int>(threadIdx.x) * per, p.f.nseg), seg1 = min(seg0 + per, p.f.nseg);
     auto places = [&](const Seq& s) { return static_cast<long long>(s.blocks) * p.kv_heads * places_of(s); };
@@ -641,7 +642,7 @@ flash_paged_rows_kernel(const __grid_constant__ PagedMap tm_k, const __grid_cons
       next_block();
     }
   }
-  if (*reinterpret_cast<volatile int*>(p.f.status) != 0) __nanosleep(1000000);   // let copies in flight land
+  if (!ok) __nanosleep(1000000);           // let copies in flight land  (a warp whose waits were all met has met all of its CTA's loads)
   if constexpr (kCluster) {
     // the CTAs' states, four columns of a row per thread, the rows dealt out over the cluster
     cg::cluster_group cluster = cg::this_cluster();
@@ -649,7 +650,6 @@ flash_paged_rows_kernel(const __grid_constant__ PagedMap tm_k, const __grid_cons
     const int ranks = static_cast<int>(cluster.num_blocks());
     const Block b = make_block<R>(p, s, unit0);
     const float c = p.f.scale_log2;
-    const bool stores = *reinterpret_cast<volatile int*>(p.f.status) == 0;
     for (int u = static_cast<int>(cluster.block_rank()) * kThreads + threadIdx.x; u < b.rows * (D / 4); u += ranks * kThreads) {
       const int r = u / (D / 4), col = u % (D / 4) * 4;
       // (all reads of the other CTAs' memory are under way before one is used)
@@ -683,7 +683,7 @@ flash_paged_rows_kernel(const __grid_constant__ PagedMap tm_k, const __grid_cons
         acc.w = fmaf(v[i].w, f, acc.w);
       }
       const int row = b.row0 + r;
-      if (stores && !is_lost(least))
+      if (!is_lost(least))
         store_row4<D>(p, seg, s.w.q_begin, row / s.group, b.kv_head * s.group + row % s.group, col, acc, mm, ll, col == 0,
                       D == 128 ? 0xffffffffu : 0xffffu << (lane & 16));
     }
