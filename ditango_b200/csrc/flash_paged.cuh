@@ -107,7 +107,8 @@ __device__ __forceinline__ void tma_load_token(void* smem_dst, const QueryMap* m
 // Loads of tiles over pages.  The thread that walks a block's tiles asks for them, and two warps that have no other role look the pages up and
 // issue the loads, a lane to each 64 channels of a box.  (One thread that does all of it is what bounds a launch: 16 loads of 2 KB and 8
 // look-ups for a tile at D = 128 and pages of 16, which a step of 1.6 us takes two of.)  A request's place in the queue is taken again only
-// when the tile's slot in the ring is, that is, after its loads have landed: there are more places than loads in the ring, and nothing to wait for.
+// when the tile's slot in the ring is, that is, after its loads have landed: there are more places than loads in the ring (checked where the ring's size is
+// known), and nothing to wait for.
 // (us, from a graph, one thread and two warps: two CogVideoX frames over pages of 64 770 -> 654, as dense keys 637; chunks and tokens over pages of 16
 // mixed 1297 -> 924.)
 constexpr int kLoadPlaces = 16;

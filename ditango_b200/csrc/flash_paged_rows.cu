@@ -11,9 +11,9 @@
 // Small batches take one launch: a cluster of up to 8 CTAs to each block, which share its tiles out and join their states through distributed
 // shared memory, and nothing to add up beforehand.
 //
-// HBM-bound: a key and a value are read once for the rows of a block.  Warp 4 loads (TMA, 128-byte swizzle, every lane a page), warps
-// 0-3 compute with mma.sync, because 16 rows fill an instruction of it and a 128-row tile of tcgen05 would be empty for the most part.  With more
-// than 16 rows the warps share the rows out, not the keys, so that what a key costs in shared memory reads stays below what it costs in HBM.
+// HBM-bound: a key and a value are read once for the rows of a block.  The last warp loads (TMA, 128-byte swizzle, every lane a page), the others, three for
+// blocks of 48 rows and else four, compute with mma.sync, because 16 rows fill an instruction of it and a 128-row tile of tcgen05 would be empty for the most
+// part.  With more than 16 rows the warps share the rows out, not the keys, so that what a key costs in shared memory reads stays below what it costs in HBM.
 // P is rounded to bf16 for the product (by 2^-8 of each weight at most, as in the other attention kernels); scores, sums and states are fp32.
 //
 // us, one launch after another, and keys and values a second: 32 heads over 8 of 128, 24 tokens against 200 to 30000 keys each 106 (5.9 TB/s); a

@@ -964,6 +964,7 @@ cudaError_t launch_window_tiles(const CUtensorMap& tq, const CUtensorMap& tk, co
 }
 template <int D>
 cudaError_t launch_paged_tiles(const QueryMap& tq, const PagedMap& tk, const PagedMap& tv, const PagedParams& p, cudaStream_t stream) {
+  static_assert(kLoadPlaces >= Cfg<D>::kStages + kLoadWarps, "requests that have not been read, and those that end the queue, have places of their own");
   return launch_tiles<D>(tq, tk, tv, p, stream);
 }
 
