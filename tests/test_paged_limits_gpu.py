@@ -126,3 +126,16 @@ def test_of_sequences_longer_than_said_the_first_rows_are_as_they_were(most, lef
         assert bool((out[rows] - whole[rows]).abs().max() <= 2 * (2.0 ** -8 + 2e-4) * max(1.0, cache.v[b].abs().max().item()))
         same = (lse[rows] == whole_lse[rows]) | ((lse[rows] - whole_lse[rows]).abs() <= 2e-4)
         assert bool(same.all())
+
+
+def test_tables_of_as_many_streams_as_there_can_be():
+    import random
+
+    from tests.test_paged_gpu import _Pages
+    rng, P, streams = random.Random(5), 16, 16384
+    pages = _Pages([rng.choice((0, 1, P, rng.randrange(3 * P))) for _ in range(streams)], P, 5, 3 * streams, seed=6)
+    pages.extend([1] * streams, streams + 7)
+    pages.extend([rng.choice((0, 0, 1, rng.randrange(P))) for _ in range(streams)], streams * P)
+    pages.release([0] * streams, [rng.choice((0, P, n)) for n in pages.lens], True)
+    pages.release([rng.choice((0, 5)) for _ in range(streams)], [10 ** 6] * streams, False)
+    pages.extend([2] * streams, 2 * streams)
