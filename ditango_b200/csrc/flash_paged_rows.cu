@@ -194,10 +194,13 @@ __device__ __forceinline__ bool is_lost(float l) { return l < 0.f; }
 template <int N>
 __device__ __forceinline__ void math_warps_sync() { asm volatile("bar.sync 1, %0;" ::"n"(N) : "memory"); }
 
+// The lse of a row: of the maximum of its raw scores and the sum of its weights.
+__device__ __forceinline__ float lse_of(const PagedParams& p, float m, float l) { return (m * p.f.scale_log2 + log2f(l)) * kLn2; }
+
 // Four columns of a finished row: normalised, merged with the state in memory where the launch accumulates, stored.  `write_lse`: this thread
 // writes the row's lse; the threads of a row that read it before are all in its warp (`mask`) or behind a barrier.
 template <int D>
-__device__ __forceinline__ void store_row4(const PagedParams& p, int seg, int q_begin, int i, int head, int col, float4 acc, float m, float l,
+__device__ __forceinline__ void store_row4(const PagedParams& p, int seg, int q_begin, int i, int head, int col, float4 acc, float lse, float l,
                                            bool write_lse, uint32_t mask) {
   const int64_t tok = p.f.cu_q != nullptr ? static_cast<int64_t>(q_begin) + i : static_cast<int64_t>(seg) * p.f.seqlen_q + i;
   const int64_t li = lse_index(p.f, seg, head, i, tok), oi = tok * p.f.out_tok_stride + static_cast<int64_t>(head) * D + col;
@@ -206,7 +209,7 @@ __device__ __forceinline__ void store_row4(const PagedParams& p, int seg, int q_
   float lse_out = -INFINITY;
   if (!keep) {
     float w_new = 0.f, w_old = 0.f;
-    if (!empty) merge_weights(p.f.accumulate != 0, p.f.accumulate ? p.f.lse[li] : -INFINITY, (m * p.f.scale_log2 + log2f(l)) * kLn2, l, w_new, w_old, lse_out);
+    if (!empty) merge_weights(p.f.accumulate != 0, p.f.accumulate ? p.f.lse[li] : -INFINITY, lse, l, w_new, w_old, lse_out);
     acc.x *= w_new;
     acc.y *= w_new;
     acc.z *= w_new;
@@ -628,7 +631,7 @@ flash_paged_rows_kernel(const __grid_constant__ PagedMap tm_k, const __grid_cons
           const bool last = x == D / kColumns - 1 && col == 0;
           if (whole) {
             const int row = b.row0 + r;
-            store_row4<D>(p, seg, s.w.q_begin, row / group, b.kv_head * group + row % group, x * kColumns + col, acc, mm, ll, last, mask);
+            store_row4<D>(p, seg, s.w.q_begin, row / group, b.kv_head * group + row % group, x * kColumns + col, acc, lse_of(p, mm, ll), ll, last, mask);
           } else if (kCluster) {
             *reinterpret_cast<float4*>(s_state + r * D + x * kColumns + col) = acc;
             if (last) s_state_ml[r] = lost ? lost_state() : make_float2(mm, ll);
@@ -684,7 +687,7 @@ flash_paged_rows_kernel(const __grid_constant__ PagedMap tm_k, const __grid_cons
       }
       const int row = b.row0 + r;
       if (!is_lost(least))
-        store_row4<D>(p, seg, s.w.q_begin, row / s.group, b.kv_head * s.group + row % s.group, col, acc, mm, ll, col == 0,
+        store_row4<D>(p, seg, s.w.q_begin, row / s.group, b.kv_head * s.group + row % s.group, col, acc, lse_of(p, mm, ll), ll, col == 0,
                       D == 128 ? 0xffffffffu : 0xffffu << (lane & 16));
     }
     cluster.sync();                         // nobody leaves while its shared memory is read
@@ -770,7 +773,7 @@ __global__ void __launch_bounds__(128) flash_paged_join_kernel(const __grid_cons
         l += s_sum[w];
       }
       const int row = j.row0 + r;
-      store_row4<D>(p, j.seg, j.q_begin, row / group, j.kv_head * group + row % group, lane * 4, a, mm, l, lane == 0, D == 128 ? 0xffffffffu : 0xffffu);
+      store_row4<D>(p, j.seg, j.q_begin, row / group, j.kv_head * group + row % group, lane * 4, a, lse_of(p, mm, l), l, lane == 0, D == 128 ? 0xffffffffu : 0xffffu);
     }
     __syncthreads();
   }
@@ -824,10 +827,10 @@ __global__ void __launch_bounds__(256) flash_tile_join_kernel(const __grid_const
 #pragma unroll
     for (int k = 0; k < kCols; ++k) s_row[warp][lane * kCols + k] = acc[k];
     __syncwarp();
-    if (lane < D / 4)          // (the maximum in units of raw scores, as store_row4 takes it)
+    if (lane < D / 4)
       store_row4<D>(p, j.seg, j.q_begin >> p.pack_shift, (j.q0 + r) >> p.pack_shift, (j.head << p.pack_shift) + ((j.q0 + r) & ((1 << p.pack_shift) - 1)), lane * 4,
                     *reinterpret_cast<const float4*>(&s_row[warp][lane * 4]),
-                    top / (p.f.scale_log2 * kLn2), sum, lane == 0, D == 128 ? 0xffffffffu : 0xffffu);
+                    top + __logf(sum), sum, lane == 0, D == 128 ? 0xffffffffu : 0xffffu);
     __syncwarp();
   }
 }

@@ -139,3 +139,26 @@ def test_tables_of_as_many_streams_as_there_can_be():
     pages.release([0] * streams, [rng.choice((0, P, n)) for n in pages.lens], True)
     pages.release([rng.choice((0, 5)) for _ in range(streams)], [10 ** 6] * streams, False)
     pages.extend([2] * streams, 2 * streams)
+
+
+@pytest.mark.parametrize("accumulate", [False, True])
+@pytest.mark.parametrize("scale", [2.0 ** -126, 2.0 ** -20, 8.0])
+@pytest.mark.parametrize("lens,n", [([700], 1), ([60000], 1), ([9000, 40, 3000], 9), ([5000], 300)])
+def test_scales_from_the_smallest(lens, n, scale, accumulate):
+    """Clusters, shares, tiles whose keys are split: with a scale of nearly 0 the mean of the values, and the logarithm of their number."""
+    from ditango_b200 import ops
+    from tests.test_flash_window_gpu import SCORE, _exact, _rand
+    from tests.test_paged_gpu import _Cache
+    cache = _Cache(lens, 2, 64, 16, seed=24)
+    q = _rand((n * len(lens), 4, 64), 73)
+    out, lse = (torch.zeros(q.shape, device="cuda"), torch.full(q.shape[:2], float("-inf"), device="cuda")) if accumulate else (None, None)
+    out, lse = ops.flash_paged(q.cuda(), cache.k_pages, cache.v_pages, cache.table, cache.seqlens, cu_seqlens_q=_i([n * i for i in range(len(lens) + 1)]), max_seqlen_q=n,
+                               softmax_scale=scale, lse_layout=ops.LSE_BSH, out=out, lse=lse, accumulate=accumulate)
+    assert ops.read_status() == 0
+    for b, total in enumerate(lens):
+        rows = slice(n * b, n * (b + 1))
+        want, top, spread = _exact(q[rows], cache.k[b], cache.v[b], torch.ones(n, total, dtype=torch.bool), scale)
+        # scores are off by 2^-21 of |q||k|, which 8 makes 64 times what 1/8 makes of it: the weights by as much more than SCORE says
+        score = SCORE * max(1.0, scale * 8)
+        assert bool(((out[rows].cpu().double() - want).abs() <= (2.0 ** -8 + 2 * score) * spread + 1e-30).all())
+        assert bool(((lse[rows].cpu().double() - top).abs() <= score).all())
