@@ -74,7 +74,8 @@ class StreamCache:
                softmax_scale: Optional[float] = None) -> Tuple[torch.Tensor, torch.Tensor]:
         """Writes the new tokens' k, v [tokens, kv_heads, head_dim] into the layer's pages and attends q [tokens, heads, head_dim] over them:
         (out, lse) of ops.flash_paged, packed, rows of padding left unwritten.  `max_new` is the largest of new_lens (`tokens` if not
-        given), `max_len` about the longest stream's length, if the host knows it."""
+        given), `max_len` about the longest stream's length, if the host knows them: kernels are chosen by both, and a token of each of many streams
+        takes up to 1.7 times as long without `max_new`."""
         plan = self.plan
         if plan is None:
             raise ExtensionError("attend comes behind extend")

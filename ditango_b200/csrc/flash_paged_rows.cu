@@ -16,8 +16,8 @@
 // part.  With more than 16 rows the warps share the rows out, not the keys, so that what a key costs in shared memory reads stays below what it costs in HBM.
 // P is rounded to bf16 for the product (by 2^-8 of each weight at most, as in the other attention kernels); scores, sums and states are fp32.
 //
-// us, one launch after another, and keys and values a second: 32 heads over 8 of 128, 24 tokens against 200 to 30000 keys each 106 (5.9 TB/s); a
-// token of 24 heads of 128 against 119056 keys 209; of 32 over 8 of 64 against 1500 keys 7.1.  What a launch takes beside its keys: 2 us until a share is
+// us, one launch after another, and keys and values a second: 32 heads over 8 of 128, 24 tokens against 200 to 30000 keys each 105 (5.9 TB/s); a
+// token of 24 heads of 128 against 119056 keys 209; of 32 over 8 of 64 against 1500 keys 6.8 to 7.2.  What a launch takes beside its keys: 2 us until a share is
 // known, 3 until the first tile is there, 2 to 5 for the join.  Five queries of 32 heads over 4 of 64 against seven sequences of 5003 to 20011 keys: 29 us,
 // bound by those and by the rate of mma.sync on 40 rows.  Two CTAs to an SM: with one the 24 tokens take 142, with three CTAs to two SMs 110.
 #include "flash_common.cuh"
@@ -847,14 +847,14 @@ template cudaError_t launch_tile_join<128>(const PagedParams&, cudaStream_t);
 // between); sharing out and joining take 3.5 us, and lengths that the host does not know are taken to be two thirds of the longest on average.  us, clusters /
 // shared out, sequences of one length, pages of 64:
 //   keys                              200        1500        4000        8000        16000       32000       64000
-//   1 x 8 heads over 1 of 64       6.4/8.1    6.9/8.8     9.1/8.5    13.0/9.0    20.9/10.3   36.2/14.0   67.0/20.3
-//   1 x 32 over 8 of 64            6.4/8.4    6.8/9.0     9.1/9.3    13.1/11.5   22.0/14.0   37.6/20.5   68.9/31.0
-//   4 x 32 over 8 of 64            6.4/8.9    7.7/10.9   11.2/14.3   16.9/20.9   26.2/31.0   44.6/51.5   81.2/92.5
-//   1 x 32 over 8 of 128           7.2/9.3    7.9/10.2   11.1/10.7   16.7/14.3   27.3/21.8   47.0/31.9   86.3/52.1
-//   1 x 24 over 24 of 128          7.4/9.6    8.8/11.7   14.8/18.6   21.9/26.1   35.8/40.6   62.8/69.9    117/128
-//   3 x 8 over 2 of 128            7.2/9.2    7.9/10.0   11.1/10.7   16.2/13.1   27.0/19.1   47.0/26.7   86.1/41.5
-// ... and over pages of 16, at 1500, 4000 and 8000 keys: the second 7.4/9.1, 10.5/9.4, 16.0/12.1, the third 8.1/11.2, 12.5/15.3, 18.3/20.6, the fourth
-// 8.4/10.5, 13.3/10.9, 21.3/14.6.
+//   1 x 8 heads over 1 of 64       6.0/8.0    6.8/9.0     9.2/8.4    12.8/9.2    20.9/11.3   36.3/16.6   67.0/17.8
+//   1 x 32 over 8 of 64            6.2/8.2    6.7/8.9     9.0/9.3    12.7/11.1   21.7/13.7   37.5/20.4   68.8/31.7
+//   4 x 32 over 8 of 64            6.2/8.8    7.5/10.3   11.1/13.9   16.8/19.9   25.9/30.5   44.7/50.9   81.9/90.7
+//   1 x 32 over 8 of 128           6.9/9.0    7.7/10.2   10.8/10.4   16.4/15.1   26.8/21.6   46.5/31.6   85.7/51.4
+//   1 x 24 over 24 of 128          7.0/9.6    8.3/11.7   14.6/18.4   21.7/25.8   35.2/40.2   62.6/70.0    117/127
+//   3 x 8 over 2 of 128            6.9/9.1    7.7/9.9    10.8/10.5   15.9/12.9   26.6/18.8   46.5/26.6   85.6/41.7
+// ... and over pages of 16, at 1500, 4000 and 8000 keys: the second 7.0/8.9, 10.4/9.4, 15.8/11.7, the third 7.9/10.6, 11.9/14.9, 18.1/19.8, the fourth
+// 8.4/10.4, 13.0/10.8, 21.3/14.9.  The two thirds cost sequences of one length: the third row's last three are shared out, 11 to 18 % above clusters.
 PagedRowsPlan plan_paged_rows(int64_t rows_of_a_head, int64_t keys, int64_t kv_heads, int64_t nseg, int head_dim, int sm_count) {
   PagedRowsPlan plan = {};
   // As few blocks as there can be, and of these the smallest, three warps instead of four.  (us, blocks of 64 and of 48: seven sequences of 5003 to 20011
